@@ -57,7 +57,8 @@ extern "C" {
 #define TGOHIP_F16 1
 /* An f32 activation [M,K] already split for tgo's arithmetic (precision mode 1):
  * the f16 plane hi = f16(x) [M,K] followed by the f16 plane lo = f16(x - hi)
- * [M,K]; the same bytes as f32. tgohip_linear's x_dtype only. */
+ * [M,K]; the same bytes as f32. The x_dtype of tgohip_linear and tgohip_adapters,
+ * the out_dtype of tgohip_packed_attention. */
 #define TGOHIP_F16X2 2
 
 const char* tgohip_last_error(void);
@@ -305,6 +306,124 @@ int tgohip_dequant(tgohip_ctx* ctx, int handle, float* y);
 /* The values the MFMA path multiplies: the dequantized weight rounded once
  * to f16 (round to nearest even). y: device [K,N] f16. */
 int tgohip_dequant_f16(tgohip_ctx* ctx, int handle, uint16_t* y);
+
+/* ---- operators beside the projections and paged attention -----------------
+ * For a caller that composes its own layer: what its requests, positions and
+ * sequences need is made once (per model, per batch) under a handle, and every
+ * layer's calls then only launch kernels on the context's stream. Such calls
+ * can be captured into a HIP graph; making, changing or freeing a handle can
+ * not. No counterpart in the reference, whose step has one unscaled rotary
+ * layout, no adapters, and attention over the block pool only. */
+
+/* Rotary positions. Pair i of a head's first rotary_dim dims turns by
+ * position * w_i: (a, b) becomes m (a cos - b sin, a sin + b cos); the dims from
+ * rotary_dim on stay as they are. layout INTERLEAVED pairs dims (2i, 2i + 1)
+ * (nn/attention.go:203-211), HALF pairs (i, i + rotary_dim / 2), the order of
+ * checkpoints before weights/convert.go permutes q and k. Unscaled,
+ * w_i = base^(-2i / rotary_dim) and m = 1. Scaled for contexts longer than the
+ * trained one:
+ *   LINEAR  w_i / factor.
+ *   YARN    (YaRN, NTK by parts) pairs that turn more than `fast` times over the
+ *           `original` positions keep w_i, pairs below `slow` turns take
+ *           w_i / factor, a ramp over the pair index between the two; m is
+ *           0.1 ln(factor) + 1.
+ *   BANDS   the same ends, the ramp over the turns themselves; m = 1.
+ * attention, where not 0, is m. */
+#define TGOHIP_ROPE_INTERLEAVED 0
+#define TGOHIP_ROPE_HALF 1
+#define TGOHIP_ROPE_UNSCALED 0
+#define TGOHIP_ROPE_LINEAR 1
+#define TGOHIP_ROPE_YARN 2
+#define TGOHIP_ROPE_BANDS 3
+typedef struct {
+  int32_t head_dim;   /* even, 2 to 256 */
+  int32_t rotary_dim; /* even, 2 to head_dim */
+  int32_t layout, scaling;
+  double base;        /* rope_theta, above 1 */
+  double factor;      /* LINEAR, YARN, BANDS: at least 1 */
+  double original;    /* YARN, BANDS: the positions trained on */
+  double fast, slow;  /* YARN, BANDS: turns, fast above slow above 0 */
+  double attention;
+} tgohip_rope_cfg;
+/* A configuration's w_i (host, [rotary_dim / 2]) and m. No device. */
+int tgohip_rope_freqs(const tgohip_rope_cfg* cfg, double* inv_freq, double* attention);
+int tgohip_rope_new(tgohip_ctx* ctx, const tgohip_rope_cfg* cfg, int* handle);
+int tgohip_rope_free(tgohip_ctx* ctx, int handle);
+/* One tensor of heads: element j of head h of row t at x[t x_row + h x_head + j].
+ * Strides are in elements; x's may be 0 (one row or head for all), y's heads
+ * must not overlap. rotate 0 copies x to y (a value head narrowed to f16 beside
+ * the rotated ones). */
+typedef struct {
+  const void* x;
+  void* y;
+  int64_t x_row, x_head, y_row, y_head;
+  int32_t heads, x_dtype, y_dtype, rotate; /* TGOHIP_F32 or TGOHIP_F16 */
+} tgohip_rope_heads;
+/* Rotates n (1 to 3) tensors of T rows in one launch, row t at positions[t]
+ * (device int32, any value). Angles are reduced in double, products are f32 and
+ * a f16 y is rounded once. y may be its own x (same type and strides: in place)
+ * or lie apart from every x and other y of the call, also between the columns
+ * of the same rows; anything else is refused. */
+int tgohip_rope(tgohip_ctx* ctx, int handle, const int32_t* positions, int T,
+                const tgohip_rope_heads* heads, int n);
+
+/* Attention over packed sequences. Sequence s has q_lengths[s] query rows and
+ * kv_lengths[s] key rows, each packed one sequence behind the other (either may
+ * be 0). causal: query i of n_q sits at position n_kv - n_q + i and sees the keys
+ * up to it; otherwise every key. A query that sees no key gives zeros, and no
+ * key or value that a query does not see (another sequence's, a later token's)
+ * reaches its output, infinities and NaN included (a value it does see may turn
+ * an infinity into NaN with f32 queries: a pair's lo part may be 0). Each kv head
+ * serves H / H_kv neighbouring query heads. head_dim 64 or 128.
+ * packed_plan decomposes the batch under *handle (host arrays; *handle 0: a new
+ * one; a plan's handle: that plan is replaced in stream order, its memory
+ * reused). It holds the partial results of contexts split over several
+ * workgroups, so calls that use one plan run in stream order, not at once: two
+ * streams, or two graphs replayed at once, take a plan each. */
+int tgohip_packed_plan(tgohip_ctx* ctx, int B, const int32_t* q_lengths, const int32_t* kv_lengths,
+                       int H, int H_kv, int head_dim, int causal, int q_dtype, int* handle);
+int tgohip_packed_free(tgohip_ctx* ctx, int handle);
+/* out = softmax(scale q k^T) v over a plan's rows. q [rows, H, head_dim] in the
+ * plan's q_dtype, k and v [key rows, H_kv, head_dim] f16, out like q in f32, f16
+ * or as a pair (TGOHIP_F16X2, dense rows, the lo plane behind the hi plane). Rows
+ * are *_row elements apart, heads dense; rows start on 16-byte boundaries.
+ * scale > 0. With f32 queries the products are those of tgohip_paged_attention's
+ * f32 form (q and the probabilities as f16 hi + lo pairs, so |q| < 65504); with
+ * f16 queries the probabilities are rounded to f16. Sums, maxima and partial
+ * results are f32. Memory behind the last row stays as it is; out meets none of
+ * q, k and v. */
+int tgohip_packed_attention(tgohip_ctx* ctx, int handle, const void* q, int64_t q_row, const void* k,
+                            int64_t k_row, const void* v, int64_t v_row, float scale, void* out,
+                            int64_t out_row, int out_dtype);
+
+/* Low-rank adapters of many requests beside a shared projection [K,N]:
+ *   y[t] = base[t] + scale (x[t] . down^T) . up^T
+ * with the adapter of the request row t belongs to, y[t] = base[t] for a request
+ * without one. base is what tgohip_linear wrote.
+ * adapters_new makes a set of up to `capacity` adapters of one projection (K a
+ * multiple of 64, N of 32). adapters_put loads one at an index, replacing what
+ * was there: host planes down [rank,K] and up [N,rank], f32 (rounded to the
+ * nearest f16, refused past its range) or f16, rank 1 to 128. adapters_drop empties an index. An
+ * empty index is no adapter. put, drop and free wait for the context's stream. */
+int tgohip_adapters_new(tgohip_ctx* ctx, int K, int N, int capacity, int* handle);
+int tgohip_adapters_put(tgohip_ctx* ctx, int handle, int index, int rank, int dtype,
+                        const void* down, const void* up, float scale);
+int tgohip_adapters_drop(tgohip_ctx* ctx, int handle, int index);
+int tgohip_adapters_free(tgohip_ctx* ctx, int handle);
+/* A batch's rows, for every set and layer: request b has extents[b] rows, one
+ * request behind the other, and adapter adapters[b] (-1: none). Host arrays;
+ * *handle as for packed_plan. It holds the rows' x . down^T between the two
+ * kernels of a call, so calls that use one run in stream order, not at once. */
+int tgohip_adapter_rows(tgohip_ctx* ctx, int B, const int32_t* extents, const int32_t* adapters,
+                        int* handle);
+int tgohip_adapter_rows_free(tgohip_ctx* ctx, int handle);
+/* x [rows,K] f32, f16 or a pair; base (or NULL: zeros) and y [rows,N] in y_dtype
+ * (f32 or f16), y may be base. 16-byte aligned. Both products are f32 sums over
+ * f16 adapters; f32 and pair activations are carried as hi + lo (|x| < 65504),
+ * x . down^T as a pair scaled by a power of two per row. Rows behind the last
+ * request stay as they are. */
+int tgohip_adapters(tgohip_ctx* ctx, int set, int rows, const void* x, int x_dtype,
+                    const void* base, void* y, int y_dtype);
 
 /* ---- host-side mirrors of the reference's batched path ------------------ */
 

@@ -1,0 +1,149 @@
+"""Rotary frequencies (tgohip_rope_freqs) against their definitions, and the refusals of the
+rotary, packed-attention and adapter entry points that need no GPU: every argument a handle is
+made from is checked before the context is touched."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+import tgo_amd
+from tgo_amd import TgoError
+
+NAN = float("nan")
+YARN = dict(scaling=tgo_amd.ROPE_YARN, factor=4.0, original=32768.0, fast=32.0, slow=1.0)
+BANDS = dict(scaling=tgo_amd.ROPE_BANDS, factor=8.0, original=8192.0, fast=4.0, slow=1.0)
+
+
+def by_hand(rd, base, scaling, factor, original, fast, slow):
+    w = []
+    for i in range(rd // 2):
+        f = base ** (-2 * i / rd)
+        wave = 2 * math.pi / f  # positions per turn
+        if scaling == tgo_amd.ROPE_LINEAR:
+            f /= factor
+        elif scaling == tgo_amd.ROPE_YARN:
+            at = lambda turns: rd / 2 * math.log(original / (2 * math.pi * turns), base)  # the pair with `turns` turns
+            lo, hi = max(0, math.floor(at(fast))), min(rd - 1, math.ceil(at(slow)))
+            t = min(1, max(0, (i - lo) / max(hi - lo, 1e-3)))
+            f = (1 - t) * f + t * f / factor
+        elif scaling == tgo_amd.ROPE_BANDS:
+            if wave > original / slow:
+                f /= factor
+            elif wave > original / fast:
+                t = (original / wave - slow) / (fast - slow)
+                f = t * f + (1 - t) * f / factor
+        w.append(f)
+    return np.array(w)
+
+
+@pytest.mark.parametrize("rd", [2, 32, 96, 128, 256])
+@pytest.mark.parametrize("kw", [dict(), dict(scaling=tgo_amd.ROPE_LINEAR, factor=2.5), YARN, BANDS,
+                                dict(YARN, original=64.0), dict(BANDS, factor=1.0)])
+def test_rope_frequencies(rd, kw):
+    w, m = tgo_amd.rope_freqs(256, 1e6, rotary_dim=rd, **kw)
+    full = dict(dict(scaling=tgo_amd.ROPE_UNSCALED, factor=1.0, original=0.0, fast=0.0, slow=0.0), **kw)
+    # both sides are a few float64 operations on exp and log
+    assert np.allclose(w, by_hand(rd, 1e6, **full), rtol=1e-13, atol=0)
+    want = 0.1 * math.log(full["factor"]) + 1 if full["scaling"] == tgo_amd.ROPE_YARN else 1.0
+    assert abs(m - want) < 1e-15
+    assert tgo_amd.rope_freqs(256, 1e6, rotary_dim=rd, attention=1.25, **kw)[1] == 1.25
+
+
+def test_scaled_frequencies_keep_the_fast_pairs_and_stretch_the_slow_ones():
+    plain, _ = tgo_amd.rope_freqs(128, 1e6)
+    for kw in (YARN, BANDS):
+        w, _ = tgo_amd.rope_freqs(128, 1e6, **kw)
+        assert w[0] == plain[0]
+        assert abs(w[-1] * kw["factor"] / plain[-1] - 1) < 1e-14
+        assert (np.diff(w) < 0).all()
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(head_dim=0), "head_dim is 0"), (dict(head_dim=7), "head_dim is 7"), (dict(head_dim=258), "head_dim is 258"),
+    (dict(rotary_dim=0), "rotary_dim is 0"), (dict(rotary_dim=5), "rotary_dim is 5"),
+    (dict(rotary_dim=130), "rotary_dim is 130 of head_dim 128"), (dict(layout=2), "layout is 2"),
+    (dict(scaling=4), "scaling is 4"), (dict(scaling=-1), "scaling is -1"), (dict(base=1.0), "base is 1"),
+    (dict(base=NAN), "base is nan"), (dict(base=math.inf), "base is inf"), (dict(attention=-1.0), "attention is -1"),
+    (dict(attention=NAN), "attention is nan"), (dict(scaling=tgo_amd.ROPE_LINEAR, factor=0.5), "factor is 0.5"),
+    (dict(YARN, factor=NAN), "factor is nan"), (dict(YARN, original=0.0), "original is 0"),
+    (dict(BANDS, slow=0.0), "slow 0"), (dict(BANDS, fast=1.0), "fast is 1 and slow 1"),
+    (dict(YARN, fast=math.inf), "fast is inf"), (dict(BANDS, slow=NAN), "slow nan"),
+])
+def test_rope_refusals(change, word):
+    args = dict(dict(head_dim=128, base=1e6), **change)
+    with pytest.raises(TgoError, match=word):
+        tgo_amd.rope_freqs(**args)
+    c, h = tgo_amd.rope_cfg(**args), ctypes.c_int(0)
+    assert tgo_amd.lib().tgohip_rope_new(None, ctypes.byref(c), ctypes.byref(h)) == tgo_amd.EINVAL
+    assert word in tgo_amd.last_error() and h.value == 0
+
+
+def plan(nq, nk, H=8, Hkv=2, d=128, q=tgo_amd.F32, B=None):
+    a, b, h = tgo_amd.i32(nq), tgo_amd.i32(nk), ctypes.c_int(0)
+    rc = tgo_amd.lib().tgohip_packed_plan(None, len(nq) if B is None else B, tgo_amd.ptr(a) if len(nq) else None,
+                                          tgo_amd.ptr(b) if len(nk) else None, H, Hkv, d, 1, q, ctypes.byref(h))
+    assert h.value == 0
+    return rc, tgo_amd.last_error()
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(nq=[1], nk=[1], B=-1), "-1 sequences"), (dict(nq=[], nk=[], B=2), "q_lengths and kv_lengths"),
+    (dict(nq=[1], nk=[1], d=96), "head_dim is 96"), (dict(nq=[1], nk=[1], H=6, Hkv=4), "6 query heads over 4"),
+    (dict(nq=[1], nk=[1], H=0), "0 query heads"), (dict(nq=[1], nk=[1], Hkv=0), "over 0 kv heads"),
+    (dict(nq=[1], nk=[1], q=tgo_amd.F16X2), "q_dtype is 2"), (dict(nq=[4, -1], nk=[4, 4]), "sequence 1 has -1 queries"),
+    (dict(nq=[4, 1], nk=[-7, 4]), "and -7 keys"), (dict(nq=[1 << 28], nk=[4]), "below 2\\^30"),
+    (dict(nq=[1] * 4, nk=[1 << 29] * 4), "below 2\\^30"), (dict(nq=[3], nk=[5]), "context is missing"),
+    (dict(nq=[], nk=[]), "context is missing"),
+])
+def test_packed_plan_refusals(kw, word):
+    import re
+    rc, msg = plan(**kw)
+    assert rc == tgo_amd.EINVAL and re.search(word, msg), msg
+
+
+@pytest.mark.parametrize("K,N,cap,word", [
+    (0, 64, 1, "projection is"), (96, 64, 1, "K a multiple of 64"), (64, 48, 1, "N of 32|N a multiple of 32"),
+    (-64, 64, 1, "projection is"), (64, 64, 0, "capacity is 0"), (64, 64, 65537, "capacity is 65537"),
+    (64, 64, 4, "context is missing"),
+])
+def test_adapter_set_refusals(K, N, cap, word):
+    import re
+    h = ctypes.c_int(0)
+    assert tgo_amd.lib().tgohip_adapters_new(None, K, N, cap, ctypes.byref(h)) == tgo_amd.EINVAL
+    assert re.search(word, tgo_amd.last_error())
+
+
+@pytest.mark.parametrize("change,word", [
+    (dict(rank=0), "rank is 0"), (dict(rank=129), "rank is 129"), (dict(dtype=2), "dtype is 2"),
+    (dict(down=None), "host planes"), (dict(up=None), "host planes"), (dict(scale=math.inf), "scale is inf"),
+    (dict(scale=NAN), "scale is nan"), (dict(), "context is missing"),
+])
+def test_adapter_put_refusals(change, word):
+    plane = np.zeros(64 * 128, np.float32)
+    a = dict(dict(rank=4, dtype=tgo_amd.F32, down=plane, up=plane, scale=1.0), **change)
+    assert tgo_amd.lib().tgohip_adapters_put(None, 1, 0, a["rank"], a["dtype"], tgo_amd.ptr(a["down"]),
+                                             tgo_amd.ptr(a["up"]), a["scale"]) == tgo_amd.EINVAL
+    assert word in tgo_amd.last_error()
+
+
+@pytest.mark.parametrize("extents,who,B,word", [
+    ([1], [0], -1, "-1 requests"), ([], [], 1, "host arrays"), ([1, -2], [0, 0], 2, "request 1 has -2 rows"),
+    ([1, 1], [0, -2], 2, "names adapter -2"), ([1], [65536], 1, "names adapter 65536"),
+    ([1 << 19, 1 << 19], [0, 0], 2, "below 2\\^20"), ([3, 0], [0, -1], 2, "context is missing"),
+])
+def test_adapter_rows_refusals(extents, who, B, word):
+    import re
+    e, w, h = tgo_amd.i32(extents), tgo_amd.i32(who), ctypes.c_int(0)
+    assert tgo_amd.lib().tgohip_adapter_rows(None, B, tgo_amd.ptr(e) if extents else None,
+                                             tgo_amd.ptr(w) if who else None, ctypes.byref(h)) == tgo_amd.EINVAL
+    assert re.search(word, tgo_amd.last_error())
+
+
+def test_calls_without_a_context_are_refused():
+    L, g = tgo_amd.lib(), (tgo_amd.RopeHeads * 1)()
+    for rc in (L.tgohip_rope(None, 1, None, 1, g, 1), L.tgohip_rope_free(None, 1), L.tgohip_packed_free(None, 1),
+               L.tgohip_packed_attention(None, 1, None, 0, None, 0, None, 0, 1.0, None, 0, 0),
+               L.tgohip_adapters(None, 1, 1, None, 0, None, None, 0), L.tgohip_adapters_drop(None, 1, 0),
+               L.tgohip_adapters_free(None, 1), L.tgohip_adapter_rows_free(None, 1)):
+        assert rc == tgo_amd.EINVAL and "context is missing" in tgo_amd.last_error()

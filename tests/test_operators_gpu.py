@@ -1,0 +1,814 @@
+"""Rotary positions, packed attention and request adapters against plain float64 forms.
+
+Tolerances count roundings: u = 2^-24 for an f32 operation, 2^-22 for an operand carried as an f16
+hi + lo pair (its lo part is rounded at 2^-11 of 2^-11 of it), half an ulp of f16 (2^-11 of the
+value, 2^-25 below its normal range) for an f16 result. A product of n terms summed in f32 is off by
+4 sqrt(n) u of the sum of the terms' magnitudes, the budget of test_gemm_gpu."""
+import math
+
+import numpy as np
+import pytest
+
+import tgo_amd
+from tgo_amd import TgoError
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+HALF = 2.0 ** -11
+
+
+def f16_step(y):
+    return HALF * y.abs() + 2.0 ** -25
+
+
+# ---------------------------------------------------------------------------
+# rotary positions
+# ---------------------------------------------------------------------------
+
+SCALINGS = {"none": {}, "linear": dict(scaling=tgo_amd.ROPE_LINEAR, factor=3.0),
+            "yarn": dict(scaling=tgo_amd.ROPE_YARN, factor=4.0, original=4096.0, fast=32.0, slow=1.0),
+            "bands": dict(scaling=tgo_amd.ROPE_BANDS, factor=8.0, original=8192.0, fast=4.0, slow=1.0)}
+
+
+def rope64(torch, x, pos, rd, layout, w, m):
+    """The definition in float64, and each output's |a| + |b|."""
+    x = x.double()
+    ang = pos.double().cpu()[:, None] * torch.from_numpy(w)[None, :]
+    c, s = (m * ang.cos()).to(x.device)[:, None], (m * ang.sin()).to(x.device)[:, None]
+    y, mag = x.clone(), torch.zeros_like(x)
+    ia = torch.arange(rd // 2, device=x.device)
+    ia, ib = (ia, ia + rd // 2) if layout == tgo_amd.ROPE_HALF else (2 * ia, 2 * ia + 1)
+    a, b = x[..., ia], x[..., ib]
+    y[..., ia], y[..., ib] = a * c - b * s, a * s + b * c
+    mag[..., ia] = mag[..., ib] = m * (a.abs() + b.abs())
+    return y, mag
+
+
+def check_rope(torch, got, x, pos, rd, layout, w, m):
+    want, mag = rope64(torch, x, pos, rd, layout, w, m)
+    # cos and sin in f32 to 2 ulp of 1 (the angle itself to 2^-30 turns at |position| < 2^31), two
+    # products and a sum: 2^-23 + 2^-24 * 3 < 2^-21
+    tol = 2.0 ** -21 * mag
+    if got.dtype == torch.float16:
+        tol = tol + f16_step(want)
+    err = (got.double() - want).abs()
+    assert bool((err <= tol).all()), float((err - tol).max())
+
+
+@pytest.mark.parametrize("scaling", sorted(SCALINGS))
+@pytest.mark.parametrize("layout", [tgo_amd.ROPE_INTERLEAVED, tgo_amd.ROPE_HALF])
+@pytest.mark.parametrize("d,rd,T,H,Hkv", [(128, 128, 1, 32, 8), (128, 64, 37, 5, 3), (64, 64, 300, 2, 1),
+                                          (80, 20, 65, 3, 1), (96, 96, 9, 24, 8), (256, 256, 130, 4, 2), (2, 2, 3, 1, 1),
+                                          (10, 6, 5, 7, 1), (128, 32, 1153, 16, 8)])
+def test_rope_over_a_fused_row(ctx, torch_gpu, d, rd, T, H, Hkv, layout, scaling):
+    torch = torch_gpu
+    g = torch.Generator(device="cuda").manual_seed(d * T + rd)
+    row = torch.randn(T, H + 2 * Hkv, d, device="cuda", generator=g)
+    pos = torch.randint(-70000, 200000, (T,), device="cuda", generator=g, dtype=torch.int32)
+    w, m = tgo_amd.rope_freqs(d, 1e6, rotary_dim=rd, layout=layout, **SCALINGS[scaling])
+    h = ctx.rope_new(d, 1e6, rotary_dim=rd, layout=layout, **SCALINGS[scaling])
+    try:
+        q = torch.full((T, H, d), float("nan"), device="cuda")
+        k = torch.full((T, Hkv, d), float("nan"), device="cuda", dtype=torch.float16)
+        v = torch.full((T, Hkv, d), float("nan"), device="cuda", dtype=torch.float16)
+        xq, xk, xv = row[:, :H], row[:, H:H + Hkv], row[:, H + Hkv:]
+        ctx.rope(h, pos, [(xq, q), (xk, k), (xv, v, False)])
+        torch.cuda.synchronize()
+        check_rope(torch, q, xq, pos, rd, layout, w, m)
+        check_rope(torch, k, xk, pos, rd, layout, w, m)
+        assert torch.equal(v, xv.half())
+        # in place, f16, and apart: the same bits
+        f = row.half()
+        apart = torch.empty_like(f)
+        ctx.rope(h, pos, [(f, apart)])
+        ctx.rope(h, pos, [(f[:, :H], f[:, :H]), (f[:, H:], f[:, H:])])
+        torch.cuda.synchronize()
+        check_rope(torch, apart, row.half(), pos, rd, layout, w, m)
+        assert torch.equal(f, apart)
+    finally:
+        ctx.rope_free(h)
+
+
+@pytest.mark.parametrize("layout", [tgo_amd.ROPE_INTERLEAVED, tgo_amd.ROPE_HALF])
+def test_rope_strides_orders_and_alignments(ctx, torch_gpu, layout):
+    """Heads-major order, rows and heads apart by odd distances, starts off 16 bytes, one row or head
+    read by all: the values of the dense call, to the bit, and nothing outside y written."""
+    torch = torch_gpu
+    T, H, d, rd = 33, 6, 64, 48
+    w, m = tgo_amd.rope_freqs(d, 1e4, rotary_dim=rd, layout=layout)
+    h = ctx.rope_new(d, 1e4, rotary_dim=rd, layout=layout)
+    pos = torch.arange(T, device="cuda", dtype=torch.int32) * 977
+    try:
+        for xt in (torch.float32, torch.float16):
+            for yt in (torch.float32, torch.float16):
+                x = torch.randn(T, H, d, device="cuda").to(xt)
+                dense = torch.empty(T, H, d, device="cuda", dtype=yt)
+                ctx.rope(h, pos, [(x, dense)])
+                check_rope(torch, dense, x, pos, rd, layout, w, m)
+                for off, pad, order in ((0, 0, "hm"), (1, 3, "rm"), (2, 6, "rm"), (5, 1, "hm"), (4, 8, "rm")):
+                    shape = (T, H, d + pad) if order == "rm" else (H, T, d + pad)
+
+                    def strided(ty):
+                        buf = torch.full((off + math.prod(shape),), -7.0, device="cuda", dtype=ty)
+                        t = buf[off:].view(shape)[..., :d]
+                        return buf, t if order == "rm" else t.transpose(0, 1)
+                    _, xs = strided(xt)
+                    xs.copy_(x)
+                    buf, ys = strided(yt)
+                    ctx.rope(h, pos, [(xs, ys)])
+                    torch.cuda.synchronize()
+                    assert torch.equal(ys, dense), (xt, yt, off, pad, order)
+                    ys.fill_(-7.0)
+                    assert bool((buf == -7.0).all())
+        x = torch.randn(1, 1, d, device="cuda").expand(T, H, d)
+        y = torch.empty(T, H, d, device="cuda")
+        ctx.rope(h, pos, [(x, y)])
+        check_rope(torch, y, x, pos, rd, layout, w, m)
+    finally:
+        ctx.rope_free(h)
+
+
+def test_rope_far_positions(ctx, torch_gpu):
+    torch = torch_gpu
+    pos = torch.tensor([0, 1, -1, 2 ** 31 - 1, -2 ** 31, 131071, 10 ** 9], dtype=torch.int32, device="cuda")
+    h = ctx.rope_new(128, 1e6)
+    try:
+        w, m = tgo_amd.rope_freqs(128, 1e6)
+        x = torch.randn(7, 4, 128, device="cuda")
+        y = torch.empty_like(x)
+        ctx.rope(h, pos, [(x, y)])
+        check_rope(torch, y, x, pos, 128, tgo_amd.ROPE_INTERLEAVED, w, m)
+        assert torch.equal(y[0], x[0])
+    finally:
+        ctx.rope_free(h)
+
+
+def test_rope_nonfinite_values_stay_in_their_pair(ctx, torch_gpu):
+    torch = torch_gpu
+    h = ctx.rope_new(128, 1e6, rotary_dim=64, layout=tgo_amd.ROPE_HALF)
+    try:
+        x = torch.randn(5, 2, 128, device="cuda")
+        pos = torch.arange(5, device="cuda", dtype=torch.int32)
+        y0, y1 = torch.empty_like(x), torch.empty_like(x)
+        ctx.rope(h, pos, [(x, y0)])
+        x[2, 1, 3] = float("nan")
+        x[3, 0, 100] = float("inf")
+        ctx.rope(h, pos, [(x, y1)])
+        torch.cuda.synchronize()
+        same = torch.ones_like(x, dtype=torch.bool)
+        same[2, 1, 3] = same[2, 1, 35] = same[3, 0, 100] = False
+        assert torch.equal(y0[same], y1[same])
+        assert y1[2, 1, 3].isnan() and y1[2, 1, 35].isnan() and y1[3, 0, 100] == float("inf")
+    finally:
+        ctx.rope_free(h)
+
+
+def test_rope_refusals(ctx, torch_gpu):
+    torch = torch_gpu
+    h = ctx.rope_new(64, 1e4)
+    L = tgo_amd.lib()
+    try:
+        x, y = torch.randn(4, 2, 64, device="cuda"), torch.zeros(4, 2, 64, device="cuda")
+        pos = torch.zeros(4, device="cuda", dtype=torch.int32)
+        xa, ya = x.data_ptr(), y.data_ptr()
+
+        def call(n=1, T=4, p=pos.data_ptr(), handle=h, **kw):
+            g = (tgo_amd.RopeHeads * 3)()
+            for i in range(3):
+                a = dict(x=xa, y=ya, x_row=128, x_head=64, y_row=128, y_head=64, heads=2, x_dtype=0, y_dtype=0, rotate=1)
+                a.update(kw)
+                for f, v in a.items():
+                    setattr(g[i], f, v)
+            rc = L.tgohip_rope(ctx.h, handle, p, T, g, n)
+            return "" if rc == 0 else tgo_amd.last_error()
+
+        for msg, kw in (("no handle 99999", dict(handle=99999)), ("rows; 0 to", dict(T=-1)), ("rows; 0 to", dict(T=1 << 24)),
+                        ("1 to 3", dict(n=0)), ("1 to 3", dict(n=4)), ("positions is a device", dict(p=None)),
+                        ("x and y are device", dict(x=None)), ("x and y are device", dict(y=None)), ("0 heads", dict(heads=0)),
+                        ("f32 or f16", dict(x_dtype=2)), ("f32 or f16", dict(y_dtype=-1)), ("not aligned", dict(x=xa + 2)),
+                        ("not aligned", dict(y=ya + 1)), ("strides are not negative", dict(x_row=-1)),
+                        ("strides are not negative", dict(x_head=1 << 41)), ("heads of y overlap", dict(y_head=63)),
+                        ("heads of y overlap", dict(y_row=127)), ("heads of y overlap", dict(y_row=0)),
+                        ("meets x", dict(y=xa + 4)), ("meets x", dict(y=xa, y_dtype=1)), ("meets x", dict(y=xa, y_row=256)),
+                        ("and 1 meet in memory", dict(n=2))):
+            assert msg in call(**kw), (msg, kw, tgo_amd.last_error())
+        assert call(T=0, p=None) == ""
+        torch.cuda.synchronize()
+        assert bool((y == 0).all())
+        with pytest.raises(TgoError, match="float32 or float16"):
+            ctx.rope(h, pos, [(x.bfloat16(), y)])
+        with pytest.raises(TgoError, match="tensor 0 is"):
+            ctx.rope(h, pos, [(x[:, :, :32], y[:, :, :32])])
+        with pytest.raises(TgoError, match="dense head rows"):
+            ctx.rope(h, pos, [(x.transpose(1, 2).contiguous().transpose(1, 2), y)])
+        with pytest.raises(TgoError, match="positions is int32"):
+            ctx.rope(h, pos.long(), [(x, y)])
+    finally:
+        ctx.rope_free(h)
+    with pytest.raises(TgoError, match="no handle"):
+        ctx.rope_free(h)
+
+
+# ---------------------------------------------------------------------------
+# packed attention
+# ---------------------------------------------------------------------------
+
+def attention64(torch, q, k, v, nq, nk, scale, causal):
+    """(output, tolerance of an f32 result before its own rounding) in float64."""
+    H, d = q.shape[1:]
+    G = H // k.shape[1]
+    f16 = q.dtype == torch.float16
+    out = torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    tol = torch.zeros_like(out)
+    tq = tk = 0
+    for n, m in zip(nq, nk):
+        for i0 in range(0, n if m else 0, 1024):
+            i1 = min(n, i0 + 1024)
+            qs = q[tq + i0:tq + i1].double()
+            ks, vs = k[tk:tk + m].double(), v[tk:tk + m].double()
+            for h in range(H):
+                kh, vh = ks[:, h // G], vs[:, h // G]
+                s = scale * (qs[:, h] @ kh.t())
+                seen = torch.ones_like(s, dtype=torch.bool)
+                if causal:
+                    seen = torch.arange(m, device=q.device)[None] <= torch.arange(m - n + i0, m - n + i1, device=q.device)[:, None]
+                s = s.masked_fill(~seen, -math.inf)
+                top = s.max(1, keepdim=True)[0]
+                live = seen.any(1, keepdim=True)
+                p = torch.where(seen, (s - torch.where(live, top, 0.0)).exp(), 0.0)
+                l = p.sum(1, keepdim=True).clamp_min(1e-300)
+                o = p @ vh / l
+                out[tq + i0:tq + i1, h] = torch.where(live, o, 0.0)
+                # relative error of a probability: its score's (the operands' pairs, d terms summed, the
+                # scaling and subtraction in log2 units up to |s| 1.45 each), the exponential's 2^-23 and the
+                # rounding to f16 (or a pair)
+                mag = scale * (qs[:, h].abs() @ kh.abs().t())
+                ds = ((0 if f16 else 2.0 ** -22) + 4 * math.sqrt(d) * U) * mag + 3 * U * 1.45 * (s.abs() + top.abs())
+                e = torch.where(seen, p * (ds + 2.0 ** -23 + (HALF if f16 else 2.0 ** -22)), 0.0)
+                # an f16 probability's absolute floor (2^-32 of the largest), the f32 sums
+                e = e + seen * 2.0 ** -32 + p * 4 * math.sqrt(m) * U
+                bound = (e @ vh.abs() + (e.sum(1, keepdim=True) / l) * (p @ vh.abs())) / l
+                tol[tq + i0:tq + i1, h] = torch.where(live, bound, 0.0)
+        tq, tk = tq + n, tk + m
+    return out, tol
+
+
+def attend(ctx, torch, q, k, v, nq, nk, causal=True, out=None, scale=None, plan=0, free=True):
+    H, d = q.shape[1:]
+    plan = ctx.packed_plan(nq, nk, H, k.shape[1], head_dim=d, causal=causal,
+                           q_dtype=tgo_amd.F16 if q.dtype == torch.float16 else tgo_amd.F32, plan=plan)
+    if out is None:
+        out = torch.full(q.shape, float("nan"), device="cuda", dtype=q.dtype)
+    ctx.packed_attention(plan, q, k, v, out, scale or 1 / math.sqrt(d))
+    if free:
+        ctx.packed_free(plan)
+    return out
+
+
+def inputs(torch, nq, nk, H, Hkv, d, f16, seed=1, spread=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.randn(sum(nq), H, d, device="cuda", generator=g) * spread
+    k = torch.randn(sum(nk), Hkv, d, device="cuda", generator=g).half()
+    v = torch.randn(sum(nk), Hkv, d, device="cuda", generator=g).half()
+    return (q.half() if f16 else q), k, v
+
+
+def check_attention(torch, got, q, k, v, nq, nk, causal, scale=None):
+    want, tol = attention64(torch, q, k, v, nq, nk, scale or 1 / math.sqrt(q.shape[2]), causal)
+    tol = tol + (f16_step(want) if got.dtype == torch.float16 else U * want.abs())
+    err = (got.double() - want).abs()
+    assert bool((err <= tol).all()), (float((err / (tol + 1e-30)).max()), int((~(err <= tol)).sum()))
+
+
+BATCHES = {
+    "one": ([1], [1]), "tiny": ([3, 1, 2], [3, 1, 2]), "edges": ([31, 32, 33, 63, 64, 65], [31, 32, 33, 63, 64, 65]),
+    "empty": ([0, 5, 0, 7, 1], [4, 0, 0, 7, 300]), "decode": ([1] * 9, [1, 2, 63, 64, 65, 700, 127, 129, 2049]),
+    "few": ([2, 5, 8, 1, 7], [500, 5, 1025, 33, 1000]), "chunks": ([100, 17, 257], [1000, 17, 700]),
+    "more_queries": ([50, 130, 3], [20, 1, 2]), "prompt": ([777], [777]), "mixed": ([1, 300, 1, 40], [3000, 300, 64, 2000]),
+}
+
+
+@pytest.mark.parametrize("batch", sorted(BATCHES))
+@pytest.mark.parametrize("H,Hkv,d", [(8, 2, 128), (4, 4, 64), (7, 1, 128), (64, 1, 64), (6, 2, 128), (10, 2, 64)])
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("causal", [True, False])
+def test_packed_attention(ctx, torch_gpu, batch, H, Hkv, d, f16, causal):
+    torch = torch_gpu
+    nq, nk = BATCHES[batch]
+    q, k, v = inputs(torch, nq, nk, H, Hkv, d, f16)
+    out = attend(ctx, torch, q, k, v, nq, nk, causal)
+    check_attention(torch, out, q, k, v, nq, nk, causal)
+
+
+@pytest.mark.parametrize("nq,nk,H,Hkv,d,f16,causal", [
+    ([1, 1], [40000, 9000], 32, 8, 128, False, True),    # long contexts of single tokens, split and merged
+    ([4], [30011], 16, 2, 64, True, True),
+    ([300], [20000], 8, 1, 128, True, True),             # a chunk far behind its keys
+    ([64], [16001], 4, 2, 128, False, False),
+    ([3000, 1100, 2047], [3000, 1100, 2047], 16, 8, 128, True, True),
+    ([2500], [2500], 28, 4, 128, False, True),
+    ([1500, 700], [1500, 700], 16, 16, 64, False, False),
+])
+def test_packed_attention_over_long_contexts(ctx, torch_gpu, nq, nk, H, Hkv, d, f16, causal):
+    torch = torch_gpu
+    q, k, v = inputs(torch, nq, nk, H, Hkv, d, f16, seed=3)
+    out = attend(ctx, torch, q, k, v, nq, nk, causal)
+    check_attention(torch, out, q, k, v, nq, nk, causal)
+    again = attend(ctx, torch, q, k, v, nq, nk, causal)
+    torch.cuda.synchronize()
+    assert torch.equal(out, again)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_attention_with_peaked_scores(ctx, torch_gpu, f16, d):
+    """Scores of some tens: the largest key anywhere, rising and falling along the context, and one
+    scale that makes every probability but one vanish."""
+    torch = torch_gpu
+    nq, nk = [200, 1, 6], [200, 1500, 900]
+    q, k, v = inputs(torch, nq, nk, 4, 2, d, f16, seed=5, spread=4.0)
+    slope = torch.linspace(0.2, 3.0, sum(nk), device="cuda")[:, None, None]
+    for keys in (k, (k * slope).half(), (k * slope.flip(0)).half()):
+        for scale in (1 / math.sqrt(d), 0.5):
+            out = attend(ctx, torch, q, keys, v, nq, nk, True, scale=scale)
+            check_attention(torch, out, q, keys, v, nq, nk, True, scale)
+
+
+@pytest.mark.parametrize("q_f16", [False, True])
+def test_packed_outputs_in_every_type(ctx, torch_gpu, q_f16):
+    """An f16 result and a pair's planes are the f32 result, rounded."""
+    torch = torch_gpu
+    nq, nk = [70, 1, 5], [70, 3000, 40]
+    q, k, v = inputs(torch, nq, nk, 8, 2, 128, q_f16)
+    f32 = attend(ctx, torch, q, k, v, nq, nk, out=torch.full(q.shape, float("nan"), device="cuda"))
+    f16 = attend(ctx, torch, q, k, v, nq, nk, out=torch.full(q.shape, float("nan"), device="cuda", dtype=torch.float16))
+    pair = attend(ctx, torch, q, k, v, nq, nk, out=torch.full((2,) + q.shape, float("nan"), device="cuda", dtype=torch.float16))
+    torch.cuda.synchronize()
+    assert torch.equal(f16, f32.half()) and torch.equal(pair[0], f32.half())
+    assert torch.equal(pair[1], (f32 - f32.half().float()).half())
+
+
+@pytest.mark.parametrize("q_f16", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_packed_rows_of_wider_buffers(ctx, torch_gpu, q_f16, d):
+    """q, k, v and out as columns of wider rows; what lies between and behind the rows stays."""
+    torch = torch_gpu
+    nq, nk, H, Hkv = [40, 1, 9], [90, 1800, 9], 6, 2
+    q, k, v = inputs(torch, nq, nk, H, Hkv, d, q_f16)
+    dense = attend(ctx, torch, q, k, v, nq, nk)
+
+    def wide(t, extra, rows=0):
+        buf = torch.full((t.shape[0] + rows, t.shape[1] + extra, d), 3.0, device="cuda", dtype=t.dtype)
+        buf[:t.shape[0], 1:1 + t.shape[1]] = t
+        return buf, buf[:t.shape[0], 1:1 + t.shape[1]]
+    _, qs = wide(q, 3)
+    kv = torch.full((k.shape[0], 3 * Hkv, d), float("nan"), device="cuda", dtype=torch.float16)
+    kv[:, :Hkv], kv[:, 2 * Hkv:] = k, v
+    buf, out = wide(torch.full_like(dense, 3.0), 2, rows=5)
+    attend(ctx, torch, qs, kv[:, :Hkv], kv[:, 2 * Hkv:], nq, nk, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(out, dense)
+    out.fill_(3.0)
+    assert bool((buf == 3.0).all())
+
+
+@pytest.mark.parametrize("q_f16", [False, True])
+@pytest.mark.parametrize("H,Hkv,d,nq,nk", [(8, 2, 128, [130, 5, 1, 64], [130, 70, 900, 64]), (3, 3, 64, [90, 33], [90, 33]),
+                                           (2, 1, 128, [3, 1], [2500, 4000])])
+def test_nothing_unseen_reaches_a_row(ctx, torch_gpu, H, Hkv, d, q_f16, nq, nk):
+    """NaN and infinities in rows behind the sequences, in other sequences' rows and in later tokens'
+    keys and values leave every row that does not see them as it was, to the bit; rows that see a value
+    get it."""
+    torch = torch_gpu
+    q, k, v = inputs(torch, nq, nk, H, Hkv, d, q_f16)
+    pad = torch.full((128, Hkv, d), float("nan"), device="cuda", dtype=torch.float16)
+    kp, vp = torch.cat([k, pad]), torch.cat([v, -pad / 0])
+    clean = attend(ctx, torch, q, kp[:len(k)], vp[:len(v)], nq, nk)
+    tk = tq = 0
+    for n, m in zip(nq, nk):
+        for at, bad in ((m - 1, float("nan")), (m - max(1, n // 2), float("inf")), (m - n, float("-inf"))):
+            for what in "kv":
+                kb, vb = kp.clone(), vp.clone()
+                (kb if what == "k" else vb)[tk + at, :, 3] = bad
+                out = attend(ctx, torch, q, kb[:len(k)], vb[:len(v)], nq, nk)
+                torch.cuda.synchronize()
+                sees = torch.zeros(len(q), dtype=torch.bool, device="cuda")
+                first = tq + max(0, at - (m - n))  # the first query at position `at` or later
+                sees[first:tq + n] = True
+                assert torch.equal(out[~sees], clean[~sees]), (m, at, bad, what)
+                if what == "v":
+                    hit = out[sees][..., 3]
+                    # a pair's product with an infinity may be NaN (its lo part is 0 or of the other sign)
+                    good = hit.isnan() if bad != bad else (hit == bad) | (hit.isnan() & (not q_f16))
+                    assert bool(good.all()), (m, at, bad)
+                    keep = [j for j in range(d) if j != 3]
+                    assert torch.equal(out[sees][..., keep], clean[sees][..., keep])
+                elif bad != bad:
+                    assert bool(out[sees].isnan().all())
+        tq, tk = tq + n, tk + m
+
+
+def test_packed_offsets_past_32_bits(ctx, torch_gpu):
+    """Key rows a megabyte apart: the last lie beyond 4 GiB (and 2^31 elements) of the first."""
+    torch = torch_gpu
+    nq, nk, H, Hkv, d = [1, 40], [2900, 1400], 4, 2, 128
+    q, k, v = inputs(torch, nq, nk, H, Hkv, d, False)
+    dense = attend(ctx, torch, q, k, v, nq, nk)
+    buf = torch.empty(sum(nk), 1 << 19, device="cuda", dtype=torch.float16)
+    ks, vs = buf[:, 256:512].view(-1, Hkv, d), buf[:, 1024:1280].view(-1, Hkv, d)
+    ks.copy_(k)
+    vs.copy_(v)
+    out = attend(ctx, torch, q, ks, vs, nq, nk)
+    torch.cuda.synchronize()
+    assert torch.equal(out, dense)
+
+
+def test_packed_plans_are_replaced_and_shared_by_layers(ctx, torch_gpu):
+    torch = torch_gpu
+    H, Hkv, d = 8, 2, 128
+    plan, queued = 0, []
+    for i, (nq, nk) in enumerate([([1] * 4, [500, 6000, 9, 40]), ([300], [300]), ([], []), ([2, 3], [2000, 7])]):
+        layers = [inputs(torch, nq, nk, H, Hkv, d, False, seed=10 * i + l) for l in range(2)]
+        plan = ctx.packed_plan(nq, nk, H, Hkv, plan=plan)
+        for q, k, v in layers:
+            out = torch.full(q.shape, float("nan"), device="cuda")
+            ctx.packed_attention(plan, q, k, v, out, 0.1)
+            queued.append((out, q, k, v, nq, nk))
+    ctx.packed_free(plan)
+    torch.cuda.synchronize()
+    for out, q, k, v, nq, nk in queued:
+        if len(q):
+            check_attention(torch, out, q, k, v, nq, nk, True, 0.1)
+
+
+def test_packed_attention_refusals(ctx, torch_gpu):
+    torch = torch_gpu
+    L = tgo_amd.lib()
+    nq, nk, H, Hkv, d = [4, 3], [10, 3], 4, 2, 64
+    q, k, v = inputs(torch, nq, nk, H, Hkv, d, False)
+    out = torch.full_like(q, 5.0)
+    plan = ctx.packed_plan(nq, nk, H, Hkv, head_dim=d)
+    try:
+        def call(handle=plan, q=q.data_ptr(), q_row=256, k=k.data_ptr(), k_row=128, v=v.data_ptr(), v_row=128, scale=0.1,
+                 out=out.data_ptr(), out_row=256, out_dtype=0):
+            rc = L.tgohip_packed_attention(ctx.h, handle, q, q_row, k, k_row, v, v_row, scale, out, out_row, out_dtype)
+            return "" if rc == 0 else tgo_amd.last_error()
+        for msg, kw in (("no handle 4444", dict(handle=4444)), ("scale is 0", dict(scale=0.0)), ("scale is -1", dict(scale=-1.0)),
+                        ("scale is nan", dict(scale=float("nan"))), ("scale is inf", dict(scale=float("inf"))),
+                        ("out_dtype is 3", dict(out_dtype=3)), ("q and out are device", dict(q=None)),
+                        ("q and out are device", dict(out=None)), ("k and v are device", dict(v=None)),
+                        ("q rows are 255", dict(q_row=255)), ("k rows are 64", dict(k_row=64)), ("v rows are -128", dict(v_row=-128)),
+                        ("out rows are 0", dict(out_row=0)), ("16-byte", dict(q=q.data_ptr() + 4)), ("16-byte", dict(k_row=132)),
+                        ("16-byte", dict(out_row=258)), ("rows are dense", dict(out_dtype=2, out_row=264)),
+                        ("out meets q", dict(out=q.data_ptr())), ("out meets k", dict(out=k.data_ptr())),
+                        ("out meets v", dict(out=v.data_ptr() + 16))):
+            assert msg in call(**kw), (msg, kw, tgo_amd.last_error())
+        with pytest.raises(TgoError, match="no handle 777"):
+            ctx.packed_plan(nq, nk, H, Hkv, plan=777)
+        with pytest.raises(TgoError, match="q is \\[7, 4, 64\\]"):
+            ctx.packed_attention(plan, q[:6], k, v, out, 0.1)
+        with pytest.raises(TgoError, match="q is float32"):
+            ctx.packed_attention(plan, q.half(), k, v, out, 0.1)
+        with pytest.raises(TgoError, match="k is float16"):
+            ctx.packed_attention(plan, q, k.float(), v, out, 0.1)
+        torch.cuda.synchronize()
+        assert bool((out == 5.0).all())
+    finally:
+        ctx.packed_free(plan)
+    empty = ctx.packed_plan([], [], H, Hkv, head_dim=d)
+    ctx.packed_attention(empty, q[:0], k[:0], v[:0], out[:0], 0.1)
+    ctx.packed_free(empty)
+
+
+# ---------------------------------------------------------------------------
+# adapters
+# ---------------------------------------------------------------------------
+
+def adapters64(torch, x, base, extents, who, loaded, K, N, x_pair):
+    """(y, tolerance before y's own rounding) in float64; loaded: {index: (down, up, scale)}, float64."""
+    y = base.double().clone() if base is not None else torch.zeros(sum(extents), N, dtype=torch.float64, device="cuda")
+    tol = torch.zeros_like(y)
+    at = 0
+    for n, a in zip(extents, who):
+        if a in loaded and n:
+            down, up, s = loaded[a]
+            xs = x[at:at + n]
+            u = xs @ down.t()
+            du = ((2.0 ** -22 if x_pair else 0) + 4 * math.sqrt(K) * U) * (xs.abs() @ down.abs().t())
+            top = u.abs().max(1, keepdim=True)[0]
+            r = down.shape[0]
+            y[at:at + n] += s * (u @ up.t())
+            tol[at:at + n] = abs(s) * ((du + (2.0 ** -22) * (top + du)) @ up.abs().t()
+                                       + (4 * math.sqrt(r) + 1) * U * (u.abs() @ up.abs().t()))
+        at += n
+    return y, tol + U * y.abs()
+
+
+def make_adapter(torch, K, N, r, seed, spread=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    down = (torch.randn(r, K, device="cuda", generator=g) * spread / math.sqrt(K)).half()
+    return down, (torch.randn(N, r, device="cuda", generator=g) * 0.05).half()
+
+
+def stored(torch, x, xk):
+    """(the stored activation, its dtype code, its values in float64)"""
+    if xk == "f32":
+        return x, tgo_amd.F32, x.double()
+    hi = x.half()
+    if xk == "f16":
+        return hi, tgo_amd.F16, hi.double()
+    lo = (x - hi.float()).half()
+    return torch.stack([hi, lo]), tgo_amd.F16X2, hi.double() + lo.double()
+
+
+def check_adapters(ctx, torch, K, N, ranks, extents, who, xk, yk, seed=1, base="apart", spread=1.0):
+    loaded = {}
+    h = ctx.adapters_new(K, N, max([len(ranks)] + [w + 1 for w in who]))
+    rows = ctx.adapter_rows(extents, who)
+    try:
+        for i, r in enumerate(ranks):
+            if r:
+                down, up = make_adapter(torch, K, N, r, 100 * seed + i, spread)
+                s = 0.5 + i
+                ctx.adapters_put(h, i, down.cpu().numpy(), up.cpu().numpy(), s)
+                loaded[i] = (down.double(), up.double(), s)
+        T = sum(extents)
+        x, xd, x64 = stored(torch, torch.randn(T, K, device="cuda"), xk)
+        yt = torch.float16 if yk == "f16" else torch.float32
+        b = torch.randn(T, N, device="cuda").to(yt) if base else None
+        # behind the last row stays as it is
+        buf = torch.full((T + 3, N), float("nan"), device="cuda", dtype=yt)
+        if base == "same":
+            buf[:T] = b
+        buf[T:] = 9.0
+        print("adapters: [%d,%d] ranks %s rows %d %s %s" % (K, N, ranks, T, xk, yk), flush=True)
+        ctx.adapters(h, rows, x, buf[:T] if base == "same" else b, buf[:T], x_dtype=xd,
+                     y_dtype=tgo_amd.F16 if yk == "f16" else tgo_amd.F32)
+        torch.cuda.synchronize()
+        want, tol = adapters64(torch, x64, b, extents, who, loaded, K, N, xk != "f16")
+        if yk == "f16":
+            tol = tol + f16_step(want)
+        err = (buf[:T].double() - want).abs()
+        assert bool((err <= tol).all()), (float((err / (tol + 1e-30)).max()), int((~(err <= tol)).sum()))
+        assert bool((buf[T:] == 9.0).all())
+        at = 0
+        for n, a in zip(extents, who):
+            if a not in loaded:
+                assert torch.equal(buf[at:at + n], b[at:at + n] if b is not None else torch.zeros_like(buf[at:at + n]))
+            at += n
+    finally:
+        ctx.adapter_rows_free(rows)
+        ctx.adapters_free(h)
+
+
+@pytest.mark.parametrize("xk,yk", [("f32", "f32"), ("x2", "f32"), ("f16", "f16"), ("f32", "f16"), ("f16", "f32")])
+@pytest.mark.parametrize("K,N,ranks,extents,who", [
+    (64, 32, [1], [1], [0]),
+    (64, 32, [5], [70], [0]),
+    (4096, 6144, [16, 8, 16], [1] * 13, [0, 1, 2, 2, 1, 0, -1, 0, 0, 0, 2, 1, 0]),
+    (1024, 2048, [64, 128, 24, 1], [1, 40, 1, 129, 0, 31, 32, 33], [0, 1, -1, 2, 3, 3, 0, 1]),
+    (640, 1056, [20, 0, 48], [17, 65, 3], [2, 1, 0]),
+    (12288, 96, [100], [5, 5], [0, 0]),
+    (192, 4128, [17], [257], [0]),
+    (2048, 1024, [16, 32], [3, 4], [-1, -1]),
+])
+def test_adapters(ctx, torch_gpu, K, N, ranks, extents, who, xk, yk):
+    check_adapters(ctx, torch_gpu, K, N, ranks, extents, who, xk, yk)
+
+
+@pytest.mark.parametrize("base", ["apart", "same", None])
+@pytest.mark.parametrize("yk", ["f32", "f16"])
+def test_adapters_bases(ctx, torch_gpu, base, yk):
+    check_adapters(ctx, torch_gpu, 256, 160, [8, 40], [9, 1, 50], [0, -1, 1], "f32", yk, base=base)
+
+
+@pytest.mark.parametrize("spread", [2.0 ** -9, 2.0 ** 9])
+def test_adapters_far_from_unit_size(ctx, torch_gpu, spread):
+    """x . down^T of 1e-3 and of some thousands (its values as f16 hi + lo parts, scaled per row)."""
+    check_adapters(ctx, torch_gpu, 1024, 512, [16, 64], [1, 70, 30], [0, 1, 0], "f32", "f32", spread=spread)
+
+
+@pytest.mark.parametrize("extents", [[2000, 1, 700], [1] * 300])
+def test_adapters_many_rows(ctx, torch_gpu, extents):
+    who = [(7 * i) % 40 - 1 for i in range(len(extents))]
+    check_adapters(ctx, torch_gpu, 1024, 1536, [8 + i for i in range(39)], extents, who, "x2", "f32")
+
+
+def test_adapters_are_replaced_and_dropped(ctx, torch_gpu):
+    torch = torch_gpu
+    K, N = 256, 128
+    h, rows = ctx.adapters_new(K, N, 3), ctx.adapter_rows([4, 3], [2, 0])
+    x, base = torch.randn(7, K, device="cuda"), torch.randn(7, N, device="cuda")
+    try:
+        def run():
+            y = torch.full((7, N), float("nan"), device="cuda")
+            ctx.adapters(h, rows, x, base, y)
+            return y
+        assert torch.equal(run(), base)  # no adapter loaded yet
+        for r in (16, 40, 3):
+            down, up = make_adapter(torch, K, N, r, r)
+            ctx.adapters_put(h, 2, down.float().cpu().numpy(), up.float().cpu().numpy(), 2.0)  # f32 planes
+            want, tol = adapters64(torch, x.double(), base, [4, 3], [2, 0], {2: (down.double(), up.double(), 2.0)}, K, N, True)
+            assert bool(((run().double() - want).abs() <= tol).all())
+        ctx.adapters_drop(h, 2)
+        assert torch.equal(run(), base)
+        rows = ctx.adapter_rows([7], [1], rows=rows)
+        down, up = make_adapter(torch, K, N, 8, 8)
+        ctx.adapters_put(h, 1, down.cpu().numpy(), up.cpu().numpy(), -1.5)
+        want, tol = adapters64(torch, x.double(), base, [7], [1], {1: (down.double(), up.double(), -1.5)}, K, N, True)
+        assert bool(((run().double() - want).abs() <= tol).all())
+        rows = ctx.adapter_rows([], [], rows=rows)
+        ctx.adapters(h, rows, x[:0], base[:0], base[:0])
+    finally:
+        ctx.adapter_rows_free(rows)
+        ctx.adapters_free(h)
+
+
+def test_adapter_rows_do_not_depend_on_each_other(ctx, torch_gpu):
+    """A row's result is the same bits alone, among others and with NaN in every other row."""
+    torch = torch_gpu
+    K, N = 512, 256
+    h = ctx.adapters_new(K, N, 2)
+    one, many = ctx.adapter_rows([1], [1]), ctx.adapter_rows([20, 1, 9], [0, 1, 1])
+    try:
+        for i in range(2):
+            down, up = make_adapter(torch, K, N, 16, i)
+            ctx.adapters_put(h, i, down.cpu().numpy(), up.cpu().numpy(), 1.0)
+        x, base = torch.randn(30, K, device="cuda"), torch.randn(30, N, device="cuda")
+        y1, y30, ynan = (torch.empty(n, N, device="cuda") for n in (1, 30, 30))
+        ctx.adapters(h, one, x[20:21], base[20:21], y1)
+        ctx.adapters(h, many, x, base, y30)
+        xb = torch.full_like(x, float("nan"))
+        xb[20] = x[20]
+        ctx.adapters(h, many, xb, base, ynan)
+        torch.cuda.synchronize()
+        assert torch.equal(y30[20], ynan[20])
+        want, tol = adapters64(torch, x[20:21].double(), base[20:21], [1], [0], {0: (down.double(), up.double(), 1.0)}, K, N, True)
+        assert bool(((y1.double() - want).abs() <= tol).all()) and bool(((y30[20:21].double() - want).abs() <= tol).all())
+        assert bool(ynan[:20].isnan().all()) and bool(ynan[21:].isnan().all())
+    finally:
+        for r in (one, many):
+            ctx.adapter_rows_free(r)
+        ctx.adapters_free(h)
+
+
+def test_adapter_refusals(ctx, torch_gpu):
+    torch = torch_gpu
+    L, K, N = tgo_amd.lib(), 128, 64
+    h, rows, far = ctx.adapters_new(K, N, 2), ctx.adapter_rows([5], [1]), ctx.adapter_rows([5, 0], [2, 1])
+    x, b, y = torch.randn(5, K, device="cuda"), torch.randn(5, N, device="cuda"), torch.full((5, N), 4.0, device="cuda")
+    try:
+        def call(s=h, r=rows, x=x.data_ptr(), xd=0, base=b.data_ptr(), y=y.data_ptr(), yd=0):
+            rc = L.tgohip_adapters(ctx.h, s, r, x, xd, base, y, yd)
+            return "" if rc == 0 else tgo_amd.last_error()
+        for msg, kw in (("set: no handle 9", dict(s=99999)), ("rows: no handle 9", dict(r=99999)), ("x_dtype is 3", dict(xd=3)),
+                        ("y_dtype is 2", dict(yd=2)), ("rows name adapter 2 and the set holds 2", dict(r=far)),
+                        ("x and y are device", dict(x=None)), ("x and y are device", dict(y=None)),
+                        ("16-byte", dict(x=x.data_ptr() + 4)), ("16-byte", dict(base=b.data_ptr() + 8)),
+                        ("16-byte", dict(y=y.data_ptr() + 2)), ("y meets x", dict(y=x.data_ptr() + 256)),
+                        ("y meets base", dict(y=b.data_ptr() + 16))):
+            assert msg in call(**kw), (msg, kw, tgo_amd.last_error())
+        down, up = np.zeros((4, K), np.float32), np.zeros((N, 4), np.float32)
+        with pytest.raises(TgoError, match="index 2 of a set of 2"):
+            ctx.adapters_put(h, 2, down, up, 1.0)
+        with pytest.raises(TgoError, match="index -1 of a set"):
+            ctx.adapters_drop(h, -1)
+        with pytest.raises(TgoError, match="down is"):
+            ctx.adapters_put(h, 0, down[:, :64], up, 1.0)
+        with pytest.raises(TgoError, match="down is"):
+            ctx.adapters_put(h, 0, down, up[:, :3], 1.0)
+        with pytest.raises(TgoError, match="past f16's range"):
+            ctx.adapters_put(h, 0, down, up + 65536, 1.0)
+        torch.cuda.synchronize()
+        assert bool((y == 4.0).all())
+    finally:
+        for r in (rows, far):
+            ctx.adapter_rows_free(r)
+        ctx.adapters_free(h)
+
+
+# ---------------------------------------------------------------------------
+# together
+# ---------------------------------------------------------------------------
+
+def test_an_attention_block_of_adapted_requests(ctx, torch_gpu):
+    """One layer's attention over packed prompts and a decoding request: projection, the requests'
+    adapters, rotary positions (scaled, half layout), attention over the rotated rows."""
+    torch = torch_gpu
+    K, H, Hkv, d = 256, 4, 2, 128
+    N = (H + 2 * Hkv) * d
+    nq, who = [70, 1, 33, 128], [0, -1, 1, 0]
+    T = sum(nq)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    w = (torch.randn(K, N, device="cuda", generator=g) / 16).half()
+    x = torch.randn(T, K, device="cuda", generator=g)
+    pos = torch.cat([torch.arange(n) for n in nq]).int().cuda() + 5000
+    wh = ctx.weight_upload(tgo_amd.FORM_F16, K, N, w.cpu())
+    kw = dict(layout=tgo_amd.ROPE_HALF, **SCALINGS["yarn"])
+    rope, s = ctx.rope_new(d, 1e6, **kw), ctx.adapters_new(K, N, 2)
+    rows, plan = ctx.adapter_rows(nq, who), ctx.packed_plan(nq, nq, H, Hkv)
+    try:
+        loaded = {}
+        for i, r in enumerate((8, 24)):
+            down, up = make_adapter(torch, K, N, r, i)
+            ctx.adapters_put(s, i, down.cpu().numpy(), up.cpu().numpy(), 2.0)
+            loaded[i] = (down.double(), up.double(), 2.0)
+        qkv = torch.empty(T, H + 2 * Hkv, d, device="cuda")
+        q = torch.empty(T, H, d, device="cuda")
+        k, v = (torch.empty(T, Hkv, d, device="cuda", dtype=torch.float16) for _ in "kv")
+        out = torch.empty(T, H, d, device="cuda")
+
+        def layer():
+            ctx.linear(wh, x, T, qkv)
+            ctx.adapters(s, rows, x, qkv, qkv)
+            ctx.rope(rope, pos, [(qkv[:, :H], q), (qkv[:, H:H + Hkv], k), (qkv[:, H + Hkv:], v, False)])
+            ctx.packed_attention(plan, q, k, v, out, d ** -0.5)
+        layer()
+        torch.cuda.synchronize()
+        # each stage against float64 of what the stage before left, then the attention
+        want, tol = adapters64(torch, x.double(), (x.double() @ w.double()), nq, who, loaded, K, N, True)
+        lin = (4 * math.sqrt(K) * U + 2.0 ** -22) * (x.double().abs() @ w.double().abs())
+        assert bool(((qkv.view(T, N).double() - want).abs() <= tol + lin + U * want.abs()).all())
+        fr, m = tgo_amd.rope_freqs(d, 1e6, **kw)
+        check_rope(torch, q, qkv[:, :H], pos, d, tgo_amd.ROPE_HALF, fr, m)
+        check_rope(torch, k, qkv[:, H:H + Hkv], pos, d, tgo_amd.ROPE_HALF, fr, m)
+        check_attention(torch, out, q, k, v, nq, nq, True)
+        # the whole block against float64 throughout: k and v are rounded to f16 (2^-11 of scores and
+        # values of size 1 to 10), everything else far below
+        w64 = want.view(T, H + 2 * Hkv, d)
+        q64, _ = rope64(torch, w64[:, :H], pos, d, tgo_amd.ROPE_HALF, fr, m)
+        k64, _ = rope64(torch, w64[:, H:H + Hkv], pos, d, tgo_amd.ROPE_HALF, fr, m)
+        v64 = w64[:, H + Hkv:]
+        full, _ = attention64(torch, q64, k64, v64, nq, nq, d ** -0.5, True)
+        shift = HALF * d ** -0.5 * float(q64.abs().sum(-1).max() * k64.abs().max())  # of a score, by k's rounding
+        assert float((out.double() - full).abs().max()) <= (2.1 * shift + 1.1 * HALF) * float(v64.abs().max())
+        # captured once and replayed: the eager bits, other calls between the replays
+        eager = out.clone()
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        ctx.set_stream(side.cuda_stream)
+        try:
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph, stream=side):
+                ctx.rope(rope, pos, [(qkv[:, :H], q), (qkv[:, H:H + Hkv], k), (qkv[:, H + Hkv:], v, False)])
+                ctx.packed_attention(plan, q, k, v, out, d ** -0.5)
+        finally:
+            ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+        for _ in range(4):
+            for t in (q, k, v, out):
+                t.fill_(float("nan"))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, eager)
+            layer()
+            torch.cuda.synchronize()
+    finally:
+        ctx.weight_free(wh)
+        ctx.rope_free(rope)
+        ctx.adapters_free(s)
+        ctx.adapter_rows_free(rows)
+        ctx.packed_free(plan)
+
+
+def test_captured_adapters_and_split_attention_replay(ctx, torch_gpu):
+    """Both kernels of the adapters and a context split over many workgroups, captured; a second plan and
+    row handle run eagerly between the replays."""
+    torch = torch_gpu
+    K, N, H, Hkv, d = 1024, 512, 8, 2, 128
+    nq, nk, who = [1, 1, 1], [6000, 90, 3000], [0, 1, 0]
+    q, k, v = inputs(torch, nq, nk, H, Hkv, d, False)
+    x, base = torch.randn(3, K, device="cuda"), torch.randn(3, N, device="cuda")
+    s = ctx.adapters_new(K, N, 2)
+    rows, rows2 = ctx.adapter_rows([1] * 3, who), ctx.adapter_rows([3], [1])
+    plan, plan2 = ctx.packed_plan(nq, nk, H, Hkv), ctx.packed_plan([3], [500], H, Hkv)
+    try:
+        for i in range(2):
+            down, up = make_adapter(torch, K, N, 16, i)
+            ctx.adapters_put(s, i, down.cpu().numpy(), up.cpu().numpy(), 1.0)
+        y, out, y2, out2 = torch.empty_like(base), torch.empty_like(q), torch.empty_like(base), torch.empty_like(q)
+
+        def run():
+            ctx.adapters(s, rows, x, base, y)
+            ctx.packed_attention(plan, q, k, v, out, 0.09)
+        run()
+        torch.cuda.synchronize()
+        ey, eo = y.clone(), out.clone()
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        ctx.set_stream(side.cuda_stream)
+        try:
+            with torch.cuda.graph(graph, stream=side):
+                run()
+        finally:
+            ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+        for _ in range(4):
+            y.fill_(float("nan"))
+            out.fill_(float("nan"))
+            graph.replay()
+            ctx.adapters(s, rows2, x, base, y2)
+            ctx.packed_attention(plan2, q, k[:500], v[:500], out2, 0.09)
+            torch.cuda.synchronize()
+            assert torch.equal(y, ey) and torch.equal(out, eo)
+    finally:
+        for f, a in ((ctx.adapters_free, s), (ctx.adapter_rows_free, rows), (ctx.adapter_rows_free, rows2),
+                     (ctx.packed_free, plan), (ctx.packed_free, plan2)):
+            f(a)

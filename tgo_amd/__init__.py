@@ -17,6 +17,8 @@ LIB_PATH = os.path.join(HERE, "libtgohip.so")
 FORM_F16, FORM_I8, FORM_I4_TGO, FORM_I4_SYM = 0, 1, 2, 3
 F32, F16, F16X2 = 0, 1, 2
 LINEAR_ROWS, LINEAR_PIPE, LINEAR_GEMV, LINEAR_TILES = range(4)  # LinearPlan.kernel
+ROPE_INTERLEAVED, ROPE_HALF = 0, 1
+ROPE_UNSCALED, ROPE_LINEAR, ROPE_YARN, ROPE_BANDS = range(4)
 PROF_ATTN, PROF_QKV, PROF_O, PROF_GATEUP, PROF_DOWN, PROF_LMHEAD = range(6)
 PROF_NAMES = ("attention", "qkv", "o", "gateup", "down", "lm_head")
 
@@ -42,6 +44,17 @@ class BatchStepC(ctypes.Structure):
                 ("max_pages", ctypes.c_int32)] + [
         (n, ctypes.c_void_p) for n in ("ids", "posq", "posk", "slots", "lengths", "extents",
                                        "last", "pages")]
+
+
+class RopeCfg(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("head_dim", "rotary_dim", "layout", "scaling")] + [
+        (n, ctypes.c_double) for n in ("base", "factor", "original", "fast", "slow", "attention")]
+
+
+class RopeHeads(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("y", ctypes.c_void_p)] + [
+        (n, ctypes.c_int64) for n in ("x_row", "x_head", "y_row", "y_head")] + [
+        (n, ctypes.c_int32) for n in ("heads", "x_dtype", "y_dtype", "rotate")]
 
 
 class LinearPlan(ctypes.Structure):
@@ -70,6 +83,7 @@ def lib():
         raise RuntimeError("tgo_amd: %s is not built; run `python -m tgo_amd.build`" % LIB_PATH)
     L = ctypes.CDLL(LIB_PATH)
     P, I, U64, D, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_double, ctypes.c_float
+    I64 = ctypes.c_int64
     sig = {
         "tgohip_last_error": (ctypes.c_char_p, []),
         "tgohip_version": (ctypes.c_char_p, []),
@@ -104,6 +118,20 @@ def lib():
         "tgohip_dequant_f16": (I, [P, I, P]),
         "tgohip_greedy": (I, [P, P, I, I, P, P]),
         "tgohip_step_margins": (I, [P, P, I]),
+        "tgohip_rope_freqs": (I, [ctypes.POINTER(RopeCfg), P, P]),
+        "tgohip_rope_new": (I, [P, ctypes.POINTER(RopeCfg), P]),
+        "tgohip_rope_free": (I, [P, I]),
+        "tgohip_rope": (I, [P, I, P, I, ctypes.POINTER(RopeHeads), I]),
+        "tgohip_packed_plan": (I, [P, I, P, P, I, I, I, I, I, P]),
+        "tgohip_packed_free": (I, [P, I]),
+        "tgohip_packed_attention": (I, [P, I, P, I64, P, I64, P, I64, F, P, I64, I]),
+        "tgohip_adapters_new": (I, [P, I, I, I, P]),
+        "tgohip_adapters_put": (I, [P, I, I, I, I, P, P, F]),
+        "tgohip_adapters_drop": (I, [P, I, I]),
+        "tgohip_adapters_free": (I, [P, I]),
+        "tgohip_adapter_rows": (I, [P, I, P, P, P]),
+        "tgohip_adapter_rows_free": (I, [P, I]),
+        "tgohip_adapters": (I, [P, I, I, P, I, P, P, I]),
         "tgohip_new_batch_step": (I, [I, I, I, I, I, P, P, P, P, P, I, I, I, P, P, P, P, P, P, P]),
         "tgohip_next_step": (I, [I, P, P, P, I, I, P, P, P, P, P, P]),
         "tgohip_victim": (I, [I, P, P, P, P]),
@@ -260,6 +288,40 @@ def attention_plan(T, H, Hkv, capacity, lengths, extents, pages, max_pages, bloc
     check(lib().tgohip_attention_plan(T, H, Hkv, capacity, len(lengths), ptr(lengths), ptr(extents), ptr(pages),
                                       max_pages, block, q_dtype, ctypes.byref(p)))
     return p
+
+
+def rope_cfg(head_dim, base, rotary_dim=None, layout=ROPE_INTERLEAVED, scaling=ROPE_UNSCALED, factor=1.0,
+             original=0.0, fast=0.0, slow=0.0, attention=0.0):
+    return RopeCfg(head_dim, head_dim if rotary_dim is None else rotary_dim, layout, scaling, base, factor, original,
+                   fast, slow, attention)
+
+
+def rope_freqs(*args, **kw):
+    """(w [rotary_dim / 2] float64, m) of a rotary configuration (rope_cfg's arguments), without a GPU."""
+    c = rope_cfg(*args, **kw)
+    w, m = np.zeros(max(c.rotary_dim // 2, 1), np.float64), ctypes.c_double()
+    check(lib().tgohip_rope_freqs(ctypes.byref(c), ptr(w), ctypes.byref(m)))
+    return w, m.value
+
+
+def _heads_view(t, what):
+    """(address, row stride, head stride, dtype code) of a device tensor [rows, heads, head_dim]."""
+    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise TgoError(EINVAL, "%s is a [rows, heads, head_dim] tensor with dense head rows" % what)
+    kind = {"torch.float32": F32, "torch.float16": F16}.get(str(t.dtype))
+    if kind is None:
+        raise TgoError(EINVAL, "%s is %s; float32 or float16" % (what, t.dtype))
+    return t.data_ptr(), t.stride(0), t.stride(1), kind
+
+
+def _packed_rows(t, what, rows, heads, d, kind):
+    """(address, row stride) of a packed operand [rows, heads, d] whose heads are dense."""
+    at, row, head, dt = _heads_view(t, what)
+    if tuple(t.shape) != (rows, heads, d) or (heads > 1 and head != d):
+        raise TgoError(EINVAL, "%s is [%d, %d, %d] with dense heads" % (what, rows, heads, d))
+    if kind is not None and dt != kind:
+        raise TgoError(EINVAL, "%s is %s" % (what, "float16" if kind == F16 else "float32"))
+    return ctypes.c_void_p(at), row, dt
 
 
 def sha256(data: bytes):
@@ -453,6 +515,7 @@ class Context:
         if not self.h:
             raise TgoError(EDEVICE, last_error())
         self.cfg = None
+        self._ropes, self._packed, self._sets = {}, {}, {}  # what this binding checks shapes by
 
     def close(self):
         if self.h:
@@ -617,6 +680,107 @@ class Context:
 
     def linear(self, handle, x, M, y, x_dtype=F32, y_dtype=F32):
         check(lib().tgohip_linear(self.h, handle, ptr(x), x_dtype, M, ptr(y), y_dtype))
+
+    # ---- rotary positions, packed attention, adapters of many requests ----
+    def rope_new(self, *args, **kw):
+        """A rotary table (rope_cfg's arguments); returns its handle."""
+        c, h = rope_cfg(*args, **kw), ctypes.c_int()
+        check(lib().tgohip_rope_new(self.h, ctypes.byref(c), ctypes.byref(h)))
+        self._ropes[h.value] = c.head_dim
+        return h.value
+
+    def rope_free(self, handle):
+        check(lib().tgohip_rope_free(self.h, handle))
+        self._ropes.pop(handle, None)
+
+    def rope(self, handle, positions, heads):
+        """Rotates up to three tensors in one launch. positions: device int32 [T]; heads: a list of
+        (x, y) or (x, y, rotate) device tensors [T, heads, head_dim] (any row and head strides)."""
+        d, T = self._ropes.get(handle), positions.numel()
+        if "int32" not in str(positions.dtype):
+            raise TgoError(EINVAL, "positions is int32, not %s" % positions.dtype)
+        g = (RopeHeads * max(len(heads), 1))()
+        for i, (x, y, *turn) in enumerate(heads):
+            if x.shape != y.shape or x.shape[0] != T or (d is not None and x.shape[2] != d):
+                raise TgoError(EINVAL, "rope: tensor %d is %s and %s for %d positions and heads of %s" %
+                               (i, tuple(x.shape), tuple(y.shape), T, d))
+            xa, xr, xh, xd = _heads_view(x, "rope: x")
+            ya, yr, yh, yd = _heads_view(y, "rope: y")
+            g[i] = RopeHeads(xa, ya, xr, xh, yr, yh, x.shape[1], xd, yd, int(turn[0]) if turn else 1)
+        check(lib().tgohip_rope(self.h, handle, ptr(positions), T, g, len(heads)))
+
+    def packed_plan(self, q_lengths, kv_lengths, H, Hkv, head_dim=128, causal=True, q_dtype=F32, plan=0):
+        """Decomposes a batch for packed_attention; returns the plan's handle. plan: a handle whose plan
+        this one replaces."""
+        nq, nk, h = i32(q_lengths), i32(kv_lengths), ctypes.c_int(plan)
+        if len(nq) != len(nk):
+            raise TgoError(EINVAL, "packed_plan: %d query lengths and %d key lengths" % (len(nq), len(nk)))
+        check(lib().tgohip_packed_plan(self.h, len(nq), ptr(nq), ptr(nk), H, Hkv, head_dim, int(causal), q_dtype,
+                                       ctypes.byref(h)))
+        self._packed[h.value] = (int(nq.sum(dtype=np.int64)), int(nk.sum(dtype=np.int64)), H, Hkv, head_dim, q_dtype)
+        return h.value
+
+    def packed_free(self, plan):
+        check(lib().tgohip_packed_free(self.h, plan))
+        self._packed.pop(plan, None)
+
+    def packed_attention(self, plan, q, k, v, out, scale):
+        """Attention over a plan's packed rows. q, out [rows, H, head_dim], k, v [key rows, H_kv, head_dim]
+        float16 device tensors (any row stride); out float32, float16, or [2, rows, H, head_dim] float16
+        for the hi and lo planes of a pair."""
+        tq, tk, H, Hkv, d, qd = self._packed.get(plan, (0, 0, 1, 1, 64, F32))
+        qa, qr, _ = _packed_rows(q, "q", tq, H, d, qd)
+        ka, kr, _ = _packed_rows(k, "k", tk, Hkv, d, F16)
+        va, vr, _ = _packed_rows(v, "v", tk, Hkv, d, F16)
+        if out.dim() == 4:
+            if tuple(out.shape) != (2, tq, H, d) or not out.is_contiguous() or "float16" not in str(out.dtype):
+                raise TgoError(EINVAL, "out as a pair is a dense float16 [2, %d, %d, %d]" % (tq, H, d))
+            oa, orow, od = ptr(out), H * d, F16X2
+        else:
+            oa, orow, od = _packed_rows(out, "out", tq, H, d, None)
+        check(lib().tgohip_packed_attention(self.h, plan, qa, qr, ka, kr, va, vr, scale, oa, orow, od))
+
+    def adapters_new(self, K, N, capacity):
+        """A set of up to `capacity` adapters of a projection [K,N]; returns its handle."""
+        h = ctypes.c_int()
+        check(lib().tgohip_adapters_new(self.h, K, N, capacity, ctypes.byref(h)))
+        self._sets[h.value] = (K, N)
+        return h.value
+
+    def adapters_put(self, handle, index, down, up, scale):
+        """Loads an adapter: down [rank, K], up [N, rank], host arrays, both float16 or taken as float32."""
+        K, N = self._sets.get(handle, (None, None))
+        half = np.asarray(down).dtype == np.float16 and np.asarray(up).dtype == np.float16
+        down, up = (np.ascontiguousarray(a, dtype=np.float16 if half else np.float32) for a in (down, up))
+        if down.ndim != 2 or up.ndim != 2 or up.shape[1] != down.shape[0] or (
+                K is not None and (down.shape[1], up.shape[0]) != (K, N)):
+            raise TgoError(EINVAL, "adapters_put: down is %s and up %s; [rank, %s] and [%s, rank]" %
+                           (down.shape, up.shape, K, N))
+        check(lib().tgohip_adapters_put(self.h, handle, index, down.shape[0], F16 if half else F32, ptr(down), ptr(up),
+                                        scale))
+
+    def adapters_drop(self, handle, index):
+        check(lib().tgohip_adapters_drop(self.h, handle, index))
+
+    def adapters_free(self, handle):
+        check(lib().tgohip_adapters_free(self.h, handle))
+        self._sets.pop(handle, None)
+
+    def adapter_rows(self, extents, adapters, rows=0):
+        """A batch's rows: extents[b] of them for request b with adapter adapters[b] (-1: none); returns
+        the handle. rows: a handle that this batch replaces."""
+        e, a, h = i32(extents), i32(adapters), ctypes.c_int(rows)
+        if len(e) != len(a):
+            raise TgoError(EINVAL, "adapter_rows: %d extents and %d adapters" % (len(e), len(a)))
+        check(lib().tgohip_adapter_rows(self.h, len(e), ptr(e), ptr(a), ctypes.byref(h)))
+        return h.value
+
+    def adapter_rows_free(self, rows):
+        check(lib().tgohip_adapter_rows_free(self.h, rows))
+
+    def adapters(self, handle, rows, x, base, y, x_dtype=F32, y_dtype=F32):
+        """y = base + the adapters' product of x (base None: zeros; y may be base)."""
+        check(lib().tgohip_adapters(self.h, handle, rows, ptr(x), x_dtype, ptr(base), ptr(y), y_dtype))
 
     def greedy(self, logits, B, V, ids, margins=None):
         """sample argmax (first strict maximum) and TopTwoMargin over device rows."""

@@ -13,7 +13,8 @@ LIB = os.path.join(HERE, "libtgohip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 HIP_SOURCES = ["runtime.hip", "kernels/attention.hip", "kernels/gemm.hip", "kernels/gemm_rows.hip",
-               "kernels/elementwise.hip", "kernels/probe.hip"]
+               "kernels/elementwise.hip", "kernels/probe.hip", "operators.hip", "kernels/rope.hip",
+               "kernels/packed_attention.hip", "kernels/adapters.hip"]
 CXX_SOURCES = ["host/hostlogic.cpp", "host/checkpoint.cpp"]
 
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall",

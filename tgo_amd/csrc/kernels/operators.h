@@ -1,0 +1,97 @@
+// operators.h -- the op-level operators beside the projections and paged
+// attention: rotary positions, packed attention, the adapters of many requests.
+// Arguments and launches of kernels/rope.hip, packed_attention.hip, adapters.hip.
+#pragma once
+
+#include "../common.h"
+
+namespace tgohip {
+
+// ---- rotary positions (rope.hip) -------------------------------------------
+constexpr int kRopeGroups = 3;      // tensors of heads per call
+constexpr int kRopeMaxHeadDim = 256;
+struct RopeGroup {
+  const void* x;
+  void* y;
+  int64_t x_row, x_head, y_row, y_head;  // elements
+  int32_t heads, x_f16, y_f16, rotate;
+};
+struct RopeArgs {
+  const int32_t* positions;
+  const double* inv_freq;  // [rotary_dim / 2], turns per position (angle / 2 pi)
+  float attention;         // cos and sin are multiplied by it
+  int T, d, rd, half;      // half: pairs (i, i + rd/2), else (2i, 2i + 1)
+  int n;
+  RopeGroup g[kRopeGroups];
+};
+void launch_rope(const RopeArgs& a, hipStream_t st);
+
+// ---- packed attention (packed_attention.hip) --------------------------------
+// A work item: rows [r0, r0 + nr) of one sequence and kv head against its keys
+// [kv_lo, kv_hi). Row r is query head kvh * G + r % G of token r / G.
+struct PackedItem {
+  int32_t q0, k0;   // the sequence's first packed query and key row
+  int32_t nk;       // its keys
+  int32_t shift;    // token t sees keys 0 .. min(t + shift, nk - 1)
+  int32_t r0, nr;
+  int32_t kv_lo, kv_hi;
+  int32_t kvh;      // -1: an empty slot of the launch order
+  int32_t part;     // first row of its partial result, -1 when it writes out
+};
+// Rows [r0, r0 + nr) of a (sequence, kv head): `parts` partial results, row i of
+// part p at partial row part + p * step + i.
+struct PackedMerge {
+  int32_t q0, r0, nr, kvh, part, parts, step;
+};
+struct PackedPlan {
+  int H = 0, Hkv = 0, D = 0, q_f16 = 0;
+  int64_t tq = 0, tk = 0;  // packed query and key rows
+  std::vector<PackedItem> items;
+  std::vector<PackedMerge> merges;
+  int64_t part_rows = 0;
+};
+// Decomposes a call (host only). nq, nk: [B], checked by the caller.
+void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int Hkv, int D, bool causal,
+                       bool q_f16, int ncu, PackedPlan& plan);
+struct PackedArgs {
+  const void* q;
+  const half_t* k;
+  const half_t* v;
+  void* out;
+  float* part_o;   // [part_rows][D]
+  float* part_ml;  // [part_rows][2]: the reference maximum (log2) and the sum
+  const PackedItem* items;
+  const PackedMerge* merges;
+  int64_t q_row, k_row, v_row, out_row, out_lo;  // elements
+  int G, out_form;                               // OUT_F32, OUT_F16, OUT_X2 (lo plane out_lo on)
+  float qscale;                                  // scale * log2(e)
+};
+int packed_enqueue(const PackedArgs& a, int D, int q_f16, int items, int merges, hipStream_t st);
+
+// ---- adapters (adapters.hip) --------------------------------------------------
+constexpr int kAdapterMaxRank = 128;
+struct AdapterEntry {
+  const half_t* down;  // [rank_pad][K]
+  const half_t* up;    // [N][rank_pad]
+  int32_t rank_pad;    // 0: no adapter at this index
+  float scale;
+};
+// Rows perm[start .. start + n) carry the adapter (-1: none).
+struct AdapterTile {
+  int32_t adapter, start, n;
+};
+struct AdapterArgs {
+  const AdapterEntry* table;
+  const AdapterTile* tiles;
+  const int32_t* perm;
+  int ntiles, T, K, N;
+  const void* x;
+  int xk;  // XK_F16, XK_F32, XK_X2
+  const void* base;
+  void* y;
+  int y_f16;
+  float* u;  // [T][kAdapterMaxRank]: x . down^T of the permuted rows
+};
+void launch_adapters(const AdapterArgs& a, hipStream_t st);
+
+}  // namespace tgohip

@@ -1,7 +1,7 @@
 // runtime.hip -- the C ABI of libtgohip: context, weight upload and repack,
 // KV pool, the batched step (Batch.step, batch.go:314-458), the op-level entry
 // points, and the Scheduler (scheduler.go) driving it.
-#include "common.h"
+#include "runtime.h"
 #include "host/hostlogic.h"
 
 #include <algorithm>
@@ -28,8 +28,6 @@ int fail(int code, const std::string& m) {
 std::string hip_message(hipError_t e, const char* what) {
   return std::string("hip: ") + what + ": " + hipGetErrorString(e);
 }
-
-constexpr size_t kBufAlign = (size_t)2 << 20;
 
 // The allocation-free linear's split-K workspace: a static device array, one
 // copy per GPU the library runs on, held until the process ends. Host code
@@ -58,122 +56,7 @@ int scratch_setup(int device, void** out) {
   return 0;
 }
 
-// Grow-only device buffer.
-struct DevBuf {
-  void* p = nullptr;
-  size_t bytes = 0;
-  int ensure(size_t n) {
-    if (n <= bytes) return 0;
-    // Whole 2 MiB pages: each buffer starts on its own page. With sizes as
-    // asked, the step's attention ran 4% slower or not depending on how the
-    // buffers happened to fall (one process or the other); rounded, it
-    // always runs the faster way.
-    n = (n + kBufAlign - 1) / kBufAlign * kBufAlign;
-    // a step still in flight may read the old buffer (the scheduler's
-    // overlap mode): let the device drain before it goes
-    if (p) (void)hipDeviceSynchronize();
-    if (p) (void)hipFree(p);
-    p = nullptr;
-    bytes = 0;
-    hipError_t e = hipMalloc(&p, n);
-    if (e != hipSuccess) {
-      p = nullptr;
-      return fail(TGOHIP_ENOMEM, "device allocation of " + std::to_string(n) + " bytes: " +
-                                     hipGetErrorString(e));
-    }
-    bytes = n;
-    // TGOHIP_DEBUG_NAN_FILL=1: every activation and workspace buffer starts as
-    // all-ones bytes (NaN in f32 and f16), so a kernel that reads memory no
-    // earlier kernel wrote shows up as NaN logits or changed tokens.
-    static const bool nan_fill = [] {
-      const char* v = getenv("TGOHIP_DEBUG_NAN_FILL");
-      return v && atoi(v) != 0;
-    }();
-    if (nan_fill) {
-      e = hipMemset(p, 0xff, n);
-      if (e == hipSuccess) e = hipDeviceSynchronize();
-      if (e != hipSuccess) return fail(TGOHIP_EDEVICE, hip_message(e, "debug fill"));
-    }
-    return 0;
-  }
-  void release() {
-    if (p) (void)hipFree(p);
-    p = nullptr;
-    bytes = 0;
-  }
-};
-
-// Sub-ports of a layer's fused projections, one bit each once uploaded.
-enum { SUB_WQ = 1, SUB_WK = 2, SUB_WV = 4, SUB_WGATE = 8, SUB_WUP = 16, SUB_ALL = 31 };
-
-struct Layer {
-  PackedWeight qkv, wo, gateup, down;
-  int bound = 0;  // SUB_* bits of the fused QKV and gate/up sub-ports written
-  float* g_attn = nullptr;
-  float* g_ffn = nullptr;
-  float* g_q = nullptr;
-  float* g_k = nullptr;
-};
-
 }  // namespace tgohip
-
-using namespace tgohip;
-
-constexpr int kPinnedSlots = 4;
-
-struct tgohip_ctx {
-  int device = 0;
-  hipStream_t own_stream = nullptr;
-  hipStream_t stream = nullptr;
-  int ncu = 256;
-  bool configured = false;
-  tgohip_model_cfg cfg{};
-  std::vector<Layer> layers;
-  void* embed = nullptr;
-  uint16_t* embed_scales = nullptr;
-  int embed_form = -1;
-  PackedWeight lm_head;
-  float* g_final = nullptr;
-  double* inv_freq = nullptr;
-  half_t* kc = nullptr;
-  half_t* vc = nullptr;
-  int kv_positions = 0;
-  int precision = 1;  // 1 (default): tgo's f32 arithmetic (hi+lo pairs), 0: f16 operands
-  int cascade = 0;    // minimum sequences sharing a prefix for prefix-shared attention (0: off)
-  // activations and workspaces
-  DevBuf h, xn, qkv, q, attn, act, lastn, logits, argmax, margin, meta, gemm_ws, part_o, part_ml;
-  DevBuf amax_part;  // per-chunk partials of the greedy selection
-  DevBuf rows;  // [2][rows]: positions and slots derived on the device
-  DevBuf rope;  // [rows][32] float4: the rows' rotary cos and sin (rope_table)
-  int rows_cap = 0, batch_cap = 0;
-  int last_batch = 0;  // members of the last launched step (its margins are in `margin`)
-  // The head of the last launched step ran over the members that worked only:
-  // logits row i is member head_rows[i]'s (empty: one row per member).
-  std::vector<int32_t> head_rows;
-  // pinned staging for per-call metadata: a call writes the next slot while the
-  // device still reads the ones before, and waits only for the slot it takes
-  struct Pinned {
-    void* p = nullptr;
-    size_t bytes = 0;
-    hipEvent_t read = nullptr;  // the device's last read of it
-  };
-  Pinned pinned[kPinnedSlots];
-  int pinned_next = 0;
-  hipEvent_t ev0 = nullptr, ev1 = nullptr;
-  std::vector<void*> allocs;  // weight and gain allocations owned by the context
-  std::map<int, PackedWeight> handles;
-  int next_handle = 1;
-  // profiling: HIP events around the launches of the kernels in prof_mask
-  // (TGOHIP_PROF_* bits) in every prof_stride-th layer of a step
-  bool profile = false;
-  int prof_stride = 1;
-  int prof_mask = 1 << TGOHIP_PROF_ATTN;
-  std::vector<hipEvent_t> prof_ev;  // [2 sets][layers][kinds][begin, end]
-  double prof_ms[TGOHIP_PROF_KINDS] = {}, prof_bytes[TGOHIP_PROF_KINDS] = {},
-         prof_flops[TGOHIP_PROF_KINDS] = {};
-  int64_t prof_launches[TGOHIP_PROF_KINDS] = {};
-  void* scratch = nullptr;  // this device's address of the static split-K workspace
-};
 
 namespace {
 
@@ -192,62 +75,6 @@ void free_owned(tgohip_ctx* c, void* p) {
   if (it != c->allocs.end()) c->allocs.erase(it);
   (void)hipFree(p);
 }
-
-// The next staging slot, free and of at least `bytes`.
-int take_pinned(tgohip_ctx* c, size_t bytes, tgohip_ctx::Pinned** out) {
-  tgohip_ctx::Pinned& s = c->pinned[c->pinned_next];
-  c->pinned_next = (c->pinned_next + 1) % kPinnedSlots;
-  TGOHIP_HIP(hipEventSynchronize(s.read));
-  if (bytes > s.bytes) {
-    if (s.p) (void)hipHostFree(s.p);
-    s.p = nullptr;
-    s.bytes = 0;
-    TGOHIP_HIP(hipHostMalloc(&s.p, bytes, hipHostMallocDefault));
-    s.bytes = bytes;
-  }
-  *out = &s;
-  return 0;
-}
-
-// Metadata packer: appends arrays into a pinned staging slot at 256-byte
-// aligned offsets, then one kernel reads all of them into c->meta, or, above
-// kFetchBytes (a page table of some thousand pages for each of hundreds of
-// sequences), the copy engine, whose rate across PCIe is higher. Attention over
-// 64-position contexts, us a call back to back / alone, kernel : engine:
-// 0.03 MB of page table 26-30 / 45 : 35 / 50; 1.0 MB 46 / 85 : 55 / 83; 2.1 MB
-// 82 / 144 : 82 / 134; 4.2 MB 135 / 221 : 120 / 199; 8.4 MB 231 / 372 : 196 / 326.
-constexpr size_t kFetchBytes = (size_t)3 << 19;
-struct Stager {
-  std::vector<std::pair<const void*, size_t>> parts;
-  std::vector<size_t> offs;
-  size_t total = 0;
-  size_t add(const void* p, size_t bytes) {
-    const size_t o = total;
-    parts.push_back({p, bytes});
-    offs.push_back(o);
-    total += (bytes + 255) / 256 * 256;
-    return o;
-  }
-  int upload(tgohip_ctx* c) {
-    if (total == 0) return 0;
-    tgohip_ctx::Pinned* s = nullptr;
-    int rc = take_pinned(c, total, &s);
-    if (rc) return rc;
-    rc = c->meta.ensure(total);
-    if (rc) return rc;
-    for (size_t i = 0; i < parts.size(); i++)
-      if (parts[i].second) memcpy((char*)s->p + offs[i], parts[i].first, parts[i].second);
-    if (total <= kFetchBytes) {
-      launch_fetch(s->p, c->meta.p, total, c->stream);
-      TGOHIP_HIP(hipGetLastError());
-    } else {
-      TGOHIP_HIP(hipMemcpyAsync(c->meta.p, s->p, total, hipMemcpyHostToDevice, c->stream));
-    }
-    TGOHIP_HIP(hipEventRecord(s->read, c->stream));
-    return 0;
-  }
-  template <class T> T* dev(tgohip_ctx* c, size_t off) { return (T*)((char*)c->meta.p + off); }
-};
 
 int check_shape(int form, int K, int N, const char* what) {
   if (form < TGOHIP_FORM_F16 || form > TGOHIP_FORM_I4_SYM)
@@ -600,6 +427,7 @@ void tgohip_close(tgohip_ctx* c) {
                     &c->argmax, &c->margin, &c->amax_part, &c->meta, &c->gemm_ws, &c->part_o, &c->part_ml,
                     &c->rows, &c->rope})
     b->release();
+  c->ops.release();
   if (c->kc) (void)hipFree(c->kc);
   if (c->vc) (void)hipFree(c->vc);
   for (tgohip_ctx::Pinned& p : c->pinned) {
