@@ -404,7 +404,10 @@ int tgohip_packed_attention(tgohip_ctx* ctx, int handle, const void* q, int64_t 
  * multiple of 64, N of 32). adapters_put loads one at an index, replacing what
  * was there: host planes down [rank,K] and up [N,rank], f32 (rounded to the
  * nearest f16, refused past its range) or f16, rank 1 to 128. adapters_drop empties an index. An
- * empty index is no adapter. put, drop and free wait for the context's stream. */
+ * empty index is no adapter. put, drop and free wait for the context's stream. A
+ * captured call sees later puts and drops; it is captured for the largest rank
+ * loaded so far (of 16, 32, 64 and 128), and rows of an adapter put later beyond
+ * that are NaN in its replays. */
 int tgohip_adapters_new(tgohip_ctx* ctx, int K, int N, int capacity, int* handle);
 int tgohip_adapters_put(tgohip_ctx* ctx, int handle, int index, int rank, int dtype,
                         const void* down, const void* up, float scale);

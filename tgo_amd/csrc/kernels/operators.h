@@ -5,6 +5,8 @@
 
 #include "../common.h"
 
+#include <algorithm>
+
 namespace tgohip {
 
 // ---- rotary positions (rope.hip) -------------------------------------------
@@ -73,7 +75,7 @@ constexpr int kAdapterMaxRank = 128;
 struct AdapterEntry {
   const half_t* down;  // [rank_pad][K]
   const half_t* up;    // [N][rank_pad]
-  int32_t rank_pad;    // 0: no adapter at this index
+  int32_t rank_pad;    // 16, 32, 64 or 128; 0: no adapter at this index
   float scale;
 };
 // Rows perm[start .. start + n) carry the adapter (-1: none).
@@ -90,8 +92,13 @@ struct AdapterArgs {
   const void* base;
   void* y;
   int y_f16;
-  float* u;  // [T][kAdapterMaxRank]: x . down^T of the permuted rows
+  int splits;  // shares of K
+  int cols;    // columns per workgroup of the second kernel (set by launch_adapters)
+  float* u;    // [splits][T][kAdapterMaxRank]: x . down^T of the permuted rows, by share
 };
-void launch_adapters(const AdapterArgs& a, hipStream_t st);
+// The shares of K for a batch of `tiles` tiles (their planes are the workspace).
+inline int adapter_splits(int tiles, int ncu) { return tiles > 0 ? std::min(16, std::max(1, 2 * ncu / tiles)) : 1; }
+// tile_rows: the most rows of a tile; rank_pad: the set's largest.
+void launch_adapters(const AdapterArgs& a, int tile_rows, int rank_pad, int ncu, hipStream_t st);
 
 }  // namespace tgohip

@@ -485,7 +485,7 @@ int tgohip_adapters_put(tgohip_ctx* c, int handle, int index, int rank, int dtyp
     OnDevice on(c->device);
     // down [rank][K] with rows of zeros, up [N][rank] with columns of zeros, to a
     // rank the kernels' products take whole; one allocation
-    const int rp = (rank + 15) / 16 * 16;
+    const int rp = rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128;
     const size_t nd = (size_t)rp * s->K, nu = (size_t)s->N * rp;
     std::vector<uint16_t> h(nd + nu, 0), tmp;
     const uint16_t *d16 = (const uint16_t*)down, *u16 = (const uint16_t*)up;
@@ -507,6 +507,7 @@ int tgohip_adapters_put(tgohip_ctx* c, int handle, int index, int rank, int dtyp
     int rc = e == hipSuccess ? 0 : fail(TGOHIP_EDEVICE, hip_message(e, "adapter planes"));
     if (!rc) rc = adapter_set(c, s, index, AdapterEntry{(const half_t*)dev, (const half_t*)dev + nd, rp, scale});
     if (rc) (void)hipFree(dev);
+    else s->rank_pad = std::max(s->rank_pad, rp);
     return rc;
   });
 }
@@ -551,7 +552,7 @@ int tgohip_adapter_rows(tgohip_ctx* c, int B, const int32_t* extents, const int3
     if (!handle) return fail(TGOHIP_EINVAL, "adapter_rows: handle is missing");
     if (*handle && !find(c->ops.rows, *handle, "adapter_rows")) return TGOHIP_EINVAL;
     OnDevice on(c->device);
-    // rows by adapter, in their own order within one
+    // rows by adapter, in their own order within one, in tiles of 64
     std::vector<std::vector<int32_t>> by((size_t)top + 2);
     int32_t row = 0;
     for (int b = 0; b < B; b++)
@@ -559,9 +560,11 @@ int tgohip_adapter_rows(tgohip_ctx* c, int B, const int32_t* extents, const int3
     std::vector<int32_t> perm;
     perm.reserve((size_t)T);
     std::vector<AdapterTile> tiles;
+    int tile_rows = 0;
     for (size_t a = 0; a < by.size(); a++)
-      for (size_t i = 0; i < by[a].size(); i += 32) {
-        const int n = (int)std::min<size_t>(32, by[a].size() - i);
+      for (size_t i = 0; i < by[a].size(); i += 64) {
+        const int n = (int)std::min<size_t>(64, by[a].size() - i);
+        tile_rows = std::max(tile_rows, n);
         tiles.push_back(AdapterTile{(int32_t)a - 1, (int32_t)perm.size(), n});
         perm.insert(perm.end(), by[a].begin() + i, by[a].begin() + i + n);
       }
@@ -573,7 +576,8 @@ int tgohip_adapter_rows(tgohip_ctx* c, int B, const int32_t* extents, const int3
     sg.add(perm.data(), perm.size() * 4);
     const size_t off = sg.add(tiles.data(), tiles.size() * sizeof(AdapterTile));
     int rc = 0;
-    if (T) rc = r.u.ensure((size_t)T * kAdapterMaxRank * sizeof(float));
+    const int splits = adapter_splits((int)tiles.size(), c->ncu);
+    if (T) rc = r.u.ensure((size_t)splits * T * kAdapterMaxRank * sizeof(float));
     if (!rc) rc = sg.upload(c, r.meta);
     if (rc) {
       if (fresh) {
@@ -585,6 +589,8 @@ int tgohip_adapter_rows(tgohip_ctx* c, int B, const int32_t* extents, const int3
     }
     r.T = (int)T;
     r.ntiles = (int)tiles.size();
+    r.tile_rows = tile_rows;
+    r.splits = splits;
     r.max_adapter = top;
     r.tiles_off = off;
     *handle = h;
@@ -642,7 +648,8 @@ int tgohip_adapters(tgohip_ctx* c, int set, int rows, const void* x, int x_dtype
   a.y_f16 = y_dtype == TGOHIP_F16;
   a.u = (float*)r->u.p;
   OnDevice on(c->device);
-  launch_adapters(a, c->stream);
+  a.splits = r->splits;
+  launch_adapters(a, r->tile_rows, s->rank_pad, c->ncu, c->stream);
   TGOHIP_HIP(hipGetLastError());
   return 0;
 }

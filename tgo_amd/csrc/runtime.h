@@ -88,11 +88,12 @@ struct PackedHandle {
 };
 struct AdapterSet {
   int K = 0, N = 0;
+  int rank_pad = 0;  // the largest loaded so far
   std::vector<AdapterEntry> table;
   DevBuf table_dev;
 };
 struct AdapterRows {
-  int T = 0, ntiles = 0, max_adapter = -1;
+  int T = 0, ntiles = 0, tile_rows = 0, splits = 1, max_adapter = -1;
   size_t tiles_off = 0;
   DevBuf meta, u;
 };
