@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(AdapterArgs a) {
   const AdapterEntry e = a.table[t.adapter];
   if (e.rank_pad == 0 || e.rank_pad > RB * 16) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, q = lane >> 4;
-  const int nrb = e.rank_pad / 16, ntb = (t.n + 15) / 16;
+  const int nrb = e.rank_pad / 16;
   const int steps = a.K / 32;
   const int s0 = (int)((int64_t)steps * blockIdx.y / gridDim.y), s1 = (int)((int64_t)steps * (blockIdx.y + 1) / gridDim.y);
   int64_t row[TB];
@@ -52,70 +52,151 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(AdapterArgs a) {
   for (int b = 0; b < TB; b++) row[b] = (int64_t)a.perm[t.start + min(b * 16 + l16, t.n - 1)] * a.K + 8 * q;
   const half_t* dn = e.down + (int64_t)l16 * a.K + 8 * q;
   float4_t acc[TB][RB] = {};
-#pragma unroll 2
+  // branch-free (rows past the tile and ranks past the adapter repeat the last ones,
+  // whose results are not stored), one step loaded ahead
+  half8_t d[RB], hi[TB], lo[TB];
+  auto load = [&](int s) {
+#pragma unroll
+    for (int b = 0; b < TB; b++) adapter_load_x<XK>(a, row[b] + 32 * s, hi[b], lo[b]);
+#pragma unroll
+    for (int r = 0; r < RB; r++) d[r] = *(const half8_t*)(dn + (int64_t)min(r, nrb - 1) * 16 * a.K + 32 * s);
+  };
+  if (s0 + wave < s1) load(s0 + wave);
   for (int s = s0 + wave; s < s1; s += 4) {
-    half8_t d[RB], hi[TB], lo[TB];
+    half8_t dc[RB], hc[TB], lc[TB];
+#pragma unroll
+    for (int r = 0; r < RB; r++) dc[r] = d[r];
+#pragma unroll
+    for (int b = 0; b < TB; b++) {
+      hc[b] = hi[b];
+      if (XK != XK_F16) lc[b] = lo[b];
+    }
+    load(min(s + 4, s1 - 1));
 #pragma unroll
     for (int b = 0; b < TB; b++)
-      if (b < ntb) adapter_load_x<XK>(a, row[b] + 32 * s, hi[b], lo[b]);
 #pragma unroll
-    for (int r = 0; r < RB; r++)
-      if (r < nrb) d[r] = *(const half8_t*)(dn + (int64_t)r * 16 * a.K + 32 * s);
-#pragma unroll
-    for (int b = 0; b < TB; b++)
-#pragma unroll
-      for (int r = 0; r < RB; r++)
-        if (b < ntb && r < nrb) {
-          acc[b][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[b], d[r], acc[b][r], 0, 0, 0);
-          if (XK != XK_F16) acc[b][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[b], d[r], acc[b][r], 0, 0, 0);
-        }
+      for (int r = 0; r < RB; r++) {
+        acc[b][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hc[b], dc[r], acc[b][r], 0, 0, 0);
+        if (XK != XK_F16) acc[b][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lc[b], dc[r], acc[b][r], 0, 0, 0);
+      }
   }
   float* u = a.u + ((int64_t)blockIdx.y * a.T + t.start) * kAdapterMaxRank;
 #pragma unroll
   for (int b = 0; b < TB; b++) {
-    if (b >= ntb) break;
     if (b) __syncthreads();
 #pragma unroll
     for (int r = 0; r < RB; r++)
 #pragma unroll
       for (int i = 0; i < 4; i++) part[wave][4 * q + i][r * 16 + l16] = acc[b][r][i];
     __syncthreads();
-    for (int i = tid; i < 16 * e.rank_pad; i += 256) {
-      const int m = i / e.rank_pad, r = i - m * e.rank_pad;
-      if (b * 16 + m < t.n)
+    for (int i = tid; i < 16 * RB * 16; i += 256) {
+      const int m = i / (RB * 16), r = i % (RB * 16);
+      if (b * 16 + m < t.n && r < e.rank_pad)
         u[(b * 16 + m) * kAdapterMaxRank + r] = (part[0][m][r] + part[1][m][r]) + (part[2][m][r] + part[3][m][r]);
     }
   }
 }
 
+// A piece of a row of base or y: four f32 or eight f16 columns, 16 bytes.
 template <bool YF16>
-__device__ __forceinline__ float4_t adapter_load_base(const AdapterArgs& a, int64_t off) {
-  if (!a.base) return float4_t{0.f, 0.f, 0.f, 0.f};
-  if constexpr (YF16) {
-    const half4_t h = *(const half4_t*)((const half_t*)a.base + off);
-    return float4_t{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+__device__ __forceinline__ void adapter_load_piece(const AdapterArgs& a, int64_t off, float (&v)[YF16 ? 8 : 4]) {
+  if (!a.base) {
+#pragma unroll
+    for (int j = 0; j < (YF16 ? 8 : 4); j++) v[j] = 0.f;
+  } else if constexpr (YF16) {
+    const half8_t h = *(const half8_t*)((const half_t*)a.base + off);
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = (float)h[j];
+  } else {
+    const float4_t f = *(const float4_t*)((const float*)a.base + off);
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = f[j];
   }
-  return *(const float4_t*)((const float*)a.base + off);
 }
 template <bool YF16>
-__device__ __forceinline__ void adapter_store_y(const AdapterArgs& a, int64_t off, float4_t v) {
-  if constexpr (YF16) *(half4_t*)((half_t*)a.y + off) = half4_t{(half_t)v[0], (half_t)v[1], (half_t)v[2], (half_t)v[3]};
-  else *(float4_t*)((float*)a.y + off) = v;
+__device__ __forceinline__ void adapter_store_piece(const AdapterArgs& a, int64_t off, const float (&v)[YF16 ? 8 : 4]) {
+  if constexpr (YF16) {
+    half8_t h;
+#pragma unroll
+    for (int j = 0; j < 8; j++) h[j] = (half_t)v[j];
+    *(half8_t*)((half_t*)a.y + off) = h;
+  } else {
+    *(float4_t*)((float*)a.y + off) = float4_t{v[0], v[1], v[2], v[3]};
+  }
+}
+// Orders a wave's own LDS writes before its other lanes' reads (and back).
+__device__ __forceinline__ void adapter_wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+__device__ __forceinline__ half4_t adapter_low(half8_t v) { return half4_t{v[0], v[1], v[2], v[3]}; }
+
+// The power of two that brings a row whose largest magnitude is `top` to [1, 2), and
+// its inverse: u is carried as an f16 pair of that scale, 22 bits of its largest
+// value wherever f16's range ends.
+__device__ __forceinline__ void adapter_power(float top, float& down, float& up) {
+  int ex = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+  ex = top > 0.f && ex < 128 ? max(-100, min(100, ex)) : 0;
+  down = __uint_as_float((uint32_t)(127 - ex) << 23);
+  up = __uint_as_float((uint32_t)(127 + ex) << 23);
 }
 
-// Columns [a.cols * blockIdx.y, + a.cols) of a tile's rows, 16 columns a wave at a
-// time: up's 16 rows are the A operand, so a lane holds four neighbouring columns
-// of row l16 of y.
+// Sums the planes of a tile's rows in their order and leaves them as pairs,
+// [hi 128 | lo 128] a row and 0 from the adapter's rank on, one wave per row and
+// two ranks a lane.
+__global__ __launch_bounds__(256) void adapter_pair_kernel(AdapterArgs a) {
+  const AdapterTile t = a.tiles[blockIdx.x];
+  const int m = blockIdx.y * 4 + (threadIdx.x >> 6), r = (threadIdx.x & 63) * 2;
+  if (t.adapter < 0 || m >= t.n) return;
+  const int rank_pad = a.table[t.adapter].rank_pad;
+  const int64_t pos = t.start + m;
+  float s0 = 0.f, s1 = 0.f;
+  if (r < min(rank_pad, a.rank_pad)) {
+    float2 v[kAdapterMaxSplits];
+#pragma unroll
+    for (int p = 0; p < kAdapterMaxSplits; p++)
+      v[p] = *(const float2*)(a.u + ((int64_t)min(p, a.splits - 1) * a.T + pos) * kAdapterMaxRank + r);
+#pragma unroll
+    for (int p = 0; p < kAdapterMaxSplits; p++) {
+      s0 += p < a.splits ? v[p].x : 0.f;
+      s1 += p < a.splits ? v[p].y : 0.f;
+    }
+  }
+  float top = fmaxf(fabsf(s0), fabsf(s1)), down, up;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  adapter_power(top, down, up);
+  s0 *= down;
+  s1 *= down;
+  const half2_t hi = {(half_t)s0, (half_t)s1};
+  half_t* dst = a.pair + pos * 2 * kAdapterMaxRank + r;
+  *(half2_t*)dst = hi;
+  *(half2_t*)(dst + kAdapterMaxRank) = half2_t{(half_t)(s0 - (float)hi[0]), (half_t)(s1 - (float)hi[1])};
+  if (r == 0) a.pair_scale[pos] = up;
+}
+
+// Columns [a.cols * blockIdx.y, + a.cols) of a tile's rows. A wave takes 16 of the
+// rows and 64 columns a round (up's rows are the A operand, so a lane holds four
+// neighbouring columns of row l16 of y); a tile of fewer blocks of rows shares its
+// columns among the waves instead. The next round's up and base are loaded before
+// this one's products, which cross the wave's own LDS so that base and y move in
+// runs of 64 columns of a row. With one block of rows per tile (TB = 1) the planes
+// are summed and scaled here, else they come as adapter_pair_kernel's pairs.
 template <int TB, int RB, bool YF16>
 __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a) {
   constexpr int KB = RB == 1 ? 1 : RB / 2;  // products along the rank: 32 wide, or one 16 wide
-  __shared__ __attribute__((aligned(16))) float us[TB * 16][RB * 16 + 4];
+  constexpr int E = RB == 1 ? 4 : 8;        // of which a lane holds E
+  constexpr int PE = YF16 ? 8 : 4;          // columns of a 16-byte piece of base or y
+  constexpr int PL = 64 / PE;               // lanes per row's run
+  constexpr int NP = 16 * PL / 64;          // pieces a lane holds
+  __shared__ __attribute__((aligned(16))) float us[TB == 1 ? 16 : 1][RB * 16 + 4];
+  __shared__ __attribute__((aligned(16))) float stage[4][16][68];
   const AdapterTile t = a.tiles[blockIdx.x];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, q = lane >> 4;
   const int n0 = blockIdx.y * a.cols, n1 = min(n0 + a.cols, a.N);
   AdapterEntry e{};
   if (t.adapter >= 0) e = a.table[t.adapter];
-  const int ntb = (t.n + 15) / 16;
   // an adapter of a larger rank than the launch was captured for: its rows are NaN
   if (e.rank_pad > RB * 16) {
     e.rank_pad = RB * 16;
@@ -123,121 +204,165 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a) {
   }
   if (e.rank_pad == 0) {
     if (a.base == a.y) return;
-    const int w = (n1 - n0) / 4;
+    const int w = (n1 - n0) / PE;
     for (int i = tid; i < t.n * w; i += 256) {
       const int m = i / w;
-      const int64_t off = (int64_t)a.perm[t.start + m] * a.N + n0 + 4 * (i - m * w);
-      adapter_store_y<YF16>(a, off, adapter_load_base<YF16>(a, off));
+      const int64_t off = (int64_t)a.perm[t.start + m] * a.N + n0 + PE * (i - m * w);
+      float v[PE];
+      adapter_load_piece<YF16>(a, off, v);
+      adapter_store_piece<YF16>(a, off, v);
     }
     return;
   }
-  for (int i = tid; i < TB * 16 * RB * 16; i += 256) {
-    const int m = i / (RB * 16), r = i - m * (RB * 16);
-    float s = 0.f;
-    if (m < t.n && r < e.rank_pad)
-      for (int p = 0; p < a.splits; p++) s += a.u[((int64_t)p * a.T + t.start + m) * kAdapterMaxRank + r];
-    us[m][r] = s;
-  }
-  __syncthreads();
-  // u of row l16 of each block as an f16 pair, scaled by a power of two to a
-  // largest value in [1, 2): 22 bits of it, wherever f16's range ends
-  half8_t uh[TB][KB], ul[TB][KB];
-  float scale[TB];
-  int64_t row[TB];
-  const int kq = RB == 1 ? 4 * q : 8 * q;
+  const int ntb = (t.n + 15) / 16, share = ntb == 1 ? 4 : ntb == 2 ? 2 : 1;  // waves that share a block's columns
+  const int m0 = 16 * (wave / share);
+  half8_t uh[KB], ul[KB];
+  float scale;
+  if constexpr (TB == 1) {
+    for (int i = tid; i < 16 * RB * 16; i += 256) {
+      const int m = i / (RB * 16), r = i - m * (RB * 16);
+      // every plane's load in flight, summed in their order
+      float s = 0.f, v[kAdapterMaxSplits];
+      const bool in = m < t.n && r < e.rank_pad;
+      const float* u = a.u + ((int64_t)t.start + (in ? m : 0)) * kAdapterMaxRank + (in ? r : 0);
 #pragma unroll
-  for (int b = 0; b < TB; b++) {
-    row[b] = (int64_t)a.perm[t.start + min(b * 16 + l16, t.n - 1)] * a.N + 4 * q;
-    float top = 0.f;
+      for (int p = 0; p < kAdapterMaxSplits; p++) v[p] = u[(int64_t)min(p, a.splits - 1) * a.T * kAdapterMaxRank];
+#pragma unroll
+      for (int p = 0; p < kAdapterMaxSplits; p++) s += p < a.splits ? v[p] : 0.f;
+      us[m][r] = in ? s : 0.f;
+    }
+    __syncthreads();
+    float top = 0.f, down, up;
 #pragma unroll
     for (int k = 0; k < KB; k++)
 #pragma unroll
-      for (int j = 0; j < (RB == 1 ? 4 : 8); j++) top = fmaxf(top, fabsf(us[b * 16 + l16][32 * k + kq + j]));
+      for (int j = 0; j < E; j++) top = fmaxf(top, fabsf(us[l16][32 * k + E * q + j]));
     top = fmaxf(top, __shfl_xor(top, 16, 64));
     top = fmaxf(top, __shfl_xor(top, 32, 64));
-    int ex = (int)((__float_as_uint(top) >> 23) & 255) - 127;
-    ex = top > 0.f && ex < 128 ? max(-100, min(100, ex)) : 0;
-    const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
-    scale[b] = e.scale * __uint_as_float((uint32_t)(127 + ex) << 23);
+    adapter_power(top, down, up);
+    scale = e.scale * up;
 #pragma unroll
     for (int k = 0; k < KB; k++)
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const float f = RB == 1 && j >= 4 ? 0.f : us[b * 16 + l16][32 * k + kq + j] * down;
-        uh[b][k][j] = (half_t)f;
-        ul[b][k][j] = (half_t)(f - (float)uh[b][k][j]);
+        const float f = j < E ? us[l16][32 * k + E * q + (j < E ? j : 0)] * down : 0.f;
+        uh[k][j] = (half_t)f;
+        ul[k][j] = (half_t)(f - (float)uh[k][j]);
       }
+  } else {
+    if (m0 >= t.n) return;
+    const int64_t pos = t.start + min(m0 + l16, t.n - 1);
+    const half_t* p = a.pair + pos * 2 * kAdapterMaxRank + E * q;
+    scale = e.scale * a.pair_scale[pos];
+#pragma unroll
+    for (int k = 0; k < KB; k++) {  // RB = 1 uses the first half of what it loads
+      uh[k] = *(const half8_t*)(p + 32 * k);
+      ul[k] = *(const half8_t*)(p + kAdapterMaxRank + 32 * k);
+    }
   }
-  const int nkb = RB == 1 ? 1 : (e.rank_pad + 31) / 32;
-#pragma unroll 2
-  for (int n = n0 + 16 * wave; n < n1; n += 64) {
-    const half_t* up = e.up + (int64_t)(n + l16) * e.rank_pad + kq;
-    half8_t w[KB];
-    float4_t base[TB];
+  const int prow = lane / PL, pcol = lane % PL * PE;
+  int64_t off[NP];  // this lane's pieces of the rows
+  bool live[NP];
 #pragma unroll
-    for (int k = 0; k < KB; k++) {
-      if constexpr (RB == 1) {
-        const half4_t h = *(const half4_t*)up;
-        w[0] = half8_t{h[0], h[1], h[2], h[3], 0, 0, 0, 0};
-      } else {
-        w[k] = half8_t{};
-        if (k < nkb && 32 * k + kq < e.rank_pad) w[k] = *(const half8_t*)(up + 32 * k);
+  for (int i = 0; i < NP; i++) {
+    const int m = m0 + i * (64 / PL) + prow;
+    live[i] = m < t.n;
+    off[i] = (int64_t)a.perm[t.start + min(m, t.n - 1)] * a.N + pcol;
+  }
+  half8_t w[4][KB];
+  float base[NP][PE];
+  auto load = [&](int n) {
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      const half_t* up = e.up + (int64_t)min(n + 16 * c + l16, a.N - 1) * e.rank_pad + E * q;
+#pragma unroll
+      for (int k = 0; k < KB; k++) {
+        if constexpr (RB == 1) {
+          const half4_t h = *(const half4_t*)up;
+          w[c][0] = half8_t{h[0], h[1], h[2], h[3], 0, 0, 0, 0};
+        } else {
+          // past the adapter's rank u is 0, and up reads its first values again
+          w[c][k] = *(const half8_t*)(up + (32 * k + 8 * q < e.rank_pad ? 32 * k : 8 * q < e.rank_pad ? 0 : -8 * q));
+        }
       }
     }
+    const int back = n + pcol < n1 ? 0 : pcol;  // behind the last column: the run's first piece again
 #pragma unroll
-    for (int b = 0; b < TB; b++)
-      if (b < ntb) base[b] = adapter_load_base<YF16>(a, row[b] + n);
+    for (int i = 0; i < NP; i++) adapter_load_piece<YF16>(a, off[i] + n - back, base[i]);
+  };
+  float(*ys)[68] = stage[wave];
+  int n = n0 + 64 * (wave % share);
+  if (n < n1) load(n);
+  for (; n < n1; n += 64 * share) {
+    half8_t wc[4][KB];
+    float bc[NP][PE];
 #pragma unroll
-    for (int b = 0; b < TB; b++) {
-      if (b >= ntb) break;
+    for (int c = 0; c < 4; c++)
+#pragma unroll
+      for (int k = 0; k < KB; k++) wc[c][k] = w[c][k];
+#pragma unroll
+    for (int i = 0; i < NP; i++)
+#pragma unroll
+      for (int j = 0; j < PE; j++) bc[i][j] = base[i][j];
+    if (n + 64 * share < n1) load(n + 64 * share);
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
       float4_t acc = {};
-      if constexpr (RB == 1) {
-        const half4_t w4 = {w[0][0], w[0][1], w[0][2], w[0][3]};
-        const half4_t h4 = {uh[b][0][0], uh[b][0][1], uh[b][0][2], uh[b][0][3]};
-        const half4_t l4 = {ul[b][0][0], ul[b][0][1], ul[b][0][2], ul[b][0][3]};
-        acc = __builtin_amdgcn_mfma_f32_16x16x16f16(w4, l4, acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_16x16x16f16(w4, h4, acc, 0, 0, 0);
-      } else {
 #pragma unroll
-        for (int k = 0; k < KB; k++)
-          if (k < nkb) {
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[k], ul[b][k], acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(w[k], uh[b][k], acc, 0, 0, 0);
-          }
+      for (int k = 0; k < KB; k++) {
+        if constexpr (RB == 1) {
+          acc = __builtin_amdgcn_mfma_f32_16x16x16f16(adapter_low(wc[c][0]), adapter_low(ul[0]), acc, 0, 0, 0);
+          acc = __builtin_amdgcn_mfma_f32_16x16x16f16(adapter_low(wc[c][0]), adapter_low(uh[0]), acc, 0, 0, 0);
+        } else {
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(wc[c][k], ul[k], acc, 0, 0, 0);
+          acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(wc[c][k], uh[k], acc, 0, 0, 0);
+        }
       }
-      float4_t y;
-#pragma unroll
-      for (int i = 0; i < 4; i++) y[i] = fmaf(scale[b], acc[i], base[b][i]);
-      if (b * 16 + l16 < t.n) adapter_store_y<YF16>(a, row[b] + n, y);
+      *(float4_t*)&ys[l16][16 * c + 4 * q] = acc * scale;
     }
+    adapter_wave_sync();
+#pragma unroll
+    for (int i = 0; i < NP; i++) {
+      float y[PE];
+#pragma unroll
+      for (int j = 0; j < PE; j += 4) {
+        const float4_t v = *(const float4_t*)&ys[i * (64 / PL) + prow][pcol + j];
+#pragma unroll
+        for (int g = 0; g < 4; g++) y[j + g] = bc[i][j + g] + v[g];
+      }
+      if (live[i] && n + pcol < n1) adapter_store_piece<YF16>(a, off[i] + n, y);
+    }
+    adapter_wave_sync();
   }
 }
 
 template <int XK, int TB, int RB>
 static void adapters_launch(const AdapterArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((adapter_down_kernel<XK, TB, RB>), dim3((unsigned)a.ntiles, (unsigned)a.splits), dim3(256), 0, st, a);
+  if (TB > 1) hipLaunchKernelGGL(adapter_pair_kernel, dim3((unsigned)a.ntiles, 4 * TB), dim3(256), 0, st, a);
   const dim3 grid((unsigned)a.ntiles, (unsigned)((a.N + a.cols - 1) / a.cols));
   if (a.y_f16) hipLaunchKernelGGL((adapter_up_kernel<TB, RB, true>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((adapter_up_kernel<TB, RB, false>), grid, dim3(256), 0, st, a);
 }
 template <int XK, int TB>
-static void adapters_rank(const AdapterArgs& a, int rank_pad, hipStream_t st) {
-  if (rank_pad <= 16) adapters_launch<XK, TB, 1>(a, st);
-  else if (rank_pad <= 32) adapters_launch<XK, TB, 2>(a, st);
-  else if (rank_pad <= 64) adapters_launch<XK, TB, 4>(a, st);
+static void adapters_rank(const AdapterArgs& a, hipStream_t st) {
+  if (a.rank_pad <= 16) adapters_launch<XK, TB, 1>(a, st);
+  else if (a.rank_pad <= 32) adapters_launch<XK, TB, 2>(a, st);
+  else if (a.rank_pad <= 64) adapters_launch<XK, TB, 4>(a, st);
   else adapters_launch<XK, TB, 8>(a, st);
 }
 
-void launch_adapters(const AdapterArgs& args, int tile_rows, int rank_pad, int ncu, hipStream_t st) {
+void launch_adapters(const AdapterArgs& args, int tile_rows, int ncu, hipStream_t st) {
   AdapterArgs a = args;
-  // about two workgroups per CU along N, each with at least 64 columns a wave
-  const int per_tile = std::max(1, 2 * ncu / a.ntiles);
-  a.cols = std::max(256, (a.N / per_tile + 63) / 64 * 64);
   const bool few = tile_rows <= 16;
+  // Columns per workgroup of the second kernel, us for 1152 mixed rows of rank 64 over
+  // [4096, 24576] and 8000 f16 rows of rank 24 over [12288, 4096]: 128 columns 108,
+  // 100; 256 106, 96; 512 114, 97; 1024 138, 111.
+  a.cols = 256;
   switch (a.xk) {
-    case XK_F32: few ? adapters_rank<XK_F32, 1>(a, rank_pad, st) : adapters_rank<XK_F32, 4>(a, rank_pad, st); break;
-    case XK_F16: few ? adapters_rank<XK_F16, 1>(a, rank_pad, st) : adapters_rank<XK_F16, 4>(a, rank_pad, st); break;
-    default: few ? adapters_rank<XK_X2, 1>(a, rank_pad, st) : adapters_rank<XK_X2, 4>(a, rank_pad, st); break;
+    case XK_F32: few ? adapters_rank<XK_F32, 1>(a, st) : adapters_rank<XK_F32, 4>(a, st); break;
+    case XK_F16: few ? adapters_rank<XK_F16, 1>(a, st) : adapters_rank<XK_F16, 4>(a, st); break;
+    default: few ? adapters_rank<XK_X2, 1>(a, st) : adapters_rank<XK_X2, 4>(a, st); break;
   }
 }
 

@@ -72,6 +72,7 @@ int packed_enqueue(const PackedArgs& a, int D, int q_f16, int items, int merges,
 
 // ---- adapters (adapters.hip) --------------------------------------------------
 constexpr int kAdapterMaxRank = 128;
+constexpr int kAdapterFewRows = 512;  // rows up to which a batch's tiles hold 16 rows
 struct AdapterEntry {
   const half_t* down;  // [rank_pad][K]
   const half_t* up;    // [N][rank_pad]
@@ -94,11 +95,17 @@ struct AdapterArgs {
   int y_f16;
   int splits;  // shares of K
   int cols;    // columns per workgroup of the second kernel (set by launch_adapters)
-  float* u;    // [splits][T][kAdapterMaxRank]: x . down^T of the permuted rows, by share
+  int rank_pad;  // the set's largest
+  float* u;      // [splits][T][kAdapterMaxRank]: x . down^T of the permuted rows, by share
+  half_t* pair;  // [T][2][kAdapterMaxRank]: their sums as scaled hi + lo pairs
+  float* pair_scale;  // [T]
 };
 // The shares of K for a batch of `tiles` tiles (their planes are the workspace).
-inline int adapter_splits(int tiles, int ncu) { return tiles > 0 ? std::min(16, std::max(1, 2 * ncu / tiles)) : 1; }
-// tile_rows: the most rows of a tile; rank_pad: the set's largest.
-void launch_adapters(const AdapterArgs& a, int tile_rows, int rank_pad, int ncu, hipStream_t st);
+constexpr int kAdapterMaxSplits = 16;
+inline int adapter_splits(int tiles, int ncu) {
+  return tiles > 0 ? std::min(kAdapterMaxSplits, std::max(1, 2 * ncu / tiles)) : 1;
+}
+// tile_rows: 16 or 64, the most rows of a tile.
+void launch_adapters(const AdapterArgs& a, int tile_rows, int ncu, hipStream_t st);
 
 }  // namespace tgohip

@@ -552,7 +552,9 @@ int tgohip_adapter_rows(tgohip_ctx* c, int B, const int32_t* extents, const int3
     if (!handle) return fail(TGOHIP_EINVAL, "adapter_rows: handle is missing");
     if (*handle && !find(c->ops.rows, *handle, "adapter_rows")) return TGOHIP_EINVAL;
     OnDevice on(c->device);
-    // rows by adapter, in their own order within one, in tiles of 64
+    // rows by adapter, in their own order within one, in tiles of 16 (decode batches:
+    // most adapters have a few rows) or 64 (prompts: an adapter is read once per tile)
+    const size_t tile = T <= kAdapterFewRows ? 16 : 64;
     std::vector<std::vector<int32_t>> by((size_t)top + 2);
     int32_t row = 0;
     for (int b = 0; b < B; b++)
@@ -560,11 +562,9 @@ int tgohip_adapter_rows(tgohip_ctx* c, int B, const int32_t* extents, const int3
     std::vector<int32_t> perm;
     perm.reserve((size_t)T);
     std::vector<AdapterTile> tiles;
-    int tile_rows = 0;
     for (size_t a = 0; a < by.size(); a++)
-      for (size_t i = 0; i < by[a].size(); i += 64) {
-        const int n = (int)std::min<size_t>(64, by[a].size() - i);
-        tile_rows = std::max(tile_rows, n);
+      for (size_t i = 0; i < by[a].size(); i += tile) {
+        const int n = (int)std::min<size_t>(tile, by[a].size() - i);
         tiles.push_back(AdapterTile{(int32_t)a - 1, (int32_t)perm.size(), n});
         perm.insert(perm.end(), by[a].begin() + i, by[a].begin() + i + n);
       }
@@ -577,7 +577,7 @@ int tgohip_adapter_rows(tgohip_ctx* c, int B, const int32_t* extents, const int3
     const size_t off = sg.add(tiles.data(), tiles.size() * sizeof(AdapterTile));
     int rc = 0;
     const int splits = adapter_splits((int)tiles.size(), c->ncu);
-    if (T) rc = r.u.ensure((size_t)splits * T * kAdapterMaxRank * sizeof(float));
+    if (T) rc = r.u.ensure((size_t)T * ((size_t)(splits + 1) * kAdapterMaxRank + 1) * sizeof(float));
     if (!rc) rc = sg.upload(c, r.meta);
     if (rc) {
       if (fresh) {
@@ -589,7 +589,7 @@ int tgohip_adapter_rows(tgohip_ctx* c, int B, const int32_t* extents, const int3
     }
     r.T = (int)T;
     r.ntiles = (int)tiles.size();
-    r.tile_rows = tile_rows;
+    r.tile_rows = (int)tile;
     r.splits = splits;
     r.max_adapter = top;
     r.tiles_off = off;
@@ -649,7 +649,10 @@ int tgohip_adapters(tgohip_ctx* c, int set, int rows, const void* x, int x_dtype
   a.u = (float*)r->u.p;
   OnDevice on(c->device);
   a.splits = r->splits;
-  launch_adapters(a, r->tile_rows, s->rank_pad, c->ncu, c->stream);
+  a.rank_pad = s->rank_pad;
+  a.pair = (half_t*)(a.u + (size_t)r->splits * T * kAdapterMaxRank);  // as many bytes as a plane
+  a.pair_scale = a.u + (size_t)(r->splits + 1) * T * kAdapterMaxRank;
+  launch_adapters(a, r->tile_rows, c->ncu, c->stream);
   TGOHIP_HIP(hipGetLastError());
   return 0;
 }
