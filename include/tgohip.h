@@ -386,8 +386,8 @@ int tgohip_packed_free(tgohip_ctx* ctx, int handle);
 /* out = softmax(scale q k^T) v over a plan's rows. q [rows, H, head_dim] in the
  * plan's q_dtype, k and v [key rows, H_kv, head_dim] f16, out like q in f32, f16
  * or as a pair (TGOHIP_F16X2, dense rows, the lo plane behind the hi plane). Rows
- * are *_row elements apart, heads dense; rows start on 16-byte boundaries.
- * scale > 0. With f32 queries the products are those of tgohip_paged_attention's
+ * are *_row elements apart (k's and v's at most 2^24), heads dense; rows start on
+ * 16-byte boundaries. scale > 0. With f32 queries the products are those of tgohip_paged_attention's
  * f32 form (q and the probabilities as f16 hi + lo pairs, so |q| < 65504); with
  * f16 queries the probabilities are rounded to f16. Sums, maxima and partial
  * results are f32. Memory behind the last row stays as it is; out meets none of

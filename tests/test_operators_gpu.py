@@ -457,7 +457,7 @@ def test_packed_attention_refusals(ctx, torch_gpu):
                         ("scale is nan", dict(scale=float("nan"))), ("scale is inf", dict(scale=float("inf"))),
                         ("out_dtype is 3", dict(out_dtype=3)), ("q and out are device", dict(q=None)),
                         ("q and out are device", dict(out=None)), ("k and v are device", dict(v=None)),
-                        ("q rows are 255", dict(q_row=255)), ("k rows are 64", dict(k_row=64)), ("v rows are -128", dict(v_row=-128)),
+                        ("q rows are 255", dict(q_row=255)), ("k rows are 16777224", dict(k_row=(1 << 24) + 8)), ("k rows are 64", dict(k_row=64)), ("v rows are -128", dict(v_row=-128)),
                         ("out rows are 0", dict(out_row=0)), ("16-byte", dict(q=q.data_ptr() + 4)), ("16-byte", dict(k_row=132)),
                         ("16-byte", dict(out_row=258)), ("rows are dense", dict(out_dtype=2, out_row=264)),
                         ("out meets q", dict(out=q.data_ptr())), ("out meets k", dict(out=k.data_ptr())),

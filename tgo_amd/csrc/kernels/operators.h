@@ -55,6 +55,8 @@ struct PackedPlan {
 // Decomposes a call (host only). nq, nk: [B], checked by the caller.
 void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int Hkv, int D, bool causal,
                        bool q_f16, int ncu, PackedPlan& plan);
+// Key rows at most this many elements apart: offsets in a tile fit 32 bits.
+constexpr int64_t kPackMaxRow = (int64_t)1 << 24;
 struct PackedArgs {
   const void* q;
   const half_t* k;

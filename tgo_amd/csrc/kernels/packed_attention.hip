@@ -5,11 +5,15 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 namespace tgohip {
 
 constexpr int kPackTile = 64;   // keys staged in LDS per iteration
-constexpr int kPackRows = 128;  // rows per workgroup
+#ifndef PW
+#define PW 4
+#endif
+constexpr int kPackRows = 32 * PW;  // rows per workgroup
 // Online softmax with a lazy reference m (log2 units): it starts at kPackNoMax, a
 // row's probabilities are 2^(s - m), and m moves to the row's maximum - kPackLift
 // once that passes m + kPackTop. They so stay below 2^kPackTop (f16 ends at 2^16),
@@ -52,7 +56,7 @@ void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int H
   plan.tq = q0;
   plan.tk = k0;
   // Parts long enough that every workgroup slot gets about one.
-  const double slots = 2.0 * ncu;
+  const double slots = 8.0 / PW * ncu;
   const int part = std::max(512, (int)std::min(1.0e9, total / slots + kPackTile) / kPackTile * kPackTile);
   for (PackedItem it : base) {
     const int parts = (it.kv_hi + part - 1) / part;
@@ -82,27 +86,55 @@ void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int H
 // kernels
 // ---------------------------------------------------------------------------
 
-// 16-byte chunk c of tile row p: K rows are read whole by 32 lanes at one chunk,
-// V by transposing reads of 4 rows x 64 bytes; both orders touch distinct banks.
-template <int D>
-__device__ __forceinline__ int pack_k_slot(int p, int c) {
-  return p * (D / 8) + (c ^ (D == 128 ? (p & 15) : ((p >> 1) & 7)));
-}
-template <int D>
-__device__ __forceinline__ int pack_v_slot(int p, int c) {
-  return p * (D / 8) + (c ^ (D == 128 ? (p & 3) << 2 : ((p >> 1) & 1) << 2));
+// s_waitcnt vmcnt(0), the other counters not waited for.
+constexpr int kPackVm0 = 0x0f70;
+// A barrier without a memory fence, which would wait for every DMA in flight; no
+// memory access moves across it.
+__device__ __forceinline__ void pack_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
-// Eight V^T operand values of one dim: tile rows p0 + [0,4) and p0 + 8 + [0,4).
-// In each 16-lane group lane j names 8 bytes of row p0 + j/4 at dim d0 + 4(j%4)
-// and receives dim d0 + j of the four rows.
+// A tile of kPackTile keys in LDS: rows of D f16, their 16-byte chunks XOR-swizzled.
+// K's chunks by the row, so that 32 lanes reading one chunk of 32 rows touch
+// distinct banks; V's 64-byte quarters by the row's last two bits (D = 64: halves
+// by the next to last), for transposing reads of four rows x 64 bytes. Both
+// swizzles repeat every 16 rows and leave the chunk's bits to an XOR, so a lane
+// keeps one byte address for each and the rest are constants.
 template <int D>
-__device__ __forceinline__ half8_t pack_v_frag(const half_t* Vs, int p0, int d0, int j) {
+__device__ __forceinline__ int pack_k_swz(int p) {
+  return D == 128 ? (p & 15) : ((p >> 1) & 7);
+}
+template <int D>
+__device__ __forceinline__ int pack_v_swz(int p) {
+  return D == 128 ? (p & 3) << 2 : ((p >> 1) & 1) << 2;
+}
+// Byte address of the lane's K operand (row l32, dims 8kh + [0,8)); step s is at
+// that XOR 32s, 32 rows on at that + 64 D.
+template <int D>
+__device__ __forceinline__ int pack_k_at(int l32, int kh) {
+  return l32 * 2 * D + 16 * (kh ^ pack_k_swz<D>(l32));
+}
+// Byte address of the lane's V^T operand: in each 16-lane group lane j names 8
+// bytes of row 4kh + j/4 at dim d0 + 4(j%4) and receives dim d0 + j of the four
+// rows; dims 32db + .. at that XOR 64db, rows p0 on at that + 2 D p0.
+template <int D>
+__device__ __forceinline__ int pack_v_at(int lane) {
+  const int j = lane & 15, p = 4 * (lane >> 5) + (j >> 2), c = 2 * ((lane >> 4) & 1) + ((j & 3) >> 1);
+  return p * 2 * D + 16 * (c ^ pack_v_swz<D>(p)) + 8 * (j & 1);
+}
+typedef __attribute__((address_space(3))) char* lds_t;
+__device__ __forceinline__ half8_t pack_k_frag(lds_t K, int at) {
+  return *(__attribute__((address_space(3))) half8_t*)(K + at);
+}
+// Eight values of one dim: tile rows p0 + 4kh + [0,4) and those + 8.
+template <int D>
+__device__ __forceinline__ half8_t pack_v_frag(lds_t V, int at) {
   typedef short short4_t __attribute__((ext_vector_type(4)));
   typedef __attribute__((address_space(3))) short4_t* lds4;
-  const int c = (d0 >> 3) + ((j & 3) >> 1), r = p0 + (j >> 2);
-  const short4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(Vs + pack_v_slot<D>(r, c) * 8 + 4 * (j & 1)));
-  const short4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(Vs + pack_v_slot<D>(r + 8, c) * 8 + 4 * (j & 1)));
+  const short4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(V + at));
+  const short4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(V + at + 16 * D));
   return __builtin_bit_cast(half8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
@@ -134,184 +166,312 @@ __device__ __forceinline__ void pack_load_q(const void* q, int64_t off, bool val
   }
 }
 
-// S^T = K . Q^T and O^T += V^T . P^T on v_mfma_f32_32x32x16_f16: lane (r, kh) =
-// (lane % 32, lane / 32) holds row r's scores at keys 8(i/4) + 4kh + i%4 of each
-// 32-key block, which are the B operand of the second product as they stand.
+// One 32-row block of a wave: where its rows are, what they have seen. Lane (r, kh)
+// = (lane % 32, lane / 32) holds row r: its query's dims 16s + 8kh + [0,8), its
+// maximum and (its half of the keys') sum, and of O^T dims 32db + 8g + 4kh + [0,4).
 template <int D, bool QF16>
-__global__ __launch_bounds__(256, 2) void packed_kernel(PackedArgs a) {
-  __shared__ __attribute__((aligned(16))) half_t Ks[kPackTile * D], Vs[kPackTile * D];
-  constexpr int CH = D / 8, NL = kPackTile * CH / 256, KS = D / 16, DB = D / 32;
-  const PackedItem it = a.items[blockIdx.x];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int l32 = lane & 31, kh = lane >> 5;
-  const int r = wave * 32 + l32;
-  const bool valid = r < it.nr;
-  const int row = it.r0 + (valid ? r : 0), tok = row / a.G, head = it.kvh * a.G + row % a.G;
-  const int lim = min(tok + it.shift, it.nk - 1);
-  // first and last key limit of the wave's rows
-  const int w0 = wave * 32, w1 = min(w0 + 32, it.nr) - 1;
-  const int wlo = min((it.r0 + w0) / a.G + it.shift, it.nk - 1);
-  const int whi = w0 < it.nr ? min((it.r0 + w1) / a.G + it.shift, it.nk - 1) : -1;
+struct PackRows {
+  bool valid;
+  int r, tok, head, lim;  // row of the item, its token, query head and last visible key
+  half8_t qh[D / 16], ql[QF16 ? 1 : D / 16];
+  float m, l;
+  float16_t o[D / 32];
 
-  half8_t qh[KS], ql[KS];
+  __device__ __forceinline__ void init(const PackedArgs& a, const PackedItem& it, int r0, int lane) {
+    r = r0 + (lane & 31);
+    valid = r < it.nr;
+    const int row = it.r0 + (valid ? r : 0);
+    tok = row / a.G;
+    head = it.kvh * a.G + row % a.G;
+    lim = min(tok + it.shift, it.nk - 1);
 #pragma unroll
-  for (int s = 0; s < KS; s++)
-    pack_load_q<QF16>(a.q, (it.q0 + tok) * a.q_row + head * D + 16 * s + 8 * kh, valid, qh[s], ql[s]);
-
-  float m = kPackNoMax, l = 0.f;
-  float16_t o[DB];
+    for (int s = 0; s < D / 16; s++)
+      pack_load_q<QF16>(a.q, (it.q0 + tok) * a.q_row + head * D + 16 * s + 8 * (lane >> 5), valid, qh[s],
+                        ql[QF16 ? 0 : s]);
+    clear();
+  }
+  __device__ __forceinline__ void clear() {
+    m = kPackNoMax;
+    l = 0.f;
 #pragma unroll
-  for (int db = 0; db < DB; db++)
+    for (int db = 0; db < D / 32; db++) o[db] = float16_t{};
+  }
+  __device__ __forceinline__ void write(const PackedArgs& a, const PackedItem& it, int lane) {
+    l += __shfl_xor(l, 32, 64);
+    if (!valid) return;
+    const int kh = lane >> 5;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int i = 0; i < 16; i++) o[db][i] = 0.f;
-  const float qs = a.qscale;
-  const int j16 = lane & 15, dgrp = 16 * ((lane >> 4) & 1);
-
-  for (int t0 = it.kv_lo; t0 < it.kv_hi; t0 += kPackTile) {
-    __syncthreads();
+    for (int db = 0; db < D / 32; db++)
 #pragma unroll
-    for (int i = 0; i < NL; i++) {
-      const int s = i * 256 + tid, p = s / CH, c = s % CH;
-      const int64_t kr = it.k0 + min(t0 + p, it.kv_hi - 1);
-      *(half8_t*)(Ks + pack_k_slot<D>(p, c) * 8) = *(const half8_t*)(a.k + kr * a.k_row + it.kvh * D + c * 8);
-      *(half8_t*)(Vs + pack_v_slot<D>(p, c) * 8) = *(const half8_t*)(a.v + kr * a.v_row + it.kvh * D + c * 8);
-    }
-    __syncthreads();
-    if (t0 > whi) continue;  // no row of this wave sees the tile
-    const bool masked = t0 + kPackTile - 1 > wlo || t0 + kPackTile > it.kv_hi;
-    float16_t sc[2] = {};
+      for (int g = 0; g < 4; g++) {
+        float4_t v = {o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+        const int d = db * 32 + 8 * g + 4 * kh;
+        if (it.part >= 0) {
+          *(float4_t*)(a.part_o + ((int64_t)it.part + r) * D + d) = v;
+          continue;
+        }
+        const int64_t off = (it.q0 + tok) * a.out_row + head * D + d;
 #pragma unroll
-    for (int s = 0; s < KS; s++)
+        for (int e = 0; e < 4; e++) v[e] = l == 0.f ? 0.f : v[e] * inv;
+        if (a.out_form == OUT_F32) {
+          *(float4_t*)((float*)a.out + off) = v;
+          continue;
+        }
+        half4_t hv, lv;
 #pragma unroll
-      for (int pb = 0; pb < 2; pb++) {
-        const half8_t ka = *(const half8_t*)(Ks + pack_k_slot<D>(pb * 32 + l32, 2 * s + kh) * 8);
-        sc[pb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qh[s], sc[pb], 0, 0, 0);
-        if (!QF16) sc[pb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, ql[s], sc[pb], 0, 0, 0);
+        for (int e = 0; e < 4; e++) {
+          hv[e] = (half_t)v[e];
+          lv[e] = (half_t)(v[e] - (float)hv[e]);
+        }
+        *(half4_t*)((half_t*)a.out + off) = hv;
+        if (a.out_form == OUT_X2) *(half4_t*)((half_t*)a.out + a.out_lo + off) = lv;
       }
-    auto visible = [&](int pb, int i) {
-      const int p = t0 + pb * 32 + 8 * (i >> 2) + 4 * kh + (i & 3);
-      return p <= lim && p < it.kv_hi;
-    };
-    if (masked) {
+    if (it.part >= 0 && kh == 0) {
+      a.part_ml[((int64_t)it.part + r) * 2] = m;
+      a.part_ml[((int64_t)it.part + r) * 2 + 1] = l;
+    }
+  }
+};
+
+// S^T = K . Q^T on v_mfma_f32_32x32x16_f16: lane (r, kh) gets row r's scores at keys
+// 32pb + 8(i/4) + 4kh + i%4 of the tile.
+template <int D, bool QF16>
+__device__ __forceinline__ void pack_scores(const PackRows<D, QF16>& w, lds_t K, int at, float16_t (&sc)[2]) {
+  sc[0] = sc[1] = float16_t{};
+#pragma unroll
+  for (int s = 0; s < D / 16; s++)
+#pragma unroll
+    for (int pb = 0; pb < 2; pb++) {
+      const half8_t ka = pack_k_frag(K, (at ^ (32 * s)) + 64 * D * pb);
+      sc[pb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, w.qh[s], sc[pb], 0, 0, 0);
+      if (!QF16) sc[pb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, w.ql[QF16 ? 0 : s], sc[pb], 0, 0, 0);
+    }
+}
+__device__ __forceinline__ bool pack_visible(int t0, int lim, int hi, int kh, int pb, int i) {
+  const int p = t0 + pb * 32 + 8 * (i >> 2) + 4 * kh + (i & 3);
+  return p <= lim && p < hi;
+}
+// The scores of a tile to probabilities: the maximum, the sum, P as f16 (or a pair)
+// where the second product's B operand wants it: its k index 8kh + e of step u is
+// key 16u + (e < 4 ? 4kh + e : 8 + 4kh + e - 4), the lane's own scores 8(u%2) + e.
+template <int D, bool QF16>
+__device__ __forceinline__ void pack_softmax(PackRows<D, QF16>& w, const float16_t (&sc)[2], float qs,
+                                             half8_t (&ph)[4], half8_t (&pl)[QF16 ? 1 : 4]) {
+  float t = -INFINITY;
+#pragma unroll
+  for (int pb = 0; pb < 2; pb++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) t = fmaxf(t, sc[pb][i]);
+  t = fmaxf(t, __shfl_xor(t, 32, 64)) * qs;
+  const bool grow = t > w.m + kPackTop;
+  if (__builtin_amdgcn_ballot_w64(grow)) {  // uniform across the wave
+    const float mnew = grow ? t - kPackLift : w.m;
+    const float alpha = __builtin_amdgcn_exp2f(w.m - mnew);
+    w.l *= alpha;
+#pragma unroll
+    for (int db = 0; db < D / 32; db++) w.o[db] *= alpha;
+    w.m = mnew;
+  }
+#pragma unroll
+  for (int pb = 0; pb < 2; pb++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(sc[pb][i], qs, -w.m));
+      w.l += p;
+      const half_t h = (half_t)p;
+      ph[2 * pb + (i >> 3)][i & 7] = h;
+      if (!QF16) pl[QF16 ? 0 : 2 * pb + (i >> 3)][i & 7] = (half_t)(p - (float)h);
+    }
+}
+// O^T += V^T . P^T.
+template <int D, bool QF16>
+__device__ __forceinline__ void pack_values(PackRows<D, QF16>& w, lds_t V, int at, const half8_t (&ph)[4],
+                                            const half8_t (&pl)[QF16 ? 1 : 4]) {
+#pragma unroll
+  for (int u = 0; u < 4; u++)
+#pragma unroll
+    for (int db = 0; db < D / 32; db++) {
+      const half8_t va = pack_v_frag<D>(V, (at ^ (64 * db)) + 32 * D * u);
+      w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[u], w.o[db], 0, 0, 0);
+      if (!QF16) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[QF16 ? 0 : u], w.o[db], 0, 0, 0);
+    }
+}
+
+// Rows [w0, w0 + 32 blocks) of an item again, for a workgroup that met an infinite
+// or NaN value in a tile some of its rows see only part of: a masked key's
+// probability is 0, but 0 times such a value is not. The products take those
+// values as 0 (the same sums, to the bit, where none is seen); a product of
+// visibility and occurrence then tells which outputs see +inf and which -inf, NaN
+// being both. Rare, and apart from the kernel so that it costs it no registers.
+template <int D, bool QF16>
+__device__ __attribute__((noinline)) void packed_redo(const PackedArgs* ap, int item, int w0, int blocks, lds_t K, lds_t V) {
+  const PackedArgs& a = *ap;
+  const PackedItem it = a.items[item];
+  const int tid = threadIdx.x, lane = tid & 63, kh = lane >> 5;
+  const int kat = pack_k_at<D>(lane & 31, kh), vat = pack_v_at<D>(lane);
+  for (int b = 0; b < blocks; b++) {
+    PackRows<D, QF16> w;
+    w.init(a, it, w0 + 32 * b, lane);
+#pragma unroll 1
+    for (int pass = 0; pass < 3; pass++) {
+      float16_t seen[D / 32];
+#pragma unroll
+      for (int db = 0; db < D / 32; db++) seen[db] = float16_t{};
+#pragma unroll 1
+      for (int t0 = it.kv_lo; t0 < it.kv_hi; t0 += kPackTile) {
+        __syncthreads();
+        for (int i = tid; i < kPackTile * (D / 8); i += blockDim.x) {
+          const int p = i / (D / 8), c = i % (D / 8);
+          const int64_t row = it.k0 + min(t0 + p, it.kv_hi - 1);
+          *(__attribute__((address_space(3))) half8_t*)(K + p * 2 * D + 16 * (c ^ pack_k_swz<D>(p))) =
+              *(const half8_t*)(a.k + row * a.k_row + it.kvh * D + c * 8);
+          *(__attribute__((address_space(3))) half8_t*)(V + p * 2 * D + 16 * (c ^ pack_v_swz<D>(p))) =
+              *(const half8_t*)(a.v + row * a.v_row + it.kvh * D + c * 8);
+        }
+        __syncthreads();
+        half8_t ph[4], pl[QF16 ? 1 : 4];
+        if (pass == 0) {
+          float16_t sc[2];
+          pack_scores<D, QF16>(w, K, kat, sc);
+          bool any = false;
+#pragma unroll
+          for (int pb = 0; pb < 2; pb++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const bool vis = pack_visible(t0, w.lim, it.kv_hi, kh, pb, i);
+              any |= vis;
+              if (!vis) sc[pb][i] = -INFINITY;
+            }
+          if (!__builtin_amdgcn_ballot_w64(any)) continue;  // as the kernel skips it
+          pack_softmax<D, QF16>(w, sc, a.qscale, ph, pl);
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; u++)
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+              ph[u][e] = (half_t)(pack_visible(t0, w.lim, it.kv_hi, kh, u >> 1, (u & 1) * 8 + e) ? 1.f : 0.f);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+          for (int db = 0; db < D / 32; db++) {
+            half8_t va = pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const float f = (float)va[e];
+              if (pass == 0) va[e] = fabsf(f) < INFINITY ? va[e] : (half_t)0.f;
+              else va[e] = (half_t)(f != f || f == (pass == 1 ? INFINITY : -INFINITY) ? 1.f : 0.f);
+            }
+            if (pass == 0) {
+              w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[u], w.o[db], 0, 0, 0);
+              if (!QF16) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[QF16 ? 0 : u], w.o[db], 0, 0, 0);
+            } else {
+              seen[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[u], seen[db], 0, 0, 0);
+            }
+          }
+      }
+#pragma unroll
+      for (int db = 0; db < D / 32; db++)
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+          if (seen[db][i] > 0.f) w.o[db][i] += pass == 1 ? INFINITY : -INFINITY;
+    }
+    w.write(a, it, lane);
+  }
+}
+
+// The workgroup's share of a tile by DMA (global_load_lds_dwordx4): lane i of wave v's
+// instruction n writes the 16-byte slot 64 (WAVES n + v) + i of the tile, and reads
+// the chunk that the swizzle keeps there. `off`: the lane's byte offset from the
+// tile's first row, the same for every n but for whole rows.
+template <int D, int WAVES>
+__device__ __forceinline__ void pack_dma(const char* base, uint32_t off, int64_t row_bytes, lds_t tile, int wave) {
+  constexpr int RPI = 64 * WAVES / (D / 8);  // rows per instruction of the workgroup
+#pragma unroll
+  for (int n = 0; n < kPackTile / RPI; n++)
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void*)(base + n * RPI * row_bytes + off),
+        (__attribute__((address_space(3))) void*)(tile + 1024 * (WAVES * n + wave)), 16, 0, 0);
+}
+// The same where the tile ends behind the item's keys: rows from `rows` on repeat the
+// last one (no row sees them; a value there that is not finite is packed_redo's).
+template <int D, int WAVES>
+__device__ __forceinline__ void pack_dma_end(const char* base, int p, int c, int rows, int64_t row_bytes, lds_t tile, int wave) {
+  constexpr int RPI = 64 * WAVES / (D / 8);
+#pragma unroll
+  for (int n = 0; n < kPackTile / RPI; n++)
+    __builtin_amdgcn_global_load_lds(
+        (const __attribute__((address_space(1))) void*)(base + min(n * RPI + p, rows - 1) * row_bytes + 16 * c),
+        (__attribute__((address_space(3))) void*)(tile + 1024 * (WAVES * n + wave)), 16, 0, 0);
+}
+
+// WAVES waves of 32 rows each; tiles of 64 keys go through two LDS buffers, the next
+// one's DMA in flight while one is used.
+template <int D, bool QF16, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void packed_kernel(PackedArgs a) {
+  __shared__ __attribute__((aligned(1024))) char K0[kPackTile * D * 2], K1[kPackTile * D * 2];
+  __shared__ __attribute__((aligned(1024))) char V0[kPackTile * D * 2], V1[kPackTile * D * 2];
+  const PackedItem it = a.items[blockIdx.x];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kh = lane >> 5, w0 = 32 * wave;
+  PackRows<D, QF16> w;
+  w.init(a, it, w0, lane);
+  // first and last key limit of the wave's rows
+  const int wlo = min((it.r0 + w0) / a.G + it.shift, it.nk - 1);
+  const int whi = w0 < it.nr ? min((it.r0 + min(w0 + 32, it.nr) - 1) / a.G + it.shift, it.nk - 1) : -1;
+  const int kat = pack_k_at<D>(lane & 31, kh), vat = pack_v_at<D>(lane);
+
+  const int p = (64 * wave + lane) / (D / 8), c = lane % (D / 8);
+  const int kc = c ^ pack_k_swz<D>(p), vc = c ^ pack_v_swz<D>(p);
+  const int64_t kb = a.k_row * 2, vb = a.v_row * 2;
+  const uint32_t koff = (uint32_t)(p * kb + 16 * kc), voff = (uint32_t)(p * vb + 16 * vc);
+  const char* kp = (const char*)(a.k + it.k0 * a.k_row + it.kvh * D);
+  const char* vp = (const char*)(a.v + it.k0 * a.v_row + it.kvh * D);
+  auto dma = [&](int t0, lds_t K, lds_t V) {
+    if (t0 + kPackTile <= it.kv_hi) {
+      pack_dma<D, WAVES>(kp + t0 * kb, koff, kb, K, wave);
+      pack_dma<D, WAVES>(vp + t0 * vb, voff, vb, V, wave);
+    } else if (t0 < it.kv_hi) {
+      pack_dma_end<D, WAVES>(kp + t0 * kb, p, kc, it.kv_hi - t0, kb, K, wave);
+      pack_dma_end<D, WAVES>(vp + t0 * vb, p, vc, it.kv_hi - t0, vb, V, wave);
+    }
+  };
+  bool bad = false;
+  auto tile = [&](int t0, lds_t K, lds_t V, lds_t Kn, lds_t Vn) {
+    // this wave's DMA of the tile has landed, every wave's has, and every wave is
+    // done with the other buffer
+    __builtin_amdgcn_s_waitcnt(kPackVm0);
+    pack_barrier();
+    dma(t0 + kPackTile, Kn, Vn);
+    if (t0 > whi) return;  // no row of this wave sees the tile
+    float16_t sc[2];
+    half8_t ph[4], pl[QF16 ? 1 : 4];
+    pack_scores<D, QF16>(w, K, kat, sc);
+    if (t0 + kPackTile - 1 > wlo || t0 + kPackTile > it.kv_hi) {
 #pragma unroll
       for (int pb = 0; pb < 2; pb++)
 #pragma unroll
         for (int i = 0; i < 16; i++)
-          if (!visible(pb, i)) sc[pb][i] = -INFINITY;
-    }
-    float tmax = -INFINITY;
-#pragma unroll
-    for (int pb = 0; pb < 2; pb++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) tmax = fmaxf(tmax, sc[pb][i]);
-    tmax = fmaxf(tmax, __shfl_xor(tmax, 32, 64)) * qs;
-    const bool grow = tmax > m + kPackTop;
-    if (__builtin_amdgcn_ballot_w64(grow)) {
-      const float mnew = grow ? tmax - kPackLift : m;
-      const float alpha = __builtin_amdgcn_exp2f(m - mnew);
-      l *= alpha;
-#pragma unroll
-      for (int db = 0; db < DB; db++) o[db] *= alpha;
-      m = mnew;
-    }
-    half8_t pf[2][2], pl[2][2];
-#pragma unroll
-    for (int pb = 0; pb < 2; pb++)
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(sc[pb][i], qs, -m));
-        l += p;
-        pf[pb][i >> 3][i & 7] = (half_t)p;
-        pl[pb][i >> 3][i & 7] = (half_t)(p - (float)(half_t)p);
-      }
-    bool bad = false;
-    if (masked) {
-#pragma unroll
-      for (int u = 0; u < 4; u++)
-#pragma unroll
-        for (int db = 0; db < DB; db++)
-          bad |= half8_nonfinite(pack_v_frag<D>(Vs, 16 * u + 4 * kh, db * 32 + dgrp, j16));
-    }
-    if (__builtin_amdgcn_ballot_w64(bad)) {
-      // A masked key's probability is 0, but 0 times an infinite or NaN value is
-      // not: the finite values go through the product, and what a row sees of
-      // NaN, +inf and -inf is counted with products of its visibility.
-#pragma unroll
-      for (int u = 0; u < 4; u++)
-#pragma unroll
-        for (int db = 0; db < DB; db++) {
-          half8_t va = pack_v_frag<D>(Vs, 16 * u + 4 * kh, db * 32 + dgrp, j16);
-#pragma unroll
-          for (int e = 0; e < 8; e++) va[e] = __builtin_isfinite((float)va[e]) ? va[e] : (half_t)0.f;
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pf[u >> 1][u & 1], o[db], 0, 0, 0);
-          if (!QF16) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[u >> 1][u & 1], o[db], 0, 0, 0);
-        }
+          if (!pack_visible(t0, w.lim, it.kv_hi, kh, pb, i)) sc[pb][i] = -INFINITY;
 #pragma unroll 1
-      for (int kind = 0; kind < 3; kind++) {
-        const float add = kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
-#pragma unroll
-        for (int db = 0; db < DB; db++) {
-          float16_t seen = {};
-#pragma unroll
-          for (int u = 0; u < 4; u++) {
-            half8_t va = pack_v_frag<D>(Vs, 16 * u + 4 * kh, db * 32 + dgrp, j16), vis;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-              const float f = (float)va[e];
-              va[e] = (half_t)((kind == 0 ? f != f : f == add) ? 1.f : 0.f);
-              vis[e] = (half_t)(visible(u >> 1, (u & 1) * 8 + e) ? 1.f : 0.f);
-            }
-            seen = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, vis, seen, 0, 0, 0);
-          }
-#pragma unroll
-          for (int i = 0; i < 16; i++) o[db][i] += seen[i] > 0.f ? add : 0.f;
-        }
-      }
-    } else {
-#pragma unroll
       for (int u = 0; u < 4; u++)
 #pragma unroll
-        for (int db = 0; db < DB; db++) {
-          const half8_t va = pack_v_frag<D>(Vs, 16 * u + 4 * kh, db * 32 + dgrp, j16);
-          o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pf[u >> 1][u & 1], o[db], 0, 0, 0);
-          if (!QF16) o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[u >> 1][u & 1], o[db], 0, 0, 0);
-        }
+        for (int db = 0; db < D / 32; db++) bad |= half8_nonfinite(pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u));
     }
+    pack_softmax<D, QF16>(w, sc, a.qscale, ph, pl);
+    pack_values<D, QF16>(w, V, vat, ph, pl);
+  };
+  dma(it.kv_lo, (lds_t)K0, (lds_t)V0);
+  for (int t0 = it.kv_lo; t0 < it.kv_hi; t0 += 2 * kPackTile) {
+    tile(t0, (lds_t)K0, (lds_t)V0, (lds_t)K1, (lds_t)V1);
+    if (t0 + kPackTile < it.kv_hi) tile(t0 + kPackTile, (lds_t)K1, (lds_t)V1, (lds_t)K0, (lds_t)V0);
   }
-  l += __shfl_xor(l, 32, 64);
-  if (!valid) return;
-  // Lane (r, kh) holds dims 32db + 8g + 4kh + [0,4) of row r, g = 0..3.
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-#pragma unroll
-  for (int db = 0; db < DB; db++)
-#pragma unroll
-    for (int g = 0; g < 4; g++) {
-      float4_t v = {o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
-      const int d = db * 32 + 8 * g + 4 * kh;
-      if (it.part >= 0) {
-        *(float4_t*)(a.part_o + (int64_t)(it.part + r) * D + d) = v;
-        continue;
-      }
-      const int64_t off = (it.q0 + tok) * a.out_row + head * D + d;
-#pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = inv == 0.f ? 0.f : v[e] * inv;
-      if (a.out_form == OUT_F32) {
-        *(float4_t*)((float*)a.out + off) = v;
-        continue;
-      }
-      half4_t hv, lv;
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        hv[e] = (half_t)v[e];
-        lv[e] = (half_t)(v[e] - (float)hv[e]);
-      }
-      *(half4_t*)((half_t*)a.out + off) = hv;
-      if (a.out_form == OUT_X2) *(half4_t*)((half_t*)a.out + a.out_lo + off) = lv;
-    }
-  if (it.part >= 0 && kh == 0) {
-    a.part_ml[(int64_t)(it.part + r) * 2] = m;
-    a.part_ml[(int64_t)(it.part + r) * 2 + 1] = l;
+  if (__syncthreads_or(bad)) {
+    packed_redo<D, QF16>((const PackedArgs*)__builtin_amdgcn_kernarg_segment_ptr(), blockIdx.x, w0, 1, (lds_t)K0, (lds_t)V0);
+    return;
   }
+  w.write(a, it, lane);
 }
 
 // Merges the parts of up to eight rows: sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p,
@@ -356,8 +516,8 @@ __global__ __launch_bounds__(256) void packed_merge_kernel(PackedArgs a) {
 template <int D>
 static void packed_launch(const PackedArgs& a, int q_f16, int items, int merges, hipStream_t st) {
   if (items) {
-    if (q_f16) hipLaunchKernelGGL((packed_kernel<D, true>), dim3(items), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((packed_kernel<D, false>), dim3(items), dim3(256), 0, st, a);
+    if (q_f16) hipLaunchKernelGGL((packed_kernel<D, true, PW>), dim3(items), dim3(64 * PW), 0, st, a);
+    else hipLaunchKernelGGL((packed_kernel<D, false, PW>), dim3(items), dim3(64 * PW), 0, st, a);
   }
   if (merges) hipLaunchKernelGGL((packed_merge_kernel<D>), dim3(merges), dim3(256), 0, st, a);
 }

@@ -384,15 +384,16 @@ int tgohip_packed_attention(tgohip_ctx* c, int handle, const void* q, int64_t q_
   struct {
     const char* name;
     const void* p;
-    int64_t row, width, rows, unit;
-  } ops[] = {{"q", q, q_row, qw, pl.tq, pl.q_f16 ? 8 : 4},
-             {"k", k, k_row, kw, pl.tk, 8},
-             {"v", v, v_row, kw, pl.tk, 8},
-             {"out", out, out_row, qw, pl.tq, out_dtype == TGOHIP_F32 ? 4 : 8}};
+    int64_t row, width, rows, unit, most;
+  } ops[] = {{"q", q, q_row, qw, pl.tq, pl.q_f16 ? 8 : 4, top},
+             {"k", k, k_row, kw, pl.tk, 8, kPackMaxRow},
+             {"v", v, v_row, kw, pl.tk, 8, kPackMaxRow},
+             {"out", out, out_row, qw, pl.tq, out_dtype == TGOHIP_F32 ? 4 : 8, top}};
   for (auto& o : ops) {
-    if (o.rows > 1 && (o.row < o.width || o.row > top))
+    if (o.rows > 1 && (o.row < o.width || o.row > o.most))
       return fail(TGOHIP_EINVAL, std::string("packed_attention: ") + o.name + " rows are " + std::to_string(o.row) +
-                                     " elements apart and hold " + std::to_string(o.width));
+                                     " elements apart and hold " + std::to_string(o.width) + "; at most " +
+                                     std::to_string(o.most) + " apart");
     if (misaligned(o.p) || (o.rows > 1 && o.row % o.unit))
       return fail(TGOHIP_EINVAL, std::string("packed_attention: ") + o.name + " rows start on 16-byte boundaries");
   }
