@@ -95,6 +95,12 @@ __device__ __forceinline__ void pack_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+// Orders a wave's own LDS writes before its other lanes' reads (and back).
+__device__ __forceinline__ void pack_wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 // A tile of kPackTile keys in LDS: rows of D f16, their 16-byte chunks XOR-swizzled.
 // K's chunks by the row, so that 32 lanes reading one chunk of 32 rows touch
@@ -149,10 +155,7 @@ __device__ __forceinline__ bool half8_nonfinite(half8_t v) {
 }
 
 template <bool QF16>
-__device__ __forceinline__ void pack_load_q(const void* q, int64_t off, bool valid, half8_t& hi, half8_t& lo) {
-#pragma unroll
-  for (int j = 0; j < 8; j++) hi[j] = lo[j] = (half_t)0.f;
-  if (!valid) return;
+__device__ __forceinline__ void pack_load_q(const void* q, int64_t off, half8_t& hi, half8_t& lo) {
   if constexpr (QF16) {
     hi = *(const half8_t*)((const half_t*)q + off);
   } else {
@@ -171,23 +174,19 @@ __device__ __forceinline__ void pack_load_q(const void* q, int64_t off, bool val
 // maximum and (its half of the keys') sum, and of O^T dims 32db + 8g + 4kh + [0,4).
 template <int D, bool QF16>
 struct PackRows {
-  bool valid;
-  int r, tok, head, lim;  // row of the item, its token, query head and last visible key
+  int r, lim;  // row of the item and its last visible key
   half8_t qh[D / 16], ql[QF16 ? 1 : D / 16];
   float m, l;
   float16_t o[D / 32];
 
+  // Rows past the item's repeat its first one; nothing of them is stored.
   __device__ __forceinline__ void init(const PackedArgs& a, const PackedItem& it, int r0, int lane) {
     r = r0 + (lane & 31);
-    valid = r < it.nr;
-    const int row = it.r0 + (valid ? r : 0);
-    tok = row / a.G;
-    head = it.kvh * a.G + row % a.G;
+    const int row = it.r0 + (r < it.nr ? r : 0), tok = row / a.G, head = it.kvh * a.G + row % a.G;
     lim = min(tok + it.shift, it.nk - 1);
 #pragma unroll
     for (int s = 0; s < D / 16; s++)
-      pack_load_q<QF16>(a.q, (it.q0 + tok) * a.q_row + head * D + 16 * s + 8 * (lane >> 5), valid, qh[s],
-                        ql[QF16 ? 0 : s]);
+      pack_load_q<QF16>(a.q, (it.q0 + tok) * a.q_row + head * D + 16 * s + 8 * (lane >> 5), qh[s], ql[QF16 ? 0 : s]);
     clear();
   }
   __device__ __forceinline__ void clear() {
@@ -196,41 +195,66 @@ struct PackRows {
 #pragma unroll
     for (int db = 0; db < D / 32; db++) o[db] = float16_t{};
   }
-  __device__ __forceinline__ void write(const PackedArgs& a, const PackedItem& it, int lane) {
+  // The rows' results, through 128 D bytes of LDS that are the wave's own: a lane
+  // holds four dims of its row at a time, and stores leave in whole rows. Stored as
+  // they lay, 16 bytes of each row per instruction, an item cost 18 us beside 2 us
+  // a tile (8192 items of 128 rows, f16).
+  __device__ __forceinline__ void write(const PackedArgs& a, const PackedItem& it, int lane, lds_t buf) {
+    typedef __attribute__((address_space(3))) float4_t* f4;
     l += __shfl_xor(l, 32, 64);
-    if (!valid) return;
-    const int kh = lane >> 5;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int l32 = lane & 31, kh = lane >> 5;
+    const bool part = it.part >= 0;
+    const float inv = part ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int db = 0; db < D / 32; db++)
 #pragma unroll
       for (int g = 0; g < 4; g++) {
-        float4_t v = {o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
-        const int d = db * 32 + 8 * g + 4 * kh;
-        if (it.part >= 0) {
-          *(float4_t*)(a.part_o + ((int64_t)it.part + r) * D + d) = v;
-          continue;
-        }
-        const int64_t off = (it.q0 + tok) * a.out_row + head * D + d;
+        float4_t v;
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = l == 0.f ? 0.f : v[e] * inv;
-        if (a.out_form == OUT_F32) {
-          *(float4_t*)((float*)a.out + off) = v;
-          continue;
-        }
-        half4_t hv, lv;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          hv[e] = (half_t)v[e];
-          lv[e] = (half_t)(v[e] - (float)hv[e]);
-        }
-        *(half4_t*)((half_t*)a.out + off) = hv;
-        if (a.out_form == OUT_X2) *(half4_t*)((half_t*)a.out + a.out_lo + off) = lv;
+        for (int e = 0; e < 4; e++) v[e] = l == 0.f ? 0.f : o[db][4 * g + e] * inv;
+        const int c = db * 8 + 2 * g + kh;  // chunk of four dims
+        *(f4)(buf + l32 * 4 * D + 16 * (c ^ (l32 & 7))) = v;
       }
-    if (it.part >= 0 && kh == 0) {
+    if (part && kh == 0 && r < it.nr) {
       a.part_ml[((int64_t)it.part + r) * 2] = m;
       a.part_ml[((int64_t)it.part + r) * 2 + 1] = l;
     }
+    pack_wave_sync();
+    const int r0 = r - l32;
+    if (part || a.out_form == OUT_F32) {
+      constexpr int PL = D / 4;  // lanes per row
+#pragma unroll 4
+      for (int i = 0; i < 32 * PL / 64; i++) {
+        const int x = i * (64 / PL) + lane / PL, c = lane % PL;
+        const float4_t v = *(f4)(buf + x * 4 * D + 16 * (c ^ (x & 7)));
+        if (r0 + x >= it.nr) continue;
+        const int row = it.r0 + r0 + x;
+        float* dst = part ? a.part_o + ((int64_t)it.part + r0 + x) * D
+                          : (float*)a.out + (it.q0 + row / a.G) * a.out_row + (it.kvh * a.G + row % a.G) * D;
+        *(float4_t*)(dst + 4 * c) = v;
+      }
+    } else {
+      constexpr int PL = D / 8;
+#pragma unroll 4
+      for (int i = 0; i < 32 * PL / 64; i++) {
+        const int x = i * (64 / PL) + lane / PL, c = lane % PL;
+        const float4_t u = *(f4)(buf + x * 4 * D + 16 * ((2 * c) ^ (x & 7)));
+        const float4_t v = *(f4)(buf + x * 4 * D + 16 * ((2 * c + 1) ^ (x & 7)));
+        if (r0 + x >= it.nr) continue;
+        const int row = it.r0 + r0 + x;
+        half_t* dst = (half_t*)a.out + (it.q0 + row / a.G) * a.out_row + (it.kvh * a.G + row % a.G) * D + 8 * c;
+        half8_t hv, lv;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const float f = e < 4 ? u[e & 3] : v[e & 3];
+          hv[e] = (half_t)f;
+          lv[e] = (half_t)(f - (float)hv[e]);
+        }
+        *(half8_t*)dst = hv;
+        if (a.out_form == OUT_X2) *(half8_t*)(dst + a.out_lo) = lv;
+      }
+    }
+    pack_wave_sync();
   }
 };
 
@@ -305,7 +329,8 @@ __device__ __forceinline__ void pack_values(PackRows<D, QF16>& w, lds_t V, int a
 // visibility and occurrence then tells which outputs see +inf and which -inf, NaN
 // being both. Rare, and apart from the kernel so that it costs it no registers.
 template <int D, bool QF16>
-__device__ __attribute__((noinline)) void packed_redo(const PackedArgs* ap, int item, int w0, int blocks, lds_t K, lds_t V) {
+__device__ __attribute__((noinline)) void packed_redo(const PackedArgs* ap, int item, int w0, int blocks, lds_t K, lds_t V,
+                                                     lds_t buf) {
   const PackedArgs& a = *ap;
   const PackedItem it = a.items[item];
   const int tid = threadIdx.x, lane = tid & 63, kh = lane >> 5;
@@ -377,7 +402,8 @@ __device__ __attribute__((noinline)) void packed_redo(const PackedArgs* ap, int 
         for (int i = 0; i < 16; i++)
           if (seen[db][i] > 0.f) w.o[db][i] += pass == 1 ? INFINITY : -INFINITY;
     }
-    w.write(a, it, lane);
+    __syncthreads();
+    w.write(a, it, lane, buf);
   }
 }
 
@@ -410,13 +436,11 @@ __device__ __forceinline__ void pack_dma_end(const char* base, int p, int c, int
 // one's DMA in flight while one is used.
 template <int D, bool QF16, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void packed_kernel(PackedArgs a) {
-  __shared__ __attribute__((aligned(1024))) char K0[kPackTile * D * 2], K1[kPackTile * D * 2];
-  __shared__ __attribute__((aligned(1024))) char V0[kPackTile * D * 2], V1[kPackTile * D * 2];
+  constexpr int TB = kPackTile * D * 2;  // bytes of a tile
+  __shared__ __attribute__((aligned(1024))) char K0[TB], V0[TB], K1[TB], V1[TB];
   const PackedItem it = a.items[blockIdx.x];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kh = lane >> 5, w0 = 32 * wave;
-  PackRows<D, QF16> w;
-  w.init(a, it, w0, lane);
   // first and last key limit of the wave's rows
   const int wlo = min((it.r0 + w0) / a.G + it.shift, it.nk - 1);
   const int whi = w0 < it.nr ? min((it.r0 + min(w0 + 32, it.nr) - 1) / a.G + it.shift, it.nk - 1) : -1;
@@ -437,6 +461,9 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void packed_kernel(PackedArg
       pack_dma_end<D, WAVES>(vp + t0 * vb, p, vc, it.kv_hi - t0, vb, V, wave);
     }
   };
+  dma(it.kv_lo, (lds_t)K0, (lds_t)V0);
+  PackRows<D, QF16> w;
+  w.init(a, it, w0, lane);
   bool bad = false;
   auto tile = [&](int t0, lds_t K, lds_t V, lds_t Kn, lds_t Vn) {
     // this wave's DMA of the tile has landed, every wave's has, and every wave is
@@ -462,16 +489,19 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void packed_kernel(PackedArg
     pack_softmax<D, QF16>(w, sc, a.qscale, ph, pl);
     pack_values<D, QF16>(w, V, vat, ph, pl);
   };
-  dma(it.kv_lo, (lds_t)K0, (lds_t)V0);
   for (int t0 = it.kv_lo; t0 < it.kv_hi; t0 += 2 * kPackTile) {
     tile(t0, (lds_t)K0, (lds_t)V0, (lds_t)K1, (lds_t)V1);
     if (t0 + kPackTile < it.kv_hi) tile(t0 + kPackTile, (lds_t)K1, (lds_t)V1, (lds_t)K0, (lds_t)V0);
   }
+  // a wave's own 32 rows of f32 in the tiles' place
+  static_assert(4 * TB >= WAVES * 128 * D, "the tiles hold the rows");
+  const int per = TB / (128 * D);
+  lds_t buf = (lds_t)(wave < per ? K0 : wave < 2 * per ? V0 : wave < 3 * per ? K1 : V1) + wave % per * 128 * D;
   if (__syncthreads_or(bad)) {
-    packed_redo<D, QF16>((const PackedArgs*)__builtin_amdgcn_kernarg_segment_ptr(), blockIdx.x, w0, 1, (lds_t)K0, (lds_t)V0);
+    packed_redo<D, QF16>((const PackedArgs*)__builtin_amdgcn_kernarg_segment_ptr(), blockIdx.x, w0, 1, (lds_t)K0, (lds_t)V0, buf);
     return;
   }
-  w.write(a, it, lane);
+  w.write(a, it, lane, buf);
 }
 
 // Merges the parts of up to eight rows: sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p,
