@@ -22,6 +22,7 @@ constexpr int kPackRows = 32 * PW;  // rows per workgroup
 constexpr float kPackNoMax = -1.0e30f;
 constexpr float kPackLift = 7.f;
 constexpr float kPackTop = 15.f;
+constexpr float kPackSum = 32768.f;  // 2^kPackTop
 
 // ---------------------------------------------------------------------------
 // decomposition (host)
@@ -270,56 +271,117 @@ __device__ __forceinline__ void pack_scores(const PackRows<D, QF16>& w, lds_t K,
       const half8_t ka = pack_k_frag(K, (at ^ (32 * s)) + 64 * D * pb);
       sc[pb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, w.qh[s], sc[pb], 0, 0, 0);
       if (!QF16) sc[pb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, w.ql[QF16 ? 0 : s], sc[pb], 0, 0, 0);
+      if (!QF16 && pb && s % 2) __builtin_amdgcn_sched_barrier(0);
     }
 }
-__device__ __forceinline__ bool pack_visible(int t0, int lim, int hi, int kh, int pb, int i) {
-  const int p = t0 + pb * 32 + 8 * (i >> 2) + 4 * kh + (i & 3);
-  return p <= lim && p < hi;
-}
-// The scores of a tile to probabilities: the maximum, the sum, P as f16 (or a pair)
-// where the second product's B operand wants it: its k index 8kh + e of step u is
-// key 16u + (e < 4 ? 4kh + e : 8 + 4kh + e - 4), the lane's own scores 8(u%2) + e.
-template <int D, bool QF16>
-__device__ __forceinline__ void pack_softmax(PackRows<D, QF16>& w, const float16_t (&sc)[2], float qs,
-                                             half8_t (&ph)[4], half8_t (&pl)[QF16 ? 1 : 4]) {
+// Whether the lane's row sees the key of its score (pb, i); left: the row's last
+// visible key, counted from the lane's first of the tile (4kh on).
+__device__ __forceinline__ bool pack_visible(int left, int pb, int i) { return pb * 32 + 8 * (i >> 2) + (i & 3) <= left; }
+// A row's largest score of a tile, scaled.
+__device__ __forceinline__ float pack_top(const float16_t (&sc)[2], float qs) {
+  // one chain: the compiler makes it 16 three-way maxima (of pairs, it quiets every
+  // score first, 32 instructions more)
   float t = -INFINITY;
 #pragma unroll
   for (int pb = 0; pb < 2; pb++)
 #pragma unroll
     for (int i = 0; i < 16; i++) t = fmaxf(t, sc[pb][i]);
-  t = fmaxf(t, __shfl_xor(t, 32, 64)) * qs;
-  const bool grow = t > w.m + kPackTop;
-  if (__builtin_amdgcn_ballot_w64(grow)) {  // uniform across the wave
-    const float mnew = grow ? t - kPackLift : w.m;
-    const float alpha = __builtin_amdgcn_exp2f(w.m - mnew);
-    w.l *= alpha;
-#pragma unroll
-    for (int db = 0; db < D / 32; db++) w.o[db] *= alpha;
-    w.m = mnew;
-  }
-#pragma unroll
-  for (int pb = 0; pb < 2; pb++)
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-      const float p = __builtin_amdgcn_exp2f(fmaf(sc[pb][i], qs, -w.m));
-      w.l += p;
-      const half_t h = (half_t)p;
-      ph[2 * pb + (i >> 3)][i & 7] = h;
-      if (!QF16) pl[QF16 ? 0 : 2 * pb + (i >> 3)][i & 7] = (half_t)(p - (float)h);
-    }
+  return fmaxf(t, __shfl_xor(t, 32, 64)) * qs;
 }
-// O^T += V^T . P^T.
+// Moves the reference maximum of the rows that need it to their tile's largest score
+// t. A row's own scores alone decide: its result does not depend on the rows beside it.
 template <int D, bool QF16>
-__device__ __forceinline__ void pack_values(PackRows<D, QF16>& w, lds_t V, int at, const half8_t (&ph)[4],
-                                            const half8_t (&pl)[QF16 ? 1 : 4]) {
+__device__ __forceinline__ void pack_raise(PackRows<D, QF16>& w, float t, bool need) {
+  const float mnew = need ? t - kPackLift : w.m;
+  const float alpha = __builtin_amdgcn_exp2f(w.m - mnew);
+  w.l *= alpha;
 #pragma unroll
-  for (int u = 0; u < 4; u++)
+  for (int db = 0; db < D / 32; db++) w.o[db] *= alpha;
+  w.m = mnew;
+}
+// Scores 8u .. 8u + 7 of the lane to probabilities, their sum on l, as f16 (or a
+// pair) where the second product's B operand wants them: its k index 8kh + e of
+// step u is key 16u + (e < 4 ? 4kh + e : 8 + 4kh + e - 4), the lane's own score e.
+// f16 probabilities are summed as rounded, two to an instruction, in f32.
+template <bool QF16>
+__device__ __forceinline__ void pack_probs(const float16_t (&sc)[2], int u, float qs, float m, float& l, half8_t& ph,
+                                           half8_t& pl) {
+  typedef float float2_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    float2_t p;
+#pragma unroll
+    for (int g = 0; g < 2; g++) p[g] = __builtin_amdgcn_exp2f(fmaf(sc[u >> 1][8 * (u & 1) + e + g], qs, -m));
+    const half2_t h = __builtin_convertvector(p, half2_t);
+    ph[e] = h[0];
+    ph[e + 1] = h[1];
+    if (QF16) {
+      l = __builtin_amdgcn_fdot2(h, half2_t{(half_t)1.f, (half_t)1.f}, l, false);
+    } else {
+      l += p[0] + p[1];
+      const float2_t r = {fmaf((float)h[0], -1.f, p[0]), fmaf((float)h[1], -1.f, p[1])};
+      const half2_t g = __builtin_convertvector(r, half2_t);
+      pl[e] = g[0];
+      pl[e + 1] = g[1];
+    }
+  }
+}
+// A tile of f16 probabilities. They are taken with the reference maximum as it is
+// and their sum tells whether one may have passed f16 (the row's first tile, or a
+// key far above the ones before): only then is the tile's maximum looked for, and
+// the probabilities taken again. That saves the search, 25 of 165 VALU
+// instructions a tile.
+template <int D>
+__device__ __forceinline__ void pack_probs_f16(PackRows<D, true>& w, const float16_t (&sc)[2], float qs, half8_t (&ph)[4]) {
+  float l[4] = {};
+  half8_t none;
+#pragma unroll
+  for (int u = 0; u < 4; u++) pack_probs<true>(sc, u, qs, w.m, l[u], ph[u], none);
+  const bool over = (l[0] + l[1]) + (l[2] + l[3]) > kPackSum;
+  if (__builtin_amdgcn_ballot_w64(over)) {  // uniform across the wave
+    const bool other = __shfl_xor((int)over, 32, 64);  // the row's other half of the keys
+    pack_raise<D, true>(w, pack_top(sc, qs), over | other);
+#pragma unroll
+    for (int u = 0; u < 4; u++) {
+      l[u] = 0.f;
+      pack_probs<true>(sc, u, qs, w.m, l[u], ph[u], none);
+    }
+  }
+  w.l += (l[0] + l[1]) + (l[2] + l[3]);
+}
+// A tile's maximum, before its pairs of probabilities.
+template <int D>
+__device__ __forceinline__ void pack_maximum(PackRows<D, false>& w, const float16_t (&sc)[2], float qs) {
+  const float t = pack_top(sc, qs);
+  const bool grow = t > w.m + kPackTop;
+  if (__builtin_amdgcn_ballot_w64(grow)) pack_raise<D, false>(w, t, grow);
+}
+// A tile's probabilities and O^T += V^T . P^T. f16 probabilities all come first: the
+// other wave of the SIMD fills the matrix unit meanwhile. Pairs come step by step,
+// or they would not fit the registers beside q's pairs.
+template <int D, bool QF16>
+__device__ __forceinline__ void pack_values(PackRows<D, QF16>& w, const float16_t (&sc)[2], float qs, lds_t V, int at) {
+  half8_t ph[4], pl, first[D / 32];
+  if (QF16) {
+    // the first products' operands come from LDS under the exponentials
+#pragma unroll
+    for (int db = 0; db < D / 32; db++) first[db] = pack_v_frag<D>(V, at ^ (64 * db));
+  }
+  if constexpr (QF16) pack_probs_f16<D>(w, sc, qs, ph);
+  else pack_maximum<D>(w, sc, qs);
+  float l[4] = {};  // a chain of adds per step
+#pragma unroll
+  for (int u = 0; u < 4; u++) {
+    if (!QF16) pack_probs<QF16>(sc, u, qs, w.m, l[u], ph[u], pl);
 #pragma unroll
     for (int db = 0; db < D / 32; db++) {
-      const half8_t va = pack_v_frag<D>(V, (at ^ (64 * db)) + 32 * D * u);
+      const half8_t va = QF16 && u == 0 ? first[db] : pack_v_frag<D>(V, (at ^ (64 * db)) + 32 * D * u);
       w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[u], w.o[db], 0, 0, 0);
-      if (!QF16) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[QF16 ? 0 : u], w.o[db], 0, 0, 0);
+      if (!QF16) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl, w.o[db], 0, 0, 0);
     }
+    if (!QF16) __builtin_amdgcn_sched_barrier(0);
+  }
+  if (!QF16) w.l += (l[0] + l[1]) + (l[2] + l[3]);
 }
 
 // Rows [w0, w0 + 32 blocks) of an item again, for a workgroup that met an infinite
@@ -327,9 +389,9 @@ __device__ __forceinline__ void pack_values(PackRows<D, QF16>& w, lds_t V, int a
 // probability is 0, but 0 times such a value is not. The products take those
 // values as 0 (the same sums, to the bit, where none is seen); a product of
 // visibility and occurrence then tells which outputs see +inf and which -inf, NaN
-// being both. Rare, and apart from the kernel so that it costs it no registers.
+// being both. Rare: a plain loop behind the kernel's own.
 template <int D, bool QF16>
-__device__ __attribute__((noinline)) void packed_redo(const PackedArgs* ap, int item, int w0, int blocks, lds_t K, lds_t V,
+__device__ __forceinline__ void packed_redo(const PackedArgs* ap, int item, int w0, int blocks, lds_t K, lds_t V,
                                                      lds_t buf) {
   const PackedArgs& a = *ap;
   const PackedItem it = a.items[item];
@@ -355,30 +417,35 @@ __device__ __attribute__((noinline)) void packed_redo(const PackedArgs* ap, int 
               *(const half8_t*)(a.v + row * a.v_row + it.kvh * D + c * 8);
         }
         __syncthreads();
-        half8_t ph[4], pl[QF16 ? 1 : 4];
+        float16_t sc[2];
+        half8_t ps[4];
+        const int left = min(w.lim, it.kv_hi - 1) - t0 - 4 * kh;
         if (pass == 0) {
-          float16_t sc[2];
           pack_scores<D, QF16>(w, K, kat, sc);
           bool any = false;
 #pragma unroll
           for (int pb = 0; pb < 2; pb++)
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-              const bool vis = pack_visible(t0, w.lim, it.kv_hi, kh, pb, i);
+              const bool vis = pack_visible(left, pb, i);
               any |= vis;
               if (!vis) sc[pb][i] = -INFINITY;
             }
           if (!__builtin_amdgcn_ballot_w64(any)) continue;  // as the kernel skips it
-          pack_softmax<D, QF16>(w, sc, a.qscale, ph, pl);
-        } else {
+          if constexpr (QF16) pack_probs_f16<D>(w, sc, a.qscale, ps);
+          else pack_maximum<D>(w, sc, a.qscale);
+        }
+        float l[4] = {};
 #pragma unroll
-          for (int u = 0; u < 4; u++)
+        for (int u = 0; u < 4; u++) {
+          half8_t ph = ps[u], pl;
+          if (pass == 0) {
+            if (!QF16) pack_probs<QF16>(sc, u, a.qscale, w.m, l[u], ph, pl);
+          } else {
 #pragma unroll
             for (int e = 0; e < 8; e++)
-              ph[u][e] = (half_t)(pack_visible(t0, w.lim, it.kv_hi, kh, u >> 1, (u & 1) * 8 + e) ? 1.f : 0.f);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; u++)
+              ph[e] = (half_t)(pack_visible(left, u >> 1, (u & 1) * 8 + e) ? 1.f : 0.f);
+          }
 #pragma unroll
           for (int db = 0; db < D / 32; db++) {
             half8_t va = pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u);
@@ -389,12 +456,14 @@ __device__ __attribute__((noinline)) void packed_redo(const PackedArgs* ap, int 
               else va[e] = (half_t)(f != f || f == (pass == 1 ? INFINITY : -INFINITY) ? 1.f : 0.f);
             }
             if (pass == 0) {
-              w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[u], w.o[db], 0, 0, 0);
-              if (!QF16) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[QF16 ? 0 : u], w.o[db], 0, 0, 0);
+              w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, w.o[db], 0, 0, 0);
+              if (!QF16) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl, w.o[db], 0, 0, 0);
             } else {
-              seen[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[u], seen[db], 0, 0, 0);
+              seen[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, seen[db], 0, 0, 0);
             }
           }
+        }
+        w.l += (l[0] + l[1]) + (l[2] + l[3]);
       }
 #pragma unroll
       for (int db = 0; db < D / 32; db++)
@@ -473,21 +542,20 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void packed_kernel(PackedArg
     dma(t0 + kPackTile, Kn, Vn);
     if (t0 > whi) return;  // no row of this wave sees the tile
     float16_t sc[2];
-    half8_t ph[4], pl[QF16 ? 1 : 4];
     pack_scores<D, QF16>(w, K, kat, sc);
     if (t0 + kPackTile - 1 > wlo || t0 + kPackTile > it.kv_hi) {
+      const int left = min(w.lim, it.kv_hi - 1) - t0 - 4 * kh;
 #pragma unroll
       for (int pb = 0; pb < 2; pb++)
 #pragma unroll
         for (int i = 0; i < 16; i++)
-          if (!pack_visible(t0, w.lim, it.kv_hi, kh, pb, i)) sc[pb][i] = -INFINITY;
+          if (!pack_visible(left, pb, i)) sc[pb][i] = -INFINITY;
 #pragma unroll 1
       for (int u = 0; u < 4; u++)
 #pragma unroll
         for (int db = 0; db < D / 32; db++) bad |= half8_nonfinite(pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u));
     }
-    pack_softmax<D, QF16>(w, sc, a.qscale, ph, pl);
-    pack_values<D, QF16>(w, V, vat, ph, pl);
+    pack_values<D, QF16>(w, sc, a.qscale, V, vat);
   };
   for (int t0 = it.kv_lo; t0 < it.kv_hi; t0 += 2 * kPackTile) {
     tile(t0, (lds_t)K0, (lds_t)V0, (lds_t)K1, (lds_t)V1);
