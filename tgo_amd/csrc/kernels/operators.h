@@ -48,7 +48,8 @@ struct PackedMerge {
 struct PackedPlan {
   int H = 0, Hkv = 0, D = 0, q_f16 = 0;
   int64_t tq = 0, tk = 0;  // packed query and key rows
-  std::vector<PackedItem> items;
+  std::vector<PackedItem> items;  // of the tile kernel
+  std::vector<PackedItem> few;    // of the few-row kernel
   std::vector<PackedMerge> merges;
   int64_t part_rows = 0;
 };
@@ -70,7 +71,11 @@ struct PackedArgs {
   int G, out_form;                               // OUT_F32, OUT_F16, OUT_X2 (lo plane out_lo on)
   float qscale;                                  // scale * log2(e)
 };
-int packed_enqueue(const PackedArgs& a, int D, int q_f16, int items, int merges, hipStream_t st);
+// a.items: the tile kernel's, then the few-row kernel's.
+struct PackedCounts {
+  int items = 0, few = 0, merges = 0;
+};
+int packed_enqueue(const PackedArgs& a, int D, int q_f16, const PackedCounts& n, hipStream_t st);
 
 // ---- adapters (adapters.hip) --------------------------------------------------
 constexpr int kAdapterMaxRank = 128;

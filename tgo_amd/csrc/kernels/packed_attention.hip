@@ -10,10 +10,11 @@
 namespace tgohip {
 
 constexpr int kPackTile = 64;   // keys staged in LDS per iteration
-#ifndef PW
-#define PW 4
-#endif
-constexpr int kPackRows = 32 * PW;  // rows per workgroup
+constexpr int kPackFew = 32;    // rows of a sequence and kv head up to which packed_few_kernel takes them
+constexpr int kFewTile = 32;    // keys of a wave's tile there
+constexpr int kFewWaves = 2;
+constexpr int kPackWaves = 4;
+constexpr int kPackRows = 32 * kPackWaves;  // rows of an item of packed_kernel
 // Online softmax with a lazy reference m (log2 units): it starts at kPackNoMax, a
 // row's probabilities are 2^(s - m), and m moves to the row's maximum - kPackLift
 // once that passes m + kPackTop. They so stay below 2^kPackTop (f16 ends at 2^16),
@@ -28,6 +29,61 @@ constexpr float kPackSum = 32768.f;  // 2^kPackTop
 // decomposition (host)
 // ---------------------------------------------------------------------------
 
+// Orders items longest first, so that the hardware's dispatch, block by block, ends
+// evenly on `slots` workgroups at a time. Where one item is longer than a quarter
+// over a slot's share, items are cut: they fill one slot's share after the other, a
+// piece ending where a share does, at least `least` tiles long. A piece costs `fixed`
+// tiles beside its own (its start, its result and their merge).
+static void pack_cut(const std::vector<PackedItem>& whole, int tile, int slots, int fixed, int least,
+                     std::vector<PackedItem>& out, PackedPlan& plan) {
+  int64_t total = 0;
+  int longest = 0;
+  for (const PackedItem& it : whole) {
+    const int t = (it.kv_hi + tile - 1) / tile;
+    total += t + fixed;
+    longest = std::max(longest, t + fixed);
+  }
+  const int64_t share = std::max<int64_t>((total + slots - 1) / slots, least + fixed);
+  if (4 * longest <= 5 * share) {
+    out = whole;
+  } else {
+    // the pieces' own fixed costs, about one more per slot
+    const int64_t room = share + (share > least + fixed ? fixed : 0);
+    int64_t left = room;
+    for (PackedItem it : whole) {
+      const int tiles = (it.kv_hi + tile - 1) / tile, hi = it.kv_hi;
+      std::vector<int> ends;
+      for (int at = 0; at < tiles;) {
+        if (left < least + fixed) left = room;
+        int take = (int)std::min<int64_t>(tiles - at, left - fixed);
+        if (tiles - at - take < least) take = tiles - at;
+        at += take;
+        left -= take + fixed;
+        ends.push_back(at);
+      }
+      if (ends.size() <= 1) {
+        out.push_back(it);
+        continue;
+      }
+      const int parts = (int)ends.size();
+      for (int p = 0; p < parts; p++) {
+        it.kv_lo = p ? ends[p - 1] * tile : 0;
+        it.kv_hi = std::min(hi, ends[p] * tile);
+        it.part = (int32_t)(plan.part_rows + (int64_t)p * it.nr);
+        out.push_back(it);
+      }
+      // rows of a merge: few where there are many parts, whose rows then share its threads
+      const int rows = parts > 16 ? 1 : parts > 4 ? 2 : 8;
+      for (int i = 0; i < it.nr; i += rows)
+        plan.merges.push_back(PackedMerge{it.q0, it.r0 + i, std::min(rows, it.nr - i), it.kvh,
+                                          (int32_t)plan.part_rows + i, parts, it.nr});
+      plan.part_rows += (int64_t)parts * it.nr;
+    }
+  }
+  std::stable_sort(out.begin(), out.end(),
+                   [](const PackedItem& a, const PackedItem& b) { return a.kv_hi - a.kv_lo > b.kv_hi - b.kv_lo; });
+}
+
 void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int Hkv, int D, bool causal,
                        bool q_f16, int ncu, PackedPlan& plan) {
   plan = PackedPlan();
@@ -36,8 +92,16 @@ void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int H
   plan.D = D;
   plan.q_f16 = q_f16;
   const int G = H / Hkv;
-  std::vector<PackedItem> base;
-  double total = 0;
+  // Sequences of up to kPackFew rows per kv head go to the few-row kernel where they
+  // hold most of the keys; beside longer prompts they are not worth a launch of their
+  // own (16 prompts, two of a few tokens: 70 us, 77 with it).
+  int64_t few_keys = 0, keys = 0;
+  for (int s = 0; s < B; s++) {
+    keys += nk[s];
+    if ((int64_t)nq[s] * G <= kPackFew) few_keys += nk[s];
+  }
+  const int64_t few_rows = 2 * few_keys > keys ? kPackFew : 0;
+  std::vector<PackedItem> whole[2];  // tiles of rows, few rows
   int64_t q0 = 0, k0 = 0;
   for (int s = 0; s < B; s++) {
     const int64_t rows = (int64_t)nq[s] * G;
@@ -46,41 +110,16 @@ void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int H
       const int nr = (int)std::min<int64_t>(kPackRows, rows - r0);
       const int64_t last = (r0 + nr - 1) / G;
       const int hi = (int)std::max<int64_t>(0, std::min<int64_t>(nk[s], last + shift + 1));
-      for (int h = 0; h < Hkv; h++) {
-        base.push_back(PackedItem{(int32_t)q0, (int32_t)k0, nk[s], shift, (int32_t)r0, nr, 0, hi, h, -1});
-        total += hi;
-      }
+      for (int h = 0; h < Hkv; h++)
+        whole[rows <= few_rows].push_back(PackedItem{(int32_t)q0, (int32_t)k0, nk[s], shift, (int32_t)r0, nr, 0, hi, h, -1});
     }
     q0 += nq[s];
     k0 += nk[s];
   }
   plan.tq = q0;
   plan.tk = k0;
-  // Parts long enough that every workgroup slot gets about one.
-  const double slots = 8.0 / PW * ncu;
-  const int part = std::max(512, (int)std::min(1.0e9, total / slots + kPackTile) / kPackTile * kPackTile);
-  for (PackedItem it : base) {
-    const int parts = (it.kv_hi + part - 1) / part;
-    if (parts <= 1) {
-      plan.items.push_back(it);
-      continue;
-    }
-    const int tiles = (it.kv_hi + kPackTile - 1) / kPackTile;
-    const int hi = it.kv_hi;
-    for (int p = 0; p < parts; p++) {
-      it.kv_lo = (int)((int64_t)tiles * p / parts) * kPackTile;
-      it.kv_hi = std::min(hi, (int)((int64_t)tiles * (p + 1) / parts) * kPackTile);
-      it.part = (int32_t)(plan.part_rows + (int64_t)p * it.nr);
-      plan.items.push_back(it);
-    }
-    for (int i = 0; i < it.nr; i += 8)
-      plan.merges.push_back(PackedMerge{it.q0, it.r0 + i, std::min(8, it.nr - i), it.kvh,
-                                        (int32_t)plan.part_rows + i, parts, it.nr});
-    plan.part_rows += (int64_t)parts * it.nr;
-  }
-  std::stable_sort(plan.items.begin(), plan.items.end(), [](const PackedItem& a, const PackedItem& b) {
-    return a.kv_hi - a.kv_lo > b.kv_hi - b.kv_lo;
-  });
+  pack_cut(whole[0], kPackTile, 2 * ncu, 3, 4, plan.items, plan);
+  pack_cut(whole[1], kFewTile * kFewWaves, 2 * ncu, 3, 2, plan.few, plan);
 }
 
 // ---------------------------------------------------------------------------
@@ -504,7 +543,7 @@ __device__ __forceinline__ void pack_dma_end(const char* base, int p, int c, int
 // WAVES waves of 32 rows each; tiles of 64 keys go through two LDS buffers, the next
 // one's DMA in flight while one is used.
 template <int D, bool QF16, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void packed_kernel(PackedArgs a) {
+__global__ __launch_bounds__(64 * WAVES, 2) void packed_kernel(PackedArgs a) {
   constexpr int TB = kPackTile * D * 2;  // bytes of a tile
   __shared__ __attribute__((aligned(1024))) char K0[TB], V0[TB], K1[TB], V1[TB];
   const PackedItem it = a.items[blockIdx.x];
@@ -572,27 +611,247 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void packed_kernel(PackedArg
   w.write(a, it, lane, buf);
 }
 
-// Merges the parts of up to eight rows: sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p,
-// four dims per thread.
+constexpr int kNonTemporal = 2;  // the nt bit: keys of few rows are read once
+
+// Items of up to 32 rows (single tokens, a few of them): bound by the bytes of their
+// keys. Two waves take tiles of 32 keys in turn, each through two LDS buffers of its
+// own, so that nothing but its own DMA holds a wave up; their results meet in LDS.
+// 64 KiB and two waves a workgroup, two workgroups a CU: at any time about 64 KiB of
+// K and V are on their way to each CU, and one workgroup's start and end lie under
+// the other's stream.
+template <int D, bool QF16>
+__global__ __launch_bounds__(64 * kFewWaves, 1) void packed_few_kernel(PackedArgs a) {
+  constexpr int TB = kFewTile * D * 2, CH = D / 8, RPI = 64 / CH, NI = kFewTile / RPI;
+  __shared__ __attribute__((aligned(1024))) char K0[kFewWaves * TB], V0[kFewWaves * TB];
+  __shared__ __attribute__((aligned(1024))) char K1[kFewWaves * TB], V1[kFewWaves * TB];
+  const PackedItem it = a.items[blockIdx.x];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kh = lane >> 5;
+  const int kat = pack_k_at<D>(lane & 31, kh), vat = pack_v_at<D>(lane);
+  const lds_t Kw[2] = {(lds_t)K0 + wave * TB, (lds_t)K1 + wave * TB}, Vw[2] = {(lds_t)V0 + wave * TB, (lds_t)V1 + wave * TB};
+
+  const int p = lane / CH, c = lane % CH;
+  const int64_t kb = a.k_row * 2, vb = a.v_row * 2;
+  const char* kp = (const char*)(a.k + it.k0 * a.k_row + it.kvh * D);
+  const char* vp = (const char*)(a.v + it.k0 * a.v_row + it.kvh * D);
+  // Rows past the item's keys repeat its last one.
+  auto dma = [&](int t0, lds_t K, lds_t V) {
+    if (t0 >= it.kv_hi) return;
+    const int rows = it.kv_hi - t0;
+#pragma unroll
+    for (int n = 0; n < NI; n++) {
+      const int r = n * RPI + p, x = min(r, rows - 1);
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(kp + (t0 + x) * kb + 16 * (c ^ pack_k_swz<D>(r))),
+          (__attribute__((address_space(3))) void*)(K + 1024 * n), 16, 0, kNonTemporal);
+    }
+#pragma unroll
+    for (int n = 0; n < NI; n++) {
+      const int r = n * RPI + p, x = min(r, rows - 1);
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(vp + (t0 + x) * vb + 16 * (c ^ pack_v_swz<D>(r))),
+          (__attribute__((address_space(3))) void*)(V + 1024 * n), 16, 0, kNonTemporal);
+    }
+  };
+  const int first = it.kv_lo + wave * kFewTile, step = kFewWaves * kFewTile;
+  dma(first, Kw[0], Vw[0]);
+  PackRows<D, QF16> w;
+  w.init(a, it, 0, lane);
+  const int wlo = min(it.r0 / a.G + it.shift, it.nk - 1);
+  const int whi = min((it.r0 + it.nr - 1) / a.G + it.shift, it.nk - 1);
+
+  // MODE 0: the attention. Where a masked tile holds a value that is not finite, the
+  // keys run again as packed_redo does: MODE 1 with such values as 0, then 2 and 3
+  // for what the rows see of +inf and -inf.
+  bool bad = false;
+  float16_t seen[D / 32];
+  auto run = [&](auto mode) {
+    constexpr int MODE = decltype(mode)::value;
+    auto tile = [&](int t0, lds_t K, lds_t V, lds_t Kn, lds_t Vn) {
+      __builtin_amdgcn_s_waitcnt(kPackVm0);
+      asm volatile("" ::: "memory");
+      dma(t0 + step, Kn, Vn);
+      if (t0 > whi) return;
+      const int left = min(w.lim, it.kv_hi - 1) - t0 - 4 * kh;
+      const bool masked = t0 + kFewTile - 1 > wlo || t0 + kFewTile > it.kv_hi;
+      half8_t ph[2], pl[2];
+      if constexpr (MODE < 2) {
+        float16_t sc[2] = {};
+#pragma unroll
+        for (int s = 0; s < D / 16; s++) {
+          const half8_t ka = pack_k_frag(K, kat ^ (32 * s));
+          sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, w.qh[s], sc[0], 0, 0, 0);
+          if (!QF16) sc[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, w.ql[QF16 ? 0 : s], sc[0], 0, 0, 0);
+        }
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            if (!pack_visible(left, 0, i)) sc[0][i] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) sc[1][i] = -INFINITY;
+        const float t = pack_top(sc, a.qscale);
+        const bool grow = t > w.m + kPackTop;
+        if (__builtin_amdgcn_ballot_w64(grow)) pack_raise<D, QF16>(w, t, grow);
+        float l[2] = {};
+#pragma unroll
+        for (int u = 0; u < 2; u++) pack_probs<QF16>(sc, u, a.qscale, w.m, l[u], ph[u], pl[u]);
+        w.l += l[0] + l[1];
+      } else {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) ph[u][e] = (half_t)(pack_visible(left, 0, u * 8 + e) ? 1.f : 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int db = 0; db < D / 32; db++) {
+          half8_t va = pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u);
+          if constexpr (MODE == 0) {
+            if (masked) bad |= half8_nonfinite(va);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const float f = (float)va[e];
+              if (MODE == 1) va[e] = fabsf(f) < INFINITY ? va[e] : (half_t)0.f;
+              else va[e] = (half_t)(f != f || f == (MODE == 2 ? INFINITY : -INFINITY) ? 1.f : 0.f);
+            }
+          }
+          if constexpr (MODE < 2) {
+            w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[u], w.o[db], 0, 0, 0);
+            if (!QF16) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl[u], w.o[db], 0, 0, 0);
+          } else {
+            seen[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph[u], seen[db], 0, 0, 0);
+          }
+        }
+    };
+    if (MODE != 0) dma(first, Kw[0], Vw[0]);
+    for (int t0 = first; t0 < it.kv_hi; t0 += 2 * step) {
+      tile(t0, Kw[0], Vw[0], Kw[1], Vw[1]);
+      if (t0 + step < it.kv_hi) tile(t0 + step, Kw[1], Vw[1], Kw[0], Vw[0]);
+    }
+  };
+  run(std::integral_constant<int, 0>{});
+  if (__syncthreads_or(bad)) {
+    w.clear();
+    run(std::integral_constant<int, 1>{});
+    auto add = [&](float v) {
+#pragma unroll
+      for (int db = 0; db < D / 32; db++)
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+          if (seen[db][i] > 0.f) w.o[db][i] += v;
+    };
+    auto none = [&] {
+#pragma unroll
+      for (int db = 0; db < D / 32; db++) seen[db] = float16_t{};
+    };
+    none();
+    run(std::integral_constant<int, 2>{});
+    add(INFINITY);
+    none();
+    run(std::integral_constant<int, 3>{});
+    add(-INFINITY);
+    __syncthreads();
+  }
+  // The second wave's rows to the first one's maximum, through LDS.
+  static_assert(kFewWaves == 2 && 2 * TB >= 128 * D, "a buffer holds a wave's rows");
+  typedef __attribute__((address_space(3))) float16_t* f16p;
+  typedef __attribute__((address_space(3))) float* fp;
+  if (wave == 1) {
+#pragma unroll
+    for (int db = 0; db < D / 32; db++) *(f16p)((lds_t)K0 + (db * 64 + lane) * 64) = w.o[db];
+    *(fp)((lds_t)V0 + lane * 8) = w.m;
+    *(fp)((lds_t)V0 + lane * 8 + 4) = w.l;
+  }
+  __syncthreads();
+  if (wave == 1) return;
+  const float m1 = *(fp)((lds_t)V0 + lane * 8), l1 = *(fp)((lds_t)V0 + lane * 8 + 4);
+  const float m = fmaxf(w.m, m1);
+  const float x0 = __builtin_amdgcn_exp2f(w.m - m), x1 = __builtin_amdgcn_exp2f(m1 - m);
+  w.l = x0 * w.l + x1 * l1;
+  w.m = m;
+#pragma unroll
+  for (int db = 0; db < D / 32; db++) {
+    const float16_t o1 = *(f16p)((lds_t)K0 + (db * 64 + lane) * 64);
+#pragma unroll
+    for (int i = 0; i < 16; i++) w.o[db][i] = x0 * w.o[db][i] + x1 * o1[i];
+  }
+  w.write(a, it, lane, (lds_t)K1);
+}
+
+// Merges the parts of up to eight rows: sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p.
+// D / 4 lanes hold a row, four dims each; with fewer rows the lane groups share a
+// row's parts and meet in LDS, in their order.
 template <int D>
 __global__ __launch_bounds__(256) void packed_merge_kernel(PackedArgs a) {
+  constexpr int LR = D / 4, GR = 256 / LR;  // lanes per row, groups of them
+  __shared__ float4_t so[GR][LR];
+  __shared__ float sl[GR], sm[GR];
   const PackedMerge g = a.merges[blockIdx.x];
-  const int i = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
-  if (i >= g.nr) return;
-  float M = kPackNoMax;
-  for (int p = 0; p < g.parts; p++) M = fmaxf(M, a.part_ml[((int64_t)g.part + i + (int64_t)p * g.step) * 2]);
+  const int grp = threadIdx.x / LR, d = threadIdx.x % LR * 4;
+  const int slices = GR / (g.nr > 4 ? 8 : g.nr > 2 ? 4 : g.nr), i = grp / slices, sl0 = grp % slices;
   float4_t v = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
-  for (int p = 0; p < g.parts; p++) {
-    const int64_t pr = (int64_t)g.part + i + (int64_t)p * g.step;
-    const float lp = a.part_ml[pr * 2 + 1];
-    if (lp == 0.f) continue;  // the part shows this row no key
-    const float w = __builtin_amdgcn_exp2f(a.part_ml[pr * 2] - M);
-    l += w * lp;
-    const float4_t po = *(const float4_t*)(a.part_o + pr * D + d);
+  float l = 0.f, m = kPackNoMax;
+  if (i < g.nr) {
+    // eight parts' loads in flight, the reference maximum moving with them
+    float M = kPackNoMax;
+    for (int p0 = sl0; p0 < g.parts; p0 += 8 * slices) {
+      float2 ml[8];
+      float4_t po[8];
 #pragma unroll
-    for (int e = 0; e < 4; e++) v[e] += w * po[e];
+      for (int u = 0; u < 8; u++) {
+        const int p = min(p0 + u * slices, g.parts - 1);
+        const int64_t pr = (int64_t)g.part + i + (int64_t)p * g.step;
+        ml[u] = *(const float2*)(a.part_ml + pr * 2);
+        po[u] = *(const float4_t*)(a.part_o + pr * D + d);
+      }
+      float top = M;
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        if (p0 + u * slices >= g.parts) ml[u].y = 0.f;
+        if (ml[u].y != 0.f) top = fmaxf(top, ml[u].x);  // 0: the part shows this row no key
+      }
+      const float old = __builtin_amdgcn_exp2f(M - top);
+      M = top;
+      l *= old;
+      v *= old;
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        if (ml[u].y == 0.f) continue;
+        const float w = __builtin_amdgcn_exp2f(ml[u].x - M);
+        l += w * ml[u].y;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] += w * po[u][e];
+      }
+    }
+    m = M;
   }
+  if (slices > 1) {
+    so[grp][d / 4] = v;
+    if (d == 0) {
+      sl[grp] = l;
+      sm[grp] = m;
+    }
+    __syncthreads();
+    if (sl0 == 0) {
+      float top = m;
+      for (int s = 1; s < slices; s++)
+        if (sl[grp + s] != 0.f) top = fmaxf(top, sm[grp + s]);
+      float w = __builtin_amdgcn_exp2f(m - top);
+      l *= w;
+      v *= w;
+      for (int s = 1; s < slices; s++) {
+        if (sl[grp + s] == 0.f) continue;
+        w = __builtin_amdgcn_exp2f(sm[grp + s] - top);
+        l += w * sl[grp + s];
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] += w * so[grp + s][d / 4][e];
+      }
+    }
+  }
+  if (i >= g.nr || sl0) return;
   const int row = g.r0 + i, tok = row / a.G, head = g.kvh * a.G + row % a.G;
   const int64_t off = (g.q0 + tok) * a.out_row + head * D + d;
 #pragma unroll
@@ -611,18 +870,17 @@ __global__ __launch_bounds__(256) void packed_merge_kernel(PackedArgs a) {
   if (a.out_form == OUT_X2) *(half4_t*)((half_t*)a.out + a.out_lo + off) = lv;
 }
 
-template <int D>
-static void packed_launch(const PackedArgs& a, int q_f16, int items, int merges, hipStream_t st) {
-  if (items) {
-    if (q_f16) hipLaunchKernelGGL((packed_kernel<D, true, PW>), dim3(items), dim3(64 * PW), 0, st, a);
-    else hipLaunchKernelGGL((packed_kernel<D, false, PW>), dim3(items), dim3(64 * PW), 0, st, a);
-  }
-  if (merges) hipLaunchKernelGGL((packed_merge_kernel<D>), dim3(merges), dim3(256), 0, st, a);
+template <int D, bool QF16>
+static void packed_launch(PackedArgs a, const PackedCounts& n, hipStream_t st) {
+  if (n.items) hipLaunchKernelGGL((packed_kernel<D, QF16, kPackWaves>), dim3(n.items), dim3(64 * kPackWaves), 0, st, a);
+  a.items += n.items;
+  if (n.few) hipLaunchKernelGGL((packed_few_kernel<D, QF16>), dim3(n.few), dim3(64 * kFewWaves), 0, st, a);
+  if (n.merges) hipLaunchKernelGGL((packed_merge_kernel<D>), dim3(n.merges), dim3(256), 0, st, a);
 }
 
-int packed_enqueue(const PackedArgs& a, int D, int q_f16, int items, int merges, hipStream_t st) {
-  if (D == 128) packed_launch<128>(a, q_f16, items, merges, st);
-  else packed_launch<64>(a, q_f16, items, merges, st);
+int packed_enqueue(const PackedArgs& a, int D, int q_f16, const PackedCounts& n, hipStream_t st) {
+  if (D == 128) q_f16 ? packed_launch<128, true>(a, n, st) : packed_launch<128, false>(a, n, st);
+  else q_f16 ? packed_launch<64, true>(a, n, st) : packed_launch<64, false>(a, n, st);
   TGOHIP_HIP(hipGetLastError());
   return 0;
 }

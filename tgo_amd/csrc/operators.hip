@@ -322,13 +322,15 @@ int tgohip_packed_plan(tgohip_ctx* c, int B, const int32_t* q_lengths, const int
     OnDevice on(c->device);
     PackedPlan plan;
     packed_build_plan(B, q_lengths, kv_lengths, H, H_kv, head_dim, causal != 0, q_dtype == TGOHIP_F16, c->ncu, plan);
+    const size_t items = plan.items.size();
+    plan.items.insert(plan.items.end(), plan.few.begin(), plan.few.end());
     if (plan.part_rows > INT_MAX || plan.items.size() > (size_t)INT_MAX / 256 || plan.merges.size() > (size_t)INT_MAX / 256)
       return fail(TGOHIP_EINVAL, "packed_plan: the batch needs " + std::to_string(plan.items.size()) +
                                      " workgroups, more than one launch takes");
     const bool fresh = *handle == 0;
     const int h = fresh ? c->ops.next++ : *handle;
     PackedHandle& p = c->ops.packed[h];
-    p.items = p.merges = 0;
+    p.n = PackedCounts{};
     p.plan = PackedPlan();
     Stager sg;
     sg.add(plan.items.data(), plan.items.size() * sizeof(PackedItem));
@@ -343,10 +345,10 @@ int tgohip_packed_plan(tgohip_ctx* c, int B, const int32_t* q_lengths, const int
       }
       return rc;
     }
-    p.items = (int)plan.items.size();
-    p.merges = (int)plan.merges.size();
+    p.n = PackedCounts{(int)items, (int)plan.few.size(), (int)plan.merges.size()};
     p.merges_off = off;
     plan.items.clear();
+    plan.few.clear();
     plan.merges.clear();
     p.plan = plan;
     *handle = h;
@@ -425,7 +427,7 @@ int tgohip_packed_attention(tgohip_ctx* c, int handle, const void* q, int64_t q_
   a.out_form = out_dtype == TGOHIP_F32 ? OUT_F32 : out_dtype == TGOHIP_F16 ? OUT_F16 : OUT_X2;
   a.qscale = scale * 1.4426950408889634f;
   OnDevice on(c->device);
-  return packed_enqueue(a, pl.D, pl.q_f16, p->items, p->merges, c->stream);
+  return packed_enqueue(a, pl.D, pl.q_f16, p->n, c->stream);
 }
 
 // ---- adapters ---------------------------------------------------------------------

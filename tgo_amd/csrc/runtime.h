@@ -82,7 +82,7 @@ struct RopeTable {
 // A batch's decomposition on the device, and the partial results of its calls.
 struct PackedHandle {
   PackedPlan plan;  // its vectors empty: they are in meta
-  int items = 0, merges = 0;
+  PackedCounts n;
   size_t merges_off = 0;
   DevBuf meta, part;
 };
