@@ -128,6 +128,22 @@ def test_rope_strides_orders_and_alignments(ctx, torch_gpu, layout):
         ctx.rope_free(h)
 
 
+@pytest.mark.parametrize("T,heads", [(20000, 1), (3000, 3), (2, 65536), (5000, 13)])
+def test_rope_heads_and_rows_of_a_workgroup(ctx, torch_gpu, T, heads):
+    torch = torch_gpu
+    d = 8 if heads > 1000 else 64
+    h = ctx.rope_new(d, 1e4, layout=tgo_amd.ROPE_HALF)
+    try:
+        w, m = tgo_amd.rope_freqs(d, 1e4)
+        x = torch.randn(T, heads, d, device="cuda").half()
+        pos = torch.randint(0, 100000, (T,), device="cuda", dtype=torch.int32)
+        y = torch.full_like(x, float("nan"))
+        ctx.rope(h, pos, [(x, y)])
+        check_rope(torch, y, x, pos, d, tgo_amd.ROPE_HALF, w, m)
+    finally:
+        ctx.rope_free(h)
+
+
 def test_rope_far_positions(ctx, torch_gpu):
     torch = torch_gpu
     pos = torch.tensor([0, 1, -1, 2 ** 31 - 1, -2 ** 31, 131071, 10 ** 9], dtype=torch.int32, device="cuda")

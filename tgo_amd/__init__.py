@@ -8,6 +8,7 @@ unbuilt library raises -- there is no CPU fallback.
 """
 import ctypes
 import os
+import struct
 
 import numpy as np
 
@@ -121,7 +122,7 @@ def lib():
         "tgohip_rope_freqs": (I, [ctypes.POINTER(RopeCfg), P, P]),
         "tgohip_rope_new": (I, [P, ctypes.POINTER(RopeCfg), P]),
         "tgohip_rope_free": (I, [P, I]),
-        "tgohip_rope": (I, [P, I, P, I, ctypes.POINTER(RopeHeads), I]),
+        "tgohip_rope": (I, [P, I, P, I, P, I]),
         "tgohip_packed_plan": (I, [P, I, P, P, I, I, I, I, I, P]),
         "tgohip_packed_free": (I, [P, I]),
         "tgohip_packed_attention": (I, [P, I, P, I64, P, I64, P, I64, F, P, I64, I]),
@@ -219,6 +220,14 @@ def ptr(a):
     return ctypes.c_void_p(a.data_ptr())
 
 
+def _addr(t):
+    """A contiguous device tensor's address (or None)."""
+    if t is None:
+        return None
+    assert t.is_contiguous(), "tensors passed to the C ABI are contiguous"
+    return t.data_ptr()
+
+
 def u32(a):
     return np.ascontiguousarray(np.asarray(a, dtype=np.uint32))
 
@@ -304,24 +313,40 @@ def rope_freqs(*args, **kw):
     return w, m.value
 
 
+_KINDS = {}  # a torch dtype's code: F32, F16, or None for one the operators do not take
+
+
+def _kind(t):
+    k = _KINDS.get(t.dtype, -1)
+    if k == -1:
+        k = _KINDS[t.dtype] = {"torch.float32": F32, "torch.float16": F16}.get(str(t.dtype))
+    return k
+
+
 def _heads_view(t, what):
     """(address, row stride, head stride, dtype code) of a device tensor [rows, heads, head_dim]."""
-    if t.dim() != 3 or (t.shape[2] > 1 and t.stride(2) != 1):
+    s = t.stride()
+    if len(s) != 3 or (s[2] != 1 and t.shape[2] > 1):
         raise TgoError(EINVAL, "%s is a [rows, heads, head_dim] tensor with dense head rows" % what)
-    kind = {"torch.float32": F32, "torch.float16": F16}.get(str(t.dtype))
+    kind = _kind(t)
     if kind is None:
         raise TgoError(EINVAL, "%s is %s; float32 or float16" % (what, t.dtype))
-    return t.data_ptr(), t.stride(0), t.stride(1), kind
+    return t.data_ptr(), s[0], s[1], kind
 
 
 def _packed_rows(t, what, rows, heads, d, kind):
-    """(address, row stride) of a packed operand [rows, heads, d] whose heads are dense."""
+    """(address, row stride, dtype code) of a packed operand [rows, heads, d] whose heads are dense."""
     at, row, head, dt = _heads_view(t, what)
     if tuple(t.shape) != (rows, heads, d) or (heads > 1 and head != d):
         raise TgoError(EINVAL, "%s is [%d, %d, %d] with dense heads" % (what, rows, heads, d))
     if kind is not None and dt != kind:
         raise TgoError(EINVAL, "%s is %s" % (what, "float16" if kind == F16 else "float32"))
-    return ctypes.c_void_p(at), row, dt
+    return at, row, dt
+
+
+_INT32 = {}  # the int32 dtype, once met
+# tgohip_rope_heads, one to three of them
+_ROPE_HEADS = [struct.Struct("=" + n * "QQqqqqiiii") for n in range(4)]
 
 
 def sha256(data: bytes):
@@ -697,17 +722,21 @@ class Context:
         """Rotates up to three tensors in one launch. positions: device int32 [T]; heads: a list of
         (x, y) or (x, y, rotate) device tensors [T, heads, head_dim] (any row and head strides)."""
         d, T = self._ropes.get(handle), positions.numel()
-        if "int32" not in str(positions.dtype):
-            raise TgoError(EINVAL, "positions is int32, not %s" % positions.dtype)
-        g = (RopeHeads * max(len(heads), 1))()
+        if _INT32.get(positions.dtype) is None:
+            if str(positions.dtype) != "torch.int32":
+                raise TgoError(EINVAL, "positions is int32, not %s" % positions.dtype)
+            _INT32[positions.dtype] = True
+        f = []
         for i, (x, y, *turn) in enumerate(heads):
-            if x.shape != y.shape or x.shape[0] != T or (d is not None and x.shape[2] != d):
+            shape = x.shape
+            if shape != y.shape or shape[0] != T or (d is not None and shape[2] != d):
                 raise TgoError(EINVAL, "rope: tensor %d is %s and %s for %d positions and heads of %s" %
-                               (i, tuple(x.shape), tuple(y.shape), T, d))
+                               (i, tuple(shape), tuple(y.shape), T, d))
             xa, xr, xh, xd = _heads_view(x, "rope: x")
             ya, yr, yh, yd = _heads_view(y, "rope: y")
-            g[i] = RopeHeads(xa, ya, xr, xh, yr, yh, x.shape[1], xd, yd, int(turn[0]) if turn else 1)
-        check(lib().tgohip_rope(self.h, handle, ptr(positions), T, g, len(heads)))
+            f += xa, ya, xr, xh, yr, yh, shape[1], xd, yd, (1 if turn[0] else 0) if turn else 1
+        n = len(heads)
+        check(_lib.tgohip_rope(self.h, handle, _addr(positions), T, _ROPE_HEADS[n].pack(*f) if n < 4 else None, n))
 
     def packed_plan(self, q_lengths, kv_lengths, H, Hkv, head_dim=128, causal=True, q_dtype=F32, plan=0):
         """Decomposes a batch for packed_attention; returns the plan's handle. plan: a handle whose plan
@@ -733,12 +762,12 @@ class Context:
         ka, kr, _ = _packed_rows(k, "k", tk, Hkv, d, F16)
         va, vr, _ = _packed_rows(v, "v", tk, Hkv, d, F16)
         if out.dim() == 4:
-            if tuple(out.shape) != (2, tq, H, d) or not out.is_contiguous() or "float16" not in str(out.dtype):
+            if tuple(out.shape) != (2, tq, H, d) or not out.is_contiguous() or _kind(out) != F16:
                 raise TgoError(EINVAL, "out as a pair is a dense float16 [2, %d, %d, %d]" % (tq, H, d))
-            oa, orow, od = ptr(out), H * d, F16X2
+            oa, orow, od = out.data_ptr(), H * d, F16X2
         else:
             oa, orow, od = _packed_rows(out, "out", tq, H, d, None)
-        check(lib().tgohip_packed_attention(self.h, plan, qa, qr, ka, kr, va, vr, scale, oa, orow, od))
+        check(_lib.tgohip_packed_attention(self.h, plan, qa, qr, ka, kr, va, vr, scale, oa, orow, od))
 
     def adapters_new(self, K, N, capacity):
         """A set of up to `capacity` adapters of a projection [K,N]; returns its handle."""
@@ -780,7 +809,7 @@ class Context:
 
     def adapters(self, handle, rows, x, base, y, x_dtype=F32, y_dtype=F32):
         """y = base + the adapters' product of x (base None: zeros; y may be base)."""
-        check(lib().tgohip_adapters(self.h, handle, rows, ptr(x), x_dtype, ptr(base), ptr(y), y_dtype))
+        check(_lib.tgohip_adapters(self.h, handle, rows, _addr(x), x_dtype, _addr(base), _addr(y), y_dtype))
 
     def greedy(self, logits, B, V, ids, margins=None):
         """sample argmax (first strict maximum) and TopTwoMargin over device rows."""

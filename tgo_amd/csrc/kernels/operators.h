@@ -17,16 +17,18 @@ struct RopeGroup {
   void* y;
   int64_t x_row, x_head, y_row, y_head;  // elements
   int32_t heads, x_f16, y_f16, rotate;
+  uint64_t magic;  // set by launch_rope
 };
 struct RopeArgs {
   const int32_t* positions;
   const double* inv_freq;  // [rotary_dim / 2], turns per position (angle / 2 pi)
   float attention;         // cos and sin are multiplied by it
   int T, d, rd, half;      // half: pairs (i, i + rd/2), else (2i, 2i + 1)
+  int rows;  // of a workgroup, set by launch_rope
   int n;
   RopeGroup g[kRopeGroups];
 };
-void launch_rope(const RopeArgs& a, hipStream_t st);
+void launch_rope(const RopeArgs& a, int ncu, hipStream_t st);
 
 // ---- packed attention (packed_attention.hip) --------------------------------
 // A work item: rows [r0, r0 + nr) of one sequence and kv head against its keys

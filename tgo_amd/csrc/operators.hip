@@ -285,7 +285,7 @@ int tgohip_rope(tgohip_ctx* c, int handle, const int32_t* positions, int T, cons
       return fail(TGOHIP_EINVAL, at + "heads of y overlap (strides " + std::to_string(g.y_row) + ", " + std::to_string(g.y_head) + ")");
     xs[i] = Span{(const char*)g.x, T, g.heads, g.x_row * elt(xf), g.x_head * elt(xf), t->d * elt(xf)};
     ys[i] = Span{(const char*)g.y, T, g.heads, g.y_row * elt(yf), g.y_head * elt(yf), t->d * elt(yf)};
-    a.g[i] = RopeGroup{g.x, g.y, g.x_row, g.x_head, g.y_row, g.y_head, g.heads, xf, yf, g.rotate != 0};
+    a.g[i] = RopeGroup{g.x, g.y, g.x_row, g.x_head, g.y_row, g.y_head, g.heads, xf, yf, g.rotate != 0, 0};
   }
   for (int i = 0; i < n; i++)
     for (int j = 0; j < n; j++) {
@@ -304,7 +304,7 @@ int tgohip_rope(tgohip_ctx* c, int handle, const int32_t* positions, int T, cons
   a.half = t->half;
   a.n = n;
   OnDevice on(c->device);
-  launch_rope(a, c->stream);
+  launch_rope(a, c->ncu, c->stream);
   TGOHIP_HIP(hipGetLastError());
   return 0;
 }
