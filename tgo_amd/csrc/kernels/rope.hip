@@ -70,6 +70,7 @@ __device__ __forceinline__ void rope_store(void* p, int64_t off, const float (&v
 // (positions to 2^31 keep 2^-23 of a turn and better), the rest in f32 with the
 // angle's second half as a first-order correction: within 2 ulp of 1.
 __device__ __forceinline__ float2 rope_angle(int32_t pos, double turns_per_position, float m) {
+#pragma clang fp contract(off)  // every kernel that inlines this computes the same bits
   double x = (double)pos * turns_per_position;
   x = 2.0 * (x - rint(x));
   const float hi = (float)x, lo = (float)(x - (double)hi) * 3.14159265f;
@@ -104,7 +105,8 @@ __device__ __forceinline__ void rope_heads(const RopeArgs& a, const RopeGroup& g
       for (int i = 0; i < V; i++) {
         const float2 w = cs[t * pairs + V * u + i];
         const float e = HALF ? A[i] : p[2 * i], f = HALF ? B[i] : p[2 * i + 1];
-        const float e2 = e * w.x - f * w.y, f2 = e * w.y + f * w.x;
+        // written out, so that every unit width rounds alike
+        const float e2 = fmaf(e, w.x, -(f * w.y)), f2 = fmaf(e, w.y, f * w.x);
         if (HALF) A[i] = e2, B[i] = f2;
         else p[2 * i] = e2, p[2 * i + 1] = f2;
       }
