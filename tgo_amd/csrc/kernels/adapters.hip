@@ -7,7 +7,12 @@
 // With ranks up to 128 the work is far below the matrix unit's: x, base and y
 // bound it, and for a few rows the two launches' latency.
 //   adapter_down_kernel  u = x . down^T over a share of K, f32 planes
-//   adapter_up_kernel    sums the planes in order, y = base + s u . up^T
+//   adapter_pair_kernel  (tiles of 64 rows) the planes' sums, as scaled f16 pairs
+//   adapter_up_kernel    y = base + s u . up^T; with tiles of 16 rows it sums the
+//                        planes itself, a launch less
+// Both products in one launch, each workgroup computing its tile's u, was slower for
+// all but the smallest K: one row of [4096, 4096] 9.4 us for 8.0, 128 rows of
+// [12288, 4096] 27.9 for 12.0, 16 rows of [1024, 4096] 6.1 for 6.9.
 // Both use v_mfma_f32_16x16x32_f16 (16x16x16 for rank 16): lane (l16, q) =
 // (lane % 16, lane / 16) holds row or column l16 of an operand at k 8q + [0,8),
 // and of the result column l16, rows 4q + [0,4).
@@ -176,90 +181,44 @@ __global__ __launch_bounds__(256) void adapter_pair_kernel(AdapterArgs a) {
   if (r == 0) a.pair_scale[pos] = up;
 }
 
-// Columns [a.cols * blockIdx.y, + a.cols) of a tile's rows. A wave takes 16 of the
-// rows and 64 columns a round (up's rows are the A operand, so a lane holds four
-// neighbouring columns of row l16 of y); a tile of fewer blocks of rows shares its
-// columns among the waves instead. The next round's up and base are loaded before
-// this one's products, which cross the wave's own LDS so that base and y move in
-// runs of 64 columns of a row. With one block of rows per tile (TB = 1) the planes
-// are summed and scaled here, else they come as adapter_pair_kernel's pairs.
-template <int TB, int RB, bool YF16>
-__global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a) {
-  constexpr int KB = RB == 1 ? 1 : RB / 2;  // products along the rank: 32 wide, or one 16 wide
-  constexpr int E = RB == 1 ? 4 : 8;        // of which a lane holds E
-  constexpr int PE = YF16 ? 8 : 4;          // columns of a 16-byte piece of base or y
-  constexpr int PL = 64 / PE;               // lanes per row's run
-  constexpr int NP = 16 * PL / 64;          // pieces a lane holds
-  __shared__ __attribute__((aligned(16))) float us[TB == 1 ? 16 : 1][RB * 16 + 4];
-  __shared__ __attribute__((aligned(16))) float stage[4][16][68];
-  const AdapterTile t = a.tiles[blockIdx.x];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, q = lane >> 4;
-  const int n0 = blockIdx.y * a.cols, n1 = min(n0 + a.cols, a.N);
-  AdapterEntry e{};
-  if (t.adapter >= 0) e = a.table[t.adapter];
-  // an adapter of a larger rank than the launch was captured for: its rows are NaN
-  if (e.rank_pad > RB * 16) {
-    e.rank_pad = RB * 16;
-    e.scale = NAN;
-  }
-  if (e.rank_pad == 0) {
-    if (a.base == a.y) return;
-    const int w = (n1 - n0) / PE;
-    for (int i = tid; i < t.n * w; i += 256) {
-      const int m = i / w;
-      const int64_t off = (int64_t)a.perm[t.start + m] * a.N + n0 + PE * (i - m * w);
-      float v[PE];
-      adapter_load_piece<YF16>(a, off, v);
-      adapter_store_piece<YF16>(a, off, v);
+// u of row l16 (16 rows in LDS) as the lane's operands of the second product.
+template <int RB>
+__device__ __forceinline__ void adapter_operand(const float (&us)[16][RB * 16 + 4], int l16, int q, half8_t (&uh)[(RB + 1) / 2],
+                                                half8_t (&ul)[(RB + 1) / 2], float& scale) {
+  constexpr int KB = (RB + 1) / 2, E = RB == 1 ? 4 : 8;
+  float top = 0.f, down, up;
+#pragma unroll
+  for (int k = 0; k < KB; k++)
+#pragma unroll
+    for (int j = 0; j < E; j++) top = fmaxf(top, fabsf(us[l16][32 * k + E * q + j]));
+  top = fmaxf(top, __shfl_xor(top, 16, 64));
+  top = fmaxf(top, __shfl_xor(top, 32, 64));
+  adapter_power(top, down, up);
+  scale *= up;
+#pragma unroll
+  for (int k = 0; k < KB; k++)
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const float f = j < E ? us[l16][32 * k + E * q + (j < E ? j : 0)] * down : 0.f;
+      uh[k][j] = (half_t)f;
+      ul[k][j] = (half_t)(f - (float)uh[k][j]);
     }
-    return;
-  }
-  const int ntb = (t.n + 15) / 16, share = ntb == 1 ? 4 : ntb == 2 ? 2 : 1;  // waves that share a block's columns
-  const int m0 = 16 * (wave / share);
-  half8_t uh[KB], ul[KB];
-  float scale;
-  if constexpr (TB == 1) {
-    for (int i = tid; i < 16 * RB * 16; i += 256) {
-      const int m = i / (RB * 16), r = i - m * (RB * 16);
-      // every plane's load in flight, summed in their order
-      float s = 0.f, v[kAdapterMaxSplits];
-      const bool in = m < t.n && r < e.rank_pad;
-      const float* u = a.u + ((int64_t)t.start + (in ? m : 0)) * kAdapterMaxRank + (in ? r : 0);
-#pragma unroll
-      for (int p = 0; p < kAdapterMaxSplits; p++) v[p] = u[(int64_t)min(p, a.splits - 1) * a.T * kAdapterMaxRank];
-#pragma unroll
-      for (int p = 0; p < kAdapterMaxSplits; p++) s += p < a.splits ? v[p] : 0.f;
-      us[m][r] = in ? s : 0.f;
-    }
-    __syncthreads();
-    float top = 0.f, down, up;
-#pragma unroll
-    for (int k = 0; k < KB; k++)
-#pragma unroll
-      for (int j = 0; j < E; j++) top = fmaxf(top, fabsf(us[l16][32 * k + E * q + j]));
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    adapter_power(top, down, up);
-    scale = e.scale * up;
-#pragma unroll
-    for (int k = 0; k < KB; k++)
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const float f = j < E ? us[l16][32 * k + E * q + (j < E ? j : 0)] * down : 0.f;
-        uh[k][j] = (half_t)f;
-        ul[k][j] = (half_t)(f - (float)uh[k][j]);
-      }
-  } else {
-    if (m0 >= t.n) return;
-    const int64_t pos = t.start + min(m0 + l16, t.n - 1);
-    const half_t* p = a.pair + pos * 2 * kAdapterMaxRank + E * q;
-    scale = e.scale * a.pair_scale[pos];
-#pragma unroll
-    for (int k = 0; k < KB; k++) {  // RB = 1 uses the first half of what it loads
-      uh[k] = *(const half8_t*)(p + 32 * k);
-      ul[k] = *(const half8_t*)(p + kAdapterMaxRank + 32 * k);
-    }
-  }
+}
+
+// y of 16 rows (m0 on) of a tile, columns n, n + step, ... below n1, 64 at a time by
+// one wave: up's rows are the A operand, so a lane holds four neighbouring columns of
+// row l16. The next round's up and base are loaded before this one's products, which
+// cross the wave's own LDS (ys) so that base and y move in runs of 64 columns of a row.
+template <int RB, bool YF16>
+__device__ __forceinline__ void adapter_columns(const AdapterArgs& a, const AdapterTile& t, const AdapterEntry& e,
+                                                const half8_t (&uh)[(RB + 1) / 2], const half8_t (&ul)[(RB + 1) / 2],
+                                                float scale, int m0, int n, int n1, int step, float (*ys)[68]) {
+  constexpr int KB = (RB + 1) / 2;   // products along the rank: 32 wide, or one 16 wide
+  constexpr int E = RB == 1 ? 4 : 8; // of which a lane holds E
+  constexpr int PE = YF16 ? 8 : 4;   // columns of a 16-byte piece of base or y
+  constexpr int PL = 64 / PE;        // lanes per row's run
+  constexpr int NP = 16 * PL / 64;   // pieces a lane holds
+  const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
   const int prow = lane / PL, pcol = lane % PL * PE;
   int64_t off[NP];  // this lane's pieces of the rows
   bool live[NP];
@@ -290,10 +249,8 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a) {
 #pragma unroll
     for (int i = 0; i < NP; i++) adapter_load_piece<YF16>(a, off[i] + n - back, base[i]);
   };
-  float(*ys)[68] = stage[wave];
-  int n = n0 + 64 * (wave % share);
   if (n < n1) load(n);
-  for (; n < n1; n += 64 * share) {
+  for (; n < n1; n += step) {
     half8_t wc[4][KB];
     float bc[NP][PE];
 #pragma unroll
@@ -304,7 +261,7 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a) {
     for (int i = 0; i < NP; i++)
 #pragma unroll
       for (int j = 0; j < PE; j++) bc[i][j] = base[i][j];
-    if (n + 64 * share < n1) load(n + 64 * share);
+    if (n + step < n1) load(n + step);
 #pragma unroll
     for (int c = 0; c < 4; c++) {
       float4_t acc = {};
@@ -336,11 +293,82 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a) {
   }
 }
 
+// A tile's rows without an adapter: y = base. False: the rows have one, in e.
+template <int RB, bool YF16>
+__device__ __forceinline__ bool adapter_copies(const AdapterArgs& a, const AdapterTile& t, AdapterEntry& e, int n0, int n1) {
+  e = AdapterEntry{};
+  if (t.adapter >= 0) e = a.table[t.adapter];
+  // an adapter of a larger rank than the launch was captured for: its rows are NaN
+  if (e.rank_pad > RB * 16) {
+    e.rank_pad = RB * 16;
+    e.scale = NAN;
+  }
+  if (e.rank_pad) return false;
+  if (a.base == a.y) return true;
+  constexpr int PE = YF16 ? 8 : 4;
+  const int w = (n1 - n0) / PE;
+  for (int i = threadIdx.x; i < t.n * w; i += blockDim.x) {
+    const int m = i / w;
+    const int64_t off = (int64_t)a.perm[t.start + m] * a.N + n0 + PE * (i - m * w);
+    float v[PE];
+    adapter_load_piece<YF16>(a, off, v);
+    adapter_store_piece<YF16>(a, off, v);
+  }
+  return true;
+}
+
+// Columns [a.cols * blockIdx.y, + a.cols) of a tile's rows. A wave takes 16 of the
+// rows; a tile of fewer blocks of rows shares its columns among the waves instead.
+// With one block of rows per tile (TB = 1) the planes are summed and scaled here, else
+// they come as adapter_pair_kernel's pairs.
+template <int TB, int RB, bool YF16>
+__global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a) {
+  constexpr int KB = (RB + 1) / 2, E = RB == 1 ? 4 : 8;
+  __shared__ __attribute__((aligned(16))) float us[TB == 1 ? 16 : 1][RB * 16 + 4];
+  __shared__ __attribute__((aligned(16))) float stage[4][16][68];
+  const AdapterTile t = a.tiles[blockIdx.x];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, q = lane >> 4;
+  const int n0 = blockIdx.y * a.cols, n1 = min(n0 + a.cols, a.N);
+  AdapterEntry e;
+  if (adapter_copies<RB, YF16>(a, t, e, n0, n1)) return;
+  const int ntb = (t.n + 15) / 16, share = ntb == 1 ? 4 : ntb == 2 ? 2 : 1;  // waves that share a block's columns
+  const int m0 = 16 * (wave / share);
+  half8_t uh[KB], ul[KB];
+  float scale = e.scale;
+  if constexpr (TB == 1) {
+    for (int i = tid; i < 16 * RB * 16; i += 256) {
+      const int m = i / (RB * 16), r = i - m * (RB * 16);
+      // every plane's load in flight, summed in their order
+      float s = 0.f, v[kAdapterMaxSplits];
+      const bool in = m < t.n && r < e.rank_pad;
+      const float* u = a.u + ((int64_t)t.start + (in ? m : 0)) * kAdapterMaxRank + (in ? r : 0);
+#pragma unroll
+      for (int p = 0; p < kAdapterMaxSplits; p++) v[p] = u[(int64_t)min(p, a.splits - 1) * a.T * kAdapterMaxRank];
+#pragma unroll
+      for (int p = 0; p < kAdapterMaxSplits; p++) s += p < a.splits ? v[p] : 0.f;
+      us[m][r] = in ? s : 0.f;
+    }
+    __syncthreads();
+    adapter_operand<RB>(us, l16, q, uh, ul, scale);
+  } else {
+    if (m0 >= t.n) return;
+    const int64_t pos = t.start + min(m0 + l16, t.n - 1);
+    const half_t* p = a.pair + pos * 2 * kAdapterMaxRank + E * q;
+    scale *= a.pair_scale[pos];
+#pragma unroll
+    for (int k = 0; k < KB; k++) {  // RB = 1 uses the first half of what it loads
+      uh[k] = *(const half8_t*)(p + 32 * k);
+      ul[k] = *(const half8_t*)(p + kAdapterMaxRank + 32 * k);
+    }
+  }
+  adapter_columns<RB, YF16>(a, t, e, uh, ul, scale, m0, n0 + 64 * (wave % share), n1, 64 * share, stage[wave]);
+}
+
 template <int XK, int TB, int RB>
 static void adapters_launch(const AdapterArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)a.ntiles, (unsigned)((a.N + a.cols - 1) / a.cols));
   hipLaunchKernelGGL((adapter_down_kernel<XK, TB, RB>), dim3((unsigned)a.ntiles, (unsigned)a.splits), dim3(256), 0, st, a);
   if (TB > 1) hipLaunchKernelGGL(adapter_pair_kernel, dim3((unsigned)a.ntiles, 4 * TB), dim3(256), 0, st, a);
-  const dim3 grid((unsigned)a.ntiles, (unsigned)((a.N + a.cols - 1) / a.cols));
   if (a.y_f16) hipLaunchKernelGGL((adapter_up_kernel<TB, RB, true>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((adapter_up_kernel<TB, RB, false>), grid, dim3(256), 0, st, a);
 }
@@ -354,15 +382,15 @@ static void adapters_rank(const AdapterArgs& a, hipStream_t st) {
 
 void launch_adapters(const AdapterArgs& args, int tile_rows, int ncu, hipStream_t st) {
   AdapterArgs a = args;
-  const bool few = tile_rows <= 16;
+  const bool one = tile_rows <= 16;
   // Columns per workgroup of the second kernel, us for 1152 mixed rows of rank 64 over
   // [4096, 24576] and 8000 f16 rows of rank 24 over [12288, 4096]: 128 columns 108,
   // 100; 256 106, 96; 512 114, 97; 1024 138, 111.
   a.cols = 256;
   switch (a.xk) {
-    case XK_F32: few ? adapters_rank<XK_F32, 1>(a, st) : adapters_rank<XK_F32, 4>(a, st); break;
-    case XK_F16: few ? adapters_rank<XK_F16, 1>(a, st) : adapters_rank<XK_F16, 4>(a, st); break;
-    default: few ? adapters_rank<XK_X2, 1>(a, st) : adapters_rank<XK_X2, 4>(a, st); break;
+    case XK_F32: one ? adapters_rank<XK_F32, 1>(a, st) : adapters_rank<XK_F32, 4>(a, st); break;
+    case XK_F16: one ? adapters_rank<XK_F16, 1>(a, st) : adapters_rank<XK_F16, 4>(a, st); break;
+    default: one ? adapters_rank<XK_X2, 1>(a, st) : adapters_rank<XK_X2, 4>(a, st); break;
   }
 }
 
