@@ -312,7 +312,8 @@ int tgohip_dequant_f16(tgohip_ctx* ctx, int handle, uint16_t* y);
  * sequences need is made once (per model, per batch) under a handle, and every
  * layer's calls then only launch kernels on the context's stream. Such calls
  * can be captured into a HIP graph; making, changing or freeing a handle can
- * not. No counterpart in the reference, whose step has one unscaled rotary
+ * not, and a handle that a graph was captured with is not replaced or freed while
+ * the graph is used (its memory may move). No counterpart in the reference, whose step has one unscaled rotary
  * layout, no adapters, and attention over the block pool only. */
 
 /* Rotary positions. Pair i of a head's first rotary_dim dims turns by
@@ -350,8 +351,8 @@ int tgohip_rope_freqs(const tgohip_rope_cfg* cfg, double* inv_freq, double* atte
 int tgohip_rope_new(tgohip_ctx* ctx, const tgohip_rope_cfg* cfg, int* handle);
 int tgohip_rope_free(tgohip_ctx* ctx, int handle);
 /* One tensor of heads: element j of head h of row t at x[t x_row + h x_head + j].
- * Strides are in elements; x's may be 0 (one row or head for all), y's heads
- * must not overlap. rotate 0 copies x to y (a value head narrowed to f16 beside
+ * Strides are in elements, at most 2^36; x's may be 0 (one row or head for all),
+ * y's heads must not overlap. rotate 0 copies x to y (a value head narrowed to f16 beside
  * the rotated ones). */
 typedef struct {
   const void* x;
@@ -383,12 +384,22 @@ int tgohip_rope(tgohip_ctx* ctx, int handle, const int32_t* positions, int T,
 int tgohip_packed_plan(tgohip_ctx* ctx, int B, const int32_t* q_lengths, const int32_t* kv_lengths,
                        int H, int H_kv, int head_dim, int causal, int q_dtype, int* handle);
 int tgohip_packed_free(tgohip_ctx* ctx, int handle);
+/* How such a batch is decomposed on a GPU of `ncu` compute units (no device, as
+ * tgohip_attention_plan): workgroups of the tile kernel (128 rows of a sequence and
+ * kv head) and of the few-row kernel (up to 32), the most keys of each, rows of
+ * partial results, and rows merged from them. */
+typedef struct {
+  int32_t tiles, few, longest_tile, longest_few;
+  int64_t part_rows, merged_rows;
+} tgohip_packed_plan_t;
+int tgohip_packed_describe(int B, const int32_t* q_lengths, const int32_t* kv_lengths, int H, int H_kv,
+                           int head_dim, int causal, int q_dtype, int ncu, tgohip_packed_plan_t* plan);
 /* out = softmax(scale q k^T) v over a plan's rows. q [rows, H, head_dim] in the
  * plan's q_dtype, k and v [key rows, H_kv, head_dim] f16, out like q in f32, f16
  * or as a pair (TGOHIP_F16X2, dense rows, the lo plane behind the hi plane). Rows
- * are *_row elements apart (k's and v's at most 2^24), heads dense; rows start on
- * 16-byte boundaries. scale > 0. With f32 queries the products are those of tgohip_paged_attention's
- * f32 form (q and the probabilities as f16 hi + lo pairs, so |q| < 65504); with
+ * are *_row elements apart (k's and v's at most 2^24, q's and out's 2^30), heads
+ * dense; rows start on 16-byte boundaries. scale > 0. With f32 queries the products
+ * are those of tgohip_paged_attention's f32 form (q and the probabilities as f16 hi + lo pairs, so |q| < 65504); with
  * f16 queries the probabilities are rounded to f16. Sums, maxima and partial
  * results are f32. Memory behind the last row stays as it is; out meets none of
  * q, k and v. */
@@ -401,7 +412,7 @@ int tgohip_packed_attention(tgohip_ctx* ctx, int handle, const void* q, int64_t 
  * with the adapter of the request row t belongs to, y[t] = base[t] for a request
  * without one. base is what tgohip_linear wrote.
  * adapters_new makes a set of up to `capacity` adapters of one projection (K a
- * multiple of 64, N of 32). adapters_put loads one at an index, replacing what
+ * multiple of 64, N of 32, each up to 2^22). adapters_put loads one at an index, replacing what
  * was there: host planes down [rank,K] and up [N,rank], f32 (rounded to the
  * nearest f16, refused past its range) or f16, rank 1 to 128. adapters_drop empties an index. An
  * empty index is no adapter. put, drop and free wait for the context's stream. A

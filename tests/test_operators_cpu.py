@@ -104,7 +104,7 @@ def test_packed_plan_refusals(kw, word):
 
 @pytest.mark.parametrize("K,N,cap,word", [
     (0, 64, 1, "projection is"), (96, 64, 1, "K a multiple of 64"), (64, 48, 1, "N of 32|N a multiple of 32"),
-    (-64, 64, 1, "projection is"), (64, 64, 0, "capacity is 0"), (64, 64, 65537, "capacity is 65537"),
+    (-64, 64, 1, "projection is"), ((1 << 22) + 64, 64, 1, "up to 2\\^22"), (64, 1 << 23, 1, "up to 2\\^22"), (64, 64, 0, "capacity is 0"), (64, 64, 65537, "capacity is 65537"),
     (64, 64, 4, "context is missing"),
 ])
 def test_adapter_set_refusals(K, N, cap, word):
@@ -147,3 +147,54 @@ def test_calls_without_a_context_are_refused():
                L.tgohip_adapters(None, 1, 1, None, 0, None, None, 0), L.tgohip_adapters_drop(None, 1, 0),
                L.tgohip_adapters_free(None, 1), L.tgohip_adapter_rows_free(None, 1)):
         assert rc == tgo_amd.EINVAL and "context is missing" in tgo_amd.last_error()
+
+
+def describe(nq, nk, **kw):
+    p = tgo_amd.packed_describe(nq, nk, kw.pop("H", 32), kw.pop("Hkv", 8), **kw)
+    return p.tiles, p.few, p.longest_tile, p.longest_few, p.part_rows, p.merged_rows
+
+
+def test_packed_batches_are_decomposed_by_their_sizes():
+    # one short prompt: 40 tokens x 4 heads are two tiles of 128 rows for each of 8 kv heads
+    assert describe([40], [40]) == (16, 0, 40, 0, 0, 0)
+    # single tokens go to the few-row kernel, whole where they fill the chip evenly ...
+    assert describe([1] * 64, [4096] * 64) == (0, 512, 0, 4096, 0, 0)
+    # ... and cut where few of them would leave it idle: 8 items on 512 slots
+    tiles, few, _, longest, parts, merged = describe([1], [32768])
+    assert tiles == 0 and few > 400 and longest <= 640 and parts == 4 * few and merged == 32
+    # beside prompts that hold most of the keys they take a tile each
+    assert describe([1, 2000], [50, 2000])[1] == 0
+    assert describe([1, 20], [5000, 20])[1] > 0
+    # a long prompt's tiles are many and of every length: none is cut
+    assert describe([16384], [16384], q_dtype=tgo_amd.F16) == (4096, 0, 16384, 0, 0, 0)
+    # a chunk far behind its keys is cut: its partial rows hold every row at least twice
+    tiles, _, longest, _, parts, merged = describe([128], [32768])
+    assert tiles > 32 and longest < 32768 and merged == 128 * 32 and parts >= 2 * merged
+    # queries that see no key still have an item, which writes zeros
+    assert describe([7], [0]) == (8, 0, 0, 0, 0, 0)
+    assert describe([0, 0], [3, 0]) == (0, 0, 0, 0, 0, 0)
+    assert describe([], []) == (0, 0, 0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("seed", range(20))
+def test_packed_parts_cover_every_key_once(seed):
+    """Rows merged are whole items', and the keys of the parts of any batch are those of its items."""
+    r = np.random.default_rng(seed)
+    n = int(r.integers(1, 40))
+    nk = r.integers(0, 6000, n)
+    nq = np.where(r.random(n) < 0.5, r.integers(0, 5, n), r.integers(0, 900, n))
+    H, Hkv = [(32, 8), (7, 1), (16, 16), (64, 4)][seed % 4]
+    for causal in (True, False):
+        p = tgo_amd.packed_describe(nq, nk, H, Hkv, causal=causal)
+        assert p.part_rows >= 2 * p.merged_rows and (p.part_rows > 0) == (p.merged_rows > 0)
+        assert p.merged_rows <= int(nq.sum()) * H
+        assert max(p.longest_tile, p.longest_few) <= nk.max()
+        # as on one compute unit, where nothing is cut
+        one = tgo_amd.packed_describe(nq, nk, H, Hkv, causal=causal, ncu=1)
+        assert one.tiles + one.few <= p.tiles + p.few
+
+
+def test_packed_describe_refusals():
+    for kw in (dict(head_dim=80), dict(ncu=0), dict(q_dtype=2)):
+        with pytest.raises(TgoError):
+            tgo_amd.packed_describe([1], [1], 8, 2, **kw)

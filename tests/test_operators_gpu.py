@@ -335,6 +335,22 @@ def test_packed_attention_over_long_contexts(ctx, torch_gpu, nq, nk, H, Hkv, d, 
     assert torch.equal(out, again)
 
 
+@pytest.mark.parametrize("seed", range(12))
+def test_packed_attention_over_random_batches(ctx, torch_gpu, seed):
+    """Batches of single tokens, chunks and prompts, cut, merged and whole, both kernels in one call."""
+    torch = torch_gpu
+    r = np.random.default_rng(seed)
+    n = int(r.integers(2, 14))
+    nk = [int(x) for x in np.exp(r.uniform(0, math.log(9000), n))]
+    nq = [int(r.choice([0, 1, 1, 2, r.integers(1, 9), r.integers(1, min(600, k) + 1)])) for k in nk]
+    H, Hkv, d = [(32, 8, 128), (14, 2, 64), (8, 8, 128), (12, 1, 64)][seed % 4]
+    f16, causal = bool(seed & 1), seed % 3 != 0
+    print("packed: %s over %s, %d/%d heads of %d" % (nq, nk, H, Hkv, d), flush=True)
+    q, k, v = inputs(torch, nq, nk, H, Hkv, d, f16, seed=seed)
+    out = attend(ctx, torch, q, k, v, nq, nk, causal)
+    check_attention(torch, out, q, k, v, nq, nk, causal)
+
+
 @pytest.mark.parametrize("f16", [False, True])
 @pytest.mark.parametrize("d", [64, 128])
 def test_packed_attention_with_peaked_scores(ctx, torch_gpu, f16, d):
@@ -665,6 +681,43 @@ def test_adapter_rows_do_not_depend_on_each_other(ctx, torch_gpu):
     finally:
         for r in (one, many):
             ctx.adapter_rows_free(r)
+        ctx.adapters_free(h)
+
+
+def test_captured_adapters_see_later_puts(ctx, torch_gpu):
+    """A replay reads the set as it is then; an adapter beyond the captured rank makes its rows NaN, loudly."""
+    torch = torch_gpu
+    K, N = 256, 320
+    h, rows = ctx.adapters_new(K, N, 2), ctx.adapter_rows([3, 2], [0, 1])
+    x, base, y = torch.randn(5, K, device="cuda"), torch.randn(5, N, device="cuda"), torch.zeros(5, N, device="cuda")
+    try:
+        def put(i, r, seed):
+            down, up = make_adapter(torch, K, N, r, seed)
+            ctx.adapters_put(h, i, down.cpu().numpy(), up.cpu().numpy(), 1.0)
+            return down.double(), up.double(), 1.0
+        loaded = {0: put(0, 16, 1), 1: put(1, 30, 2)}
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        ctx.adapters(h, rows, x, base, y)
+        ctx.set_stream(side.cuda_stream)
+        try:
+            with torch.cuda.graph(graph, stream=side):
+                ctx.adapters(h, rows, x, base, y)
+        finally:
+            ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+        for step in range(3):
+            if step:
+                loaded[0] = put(0, 32 if step == 1 else 7, 10 + step)
+            graph.replay()
+            torch.cuda.synchronize()
+            want, tol = adapters64(torch, x.double(), base, [3, 2], [0, 1], loaded, K, N, True)
+            assert bool(((y.double() - want).abs() <= tol).all())
+        ctx.adapters_drop(h, 0)
+        put(1, 33, 20)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y[:3], base[:3]) and bool(y[3:].isnan().all())
+    finally:
+        ctx.adapter_rows_free(rows)
         ctx.adapters_free(h)
 
 

@@ -58,6 +58,11 @@ class RopeHeads(ctypes.Structure):
         (n, ctypes.c_int32) for n in ("heads", "x_dtype", "y_dtype", "rotate")]
 
 
+class PackedPlan(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("tiles", "few", "longest_tile", "longest_few")] + [
+        (n, ctypes.c_int64) for n in ("part_rows", "merged_rows")]
+
+
 class LinearPlan(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("kernel", "splits", "column_blocks")] + [
         (n, ctypes.c_size_t) for n in ("array_bytes", "limit_bytes")]
@@ -124,6 +129,7 @@ def lib():
         "tgohip_rope_free": (I, [P, I]),
         "tgohip_rope": (I, [P, I, P, I, P, I]),
         "tgohip_packed_plan": (I, [P, I, P, P, I, I, I, I, I, P]),
+        "tgohip_packed_describe": (I, [I, P, P, I, I, I, I, I, I, ctypes.POINTER(PackedPlan)]),
         "tgohip_packed_free": (I, [P, I]),
         "tgohip_packed_attention": (I, [P, I, P, I64, P, I64, P, I64, F, P, I64, I]),
         "tgohip_adapters_new": (I, [P, I, I, I, P]),
@@ -311,6 +317,15 @@ def rope_freqs(*args, **kw):
     w, m = np.zeros(max(c.rotary_dim // 2, 1), np.float64), ctypes.c_double()
     check(lib().tgohip_rope_freqs(ctypes.byref(c), ptr(w), ctypes.byref(m)))
     return w, m.value
+
+
+def packed_describe(q_lengths, kv_lengths, H, Hkv, head_dim=128, causal=True, q_dtype=F32, ncu=256):
+    """How a packed batch is decomposed (PackedPlan), without a GPU."""
+    nq, nk, p = i32(q_lengths), i32(kv_lengths), PackedPlan()
+    assert len(nq) == len(nk)
+    check(lib().tgohip_packed_describe(len(nq), ptr(nq), ptr(nk), H, Hkv, head_dim, int(causal), q_dtype, ncu,
+                                       ctypes.byref(p)))
+    return p
 
 
 _KINDS = {}  # a torch dtype's code: F32, F16, or None for one the operators do not take

@@ -105,8 +105,10 @@ __device__ __forceinline__ void rope_heads(const RopeArgs& a, const RopeGroup& g
       for (int i = 0; i < V; i++) {
         const float2 w = cs[t * pairs + V * u + i];
         const float e = HALF ? A[i] : p[2 * i], f = HALF ? B[i] : p[2 * i + 1];
-        // written out, so that every unit width rounds alike
-        const float e2 = fmaf(e, w.x, -(f * w.y)), f2 = fmaf(e, w.y, f * w.x);
+        // Written out, and kept apart from the store's rounding (some widths would
+        // otherwise round the multiply-add to f16 at once), so that all round alike.
+        float e2 = fmaf(e, w.x, -(f * w.y)), f2 = fmaf(e, w.y, f * w.x);
+        asm("" : "+v"(e2), "+v"(f2));
         if (HALF) A[i] = e2, B[i] = f2;
         else p[2 * i] = e2, p[2 * i + 1] = f2;
       }

@@ -234,79 +234,83 @@ int tgohip_rope_new(tgohip_ctx* c, const tgohip_rope_cfg* cfg, int* handle) {
 }
 
 int tgohip_rope_free(tgohip_ctx* c, int handle) {
-  if (!c) return no_ctx("rope_free");
-  RopeTable* t = find(c->ops.ropes, handle, "rope_free");
-  if (!t) return TGOHIP_EINVAL;
-  OnDevice on(c->device);
-  TGOHIP_HIP(hipStreamSynchronize(c->stream));
-  t->inv_freq.release();
-  c->ops.ropes.erase(handle);
-  return 0;
+  return guarded([&]() -> int {
+    if (!c) return no_ctx("rope_free");
+    RopeTable* t = find(c->ops.ropes, handle, "rope_free");
+    if (!t) return TGOHIP_EINVAL;
+    OnDevice on(c->device);
+    TGOHIP_HIP(hipStreamSynchronize(c->stream));
+    t->inv_freq.release();
+    c->ops.ropes.erase(handle);
+    return 0;
+  });
 }
 
 int tgohip_rope(tgohip_ctx* c, int handle, const int32_t* positions, int T, const tgohip_rope_heads* heads, int n) {
-  if (!c) return no_ctx("rope");
-  RopeTable* t = find(c->ops.ropes, handle, "rope");
-  if (!t) return TGOHIP_EINVAL;
-  if (T < 0 || T >= 1 << 24) return fail(TGOHIP_EINVAL, "rope: " + std::to_string(T) + " rows; 0 to 2^24 - 1");
-  if (n < 1 || n > kRopeGroups || !heads)
-    return fail(TGOHIP_EINVAL, "rope: " + std::to_string(n) + " tensors of heads; 1 to " + std::to_string(kRopeGroups));
-  if (T == 0) return 0;
-  if (!positions) return fail(TGOHIP_EINVAL, "rope: positions is a device buffer");
-  RopeArgs a{};
-  Span xs[kRopeGroups], ys[kRopeGroups];
-  for (int i = 0; i < n; i++) {
-    const tgohip_rope_heads& g = heads[i];
-    const std::string at = "rope: tensor " + std::to_string(i) + ": ";
-    if (!g.x || !g.y) return fail(TGOHIP_EINVAL, at + "x and y are device buffers");
-    if (g.heads < 1 || g.heads > 65536) return fail(TGOHIP_EINVAL, at + std::to_string(g.heads) + " heads; 1 to 65536");
-    if ((g.x_dtype != TGOHIP_F32 && g.x_dtype != TGOHIP_F16) || (g.y_dtype != TGOHIP_F32 && g.y_dtype != TGOHIP_F16))
-      return fail(TGOHIP_EINVAL, at + "x_dtype and y_dtype are f32 or f16");
-    const int xf = g.x_dtype == TGOHIP_F16, yf = g.y_dtype == TGOHIP_F16;
-    if (((uintptr_t)g.x & (elt(xf) - 1)) || ((uintptr_t)g.y & (elt(yf) - 1)))
-      return fail(TGOHIP_EINVAL, at + "x or y is not aligned to its type");
-    const int64_t top = (int64_t)1 << 40;  // strides beyond any tensor: the products below stay in 64 bits
-    if (g.x_row < 0 || g.x_head < 0 || g.x_row > top || g.x_head > top || g.y_row > top || g.y_head > top)
-      return fail(TGOHIP_EINVAL, at + "strides are not negative, and at most 2^40 elements");
-    // no two heads of y share an element
-    int64_t s0 = g.y_row, n0 = T, s1 = g.y_head, n1 = g.heads;
-    if (n0 == 1) s0 = 0;
-    if (n1 == 1) s1 = 0;
-    if (s0 > s1) {
-      std::swap(s0, s1);
-      std::swap(n0, n1);
+  return guarded([&]() -> int {
+    if (!c) return no_ctx("rope");
+    RopeTable* t = find(c->ops.ropes, handle, "rope");
+    if (!t) return TGOHIP_EINVAL;
+    if (T < 0 || T >= 1 << 24) return fail(TGOHIP_EINVAL, "rope: " + std::to_string(T) + " rows; 0 to 2^24 - 1");
+    if (n < 1 || n > kRopeGroups || !heads)
+      return fail(TGOHIP_EINVAL, "rope: " + std::to_string(n) + " tensors of heads; 1 to " + std::to_string(kRopeGroups));
+    if (T == 0) return 0;
+    if (!positions) return fail(TGOHIP_EINVAL, "rope: positions is a device buffer");
+    RopeArgs a{};
+    Span xs[kRopeGroups], ys[kRopeGroups];
+    for (int i = 0; i < n; i++) {
+      const tgohip_rope_heads& g = heads[i];
+      auto bad = [i](const std::string& m) { return fail(TGOHIP_EINVAL, "rope: tensor " + std::to_string(i) + ": " + m); };
+      if (!g.x || !g.y) return bad("x and y are device buffers");
+      if (g.heads < 1 || g.heads > 65536) return bad(std::to_string(g.heads) + " heads; 1 to 65536");
+      if ((g.x_dtype != TGOHIP_F32 && g.x_dtype != TGOHIP_F16) || (g.y_dtype != TGOHIP_F32 && g.y_dtype != TGOHIP_F16))
+        return bad("x_dtype and y_dtype are f32 or f16");
+      const int xf = g.x_dtype == TGOHIP_F16, yf = g.y_dtype == TGOHIP_F16;
+      if (((uintptr_t)g.x & (elt(xf) - 1)) || ((uintptr_t)g.y & (elt(yf) - 1)))
+        return bad("x or y is not aligned to its type");
+      const int64_t top = (int64_t)1 << 36;  // beyond any tensor; the products below stay in 64 bits
+      if (g.x_row < 0 || g.x_head < 0 || g.x_row > top || g.x_head > top || g.y_row > top || g.y_head > top)
+        return bad("strides are not negative, and at most 2^36 elements");
+      // no two heads of y share an element
+      int64_t s0 = g.y_row, n0 = T, s1 = g.y_head, n1 = g.heads;
+      if (n0 == 1) s0 = 0;
+      if (n1 == 1) s1 = 0;
+      if (s0 > s1) {
+        std::swap(s0, s1);
+        std::swap(n0, n1);
+      }
+      int64_t need = t->d;
+      if (n0 > 1) {
+        if (s0 < need) return bad("heads of y overlap (strides " + std::to_string(g.y_row) + ", " + std::to_string(g.y_head) + ")");
+        need = (n0 - 1) * s0 + t->d;
+      }
+      if (n1 > 1 && s1 < need)
+        return bad("heads of y overlap (strides " + std::to_string(g.y_row) + ", " + std::to_string(g.y_head) + ")");
+      xs[i] = Span{(const char*)g.x, T, g.heads, g.x_row * elt(xf), g.x_head * elt(xf), t->d * elt(xf)};
+      ys[i] = Span{(const char*)g.y, T, g.heads, g.y_row * elt(yf), g.y_head * elt(yf), t->d * elt(yf)};
+      a.g[i] = RopeGroup{g.x, g.y, g.x_row, g.x_head, g.y_row, g.y_head, g.heads, xf, yf, g.rotate != 0, 0};
     }
-    int64_t need = t->d;
-    if (n0 > 1) {
-      if (s0 < need) return fail(TGOHIP_EINVAL, at + "heads of y overlap (strides " + std::to_string(g.y_row) + ", " + std::to_string(g.y_head) + ")");
-      need = (n0 - 1) * s0 + t->d;
-    }
-    if (n1 > 1 && s1 < need)
-      return fail(TGOHIP_EINVAL, at + "heads of y overlap (strides " + std::to_string(g.y_row) + ", " + std::to_string(g.y_head) + ")");
-    xs[i] = Span{(const char*)g.x, T, g.heads, g.x_row * elt(xf), g.x_head * elt(xf), t->d * elt(xf)};
-    ys[i] = Span{(const char*)g.y, T, g.heads, g.y_row * elt(yf), g.y_head * elt(yf), t->d * elt(yf)};
-    a.g[i] = RopeGroup{g.x, g.y, g.x_row, g.x_head, g.y_row, g.y_head, g.heads, xf, yf, g.rotate != 0, 0};
-  }
-  for (int i = 0; i < n; i++)
-    for (int j = 0; j < n; j++) {
-      if (meet(ys[i], xs[j]) && !(i == j && a.g[i].x_f16 == a.g[i].y_f16 && same(ys[i], xs[i])))
-        return fail(TGOHIP_EINVAL, "rope: y of tensor " + std::to_string(i) + " meets x of tensor " + std::to_string(j) +
-                                       " in memory; y is its own x (same type and strides) or apart");
-      if (i < j && meet(ys[i], ys[j]))
-        return fail(TGOHIP_EINVAL, "rope: y of tensors " + std::to_string(i) + " and " + std::to_string(j) + " meet in memory");
-    }
-  a.positions = positions;
-  a.inv_freq = (const double*)t->inv_freq.p;
-  a.attention = t->attention;
-  a.T = T;
-  a.d = t->d;
-  a.rd = t->rd;
-  a.half = t->half;
-  a.n = n;
-  OnDevice on(c->device);
-  launch_rope(a, c->ncu, c->stream);
-  TGOHIP_HIP(hipGetLastError());
-  return 0;
+    for (int i = 0; i < n; i++)
+      for (int j = 0; j < n; j++) {
+        if (meet(ys[i], xs[j]) && !(i == j && a.g[i].x_f16 == a.g[i].y_f16 && same(ys[i], xs[i])))
+          return fail(TGOHIP_EINVAL, "rope: y of tensor " + std::to_string(i) + " meets x of tensor " + std::to_string(j) +
+                                         " in memory; y is its own x (same type and strides) or apart");
+        if (i < j && meet(ys[i], ys[j]))
+          return fail(TGOHIP_EINVAL, "rope: y of tensors " + std::to_string(i) + " and " + std::to_string(j) + " meet in memory");
+      }
+    a.positions = positions;
+    a.inv_freq = (const double*)t->inv_freq.p;
+    a.attention = t->attention;
+    a.T = T;
+    a.d = t->d;
+    a.rd = t->rd;
+    a.half = t->half;
+    a.n = n;
+    OnDevice on(c->device);
+    launch_rope(a, c->ncu, c->stream);
+    TGOHIP_HIP(hipGetLastError());
+    return 0;
+  });
 }
 
 // ---- packed attention -----------------------------------------------------------
@@ -356,87 +360,107 @@ int tgohip_packed_plan(tgohip_ctx* c, int B, const int32_t* q_lengths, const int
   });
 }
 
+int tgohip_packed_describe(int B, const int32_t* q_lengths, const int32_t* kv_lengths, int H, int H_kv, int head_dim,
+                           int causal, int q_dtype, int ncu, tgohip_packed_plan_t* out) {
+  return guarded([&]() -> int {
+    const int rc = check_packed(B, q_lengths, kv_lengths, H, H_kv, head_dim, q_dtype);
+    if (rc) return rc;
+    if (ncu < 1 || !out) return fail(TGOHIP_EINVAL, "packed_describe: ncu and plan");
+    PackedPlan plan;
+    packed_build_plan(B, q_lengths, kv_lengths, H, H_kv, head_dim, causal != 0, q_dtype == TGOHIP_F16, ncu, plan);
+    *out = tgohip_packed_plan_t{(int32_t)plan.items.size(), (int32_t)plan.few.size(), 0, 0, plan.part_rows, 0};
+    for (const PackedItem& it : plan.items) out->longest_tile = std::max(out->longest_tile, it.kv_hi - it.kv_lo);
+    for (const PackedItem& it : plan.few) out->longest_few = std::max(out->longest_few, it.kv_hi - it.kv_lo);
+    for (const PackedMerge& m : plan.merges) out->merged_rows += m.nr;
+    return 0;
+  });
+}
+
 int tgohip_packed_free(tgohip_ctx* c, int handle) {
-  if (!c) return no_ctx("packed_free");
-  PackedHandle* p = find(c->ops.packed, handle, "packed_free");
-  if (!p) return TGOHIP_EINVAL;
-  OnDevice on(c->device);
-  TGOHIP_HIP(hipStreamSynchronize(c->stream));
-  p->meta.release();
-  p->part.release();
-  c->ops.packed.erase(handle);
-  return 0;
+  return guarded([&]() -> int {
+    if (!c) return no_ctx("packed_free");
+    PackedHandle* p = find(c->ops.packed, handle, "packed_free");
+    if (!p) return TGOHIP_EINVAL;
+    OnDevice on(c->device);
+    TGOHIP_HIP(hipStreamSynchronize(c->stream));
+    p->meta.release();
+    p->part.release();
+    c->ops.packed.erase(handle);
+    return 0;
+  });
 }
 
 int tgohip_packed_attention(tgohip_ctx* c, int handle, const void* q, int64_t q_row, const void* k, int64_t k_row,
                             const void* v, int64_t v_row, float scale, void* out, int64_t out_row, int out_dtype) {
-  if (!c) return no_ctx("packed_attention");
-  PackedHandle* p = find(c->ops.packed, handle, "packed_attention");
-  if (!p) return TGOHIP_EINVAL;
-  const PackedPlan& pl = p->plan;
-  if (!pl.D) return fail(TGOHIP_ESTATE, "packed_attention: the plan was not made again after a failure");
-  if (!(scale > 0.f) || !std::isfinite(scale))
-    return fail(TGOHIP_EINVAL, "packed_attention: scale is " + num(scale) + "; a finite number above 0");
-  if (out_dtype != TGOHIP_F32 && out_dtype != TGOHIP_F16 && out_dtype != TGOHIP_F16X2)
-    return fail(TGOHIP_EINVAL, "packed_attention: out_dtype is " + std::to_string(out_dtype) + "; f32, f16 or a pair");
-  if (pl.tq == 0) return 0;
-  if (!q || !out) return fail(TGOHIP_EINVAL, "packed_attention: q and out are device buffers");
-  if (pl.tk && (!k || !v)) return fail(TGOHIP_EINVAL, "packed_attention: k and v are device buffers");
-  const int64_t qw = (int64_t)pl.H * pl.D, kw = (int64_t)pl.Hkv * pl.D, top = (int64_t)1 << 40;
-  struct {
-    const char* name;
-    const void* p;
-    int64_t row, width, rows, unit, most;
-  } ops[] = {{"q", q, q_row, qw, pl.tq, pl.q_f16 ? 8 : 4, top},
-             {"k", k, k_row, kw, pl.tk, 8, kPackMaxRow},
-             {"v", v, v_row, kw, pl.tk, 8, kPackMaxRow},
-             {"out", out, out_row, qw, pl.tq, out_dtype == TGOHIP_F32 ? 4 : 8, top}};
-  for (auto& o : ops) {
-    if (o.rows > 1 && (o.row < o.width || o.row > o.most))
-      return fail(TGOHIP_EINVAL, std::string("packed_attention: ") + o.name + " rows are " + std::to_string(o.row) +
-                                     " elements apart and hold " + std::to_string(o.width) + "; at most " +
-                                     std::to_string(o.most) + " apart");
-    if (misaligned(o.p) || (o.rows > 1 && o.row % o.unit))
-      return fail(TGOHIP_EINVAL, std::string("packed_attention: ") + o.name + " rows start on 16-byte boundaries");
-  }
-  if (out_dtype == TGOHIP_F16X2 && pl.tq > 1 && out_row != qw)
-    return fail(TGOHIP_EINVAL, "packed_attention: a pair's rows are dense (out_row " + std::to_string(out_row) + ", not " +
-                                   std::to_string(qw) + ")");
-  const int64_t ob = out_dtype == TGOHIP_F32 ? 4 : 2, planes = out_dtype == TGOHIP_F16X2 ? 2 : 1;
-  const Span so{(const char*)out, planes * pl.tq, 1, out_row * ob, 0, qw * ob};
-  const Span in[] = {{(const char*)q, pl.tq, 1, q_row * elt(pl.q_f16), 0, qw * elt(pl.q_f16)},
-                     {(const char*)k, pl.tk, 1, k_row * 2, 0, kw * 2},
-                     {(const char*)v, pl.tk, 1, v_row * 2, 0, kw * 2}};
-  for (int i = 0; i < 3; i++)
-    if (meet(so, in[i])) return fail(TGOHIP_EINVAL, std::string("packed_attention: out meets ") + ops[i].name + " in memory");
-  PackedArgs a{};
-  a.q = q;
-  a.k = (const half_t*)k;
-  a.v = (const half_t*)v;
-  a.out = out;
-  a.part_o = (float*)p->part.p;
-  a.part_ml = (float*)p->part.p + (size_t)pl.part_rows * pl.D;
-  a.items = (const PackedItem*)p->meta.p;
-  a.merges = (const PackedMerge*)((const char*)p->meta.p + p->merges_off);
-  a.q_row = q_row;
-  a.k_row = k_row;
-  a.v_row = v_row;
-  a.out_row = out_row;
-  a.out_lo = pl.tq * qw;
-  a.G = pl.H / pl.Hkv;
-  a.out_form = out_dtype == TGOHIP_F32 ? OUT_F32 : out_dtype == TGOHIP_F16 ? OUT_F16 : OUT_X2;
-  a.qscale = scale * 1.4426950408889634f;
-  OnDevice on(c->device);
-  return packed_enqueue(a, pl.D, pl.q_f16, p->n, c->stream);
+  return guarded([&]() -> int {
+    if (!c) return no_ctx("packed_attention");
+    PackedHandle* p = find(c->ops.packed, handle, "packed_attention");
+    if (!p) return TGOHIP_EINVAL;
+    const PackedPlan& pl = p->plan;
+    if (!pl.D) return fail(TGOHIP_ESTATE, "packed_attention: the plan was not made again after a failure");
+    if (!(scale > 0.f) || !std::isfinite(scale))
+      return fail(TGOHIP_EINVAL, "packed_attention: scale is " + num(scale) + "; a finite number above 0");
+    if (out_dtype != TGOHIP_F32 && out_dtype != TGOHIP_F16 && out_dtype != TGOHIP_F16X2)
+      return fail(TGOHIP_EINVAL, "packed_attention: out_dtype is " + std::to_string(out_dtype) + "; f32, f16 or a pair");
+    if (pl.tq == 0) return 0;
+    if (!q || !out) return fail(TGOHIP_EINVAL, "packed_attention: q and out are device buffers");
+    if (pl.tk && (!k || !v)) return fail(TGOHIP_EINVAL, "packed_attention: k and v are device buffers");
+    const int64_t qw = (int64_t)pl.H * pl.D, kw = (int64_t)pl.Hkv * pl.D, top = (int64_t)1 << 30;
+    struct {
+      const char* name;
+      const void* p;
+      int64_t row, width, rows, unit, most;
+    } ops[] = {{"q", q, q_row, qw, pl.tq, pl.q_f16 ? 8 : 4, top},
+               {"k", k, k_row, kw, pl.tk, 8, kPackMaxRow},
+               {"v", v, v_row, kw, pl.tk, 8, kPackMaxRow},
+               {"out", out, out_row, qw, pl.tq, out_dtype == TGOHIP_F32 ? 4 : 8, top}};
+    for (auto& o : ops) {
+      if (o.rows > 1 && (o.row < o.width || o.row > o.most))
+        return fail(TGOHIP_EINVAL, std::string("packed_attention: ") + o.name + " rows are " + std::to_string(o.row) +
+                                       " elements apart and hold " + std::to_string(o.width) + "; at most " +
+                                       std::to_string(o.most) + " apart");
+      if (misaligned(o.p) || (o.rows > 1 && o.row % o.unit))
+        return fail(TGOHIP_EINVAL, std::string("packed_attention: ") + o.name + " rows start on 16-byte boundaries");
+    }
+    if (out_dtype == TGOHIP_F16X2 && pl.tq > 1 && out_row != qw)
+      return fail(TGOHIP_EINVAL, "packed_attention: a pair's rows are dense (out_row " + std::to_string(out_row) + ", not " +
+                                     std::to_string(qw) + ")");
+    const int64_t ob = out_dtype == TGOHIP_F32 ? 4 : 2, planes = out_dtype == TGOHIP_F16X2 ? 2 : 1;
+    const Span so{(const char*)out, planes * pl.tq, 1, out_row * ob, 0, qw * ob};
+    const Span in[] = {{(const char*)q, pl.tq, 1, q_row * elt(pl.q_f16), 0, qw * elt(pl.q_f16)},
+                       {(const char*)k, pl.tk, 1, k_row * 2, 0, kw * 2},
+                       {(const char*)v, pl.tk, 1, v_row * 2, 0, kw * 2}};
+    for (int i = 0; i < 3; i++)
+      if (meet(so, in[i])) return fail(TGOHIP_EINVAL, std::string("packed_attention: out meets ") + ops[i].name + " in memory");
+    PackedArgs a{};
+    a.q = q;
+    a.k = (const half_t*)k;
+    a.v = (const half_t*)v;
+    a.out = out;
+    a.part_o = (float*)p->part.p;
+    a.part_ml = (float*)p->part.p + (size_t)pl.part_rows * pl.D;
+    a.items = (const PackedItem*)p->meta.p;
+    a.merges = (const PackedMerge*)((const char*)p->meta.p + p->merges_off);
+    a.q_row = q_row;
+    a.k_row = k_row;
+    a.v_row = v_row;
+    a.out_row = out_row;
+    a.out_lo = pl.tq * qw;
+    a.G = pl.H / pl.Hkv;
+    a.out_form = out_dtype == TGOHIP_F32 ? OUT_F32 : out_dtype == TGOHIP_F16 ? OUT_F16 : OUT_X2;
+    a.qscale = scale * 1.4426950408889634f;
+    OnDevice on(c->device);
+    return packed_enqueue(a, pl.D, pl.q_f16, p->n, c->stream);
+  });
 }
 
 // ---- adapters ---------------------------------------------------------------------
 
 int tgohip_adapters_new(tgohip_ctx* c, int K, int N, int capacity, int* handle) {
   return guarded([&]() -> int {
-    if (K <= 0 || N <= 0 || K % 64 != 0 || N % 32 != 0)
+    if (K <= 0 || N <= 0 || K % 64 != 0 || N % 32 != 0 || K > 1 << 22 || N > 1 << 22)
       return fail(TGOHIP_EINVAL, "adapters_new: the projection is [" + std::to_string(K) + "," + std::to_string(N) +
-                                     "]; this library takes K a multiple of 64 and N a multiple of 32");
+                                     "]; this library takes K a multiple of 64 and N a multiple of 32, up to 2^22");
     if (capacity < 1 || capacity > 65536)
       return fail(TGOHIP_EINVAL, "adapters_new: capacity is " + std::to_string(capacity) + "; 1 to 65536 adapters");
     if (!c) return no_ctx("adapters_new");
@@ -516,25 +540,29 @@ int tgohip_adapters_put(tgohip_ctx* c, int handle, int index, int rank, int dtyp
 }
 
 int tgohip_adapters_drop(tgohip_ctx* c, int handle, int index) {
-  if (!c) return no_ctx("adapters_drop");
-  AdapterSet* s = find(c->ops.sets, handle, "adapters_drop");
-  if (!s) return TGOHIP_EINVAL;
-  if (index < 0 || index >= (int)s->table.size())
-    return fail(TGOHIP_EINVAL, "adapters_drop: index " + std::to_string(index) + " of a set of " + std::to_string(s->table.size()));
-  OnDevice on(c->device);
-  return adapter_set(c, s, index, AdapterEntry{nullptr, nullptr, 0, 0.f});
+  return guarded([&]() -> int {
+    if (!c) return no_ctx("adapters_drop");
+    AdapterSet* s = find(c->ops.sets, handle, "adapters_drop");
+    if (!s) return TGOHIP_EINVAL;
+    if (index < 0 || index >= (int)s->table.size())
+      return fail(TGOHIP_EINVAL, "adapters_drop: index " + std::to_string(index) + " of a set of " + std::to_string(s->table.size()));
+    OnDevice on(c->device);
+    return adapter_set(c, s, index, AdapterEntry{nullptr, nullptr, 0, 0.f});
+  });
 }
 
 int tgohip_adapters_free(tgohip_ctx* c, int handle) {
-  if (!c) return no_ctx("adapters_free");
-  AdapterSet* s = find(c->ops.sets, handle, "adapters_free");
-  if (!s) return TGOHIP_EINVAL;
-  OnDevice on(c->device);
-  TGOHIP_HIP(hipStreamSynchronize(c->stream));
-  for (AdapterEntry& e : s->table) (void)hipFree((void*)e.down);
-  s->table_dev.release();
-  c->ops.sets.erase(handle);
-  return 0;
+  return guarded([&]() -> int {
+    if (!c) return no_ctx("adapters_free");
+    AdapterSet* s = find(c->ops.sets, handle, "adapters_free");
+    if (!s) return TGOHIP_EINVAL;
+    OnDevice on(c->device);
+    TGOHIP_HIP(hipStreamSynchronize(c->stream));
+    for (AdapterEntry& e : s->table) (void)hipFree((void*)e.down);
+    s->table_dev.release();
+    c->ops.sets.erase(handle);
+    return 0;
+  });
 }
 
 int tgohip_adapter_rows(tgohip_ctx* c, int B, const int32_t* extents, const int32_t* adapters, int* handle) {
@@ -602,62 +630,66 @@ int tgohip_adapter_rows(tgohip_ctx* c, int B, const int32_t* extents, const int3
 }
 
 int tgohip_adapter_rows_free(tgohip_ctx* c, int handle) {
-  if (!c) return no_ctx("adapter_rows_free");
-  AdapterRows* r = find(c->ops.rows, handle, "adapter_rows_free");
-  if (!r) return TGOHIP_EINVAL;
-  OnDevice on(c->device);
-  TGOHIP_HIP(hipStreamSynchronize(c->stream));
-  r->meta.release();
-  r->u.release();
-  c->ops.rows.erase(handle);
-  return 0;
+  return guarded([&]() -> int {
+    if (!c) return no_ctx("adapter_rows_free");
+    AdapterRows* r = find(c->ops.rows, handle, "adapter_rows_free");
+    if (!r) return TGOHIP_EINVAL;
+    OnDevice on(c->device);
+    TGOHIP_HIP(hipStreamSynchronize(c->stream));
+    r->meta.release();
+    r->u.release();
+    c->ops.rows.erase(handle);
+    return 0;
+  });
 }
 
 int tgohip_adapters(tgohip_ctx* c, int set, int rows, const void* x, int x_dtype, const void* base, void* y, int y_dtype) {
-  if (!c) return no_ctx("adapters");
-  AdapterSet* s = find(c->ops.sets, set, "adapters: set");
-  if (!s) return TGOHIP_EINVAL;
-  AdapterRows* r = find(c->ops.rows, rows, "adapters: rows");
-  if (!r) return TGOHIP_EINVAL;
-  if (r->T < 0) return fail(TGOHIP_ESTATE, "adapters: the rows were not made again after a failure");
-  if (x_dtype != TGOHIP_F32 && x_dtype != TGOHIP_F16 && x_dtype != TGOHIP_F16X2)
-    return fail(TGOHIP_EINVAL, "adapters: x_dtype is " + std::to_string(x_dtype) + "; f32, f16 or a pair");
-  if (y_dtype != TGOHIP_F32 && y_dtype != TGOHIP_F16)
-    return fail(TGOHIP_EINVAL, "adapters: y_dtype is " + std::to_string(y_dtype) + "; f32 or f16");
-  if (r->max_adapter >= (int)s->table.size())
-    return fail(TGOHIP_EINVAL, "adapters: the rows name adapter " + std::to_string(r->max_adapter) + " and the set holds " +
-                                   std::to_string(s->table.size()));
-  if (r->T == 0) return 0;
-  if (!x || !y) return fail(TGOHIP_EINVAL, "adapters: x and y are device buffers");
-  if (misaligned(x) || misaligned(base) || misaligned(y))
-    return fail(TGOHIP_EINVAL, "adapters: x, base and y start on 16-byte boundaries");
-  const int64_t T = r->T, yb = y_dtype == TGOHIP_F16 ? 2 : 4;
-  const Span sx{(const char*)x, 1, 1, 0, 0, T * s->K * (x_dtype == TGOHIP_F16 ? 2 : 4)};
-  const Span sy{(const char*)y, 1, 1, 0, 0, T * s->N * yb}, sb{(const char*)base, 1, 1, 0, 0, T * s->N * yb};
-  if (meet(sy, sx)) return fail(TGOHIP_EINVAL, "adapters: y meets x in memory");
-  if (base && base != y && meet(sy, sb)) return fail(TGOHIP_EINVAL, "adapters: y meets base in memory; y is base itself or apart");
-  AdapterArgs a{};
-  a.table = (const AdapterEntry*)s->table_dev.p;
-  a.tiles = (const AdapterTile*)((const char*)r->meta.p + r->tiles_off);
-  a.perm = (const int32_t*)r->meta.p;
-  a.ntiles = r->ntiles;
-  a.T = r->T;
-  a.K = s->K;
-  a.N = s->N;
-  a.x = x;
-  a.xk = x_dtype == TGOHIP_F32 ? XK_F32 : x_dtype == TGOHIP_F16 ? XK_F16 : XK_X2;
-  a.base = base;
-  a.y = y;
-  a.y_f16 = y_dtype == TGOHIP_F16;
-  a.u = (float*)r->u.p;
-  OnDevice on(c->device);
-  a.splits = r->splits;
-  a.rank_pad = s->rank_pad;
-  a.pair = (half_t*)(a.u + (size_t)r->splits * T * kAdapterMaxRank);  // as many bytes as a plane
-  a.pair_scale = a.u + (size_t)(r->splits + 1) * T * kAdapterMaxRank;
-  launch_adapters(a, r->tile_rows, c->ncu, c->stream);
-  TGOHIP_HIP(hipGetLastError());
-  return 0;
+  return guarded([&]() -> int {
+    if (!c) return no_ctx("adapters");
+    AdapterSet* s = find(c->ops.sets, set, "adapters: set");
+    if (!s) return TGOHIP_EINVAL;
+    AdapterRows* r = find(c->ops.rows, rows, "adapters: rows");
+    if (!r) return TGOHIP_EINVAL;
+    if (r->T < 0) return fail(TGOHIP_ESTATE, "adapters: the rows were not made again after a failure");
+    if (x_dtype != TGOHIP_F32 && x_dtype != TGOHIP_F16 && x_dtype != TGOHIP_F16X2)
+      return fail(TGOHIP_EINVAL, "adapters: x_dtype is " + std::to_string(x_dtype) + "; f32, f16 or a pair");
+    if (y_dtype != TGOHIP_F32 && y_dtype != TGOHIP_F16)
+      return fail(TGOHIP_EINVAL, "adapters: y_dtype is " + std::to_string(y_dtype) + "; f32 or f16");
+    if (r->max_adapter >= (int)s->table.size())
+      return fail(TGOHIP_EINVAL, "adapters: the rows name adapter " + std::to_string(r->max_adapter) + " and the set holds " +
+                                     std::to_string(s->table.size()));
+    if (r->T == 0) return 0;
+    if (!x || !y) return fail(TGOHIP_EINVAL, "adapters: x and y are device buffers");
+    if (misaligned(x) || misaligned(base) || misaligned(y))
+      return fail(TGOHIP_EINVAL, "adapters: x, base and y start on 16-byte boundaries");
+    const int64_t T = r->T, yb = y_dtype == TGOHIP_F16 ? 2 : 4;
+    const Span sx{(const char*)x, 1, 1, 0, 0, T * s->K * (x_dtype == TGOHIP_F16 ? 2 : 4)};
+    const Span sy{(const char*)y, 1, 1, 0, 0, T * s->N * yb}, sb{(const char*)base, 1, 1, 0, 0, T * s->N * yb};
+    if (meet(sy, sx)) return fail(TGOHIP_EINVAL, "adapters: y meets x in memory");
+    if (base && base != y && meet(sy, sb)) return fail(TGOHIP_EINVAL, "adapters: y meets base in memory; y is base itself or apart");
+    AdapterArgs a{};
+    a.table = (const AdapterEntry*)s->table_dev.p;
+    a.tiles = (const AdapterTile*)((const char*)r->meta.p + r->tiles_off);
+    a.perm = (const int32_t*)r->meta.p;
+    a.ntiles = r->ntiles;
+    a.T = r->T;
+    a.K = s->K;
+    a.N = s->N;
+    a.x = x;
+    a.xk = x_dtype == TGOHIP_F32 ? XK_F32 : x_dtype == TGOHIP_F16 ? XK_F16 : XK_X2;
+    a.base = base;
+    a.y = y;
+    a.y_f16 = y_dtype == TGOHIP_F16;
+    a.u = (float*)r->u.p;
+    OnDevice on(c->device);
+    a.splits = r->splits;
+    a.rank_pad = s->rank_pad;
+    a.pair = (half_t*)(a.u + (size_t)r->splits * T * kAdapterMaxRank);  // as many bytes as a plane
+    a.pair_scale = a.u + (size_t)(r->splits + 1) * T * kAdapterMaxRank;
+    launch_adapters(a, r->tile_rows, c->ncu, c->stream);
+    TGOHIP_HIP(hipGetLastError());
+    return 0;
+  });
 }
 
 }  // extern "C"
