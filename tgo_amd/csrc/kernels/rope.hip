@@ -89,7 +89,6 @@ __device__ __forceinline__ void rope_heads(const RopeArgs& a, const RopeGroup& g
   // where the unit's elements lie in a head: two runs of V, or one of 2V
   const int ja = !turn ? (g.rotate ? a.rd : 0) + 2 * V * (u - rot) : HALF ? V * u : 2 * V * u;
   const int jb = turn && HALF ? ja + pairs : ja + V;
-#pragma unroll 4
   for (int r = slot; r < rows * g.heads; r += slots) {
     const int t = (int)(((uint64_t)r * g.magic) >> 32), h = r - t * g.heads;
     const int64_t x = (t0 + t) * g.x_row + h * g.x_head, y = (t0 + t) * g.y_row + h * g.y_head;
