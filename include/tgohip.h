@@ -311,10 +311,11 @@ int tgohip_dequant_f16(tgohip_ctx* ctx, int handle, uint16_t* y);
  * For a caller that composes its own layer: what its requests, positions and
  * sequences need is made once (per model, per batch) under a handle, and every
  * layer's calls then only launch kernels on the context's stream. Such calls
- * can be captured into a HIP graph; making, changing or freeing a handle can
- * not, and a handle that a graph was captured with is not replaced or freed while
- * the graph is used (its memory may move). No counterpart in the reference, whose step has one unscaled rotary
- * layout, no adapters, and attention over the block pool only. */
+ * can be captured into a HIP graph; making, changing or freeing a handle is
+ * refused then (TGOHIP_ESTATE), and a handle that a graph was captured with is not
+ * replaced or freed while the graph is used (its memory may move). No counterpart
+ * in the reference, whose step has one unscaled rotary layout, no adapters, and
+ * attention over the block pool only. */
 
 /* Rotary positions. Pair i of a head's first rotary_dim dims turns by
  * position * w_i: (a, b) becomes m (a cos - b sin, a sin + b cos); the dims from
@@ -352,8 +353,8 @@ int tgohip_rope_new(tgohip_ctx* ctx, const tgohip_rope_cfg* cfg, int* handle);
 int tgohip_rope_free(tgohip_ctx* ctx, int handle);
 /* One tensor of heads: element j of head h of row t at x[t x_row + h x_head + j].
  * Strides are in elements, at most 2^36; x's may be 0 (one row or head for all),
- * y's heads must not overlap. rotate 0 copies x to y (a value head narrowed to f16 beside
- * the rotated ones). */
+ * y's heads must not overlap. rotate 0 copies x to y (a value head narrowed to f16
+ * beside the rotated ones). */
 typedef struct {
   const void* x;
   void* y;
@@ -364,7 +365,7 @@ typedef struct {
  * (device int32, any value). Angles are reduced in double, products are f32 and
  * a f16 y is rounded once. y may be its own x (same type and strides: in place)
  * or lie apart from every x and other y of the call, also between the columns
- * of the same rows; anything else is refused. */
+ * of the same rows, and from positions; anything else is refused. */
 int tgohip_rope(tgohip_ctx* ctx, int handle, const int32_t* positions, int T,
                 const tgohip_rope_heads* heads, int n);
 
@@ -373,9 +374,10 @@ int tgohip_rope(tgohip_ctx* ctx, int handle, const int32_t* positions, int T,
  * be 0). causal: query i of n_q sits at position n_kv - n_q + i and sees the keys
  * up to it; otherwise every key. A query that sees no key gives zeros, and no
  * key or value that a query does not see (another sequence's, a later token's)
- * reaches its output, infinities and NaN included (a value it does see may turn
- * an infinity into NaN with f32 queries: a pair's lo part may be 0). Each kv head
- * serves H / H_kv neighbouring query heads. head_dim 64 or 128.
+ * reaches its output, infinities and NaN included (an infinite value that it does
+ * see may give NaN in place of the infinity: its f16 probability, or the lo part of
+ * a pair's, may be 0). Each kv head serves H / H_kv neighbouring query heads, H at
+ * most 65536. head_dim 64 or 128.
  * packed_plan decomposes the batch under *handle (host arrays; *handle 0: a new
  * one; a plan's handle: that plan is replaced in stream order, its memory
  * reused). It holds the partial results of contexts split over several
@@ -398,11 +400,11 @@ int tgohip_packed_describe(int B, const int32_t* q_lengths, const int32_t* kv_le
  * plan's q_dtype, k and v [key rows, H_kv, head_dim] f16, out like q in f32, f16
  * or as a pair (TGOHIP_F16X2, dense rows, the lo plane behind the hi plane). Rows
  * are *_row elements apart (k's and v's at most 2^24, q's and out's 2^30), heads
- * dense; rows start on 16-byte boundaries. scale > 0. With f32 queries the products
- * are those of tgohip_paged_attention's f32 form (q and the probabilities as f16 hi + lo pairs, so |q| < 65504); with
- * f16 queries the probabilities are rounded to f16. Sums, maxima and partial
- * results are f32. Memory behind the last row stays as it is; out meets none of
- * q, k and v. */
+ * dense; rows start on 16-byte boundaries. scale is above 0 and at most 2^32. With
+ * f32 queries the products are those of tgohip_paged_attention's f32 form (q and
+ * the probabilities as f16 hi + lo pairs, so |q| < 65504); with f16 queries the
+ * probabilities are rounded to f16. Sums, maxima and partial results are f32.
+ * Memory behind the last row stays as it is; out meets none of q, k and v. */
 int tgohip_packed_attention(tgohip_ctx* ctx, int handle, const void* q, int64_t q_row, const void* k,
                             int64_t k_row, const void* v, int64_t v_row, float scale, void* out,
                             int64_t out_row, int out_dtype);
@@ -412,13 +414,14 @@ int tgohip_packed_attention(tgohip_ctx* ctx, int handle, const void* q, int64_t 
  * with the adapter of the request row t belongs to, y[t] = base[t] for a request
  * without one. base is what tgohip_linear wrote.
  * adapters_new makes a set of up to `capacity` adapters of one projection (K a
- * multiple of 64, N of 32, each up to 2^22). adapters_put loads one at an index, replacing what
- * was there: host planes down [rank,K] and up [N,rank], f32 (rounded to the
- * nearest f16, refused past its range) or f16, rank 1 to 128. adapters_drop empties an index. An
- * empty index is no adapter. put, drop and free wait for the context's stream. A
- * captured call sees later puts and drops; it is captured for the largest rank
- * loaded so far (of 16, 32, 64 and 128), and rows of an adapter put later beyond
- * that are NaN in its replays. */
+ * multiple of 64, N of 32, each up to 2^22). adapters_put loads one at an index,
+ * replacing what was there: host planes down [rank,K] and up [N,rank], f32 (rounded
+ * to the nearest f16, refused past its range) or f16, rank 1 to 128. adapters_drop
+ * empties an index. An empty index is no adapter. put, drop and free wait for the
+ * context's stream; a graph of other streams that uses the set is waited for by its
+ * owner. A captured call sees later puts and drops; it is captured for the largest
+ * rank loaded so far (of 16, 32, 64 and 128), and rows of an adapter put later
+ * beyond that are NaN in its replays. */
 int tgohip_adapters_new(tgohip_ctx* ctx, int K, int N, int capacity, int* handle);
 int tgohip_adapters_put(tgohip_ctx* ctx, int handle, int index, int rank, int dtype,
                         const void* down, const void* up, float scale);

@@ -94,7 +94,7 @@ def plan(nq, nk, H=8, Hkv=2, d=128, q=tgo_amd.F32, B=None):
     (dict(nq=[1], nk=[1], q=tgo_amd.F16X2), "q_dtype is 2"), (dict(nq=[4, -1], nk=[4, 4]), "sequence 1 has -1 queries"),
     (dict(nq=[4, 1], nk=[-7, 4]), "and -7 keys"), (dict(nq=[1 << 28], nk=[4]), "below 2\\^30"),
     (dict(nq=[1] * 4, nk=[1 << 29] * 4), "below 2\\^30"), (dict(nq=[3], nk=[5]), "context is missing"),
-    (dict(nq=[], nk=[]), "context is missing"),
+    (dict(nq=[], nk=[]), "context is missing"), (dict(nq=[1], nk=[1], H=65538, Hkv=2), "65538 query heads; at most 65536"),
 ])
 def test_packed_plan_refusals(kw, word):
     import re

@@ -881,3 +881,116 @@ def test_captured_adapters_and_split_attention_replay(ctx, torch_gpu):
         for f, a in ((ctx.adapters_free, s), (ctx.adapter_rows_free, rows), (ctx.adapter_rows_free, rows2),
                      (ctx.packed_free, plan), (ctx.packed_free, plan2)):
             f(a)
+
+
+def test_one_row_of_strange_strides_and_its_refusals(ctx, torch_gpu):
+    """A single row's stride says nothing: the pair's lo plane is a row's width behind the hi plane, and the
+    check of what it meets goes by that. A scale past 2^32 is refused."""
+    torch, L = torch_gpu, tgo_amd.lib()
+    H, Hkv, d, nk = 4, 2, 64, 50
+    q, k, v = inputs(torch, [1], [nk], H, Hkv, d, False)
+    out = torch.full((3, H * d), 5.0, device="cuda", dtype=torch.float16)
+    want = attend(ctx, torch, q, k, v, [1], [nk], out=torch.empty_like(q), scale=0.1)
+    plan = ctx.packed_plan([1], [nk], H, Hkv, head_dim=d)
+    try:
+        def call(q=q.data_ptr(), out=out.data_ptr(), out_row=0, scale=0.1):
+            rc = L.tgohip_packed_attention(ctx.h, plan, q, -7, k.data_ptr(), 128, v.data_ptr(), 128, scale, out, out_row,
+                                           tgo_amd.F16X2)
+            return "" if rc == 0 else tgo_amd.last_error()
+        joint = torch.zeros(4, H * d, device="cuda")  # q in the place of the lo plane
+        for row in (0, -4096, 1 << 40):
+            assert "out meets q" in call(q=joint.data_ptr() + 2 * H * d, out=joint.data_ptr(), out_row=row)
+            assert call(out_row=row) == ""
+            torch.cuda.synchronize()
+            pair = out[0].double() + out[1].double()
+            # the pair's own rounding: 2^-22 of the value and an f16 step of its lo part
+            assert bool(((pair - want.reshape(-1).double()).abs() <= 2.0 ** -22 * want.reshape(-1).double().abs() + 2.0 ** -25).all())
+            assert bool((out[2] == 5.0).all())
+        assert "at most 2^32" in call(scale=2.0 ** 33)
+    finally:
+        ctx.packed_free(plan)
+
+
+def test_operands_of_the_host_and_positions_as_an_output_are_refused(ctx, torch_gpu):
+    torch = torch_gpu
+    L = tgo_amd.lib()
+    h = ctx.rope_new(64, 1e4)
+    s, rows, plan = ctx.adapters_new(64, 32, 1), ctx.adapter_rows([2], [0]), ctx.packed_plan([2], [2], 1, 1, head_dim=64)
+    try:
+        x, pos = torch.zeros(2, 1, 64, device="cuda"), torch.zeros(2, device="cuda", dtype=torch.int32)
+        half = x.half()
+        buf = torch.zeros(256, device="cuda")
+        with pytest.raises(TgoError, match="of the host"):
+            ctx.rope(h, pos.cpu(), [(x, x)])
+        with pytest.raises(TgoError, match="of the host"):
+            ctx.rope(h, pos, [(x.cpu(), x)])
+        with pytest.raises(TgoError, match="of the host"):
+            ctx.packed_attention(plan, x, half, half.cpu(), torch.zeros_like(x), 0.1)
+        with pytest.raises(TgoError, match="of the host"):
+            ctx.packed_attention(plan, x, half, half, torch.zeros(2, 2, 1, 64, dtype=torch.float16), 0.1)
+        y = torch.zeros(2, 32, device="cuda")
+        for bad in (dict(x=x.cpu()), dict(y=y.cpu()), dict(base=y.cpu())):
+            with pytest.raises(TgoError, match="of the host"):
+                ctx.adapters(s, rows, **dict(dict(x=x, base=y, y=y), **bad))
+        # fewer rows than the batch, another type than said
+        for bad in (dict(x=x[:1]), dict(y=y[:1]), dict(base=y[:1]), dict(x=half), dict(y=y.half()), dict(x=half, x_dtype=tgo_amd.F16X2),
+                    dict(base=y.half(), y_dtype=tgo_amd.F32)):
+            with pytest.raises(TgoError, match="2 rows of \\[64, 32\\]"):
+                ctx.adapters(s, rows, **dict(dict(x=x, base=y, y=y), **bad))
+        g = (tgo_amd.RopeHeads * 1)(tgo_amd.RopeHeads(x.data_ptr(), buf.data_ptr(), 64, 64, 64, 64, 1, 0, 0, 1))
+        assert L.tgohip_rope(ctx.h, h, buf.data_ptr() + 4 * 127, 2, g, 1) == tgo_amd.EINVAL
+        assert "meets positions" in tgo_amd.last_error()
+        assert L.tgohip_rope(ctx.h, h, buf.data_ptr() + 2, 2, g, 1) == tgo_amd.EINVAL
+        assert "device buffer of int32" in tgo_amd.last_error()
+        assert L.tgohip_rope(ctx.h, h, buf.data_ptr() + 4 * 128, 2, g, 1) == 0
+        torch.cuda.synchronize()
+    finally:
+        for f, a in ((ctx.rope_free, h), (ctx.adapters_free, s), (ctx.adapter_rows_free, rows), (ctx.packed_free, plan)):
+            f(a)
+
+
+def test_handles_are_not_made_or_changed_under_capture(ctx, torch_gpu):
+    """Every call that makes, changes or frees a handle is refused while the stream is captured, and the
+    capture goes on: the graph holds the calls made between the refusals."""
+    torch = torch_gpu
+    h = ctx.rope_new(64, 1e4)
+    s, rows, plan = ctx.adapters_new(64, 32, 1), ctx.adapter_rows([2], [0]), ctx.packed_plan([2], [2], 1, 1, head_dim=64)
+    down, up = np.ones((4, 64), np.float32), np.ones((32, 4), np.float32)
+    ctx.adapters_put(s, 0, down, up, 1.0)
+    x, pos = torch.randn(2, 1, 64, device="cuda"), torch.arange(2, device="cuda", dtype=torch.int32)
+    y, base, out = torch.empty_like(x), torch.randn(2, 32, device="cuda"), torch.empty(2, 32, device="cuda")
+
+    def run():
+        ctx.rope(h, pos, [(x, y)])
+        ctx.adapters(s, rows, x, base, out)
+    try:
+        run()
+        torch.cuda.synchronize()
+        ey, eo = y.clone(), out.clone()
+        calls = [lambda: ctx.rope_new(64, 1e4), lambda: ctx.rope_free(h), lambda: ctx.packed_plan([2], [2], 1, 1, head_dim=64),
+                 lambda: ctx.packed_plan([2], [2], 1, 1, head_dim=64, plan=plan), lambda: ctx.packed_free(plan),
+                 lambda: ctx.adapters_new(64, 32, 1), lambda: ctx.adapters_put(s, 0, down, up, 2.0),
+                 lambda: ctx.adapters_drop(s, 0), lambda: ctx.adapters_free(s), lambda: ctx.adapter_rows([2], [0]),
+                 lambda: ctx.adapter_rows([1], [0], rows=rows), lambda: ctx.adapter_rows_free(rows)]
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        ctx.set_stream(side.cuda_stream)
+        try:
+            with torch.cuda.graph(graph, stream=side):
+                for c in calls[:6]:
+                    with pytest.raises(TgoError, match="being captured"):
+                        c()
+                run()
+                for c in calls[6:]:
+                    with pytest.raises(TgoError, match="being captured"):
+                        c()
+        finally:
+            ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+        for _ in range(3):
+            y.fill_(float("nan"))
+            out.fill_(float("nan"))
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, ey) and torch.equal(out, eo)
+    finally:
+        for f, a in ((ctx.rope_free, h), (ctx.adapters_free, s), (ctx.adapter_rows_free, rows), (ctx.packed_free, plan)):
+            f(a)

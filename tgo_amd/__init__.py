@@ -231,6 +231,8 @@ def _addr(t):
     if t is None:
         return None
     assert t.is_contiguous(), "tensors passed to the C ABI are contiguous"
+    if not t.is_cuda:
+        raise TgoError(EINVAL, "a %s tensor of the host; operands are device tensors" % t.dtype)
     return t.data_ptr()
 
 
@@ -346,6 +348,8 @@ def _heads_view(t, what):
     kind = _kind(t)
     if kind is None:
         raise TgoError(EINVAL, "%s is %s; float32 or float16" % (what, t.dtype))
+    if not t.is_cuda:
+        raise TgoError(EINVAL, "%s is a tensor of the host; operands are device tensors" % what)
     return t.data_ptr(), s[0], s[1], kind
 
 
@@ -555,7 +559,7 @@ class Context:
         if not self.h:
             raise TgoError(EDEVICE, last_error())
         self.cfg = None
-        self._ropes, self._packed, self._sets = {}, {}, {}  # what this binding checks shapes by
+        self._ropes, self._packed, self._sets, self._rows = {}, {}, {}, {}  # what this binding checks shapes by
 
     def close(self):
         if self.h:
@@ -779,7 +783,7 @@ class Context:
         if out.dim() == 4:
             if tuple(out.shape) != (2, tq, H, d) or not out.is_contiguous() or _kind(out) != F16:
                 raise TgoError(EINVAL, "out as a pair is a dense float16 [2, %d, %d, %d]" % (tq, H, d))
-            oa, orow, od = out.data_ptr(), H * d, F16X2
+            oa, orow, od = _addr(out), H * d, F16X2
         else:
             oa, orow, od = _packed_rows(out, "out", tq, H, d, None)
         check(_lib.tgohip_packed_attention(self.h, plan, qa, qr, ka, kr, va, vr, scale, oa, orow, od))
@@ -817,13 +821,22 @@ class Context:
         if len(e) != len(a):
             raise TgoError(EINVAL, "adapter_rows: %d extents and %d adapters" % (len(e), len(a)))
         check(lib().tgohip_adapter_rows(self.h, len(e), ptr(e), ptr(a), ctypes.byref(h)))
+        self._rows[h.value] = int(e.sum(dtype=np.int64))
         return h.value
 
     def adapter_rows_free(self, rows):
         check(lib().tgohip_adapter_rows_free(self.h, rows))
+        self._rows.pop(rows, None)
 
     def adapters(self, handle, rows, x, base, y, x_dtype=F32, y_dtype=F32):
-        """y = base + the adapters' product of x (base None: zeros; y may be base)."""
+        """y = base + the adapters' product of x (base None: zeros; y may be base). Device tensors of at least
+        the batch's rows; x_dtype F16X2: both planes of a pair."""
+        (K, N), T = self._sets.get(handle, (0, 0)), self._rows.get(rows, 0)
+        if (x.numel() < (2 * T * K if x_dtype == F16X2 else T * K) or _kind(x) != (F32 if x_dtype == F32 else F16)
+                or y.numel() < T * N or _kind(y) != y_dtype
+                or (base is not None and (base.numel() < T * N or _kind(base) != y_dtype))):
+            raise TgoError(EINVAL, "adapters: x %s, base and y %s of %d rows of [%d, %d]; x_dtype %d, y_dtype %d" %
+                           (tuple(x.shape), tuple(y.shape), T, K, N, x_dtype, y_dtype))
         check(_lib.tgohip_adapters(self.h, handle, rows, _addr(x), x_dtype, _addr(base), _addr(y), y_dtype))
 
     def greedy(self, logits, B, V, ids, margins=None):

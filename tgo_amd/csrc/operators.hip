@@ -61,6 +61,16 @@ struct OnDevice {
 
 int no_ctx(const char* what) { return fail(TGOHIP_EINVAL, std::string(what) + ": the context is missing"); }
 
+// Making, changing or freeing a handle copies, allocates and waits, which a graph
+// cannot hold.
+int no_capture(tgohip_ctx* c, const char* what) {
+  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+  const hipError_t e = hipStreamIsCapturing(c->stream, &st);
+  if (e != hipSuccess) return fail(TGOHIP_EDEVICE, hip_message(e, what));
+  if (st == hipStreamCaptureStatusNone) return 0;
+  return fail(TGOHIP_ESTATE, std::string(what) + ": the context's stream is being captured");
+}
+
 template <typename T>
 T* find(std::map<int, T>& m, int handle, const char* what) {
   auto it = m.find(handle);
@@ -95,17 +105,31 @@ bool same(const Span& a, const Span& b) {
   return a.p == b.p && a.d == b.d && (a.rows <= 1 || a.row == b.row) && (a.heads <= 1 || a.head == b.head);
 }
 
-// Rounds to the nearest f16, subnormal ones included: an adapter's values sit near
-// the bottom of f16's range, where the loader's rule (tgohip_to_f16) flushes to 0.
+// Rounds to the nearest f16 (ties to even), subnormal ones included: an adapter's
+// values sit near the bottom of f16's range, where the loader's rule
+// (tgohip_to_f16) flushes to 0. Both ranges are computed and one is taken, so that
+// the loop vectorises (a conversion by the compiler's function takes 5 ns a value).
 // False if a finite value is past f16's range.
 bool to_half(const float* src, uint16_t* dst, size_t n) {
-  bool fits = true;
+  uint32_t past = 0;
   for (size_t i = 0; i < n; i++) {
-    const half_t h = (half_t)src[i];
-    fits = fits && (std::isfinite((float)h) || !std::isfinite(src[i]));
-    memcpy(dst + i, &h, 2);
+    uint32_t w;
+    memcpy(&w, src + i, 4);
+    const uint32_t mag = w & 0x7fffffffu;
+    float f;
+    memcpy(&f, &mag, 4);
+    f += 0.5f;  // of 2^-24 an ulp, f16's subnormal step
+    uint32_t small;
+    memcpy(&small, &f, 4);
+    small -= 0x3f000000u;
+    const uint32_t normal = (mag + 0xfffu + ((mag >> 13) & 1) - (112u << 23)) >> 13;
+    uint32_t h = mag < (113u << 23) ? small : normal;
+    const uint32_t over = mag < 0x7f800000u && mag >= 0x477ff000u;  // 65520 rounds to 2^16
+    past |= over;
+    h = mag >= 0x7f800000u ? (mag > 0x7f800000u ? 0x7e00u : 0x7c00u) : h;
+    dst[i] = (uint16_t)(h | ((w >> 16) & 0x8000u));
   }
-  return fits;
+  return !past;
 }
 
 std::string num(double v) {
@@ -175,6 +199,7 @@ int check_packed(int B, const int32_t* nq, const int32_t* nk, int H, int Hkv, in
   if (H <= 0 || Hkv <= 0 || H % Hkv != 0)
     return fail(TGOHIP_EINVAL, "packed_plan: " + std::to_string(H) + " query heads over " + std::to_string(Hkv) +
                                    " kv heads; each kv head serves the same number of query heads");
+  if (H > 65536) return fail(TGOHIP_EINVAL, "packed_plan: " + std::to_string(H) + " query heads; at most 65536");
   if (q_dtype != TGOHIP_F32 && q_dtype != TGOHIP_F16)
     return fail(TGOHIP_EINVAL, "packed_plan: q_dtype is " + std::to_string(q_dtype) + "; queries are f32 or f16");
   int64_t tq = 0, tk = 0;
@@ -198,11 +223,13 @@ extern "C" {
 // ---- rotary positions ---------------------------------------------------------
 
 int tgohip_rope_freqs(const tgohip_rope_cfg* cfg, double* inv_freq, double* attention) {
-  const int rc = check_rope(cfg);
-  if (rc) return rc;
-  if (!inv_freq || !attention) return fail(TGOHIP_EINVAL, "rope_freqs: inv_freq and attention are host buffers");
-  rope_freqs(*cfg, inv_freq, attention);
-  return 0;
+  return guarded([&]() -> int {
+    const int rc = check_rope(cfg);
+    if (rc) return rc;
+    if (!inv_freq || !attention) return fail(TGOHIP_EINVAL, "rope_freqs: inv_freq and attention are host buffers");
+    rope_freqs(*cfg, inv_freq, attention);
+    return 0;
+  });
 }
 
 int tgohip_rope_new(tgohip_ctx* c, const tgohip_rope_cfg* cfg, int* handle) {
@@ -212,6 +239,7 @@ int tgohip_rope_new(tgohip_ctx* c, const tgohip_rope_cfg* cfg, int* handle) {
     if (!c) return no_ctx("rope_new");
     if (!handle) return fail(TGOHIP_EINVAL, "rope_new: handle is missing");
     OnDevice on(c->device);
+    if ((rc = no_capture(c, "rope_new"))) return rc;
     double w[kRopeMaxHeadDim / 2], attention;
     rope_freqs(*cfg, w, &attention);
     for (int i = 0; i < cfg->rotary_dim / 2; i++) w[i] /= 2.0 * M_PI;
@@ -239,6 +267,7 @@ int tgohip_rope_free(tgohip_ctx* c, int handle) {
     RopeTable* t = find(c->ops.ropes, handle, "rope_free");
     if (!t) return TGOHIP_EINVAL;
     OnDevice on(c->device);
+    if (const int rc = no_capture(c, "rope_free")) return rc;
     TGOHIP_HIP(hipStreamSynchronize(c->stream));
     t->inv_freq.release();
     c->ops.ropes.erase(handle);
@@ -255,7 +284,8 @@ int tgohip_rope(tgohip_ctx* c, int handle, const int32_t* positions, int T, cons
     if (n < 1 || n > kRopeGroups || !heads)
       return fail(TGOHIP_EINVAL, "rope: " + std::to_string(n) + " tensors of heads; 1 to " + std::to_string(kRopeGroups));
     if (T == 0) return 0;
-    if (!positions) return fail(TGOHIP_EINVAL, "rope: positions is a device buffer");
+    if (!positions || (uintptr_t)positions % 4) return fail(TGOHIP_EINVAL, "rope: positions is a device buffer of int32");
+    const Span at{(const char*)positions, 1, 1, 0, 0, (int64_t)T * 4};
     RopeArgs a{};
     Span xs[kRopeGroups], ys[kRopeGroups];
     for (int i = 0; i < n; i++) {
@@ -290,7 +320,9 @@ int tgohip_rope(tgohip_ctx* c, int handle, const int32_t* positions, int T, cons
       ys[i] = Span{(const char*)g.y, T, g.heads, g.y_row * elt(yf), g.y_head * elt(yf), t->d * elt(yf)};
       a.g[i] = RopeGroup{g.x, g.y, g.x_row, g.x_head, g.y_row, g.y_head, g.heads, xf, yf, g.rotate != 0, 0};
     }
-    for (int i = 0; i < n; i++)
+    for (int i = 0; i < n; i++) {
+      if (meet(ys[i], at))
+        return fail(TGOHIP_EINVAL, "rope: y of tensor " + std::to_string(i) + " meets positions in memory");
       for (int j = 0; j < n; j++) {
         if (meet(ys[i], xs[j]) && !(i == j && a.g[i].x_f16 == a.g[i].y_f16 && same(ys[i], xs[i])))
           return fail(TGOHIP_EINVAL, "rope: y of tensor " + std::to_string(i) + " meets x of tensor " + std::to_string(j) +
@@ -298,6 +330,7 @@ int tgohip_rope(tgohip_ctx* c, int handle, const int32_t* positions, int T, cons
         if (i < j && meet(ys[i], ys[j]))
           return fail(TGOHIP_EINVAL, "rope: y of tensors " + std::to_string(i) + " and " + std::to_string(j) + " meet in memory");
       }
+    }
     a.positions = positions;
     a.inv_freq = (const double*)t->inv_freq.p;
     a.attention = t->attention;
@@ -324,6 +357,7 @@ int tgohip_packed_plan(tgohip_ctx* c, int B, const int32_t* q_lengths, const int
     if (!handle) return fail(TGOHIP_EINVAL, "packed_plan: handle is missing");
     if (*handle && !find(c->ops.packed, *handle, "packed_plan")) return TGOHIP_EINVAL;
     OnDevice on(c->device);
+    if ((rc = no_capture(c, "packed_plan"))) return rc;
     PackedPlan plan;
     packed_build_plan(B, q_lengths, kv_lengths, H, H_kv, head_dim, causal != 0, q_dtype == TGOHIP_F16, c->ncu, plan);
     const size_t items = plan.items.size();
@@ -382,6 +416,7 @@ int tgohip_packed_free(tgohip_ctx* c, int handle) {
     PackedHandle* p = find(c->ops.packed, handle, "packed_free");
     if (!p) return TGOHIP_EINVAL;
     OnDevice on(c->device);
+    if (const int rc = no_capture(c, "packed_free")) return rc;
     TGOHIP_HIP(hipStreamSynchronize(c->stream));
     p->meta.release();
     p->part.release();
@@ -398,8 +433,8 @@ int tgohip_packed_attention(tgohip_ctx* c, int handle, const void* q, int64_t q_
     if (!p) return TGOHIP_EINVAL;
     const PackedPlan& pl = p->plan;
     if (!pl.D) return fail(TGOHIP_ESTATE, "packed_attention: the plan was not made again after a failure");
-    if (!(scale > 0.f) || !std::isfinite(scale))
-      return fail(TGOHIP_EINVAL, "packed_attention: scale is " + num(scale) + "; a finite number above 0");
+    if (!(scale > 0.f) || scale > 0x1p32f)  // scores stay below 2^72, and above kPackNoMax
+      return fail(TGOHIP_EINVAL, "packed_attention: scale is " + num(scale) + "; a number above 0, at most 2^32");
     if (out_dtype != TGOHIP_F32 && out_dtype != TGOHIP_F16 && out_dtype != TGOHIP_F16X2)
       return fail(TGOHIP_EINVAL, "packed_attention: out_dtype is " + std::to_string(out_dtype) + "; f32, f16 or a pair");
     if (pl.tq == 0) return 0;
@@ -426,7 +461,7 @@ int tgohip_packed_attention(tgohip_ctx* c, int handle, const void* q, int64_t q_
       return fail(TGOHIP_EINVAL, "packed_attention: a pair's rows are dense (out_row " + std::to_string(out_row) + ", not " +
                                      std::to_string(qw) + ")");
     const int64_t ob = out_dtype == TGOHIP_F32 ? 4 : 2, planes = out_dtype == TGOHIP_F16X2 ? 2 : 1;
-    const Span so{(const char*)out, planes * pl.tq, 1, out_row * ob, 0, qw * ob};
+    const Span so{(const char*)out, planes * pl.tq, 1, (pl.tq > 1 ? out_row : qw) * ob, 0, qw * ob};
     const Span in[] = {{(const char*)q, pl.tq, 1, q_row * elt(pl.q_f16), 0, qw * elt(pl.q_f16)},
                        {(const char*)k, pl.tk, 1, k_row * 2, 0, kw * 2},
                        {(const char*)v, pl.tk, 1, v_row * 2, 0, kw * 2}};
@@ -466,6 +501,7 @@ int tgohip_adapters_new(tgohip_ctx* c, int K, int N, int capacity, int* handle) 
     if (!c) return no_ctx("adapters_new");
     if (!handle) return fail(TGOHIP_EINVAL, "adapters_new: handle is missing");
     OnDevice on(c->device);
+    if (const int rc = no_capture(c, "adapters_new")) return rc;
     AdapterSet s;
     s.K = K;
     s.N = N;
@@ -510,6 +546,7 @@ int tgohip_adapters_put(tgohip_ctx* c, int handle, int index, int rank, int dtyp
     if (index < 0 || index >= (int)s->table.size())
       return fail(TGOHIP_EINVAL, "adapters_put: index " + std::to_string(index) + " of a set of " + std::to_string(s->table.size()));
     OnDevice on(c->device);
+    if (const int rc = no_capture(c, "adapters_put")) return rc;
     // down [rank][K] with rows of zeros, up [N][rank] with columns of zeros, to a
     // rank the kernels' products take whole; one allocation
     const int rp = rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128;
@@ -547,6 +584,7 @@ int tgohip_adapters_drop(tgohip_ctx* c, int handle, int index) {
     if (index < 0 || index >= (int)s->table.size())
       return fail(TGOHIP_EINVAL, "adapters_drop: index " + std::to_string(index) + " of a set of " + std::to_string(s->table.size()));
     OnDevice on(c->device);
+    if (const int rc = no_capture(c, "adapters_drop")) return rc;
     return adapter_set(c, s, index, AdapterEntry{nullptr, nullptr, 0, 0.f});
   });
 }
@@ -557,6 +595,7 @@ int tgohip_adapters_free(tgohip_ctx* c, int handle) {
     AdapterSet* s = find(c->ops.sets, handle, "adapters_free");
     if (!s) return TGOHIP_EINVAL;
     OnDevice on(c->device);
+    if (const int rc = no_capture(c, "adapters_free")) return rc;
     TGOHIP_HIP(hipStreamSynchronize(c->stream));
     for (AdapterEntry& e : s->table) (void)hipFree((void*)e.down);
     s->table_dev.release();
@@ -583,6 +622,7 @@ int tgohip_adapter_rows(tgohip_ctx* c, int B, const int32_t* extents, const int3
     if (!handle) return fail(TGOHIP_EINVAL, "adapter_rows: handle is missing");
     if (*handle && !find(c->ops.rows, *handle, "adapter_rows")) return TGOHIP_EINVAL;
     OnDevice on(c->device);
+    if (const int rc = no_capture(c, "adapter_rows")) return rc;
     // rows by adapter, in their own order within one, in tiles of 16 (decode batches:
     // most adapters have a few rows) or 64 (prompts: an adapter is read once per tile)
     const size_t tile = T <= kAdapterFewRows ? 16 : 64;
@@ -635,6 +675,7 @@ int tgohip_adapter_rows_free(tgohip_ctx* c, int handle) {
     AdapterRows* r = find(c->ops.rows, handle, "adapter_rows_free");
     if (!r) return TGOHIP_EINVAL;
     OnDevice on(c->device);
+    if (const int rc = no_capture(c, "adapter_rows_free")) return rc;
     TGOHIP_HIP(hipStreamSynchronize(c->stream));
     r->meta.release();
     r->u.release();
