@@ -126,8 +126,9 @@ void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int H
 // kernels
 // ---------------------------------------------------------------------------
 
-// s_waitcnt vmcnt(0), the other counters not waited for.
-constexpr int kPackVm0 = 0x0f70;
+// s_waitcnt vmcnt(0) lgkmcnt(0): the wave's DMA has landed, and its LDS reads have
+// returned, before other data goes where they read.
+constexpr int kPackWait = 0x0070;
 // A barrier without a memory fence, which would wait for every DMA in flight; no
 // memory access moves across it.
 __device__ __forceinline__ void pack_barrier() {
@@ -576,7 +577,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_kernel(PackedArgs a) {
   auto tile = [&](int t0, lds_t K, lds_t V, lds_t Kn, lds_t Vn) {
     // this wave's DMA of the tile has landed, every wave's has, and every wave is
     // done with the other buffer
-    __builtin_amdgcn_s_waitcnt(kPackVm0);
+    __builtin_amdgcn_s_waitcnt(kPackWait);
     pack_barrier();
     dma(t0 + kPackTile, Kn, Vn);
     if (t0 > whi) return;  // no row of this wave sees the tile
@@ -668,7 +669,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void packed_few_kernel(PackedArg
   auto run = [&](auto mode) {
     constexpr int MODE = decltype(mode)::value;
     auto tile = [&](int t0, lds_t K, lds_t V, lds_t Kn, lds_t Vn) {
-      __builtin_amdgcn_s_waitcnt(kPackVm0);
+      __builtin_amdgcn_s_waitcnt(kPackWait);
       asm volatile("" ::: "memory");
       dma(t0 + step, Kn, Vn);
       if (t0 > whi) return;
