@@ -10,81 +10,156 @@
 //   adapter_pair_kernel  (tiles of 64 rows) the planes' sums, as scaled f16 pairs
 //   adapter_up_kernel    y = base + s u . up^T; with tiles of 16 rows it sums the
 //                        planes itself, a launch less
+// Measured, the three together (us; bytes are x, base, y and each adapter once):
+//   1 row, rank 16, [4096, 4096]                7.5, 3.3 and 3.6 of them the kernels
+//   128 rows of 32 adapters, [4096, 6144]       10.8, 1.7 TB/s
+//   1152 rows, rank 64, [4096, 24576]           103, 3.4 TB/s: 15, 5 and 84
+//   8000 f16 rows, rank 24, [12288, 4096]       80, 3.8 TB/s: 38, 5 and 34
 // Both products in one launch, each workgroup computing its tile's u, was slower for
 // all but the smallest K: one row of [4096, 4096] 9.4 us for 8.0, 128 rows of
 // [12288, 4096] 27.9 for 12.0, 16 rows of [1024, 4096] 6.1 for 6.9.
 // Both use v_mfma_f32_16x16x32_f16 (16x16x16 for rank 16): lane (l16, q) =
-// (lane % 16, lane / 16) holds row or column l16 of an operand at k 8q + [0,8),
-// and of the result column l16, rows 4q + [0,4).
+// (lane % 16, lane / 16) holds row or column l16 of an operand at eight k of its own,
+// the same of both operands, and of the result column l16, rows 4q + [0,4).
 #include "operators.h"
 
 #include <algorithm>
 
 namespace tgohip {
 
-// x of rows `off` elements in, at k .. k + 8: the hi part, and lo where there is one.
+// Eight f32 as f16 hi + lo.
+__device__ __forceinline__ void adapter_split(float4_t u, float4_t v, half8_t& hi, half8_t& lo) {
+#pragma unroll
+  for (int j = 0; j < 8; j++) {
+    const float f = j < 4 ? u[j & 3] : v[j & 3];
+    hi[j] = (half_t)f;
+    lo[j] = (half_t)(f - (float)hi[j]);
+  }
+}
+// Eight values of x at `off` elements, as the hi part of the product (and lo).
 template <int XK>
 __device__ __forceinline__ void adapter_load_x(const AdapterArgs& a, int64_t off, half8_t& hi, half8_t& lo) {
   if constexpr (XK == XK_F32) {
     const float4_t u = *(const float4_t*)((const float*)a.x + off), v = *(const float4_t*)((const float*)a.x + off + 4);
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const float f = j < 4 ? u[j & 3] : v[j & 3];
-      hi[j] = (half_t)f;
-      lo[j] = (half_t)(f - (float)hi[j]);
-    }
+    adapter_split(u, v, hi, lo);
   } else {
     hi = *(const half8_t*)((const half_t*)a.x + off);
     if constexpr (XK == XK_X2) lo = *(const half8_t*)((const half_t*)a.x + (int64_t)a.T * a.K + off);
   }
 }
 
-// Waves take 32-k steps of the workgroup's share of K in turn, so that every
-// wave streams its own lines of x and down, and their sums meet in LDS.
-template <int XK, int TB, int RB>
-__global__ __launch_bounds__(256) void adapter_down_kernel(AdapterArgs a) {
-  __shared__ float part[4][16][RB * 16];
-  const AdapterTile t = a.tiles[blockIdx.x];
-  if (t.adapter < 0) return;
-  const AdapterEntry e = a.table[t.adapter];
-  if (e.rank_pad == 0 || e.rank_pad > RB * 16) return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l16 = lane & 15, q = lane >> 4;
-  const int nrb = e.rank_pad / 16;
-  const int steps = a.K / 32;
-  const int s0 = (int)((int64_t)steps * blockIdx.y / gridDim.y), s1 = (int)((int64_t)steps * (blockIdx.y + 1) / gridDim.y);
-  int64_t row[TB];
+// Up to 16 rows of a tile, 64-k units [s0, s1) of its workgroup's share: waves take
+// runs of two units in turn. A lane's two loads of a unit lie side by side (its k are
+// 16q + 8g + [0,8)), so that a unit is whole lines of x and down.
+template <int XK, int RB>
+__device__ __forceinline__ void adapter_down_16(const AdapterArgs& a, const AdapterTile& t, const AdapterEntry& e, int s0,
+                                                int s1, int wave, float4_t (&acc)[1][RB]) {
+  const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4, nrb = e.rank_pad / 16;
+  // rows past the tile and ranks past the adapter repeat the last ones, whose results are not stored
+  const int64_t row = (int64_t)a.perm[t.start + min(l16, t.n - 1)] * a.K + 16 * q;
+  const half_t* dn = e.down + (int64_t)l16 * a.K + 16 * q;
+  for (int j = 0; s0 + 8 * (j / 2) + 2 * wave + j % 2 < s1; j++) {
+    const int k = 64 * (s0 + 8 * (j / 2) + 2 * wave + j % 2);
+    half8_t d[RB][2], hi[2], lo[2];
 #pragma unroll
-  for (int b = 0; b < TB; b++) row[b] = (int64_t)a.perm[t.start + min(b * 16 + l16, t.n - 1)] * a.K + 8 * q;
-  const half_t* dn = e.down + (int64_t)l16 * a.K + 8 * q;
-  float4_t acc[TB][RB] = {};
-  // branch-free (rows past the tile and ranks past the adapter repeat the last ones,
-  // whose results are not stored), one step loaded ahead
-  half8_t d[RB], hi[TB], lo[TB];
-  auto load = [&](int s) {
+    for (int g = 0; g < 2; g++) {
+      adapter_load_x<XK>(a, row + k + 8 * g, hi[g], lo[g]);
 #pragma unroll
-    for (int b = 0; b < TB; b++) adapter_load_x<XK>(a, row[b] + 32 * s, hi[b], lo[b]);
-#pragma unroll
-    for (int r = 0; r < RB; r++) d[r] = *(const half8_t*)(dn + (int64_t)min(r, nrb - 1) * 16 * a.K + 32 * s);
-  };
-  if (s0 + wave < s1) load(s0 + wave);
-  for (int s = s0 + wave; s < s1; s += 4) {
-    half8_t dc[RB], hc[TB], lc[TB];
-#pragma unroll
-    for (int r = 0; r < RB; r++) dc[r] = d[r];
-#pragma unroll
-    for (int b = 0; b < TB; b++) {
-      hc[b] = hi[b];
-      if (XK != XK_F16) lc[b] = lo[b];
+      for (int r = 0; r < RB; r++) d[r][g] = *(const half8_t*)(dn + (int64_t)min(r, nrb - 1) * 16 * a.K + k + 8 * g);
     }
-    load(min(s + 4, s1 - 1));
 #pragma unroll
-    for (int b = 0; b < TB; b++)
+    for (int g = 0; g < 2; g++)
 #pragma unroll
       for (int r = 0; r < RB; r++) {
-        acc[b][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hc[b], dc[r], acc[b][r], 0, 0, 0);
-        if (XK != XK_F16) acc[b][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lc[b], dc[r], acc[b][r], 0, 0, 0);
+        acc[0][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi[g], d[r][g], acc[0][r], 0, 0, 0);
+        if (XK != XK_F16) acc[0][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo[g], d[r][g], acc[0][r], 0, 0, 0);
       }
   }
+}
+
+constexpr int kAdapterNt = 2;  // the nt bit: x is read once
+typedef __attribute__((address_space(3))) char* adapter_lds;
+// s_waitcnt vmcnt(0) lgkmcnt(0), and no memory access moves across it.
+__device__ __forceinline__ void adapter_wait() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  asm volatile("" ::: "memory");
+}
+
+// Up to 64 rows: x goes through 16 KiB of LDS that are the wave's own by DMA, whole
+// lines of a row at a time, 16-byte chunks XOR-swizzled by the row. Eight waves a CU,
+// each with its buffer on its way, keep the memory busy; no wave waits for another.
+// 7000 f16 rows of K = 12288 and a rank of 24: 37 us, 4.6 TB/s; loaded to registers as
+// half lines 56 us, as the unit above 43 (L1 holds half of what is in flight); without
+// the nt bit 40.
+template <int XK, int RB>
+__device__ __forceinline__ void adapter_down_64(const AdapterArgs& a, const AdapterTile& t, const AdapterEntry& e, int s0,
+                                                int s1, int wave, adapter_lds buf, float4_t (&acc)[4][RB]) {
+  constexpr int RBY = XK == XK_F32 ? 256 : 128;  // bytes of a row's unit in one plane
+  constexpr int CH = RBY / 16, RPI = 64 / CH, NI = 64 / RPI;  // its chunks, rows per instruction, instructions
+  constexpr int U = XK == XK_F16 && RB <= 4 ? 2 : 1;  // units in the buffer at a time (rank 128 has no registers for two)
+  const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4, nrb = e.rank_pad / 16;
+  int64_t at[NI];  // byte offset of the lane's chunk, row by row
+#pragma unroll
+  for (int n = 0; n < NI; n++) {
+    const int m = n * RPI + lane / CH;
+    at[n] = (int64_t)a.perm[t.start + min(m, t.n - 1)] * a.K * (RBY / 64) + 16 * ((lane % CH) ^ (m & 7));
+  }
+  const half_t* dn = e.down + (int64_t)l16 * a.K + 16 * q;
+  for (int s = s0 + U * wave; s < s1; s += 4 * U) {
+    half8_t d[U][RB][2];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (s + u >= s1) break;
+      const char* x = (const char*)a.x + (int64_t)(s + u) * RBY;
+#pragma unroll
+      for (int p = 0; p < (XK == XK_X2 ? 2 : 1); p++)
+#pragma unroll
+        for (int n = 0; n < NI; n++)
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(x + p * (int64_t)a.T * a.K * 2 + at[n]),
+                                           (__attribute__((address_space(3))) void*)(buf + 8192 * (u + p) + 1024 * n), 16, 0, kAdapterNt);
+#pragma unroll
+      for (int r = 0; r < RB; r++)
+#pragma unroll
+        for (int g = 0; g < 2; g++)
+          d[u][r][g] = *(const half8_t*)(dn + (int64_t)min(r, nrb - 1) * 16 * a.K + 64 * (s + u) + 8 * g);
+    }
+    adapter_wait();
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (s + u >= s1) break;
+#pragma unroll
+      for (int b = 0; b < 4; b++)
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+          const adapter_lds row = buf + (16 * b + l16) * RBY;
+          half8_t hi, lo;
+          if constexpr (XK == XK_F32) {
+            typedef __attribute__((address_space(3))) float4_t* f4;
+            const int c = 4 * q + 2 * g;
+            adapter_split(*(f4)(row + 16 * (c ^ (l16 & 7))), *(f4)(row + 16 * ((c + 1) ^ (l16 & 7))), hi, lo);
+          } else {
+            typedef __attribute__((address_space(3))) half8_t* h8;
+            const int c = 16 * ((2 * q + g) ^ (l16 & 7));
+            hi = *(h8)(row + 8192 * u + c);
+            if constexpr (XK == XK_X2) lo = *(h8)(row + 8192 + c);
+          }
+#pragma unroll
+          for (int r = 0; r < RB; r++) {
+            acc[b][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, d[u][r][g], acc[b][r], 0, 0, 0);
+            if (XK != XK_F16) acc[b][r] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, d[u][r][g], acc[b][r], 0, 0, 0);
+          }
+        }
+    }
+    adapter_wait();  // the reads have returned before the next DMA
+  }
+}
+
+// The waves' sums of TB blocks of rows meet in LDS and go to the share's plane.
+template <int TB, int RB>
+__device__ __forceinline__ void adapter_down_out(const AdapterArgs& a, const AdapterTile& t, int rank_pad, int wave,
+                                                 const float4_t (&acc)[TB][RB], float (*part)[16][RB * 16]) {
+  const int tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, q = lane >> 4;
   float* u = a.u + ((int64_t)blockIdx.y * a.T + t.start) * kAdapterMaxRank;
 #pragma unroll
   for (int b = 0; b < TB; b++) {
@@ -96,9 +171,32 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(AdapterArgs a) {
     __syncthreads();
     for (int i = tid; i < 16 * RB * 16; i += 256) {
       const int m = i / (RB * 16), r = i % (RB * 16);
-      if (b * 16 + m < t.n && r < e.rank_pad)
+      if (b * 16 + m < t.n && r < rank_pad)
         u[(b * 16 + m) * kAdapterMaxRank + r] = (part[0][m][r] + part[1][m][r]) + (part[2][m][r] + part[3][m][r]);
     }
+  }
+}
+
+template <int XK, int TB, int RB>
+__global__ __launch_bounds__(256) void adapter_down_kernel(AdapterArgs a) {
+  constexpr int kPart = 4 * 16 * RB * 16 * 4, kBuf = TB > 1 ? 4 * 16384 : 0;
+  __shared__ __attribute__((aligned(1024))) char mem[kPart > kBuf ? kPart : kBuf];
+  const AdapterTile t = a.tiles[blockIdx.x];
+  if (t.adapter < 0) return;
+  const AdapterEntry e = a.table[t.adapter];
+  if (e.rank_pad == 0 || e.rank_pad > RB * 16) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), units = a.K / 64;
+  const int s0 = (int)((int64_t)units * blockIdx.y / gridDim.y), s1 = (int)((int64_t)units * (blockIdx.y + 1) / gridDim.y);
+  float (*part)[16][RB * 16] = (float(*)[16][RB * 16])mem;
+  if (TB == 1 || t.n <= 16) {
+    float4_t acc[1][RB] = {};
+    adapter_down_16<XK, RB>(a, t, e, s0, s1, wave, acc);
+    adapter_down_out<1, RB>(a, t, e.rank_pad, wave, acc, part);
+  } else {
+    float4_t acc[4][RB] = {};
+    adapter_down_64<XK, RB>(a, t, e, s0, s1, wave, (adapter_lds)mem + 16384 * wave, acc);
+    __syncthreads();  // part lies where the DMA went
+    adapter_down_out<4, RB>(a, t, e.rank_pad, wave, acc, part);
   }
 }
 
@@ -148,29 +246,32 @@ __device__ __forceinline__ void adapter_power(float top, float& down, float& up)
 }
 
 // Sums the planes of a tile's rows in their order and leaves them as pairs,
-// [hi 128 | lo 128] a row and 0 from the adapter's rank on, one wave per row and
-// two ranks a lane.
+// [hi 128 | lo 128] a row, 0 from the adapter's rank to the launch's, two ranks a lane.
+template <int RB>
 __global__ __launch_bounds__(256) void adapter_pair_kernel(AdapterArgs a) {
+  constexpr int LR = RB * 8;  // lanes per row
   const AdapterTile t = a.tiles[blockIdx.x];
-  const int m = blockIdx.y * 4 + (threadIdx.x >> 6), r = (threadIdx.x & 63) * 2;
+  const int m = blockIdx.y * (256 / LR) + threadIdx.x / LR, r = threadIdx.x % LR * 2;
   if (t.adapter < 0 || m >= t.n) return;
-  const int rank_pad = a.table[t.adapter].rank_pad;
+  const bool in = r < a.table[t.adapter].rank_pad;
   const int64_t pos = t.start + m;
+  const float* u = a.u + pos * kAdapterMaxRank + (in ? r : 0);
   float s0 = 0.f, s1 = 0.f;
-  if (r < min(rank_pad, a.rank_pad)) {
-    float2 v[kAdapterMaxSplits];
+  for (int p0 = 0; p0 < a.splits; p0 += 4) {
+    float2 v[4];
 #pragma unroll
-    for (int p = 0; p < kAdapterMaxSplits; p++)
-      v[p] = *(const float2*)(a.u + ((int64_t)min(p, a.splits - 1) * a.T + pos) * kAdapterMaxRank + r);
+    for (int p = 0; p < 4; p++) v[p] = *(const float2*)(u + (int64_t)min(p0 + p, a.splits - 1) * a.T * kAdapterMaxRank);
 #pragma unroll
-    for (int p = 0; p < kAdapterMaxSplits; p++) {
-      s0 += p < a.splits ? v[p].x : 0.f;
-      s1 += p < a.splits ? v[p].y : 0.f;
+    for (int p = 0; p < 4; p++) {
+      s0 += p0 + p < a.splits ? v[p].x : 0.f;
+      s1 += p0 + p < a.splits ? v[p].y : 0.f;
     }
   }
+  s0 = in ? s0 : 0.f;
+  s1 = in ? s1 : 0.f;
   float top = fmaxf(fabsf(s0), fabsf(s1)), down, up;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+  for (int o = LR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
   adapter_power(top, down, up);
   s0 *= down;
   s1 *= down;
@@ -368,7 +469,7 @@ template <int XK, int TB, int RB>
 static void adapters_launch(const AdapterArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)a.ntiles, (unsigned)((a.N + a.cols - 1) / a.cols));
   hipLaunchKernelGGL((adapter_down_kernel<XK, TB, RB>), dim3((unsigned)a.ntiles, (unsigned)a.splits), dim3(256), 0, st, a);
-  if (TB > 1) hipLaunchKernelGGL(adapter_pair_kernel, dim3((unsigned)a.ntiles, 4 * TB), dim3(256), 0, st, a);
+  if (TB > 1) hipLaunchKernelGGL((adapter_pair_kernel<RB>), dim3((unsigned)a.ntiles, TB * RB / 2 ? TB * RB / 2 : 1), dim3(256), 0, st, a);
   if (a.y_f16) hipLaunchKernelGGL((adapter_up_kernel<TB, RB, true>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((adapter_up_kernel<TB, RB, false>), grid, dim3(256), 0, st, a);
 }

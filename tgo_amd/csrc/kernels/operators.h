@@ -109,7 +109,9 @@ struct AdapterArgs {
   half_t* pair;  // [T][2][kAdapterMaxRank]: their sums as scaled hi + lo pairs
   float* pair_scale;  // [T]
 };
-// The shares of K for a batch of `tiles` tiles (their planes are the workspace).
+// The shares of K for a batch of `tiles` tiles (their planes are the workspace): up to
+// two workgroups a CU, all on the chip at once. With 1, 2, 3 or 4 per CU, us: 8000 f16
+// rows of [12288, 4096] 86, 81, 92, 86; 1152 pairs of [4096, 24576] 104, 103, 107, 106.
 constexpr int kAdapterMaxSplits = 16;
 inline int adapter_splits(int tiles, int ncu) {
   return tiles > 0 ? std::min(kAdapterMaxSplits, std::max(1, 2 * ncu / tiles)) : 1;
