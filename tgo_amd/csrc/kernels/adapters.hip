@@ -13,8 +13,8 @@
 // Measured, the three together (us; bytes are x, base, y and each adapter once):
 //   1 row, rank 16, [4096, 4096]                7.5, 3.3 and 3.6 of them the kernels
 //   128 rows of 32 adapters, [4096, 6144]       10.8, 1.7 TB/s
-//   1152 rows, rank 64, [4096, 24576]           103, 3.4 TB/s: 15, 5 and 84
-//   8000 f16 rows, rank 24, [12288, 4096]       80, 3.8 TB/s: 38, 5 and 34
+//   1152 rows, rank 64, [4096, 24576]           96, 3.7 TB/s: 15, 5 and 76
+//   8000 f16 rows, rank 24, [12288, 4096]       79, 3.9 TB/s: 38, 5 and 34
 // Both products in one launch, each workgroup computing its tile's u, was slower for
 // all but the smallest K: one row of [4096, 4096] 9.4 us for 8.0, 128 rows of
 // [12288, 4096] 27.9 for 12.0, 16 rows of [1024, 4096] 6.1 for 6.9.
@@ -394,7 +394,9 @@ __device__ __forceinline__ void adapter_columns(const AdapterArgs& a, const Adap
   }
 }
 
-// A tile's rows without an adapter: y = base. False: the rows have one, in e.
+// A tile's rows without an adapter: y = base, eight pieces a thread in flight (one at a
+// time, 1152 rows of which 528 have none took 103 us instead of 96). False: the rows have
+// one, in e.
 template <int RB, bool YF16>
 __device__ __forceinline__ bool adapter_copies(const AdapterArgs& a, const AdapterTile& t, AdapterEntry& e, int n0, int n1) {
   e = AdapterEntry{};
@@ -407,13 +409,19 @@ __device__ __forceinline__ bool adapter_copies(const AdapterArgs& a, const Adapt
   if (e.rank_pad) return false;
   if (a.base == a.y) return true;
   constexpr int PE = YF16 ? 8 : 4;
-  const int w = (n1 - n0) / PE;
-  for (int i = threadIdx.x; i < t.n * w; i += blockDim.x) {
-    const int m = i / w;
-    const int64_t off = (int64_t)a.perm[t.start + m] * a.N + n0 + PE * (i - m * w);
-    float v[PE];
-    adapter_load_piece<YF16>(a, off, v);
-    adapter_store_piece<YF16>(a, off, v);
+  const int w = (n1 - n0) / PE, all = t.n * w;
+  for (int i0 = threadIdx.x; i0 < all; i0 += 8 * 256) {
+    int64_t off[8];
+    float v[8][PE];
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+      const int i = min(i0 + 256 * u, all - 1), m = i / w;
+      off[u] = (int64_t)a.perm[t.start + m] * a.N + n0 + PE * (i - m * w);
+      adapter_load_piece<YF16>(a, off[u], v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 8; u++)
+      if (i0 + 256 * u < all) adapter_store_piece<YF16>(a, off[u], v[u]);
   }
   return true;
 }
@@ -485,8 +493,8 @@ void launch_adapters(const AdapterArgs& args, int tile_rows, int ncu, hipStream_
   AdapterArgs a = args;
   const bool one = tile_rows <= 16;
   // Columns per workgroup of the second kernel, us for 1152 mixed rows of rank 64 over
-  // [4096, 24576] and 8000 f16 rows of rank 24 over [12288, 4096]: 128 columns 108,
-  // 100; 256 106, 96; 512 114, 97; 1024 138, 111.
+  // [4096, 24576] and 8000 f16 rows of rank 24 over [12288, 4096]: 128 columns 98, 84;
+  // 256 96, 79; 512 101, 79; 1024 119, 85.
   a.cols = 256;
   switch (a.xk) {
     case XK_F32: one ? adapters_rank<XK_F32, 1>(a, st) : adapters_rank<XK_F32, 4>(a, st); break;
