@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <functional>
 #include <type_traits>
 
 namespace tgohip {
@@ -29,59 +30,190 @@ constexpr float kPackSum = 32768.f;  // 2^kPackTop
 // decomposition (host)
 // ---------------------------------------------------------------------------
 
-// Orders items longest first, so that the hardware's dispatch, block by block, ends
-// evenly on `slots` workgroups at a time. Where one item is longer than a quarter
-// over a slot's share, items are cut: they fill one slot's share after the other, a
-// piece ending where a share does, at least `least` tiles long. A piece costs `fixed`
-// tiles beside its own (its start, its result and their merge).
-static void pack_cut(const std::vector<PackedItem>& whole, int tile, int slots, int fixed, int least,
+// How items are cut along their keys: the pieces of each, and their tiles, item by item.
+struct PackCut {
+  std::vector<int> pieces, tiles;
+};
+
+// What a kernel's tiles of 64 keys cost: us of one whose workgroup has its CU alone, and
+// the part of that rate each of two workgroups on a CU reaches.
+struct PackRate {
+  double tile, shared;
+};
+constexpr int kPackFixed = 3;  // tiles that a piece costs beside its own: its start and its result
+
+// us until the last piece has ended and the rows of cut items are merged. Pieces are
+// dispatched longest first, two workgroups to a CU; merging costs a launch and, for each
+// row of a partial result, its way to memory and back. Within 15% of what the kernels
+// measure for 18 batches in each of these cuts, but for batches of short pieces.
+static double pack_time(const std::vector<PackedItem>& whole, const PackCut& c, int ncu, const PackRate& rate) {
+  std::vector<int> tiles = c.tiles;
+  std::sort(tiles.begin(), tiles.end(), std::greater<int>());
+  struct Cu {
+    double now = 0, a = 0, b = 0;  // its clock, and what is left of its two pieces, a <= b
+  };
+  std::vector<Cu> cus(std::min<size_t>(tiles.size(), ncu));
+  size_t next = 0;
+  for (; next < tiles.size() && next < 2 * cus.size(); next++) {
+    Cu& u = cus[next % cus.size()];
+    (next < cus.size() ? u.b : u.a) = tiles[next] + kPackFixed;
+  }
+  // the next end on a CU: of the shorter piece while there are two
+  const auto end = [&](const Cu& u) { return u.now + (u.a > 0 ? u.a / rate.shared : u.b); };
+  typedef std::pair<double, int> Event;
+  std::vector<Event> ends;  // a heap, the soonest first
+  for (size_t i = 0; i < cus.size(); i++) ends.push_back({end(cus[i]), (int)i});
+  std::make_heap(ends.begin(), ends.end(), std::greater<Event>());
+  double last = 0;
+  while (!ends.empty()) {
+    const int cu = ends[0].second;
+    Cu& u = cus[cu];
+    last = u.now = ends[0].first;
+    u.b = u.a > 0 ? u.b - u.a : 0;
+    u.a = 0;
+    if (next < tiles.size()) {
+      u.a = tiles[next++] + kPackFixed;
+      if (u.a > u.b) std::swap(u.a, u.b);
+    }
+    // the CU's next end in the place of this one, or the heap's last
+    Event e = {end(u), cu};
+    if (u.b <= 0) {
+      e = ends.back();
+      ends.pop_back();
+    }
+    for (size_t i = 0, k; i < ends.size(); i = k) {
+      k = 2 * i + 1;
+      if (k + 1 < ends.size() && ends[k + 1].first < ends[k].first) k++;
+      if (k >= ends.size() || ends[k].first >= e.first) {
+        ends[i] = e;
+        break;
+      }
+      ends[i] = ends[k];
+    }
+  }
+  int64_t rows = 0;
+  for (size_t i = 0; i < whole.size(); i++)
+    if (c.pieces[i] > 1) rows += (int64_t)c.pieces[i] * whole[i].nr;
+  return last * rate.tile + (rows ? 4.5 + 0.35e-3 * (double)rows : 0.0);
+}
+
+// Pieces that fill the shares of `slots` workgroups one after the other, ending where a
+// share does, at least `least` tiles long.
+static PackCut pack_shares(const std::vector<int>& tiles, int slots, int least) {
+  PackCut c;
+  int64_t total = 0;
+  for (int t : tiles) total += t + kPackFixed;
+  const int64_t share = std::max<int64_t>((total + slots - 1) / slots, least + kPackFixed);
+  // the pieces' own fixed costs, about one more per slot
+  const int64_t room = share + (share > least + kPackFixed ? kPackFixed : 0);
+  int64_t left = room;
+  for (int t : tiles) {
+    int n = 0, at = 0;
+    do {
+      if (left < least + kPackFixed) left = room;
+      int take = (int)std::min<int64_t>(t - at, left - kPackFixed);
+      const int rest = t - at - take;
+      if (rest > 0 && rest < least) take = t - at >= 2 * least ? t - at - least : t - at;
+      at += take;
+      left -= take + kPackFixed;
+      c.tiles.push_back(take);
+      n++;
+    } while (at < t);
+    c.pieces.push_back(n);
+  }
+  return c;
+}
+
+// No more pieces than slots, an item's of one size, the longest as short as that allows.
+static PackCut pack_even(const std::vector<int>& tiles, int slots, int longest, int least) {
+  const auto pieces = [](int t, int most) { return t ? (t + most - 1) / most : 1; };
+  int lo = least, hi = std::max(longest, least);
+  while (lo < hi) {
+    const int most = (lo + hi) / 2;
+    int64_t n = 0;
+    for (int t : tiles) n += pieces(t, most);
+    if (n <= slots) hi = most;
+    else lo = most + 1;
+  }
+  PackCut c;
+  for (int t : tiles) {
+    const int n = pieces(t, lo);
+    c.pieces.push_back(n);
+    for (int i = 0; i < n; i++) c.tiles.push_back((int)((int64_t)t * (i + 1) / n - (int64_t)t * i / n));
+  }
+  return c;
+}
+
+// Orders items longest first and cuts them along their keys in the way that ends
+// soonest: not at all, in even pieces (one or two workgroups a CU) or in shares (two).
+// Measured, us for these four: 64 decoders of 16 to 8192 keys 187, -, -, 74; 66 of 4096
+// keys 249, -, -, 175; 4 chunks of 82 to 354 f32 queries over 2116 to 8176 keys 237, 226,
+// 130, 136; 2 of 23 and 114 over 2300 and 2700 87, 39, 41, 43; one prompt of 2048 f16
+// queries 61, -, -, 68; 3 prompts of 600 to 900 f32 queries 52, -, -, 59.
+static void pack_cut(const std::vector<PackedItem>& whole, int tile, int least, int ncu, const PackRate& rate,
                      std::vector<PackedItem>& out, PackedPlan& plan) {
+  PackCut cut;
   int64_t total = 0;
   int longest = 0;
   for (const PackedItem& it : whole) {
     const int t = (it.kv_hi + tile - 1) / tile;
-    total += t + fixed;
-    longest = std::max(longest, t + fixed);
+    cut.pieces.push_back(1);
+    cut.tiles.push_back(t);
+    total += t + kPackFixed;
+    longest = std::max(longest, t);
   }
-  const int64_t share = std::max<int64_t>((total + slots - 1) / slots, least + fixed);
-  if (4 * longest <= 5 * share) {
-    out = whole;
-  } else {
-    // the pieces' own fixed costs, about one more per slot
-    const int64_t room = share + (share > least + fixed ? fixed : 0);
-    int64_t left = room;
-    for (PackedItem it : whole) {
-      const int tiles = (it.kv_hi + tile - 1) / tile, hi = it.kv_hi;
-      std::vector<int> ends;
-      for (int at = 0; at < tiles;) {
-        if (left < least + fixed) left = room;
-        int take = (int)std::min<int64_t>(tiles - at, left - fixed);
-        if (tiles - at - take < least) take = tiles - at;
-        at += take;
-        left -= take + fixed;
-        ends.push_back(at);
-      }
-      if (ends.size() <= 1) {
-        out.push_back(it);
-        continue;
-      }
-      const int parts = (int)ends.size();
-      for (int p = 0; p < parts; p++) {
-        it.kv_lo = p ? ends[p - 1] * tile : 0;
-        it.kv_hi = std::min(hi, ends[p] * tile);
-        it.part = (int32_t)(plan.part_rows + (int64_t)p * it.nr);
-        out.push_back(it);
-      }
-      // rows of a merge: few where there are many parts, whose rows then share its threads
-      const int rows = parts > 16 ? 1 : parts > 4 ? 2 : 8;
-      for (int i = 0; i < it.nr; i += rows)
-        plan.merges.push_back(PackedMerge{it.q0, it.r0 + i, std::min(rows, it.nr - i), it.kvh,
-                                          (int32_t)plan.part_rows + i, parts, it.nr});
-      plan.part_rows += (int64_t)parts * it.nr;
+  // Nothing to gain where whole items, longest first, end within a tenth of even shares,
+  // or the longest is a quarter of a workgroup's share. A cut has to win by 5%: the
+  // estimates are no closer.
+  const double even = (double)total / ncu * rate.tile / (2 * rate.shared);
+  if (longest > least && 8.0 * longest * ncu > (double)total) {
+    double best = pack_time(whole, cut, ncu, rate);
+    if (best > 1.1 * even) {
+      const std::vector<int> tiles = cut.tiles;
+      const auto take = [&](PackCut other) {
+        const double time = pack_time(whole, other, ncu, rate);
+        if (time >= 0.95 * best) return;
+        best = time;
+        cut = std::move(other);
+      };
+      if ((int64_t)whole.size() < ncu) take(pack_even(tiles, ncu, longest, least));
+      if ((int64_t)whole.size() < 2 * ncu) take(pack_even(tiles, 2 * ncu, longest, least));
+      take(pack_shares(tiles, 2 * ncu, least));
     }
   }
-  std::stable_sort(out.begin(), out.end(),
-                   [](const PackedItem& a, const PackedItem& b) { return a.kv_hi - a.kv_lo > b.kv_hi - b.kv_lo; });
+  std::vector<PackedItem> cuts;
+  cuts.reserve(cut.tiles.size());
+  size_t at = 0;
+  for (size_t i = 0; i < whole.size(); i++) {
+    PackedItem it = whole[i];
+    const int parts = cut.pieces[i], hi = it.kv_hi;
+    if (parts == 1) {
+      at++;
+      cuts.push_back(it);
+      continue;
+    }
+    int end = 0;
+    for (int p = 0; p < parts; p++) {
+      it.kv_lo = end * tile;
+      end += cut.tiles[at++];
+      it.kv_hi = std::min(hi, end * tile);
+      it.part = (int32_t)(plan.part_rows + (int64_t)p * it.nr);
+      cuts.push_back(it);
+    }
+    // rows of a merge: few where there are many parts, whose rows then share its threads (4
+    // chunks of up to 5 parts: 130 us with 8 rows, 134 with 2)
+    const int rows = parts > 64 ? 1 : parts > 16 ? 2 : 8;
+    for (int r = 0; r < it.nr; r += rows)
+      plan.merges.push_back(PackedMerge{it.q0, it.r0 + r, std::min(rows, it.nr - r), it.kvh,
+                                        (int32_t)plan.part_rows + r, parts, it.nr});
+    plan.part_rows += (int64_t)parts * it.nr;
+  }
+  std::vector<std::pair<int, int>> order;  // minus its keys, and where it stands
+  order.reserve(cuts.size());
+  for (const PackedItem& it : cuts) order.push_back({it.kv_lo - it.kv_hi, (int)order.size()});
+  std::sort(order.begin(), order.end());
+  out.reserve(cuts.size());
+  for (const auto& o : order) out.push_back(cuts[o.second]);
 }
 
 void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int Hkv, int D, bool causal,
@@ -118,8 +250,9 @@ void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int H
   }
   plan.tq = q0;
   plan.tk = k0;
-  pack_cut(whole[0], kPackTile, 2 * ncu, 3, 4, plan.items, plan);
-  pack_cut(whole[1], kFewTile * kFewWaves, 2 * ncu, 3, 2, plan.few, plan);
+  const double dims = D / 128.0;
+  pack_cut(whole[0], kPackTile, 4, ncu, q_f16 ? PackRate{1.31 * dims, 0.64} : PackRate{1.8 * dims, 0.53}, plan.items, plan);
+  pack_cut(whole[1], kFewTile * kFewWaves, 2, ncu, PackRate{1.8 * dims, 0.7}, plan.few, plan);
 }
 
 // ---------------------------------------------------------------------------
