@@ -97,7 +97,7 @@ __device__ __forceinline__ void adapter_down_64(const AdapterArgs& a, const Adap
                                                 int s1, int wave, adapter_lds buf, float4_t (&acc)[4][RB]) {
   constexpr int RBY = XK == XK_F32 ? 256 : 128;  // bytes of a row's unit in one plane
   constexpr int CH = RBY / 16, RPI = 64 / CH, NI = 64 / RPI;  // its chunks, rows per instruction, instructions
-  constexpr int U = XK == XK_F16 && RB <= 4 ? 2 : 1;  // units in the buffer at a time (rank 128 has no registers for two)
+  constexpr int U = XK == XK_F16 && RB <= 4 ? 2 : 1;  // units in the buffer (rank 128: no registers for two)
   const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4, nrb = e.rank_pad / 16;
   int64_t at[NI];  // byte offset of the lane's chunk, row by row
 #pragma unroll
@@ -116,8 +116,9 @@ __device__ __forceinline__ void adapter_down_64(const AdapterArgs& a, const Adap
       for (int p = 0; p < (XK == XK_X2 ? 2 : 1); p++)
 #pragma unroll
         for (int n = 0; n < NI; n++)
-          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(x + p * (int64_t)a.T * a.K * 2 + at[n]),
-                                           (__attribute__((address_space(3))) void*)(buf + 8192 * (u + p) + 1024 * n), 16, 0, kAdapterNt);
+          __builtin_amdgcn_global_load_lds(
+              (const __attribute__((address_space(1))) void*)(x + p * (int64_t)a.T * a.K * 2 + at[n]),
+              (__attribute__((address_space(3))) void*)(buf + 8192 * (u + p) + 1024 * n), 16, 0, kAdapterNt);
 #pragma unroll
       for (int r = 0; r < RB; r++)
 #pragma unroll
@@ -186,7 +187,8 @@ __global__ __launch_bounds__(256) void adapter_down_kernel(AdapterArgs a) {
   const AdapterEntry e = a.table[t.adapter];
   if (e.rank_pad == 0 || e.rank_pad > RB * 16) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), units = a.K / 64;
-  const int s0 = (int)((int64_t)units * blockIdx.y / gridDim.y), s1 = (int)((int64_t)units * (blockIdx.y + 1) / gridDim.y);
+  const int s0 = (int)((int64_t)units * blockIdx.y / gridDim.y);
+  const int s1 = (int)((int64_t)units * (blockIdx.y + 1) / gridDim.y);
   float (*part)[16][RB * 16] = (float(*)[16][RB * 16])mem;
   if (TB == 1 || t.n <= 16) {
     float4_t acc[1][RB] = {};
@@ -284,8 +286,8 @@ __global__ __launch_bounds__(256) void adapter_pair_kernel(AdapterArgs a) {
 
 // u of row l16 (16 rows in LDS) as the lane's operands of the second product.
 template <int RB>
-__device__ __forceinline__ void adapter_operand(const float (&us)[16][RB * 16 + 4], int l16, int q, half8_t (&uh)[(RB + 1) / 2],
-                                                half8_t (&ul)[(RB + 1) / 2], float& scale) {
+__device__ __forceinline__ void adapter_operand(const float (&us)[16][RB * 16 + 4], int l16, int q,
+                                                half8_t (&uh)[(RB + 1) / 2], half8_t (&ul)[(RB + 1) / 2], float& scale) {
   constexpr int KB = (RB + 1) / 2, E = RB == 1 ? 4 : 8;
   float top = 0.f, down, up;
 #pragma unroll
@@ -398,7 +400,8 @@ __device__ __forceinline__ void adapter_columns(const AdapterArgs& a, const Adap
 // time, 1152 rows of which 528 have none took 103 us instead of 96). False: the rows have
 // one, in e.
 template <int RB, bool YF16>
-__device__ __forceinline__ bool adapter_copies(const AdapterArgs& a, const AdapterTile& t, AdapterEntry& e, int n0, int n1) {
+__device__ __forceinline__ bool adapter_copies(const AdapterArgs& a, const AdapterTile& t, AdapterEntry& e, int n0,
+                                               int n1) {
   e = AdapterEntry{};
   if (t.adapter >= 0) e = a.table[t.adapter];
   // an adapter of a larger rank than the launch was captured for: its rows are NaN
@@ -476,8 +479,11 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a) {
 template <int XK, int TB, int RB>
 static void adapters_launch(const AdapterArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)a.ntiles, (unsigned)((a.N + a.cols - 1) / a.cols));
-  hipLaunchKernelGGL((adapter_down_kernel<XK, TB, RB>), dim3((unsigned)a.ntiles, (unsigned)a.splits), dim3(256), 0, st, a);
-  if (TB > 1) hipLaunchKernelGGL((adapter_pair_kernel<RB>), dim3((unsigned)a.ntiles, TB * RB / 2 ? TB * RB / 2 : 1), dim3(256), 0, st, a);
+  const dim3 shares((unsigned)a.ntiles, (unsigned)a.splits);
+  hipLaunchKernelGGL((adapter_down_kernel<XK, TB, RB>), shares, dim3(256), 0, st, a);
+  constexpr int kPairRows = 256 / (RB * 8);  // rows of a workgroup
+  const dim3 pairs((unsigned)a.ntiles, (16 * TB + kPairRows - 1) / kPairRows);
+  if (TB > 1) hipLaunchKernelGGL((adapter_pair_kernel<RB>), pairs, dim3(256), 0, st, a);
   if (a.y_f16) hipLaunchKernelGGL((adapter_up_kernel<TB, RB, true>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((adapter_up_kernel<TB, RB, false>), grid, dim3(256), 0, st, a);
 }

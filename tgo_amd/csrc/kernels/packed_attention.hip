@@ -1,6 +1,30 @@
 // packed_attention.hip -- attention over packed sequences of different lengths
 // whose K and V are plain f16 rows (no pool, no page table): whole prompts,
 // chunks of new tokens, single tokens; causal or full; grouped heads.
+//
+// o = sum_k 2^(s_k - m) v_k / sum_k 2^(s_k - m), s = scale log2(e) q . k, in one pass
+// over the keys: m and the sums move along with the tiles (online softmax), and m only
+// when a probability would leave its range. Both products run transposed (S^T = K Q^T,
+// O^T = V^T P^T) on v_mfma_f32_32x32x16_f16, so that a lane holds scores of one row and
+// its own probabilities are the second product's operand: P never leaves registers.
+// f32 queries go as f16 hi + lo pairs, and so do their probabilities, two MFMAs per
+// product; f16 queries take f16 probabilities (2^-11 of each, as their outputs). Scores,
+// sums, maxima and partial results are f32.
+//   packed_kernel        128 rows of a sequence and kv head (token by token, the
+//                        group's heads side by side), tiles of 64 keys: MFMA-bound
+//   packed_few_kernel    up to 32 such rows (decoding): bound by the keys' bytes
+//   packed_merge_kernel  rows whose keys were cut into pieces
+// Measured (us, 32 heads over 8 of 128 dims unless said):
+//   one causal prompt of 16384 f16 rows           2140, 1.03 PFLOP/s, the matrix unit
+//       busy 53% at 1.93 GHz (all four SIMDs' power holds the clock), VALU 41%
+//   16 f16 prompts of 1 to 1384 rows              53, 0.64 PFLOP/s
+//   4 f32 chunks of 82 to 354 rows, 2116 to 8176 keys   122, 0.42 PFLOP/s, twice that executed
+//   32 full f32 sequences of 22 to 763 rows, 16 heads of 64   51, 0.30 PFLOP/s
+//   64 decoders of 16 to 8192 keys                73, 5.3 TB/s
+//   64 decoders of 4096 keys                      163, 6.6 TB/s
+// Tried and slower or no faster in packed_kernel, for that prompt (2240 us then): the
+// next tile's scores beside this one's softmax 2252; eight waves on four LDS buffers
+// 2666; 64 rows a wave spills; the waves' priorities by phase 2240.
 #include "operators.h"
 
 #include <algorithm>
@@ -225,8 +249,9 @@ void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int H
   plan.q_f16 = q_f16;
   const int G = H / Hkv;
   // Sequences of up to kPackFew rows per kv head go to the few-row kernel where they
-  // hold most of the keys; beside longer prompts they are not worth a launch of their
-  // own (16 prompts, two of a few tokens: 70 us, 77 with it).
+  // hold most of the keys (64 decoders of 16 to 8192 keys 73 us, 84 without); beside longer
+  // prompts they are not worth a launch of their own (16 prompts, eight of a few tokens:
+  // 60 us, 65 with it).
   int64_t few_keys = 0, keys = 0;
   for (int s = 0; s < B; s++) {
     keys += nk[s];
@@ -243,7 +268,8 @@ void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int H
       const int64_t last = (r0 + nr - 1) / G;
       const int hi = (int)std::max<int64_t>(0, std::min<int64_t>(nk[s], last + shift + 1));
       for (int h = 0; h < Hkv; h++)
-        whole[rows <= few_rows].push_back(PackedItem{(int32_t)q0, (int32_t)k0, nk[s], shift, (int32_t)r0, nr, 0, hi, h, -1});
+        whole[rows <= few_rows].push_back(
+            PackedItem{(int32_t)q0, (int32_t)k0, nk[s], shift, (int32_t)r0, nr, 0, hi, h, -1});
     }
     q0 += nq[s];
     k0 += nk[s];
@@ -251,7 +277,8 @@ void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int H
   plan.tq = q0;
   plan.tk = k0;
   const double dims = D / 128.0;
-  pack_cut(whole[0], kPackTile, 4, ncu, q_f16 ? PackRate{1.31 * dims, 0.64} : PackRate{1.8 * dims, 0.53}, plan.items, plan);
+  const PackRate rate = q_f16 ? PackRate{1.31 * dims, 0.64} : PackRate{1.8 * dims, 0.53};
+  pack_cut(whole[0], kPackTile, 4, ncu, rate, plan.items, plan);
   pack_cut(whole[1], kFewTile * kFewWaves, 2, ncu, PackRate{1.8 * dims, 0.7}, plan.few, plan);
 }
 
@@ -449,7 +476,9 @@ __device__ __forceinline__ void pack_scores(const PackRows<D, QF16>& w, lds_t K,
 }
 // Whether the lane's row sees the key of its score (pb, i); left: the row's last
 // visible key, counted from the lane's first of the tile (4kh on).
-__device__ __forceinline__ bool pack_visible(int left, int pb, int i) { return pb * 32 + 8 * (i >> 2) + (i & 3) <= left; }
+__device__ __forceinline__ bool pack_visible(int left, int pb, int i) {
+  return pb * 32 + 8 * (i >> 2) + (i & 3) <= left;
+}
 // A row's largest score of a tile, scaled.
 __device__ __forceinline__ float pack_top(const float16_t (&sc)[2], float qs) {
   // one chain: the compiler makes it 16 three-way maxima (of pairs, it quiets every
@@ -505,7 +534,8 @@ __device__ __forceinline__ void pack_probs(const float16_t (&sc)[2], int u, floa
 // the probabilities taken again. That saves the search, 25 of 165 VALU
 // instructions a tile.
 template <int D>
-__device__ __forceinline__ void pack_probs_f16(PackRows<D, true>& w, const float16_t (&sc)[2], float qs, half8_t (&ph)[4]) {
+__device__ __forceinline__ void pack_probs_f16(PackRows<D, true>& w, const float16_t (&sc)[2], float qs,
+                                               half8_t (&ph)[4]) {
   float l[4] = {};
   half8_t none;
 #pragma unroll
@@ -565,7 +595,7 @@ __device__ __forceinline__ void pack_values(PackRows<D, QF16>& w, const float16_
 // being both. Rare: a plain loop behind the kernel's own.
 template <int D, bool QF16>
 __device__ __forceinline__ void packed_redo(const PackedArgs* ap, int item, int w0, int blocks, lds_t K, lds_t V,
-                                                     lds_t buf) {
+                                            lds_t buf) {
   const PackedArgs& a = *ap;
   const PackedItem it = a.items[item];
   const int tid = threadIdx.x, lane = tid & 63, kh = lane >> 5;
@@ -665,7 +695,8 @@ __device__ __forceinline__ void pack_dma(const char* base, uint32_t off, int64_t
 // The same where the tile ends behind the item's keys: rows from `rows` on repeat the
 // last one (no row sees them; a value there that is not finite is packed_redo's).
 template <int D, int WAVES>
-__device__ __forceinline__ void pack_dma_end(const char* base, int p, int c, int rows, int64_t row_bytes, lds_t tile, int wave) {
+__device__ __forceinline__ void pack_dma_end(const char* base, int p, int c, int rows, int64_t row_bytes, lds_t tile,
+                                             int wave) {
   constexpr int RPI = 64 * WAVES / (D / 8);
 #pragma unroll
   for (int n = 0; n < kPackTile / RPI; n++)
@@ -675,7 +706,9 @@ __device__ __forceinline__ void pack_dma_end(const char* base, int p, int c, int
 }
 
 // WAVES waves of 32 rows each; tiles of 64 keys go through two LDS buffers, the next
-// one's DMA in flight while one is used.
+// one's DMA in flight while one is used. Two workgroups a CU (64 KiB of LDS and 256
+// registers each), so that one's products run under the other's softmax: without the
+// softmax the 16384-row prompt took 12% less, without the DMA 14%.
 template <int D, bool QF16, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void packed_kernel(PackedArgs a) {
   constexpr int TB = kPackTile * D * 2;  // bytes of a tile
@@ -739,7 +772,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_kernel(PackedArgs a) {
   const int per = TB / (128 * D);
   lds_t buf = (lds_t)(wave < per ? K0 : wave < 2 * per ? V0 : wave < 3 * per ? K1 : V1) + wave % per * 128 * D;
   if (__syncthreads_or(bad)) {
-    packed_redo<D, QF16>((const PackedArgs*)__builtin_amdgcn_kernarg_segment_ptr(), blockIdx.x, w0, 1, (lds_t)K0, (lds_t)V0, buf);
+    packed_redo<D, QF16>((const PackedArgs*)__builtin_amdgcn_kernarg_segment_ptr(), blockIdx.x, w0, 1, (lds_t)K0,
+                         (lds_t)V0, buf);
     return;
   }
   w.write(a, it, lane, buf);
@@ -753,6 +787,8 @@ constexpr int kNonTemporal = 2;  // the nt bit: keys of few rows are read once
 // 64 KiB and two waves a workgroup, two workgroups a CU: at any time about 64 KiB of
 // K and V are on their way to each CU, and one workgroup's start and end lie under
 // the other's stream.
+// 64 decoders of 4096 keys: 162 us, 6.6 TB/s of the 7.0 that a plain read reaches here,
+// 190 in packed_kernel; of 16 to 8192 keys 73 us, 5.3 TB/s, and 84.
 template <int D, bool QF16>
 __global__ __launch_bounds__(64 * kFewWaves, 1) void packed_few_kernel(PackedArgs a) {
   constexpr int TB = kFewTile * D * 2, CH = D / 8, RPI = 64 / CH, NI = kFewTile / RPI;
@@ -762,7 +798,8 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void packed_few_kernel(PackedArg
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kh = lane >> 5;
   const int kat = pack_k_at<D>(lane & 31, kh), vat = pack_v_at<D>(lane);
-  const lds_t Kw[2] = {(lds_t)K0 + wave * TB, (lds_t)K1 + wave * TB}, Vw[2] = {(lds_t)V0 + wave * TB, (lds_t)V1 + wave * TB};
+  const lds_t Kw[2] = {(lds_t)K0 + wave * TB, (lds_t)K1 + wave * TB};
+  const lds_t Vw[2] = {(lds_t)V0 + wave * TB, (lds_t)V1 + wave * TB};
 
   const int p = lane / CH, c = lane % CH;
   const int64_t kb = a.k_row * 2, vb = a.v_row * 2;

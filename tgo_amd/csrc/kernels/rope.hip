@@ -4,10 +4,12 @@
 //
 // Bound by the heads' bytes. A workgroup takes some rows of one tensor: its
 // threads first put the rows' cos and sin into LDS, once per pair and row
-// (computed by every thread that uses them, 72 heads of 16384 rows took 440 us
-// instead of 140), then walk the rows' heads in units of 2V elements, V pairs of
+// (computed by every thread that uses them, 72 heads of 16384 rows took 443 us
+// instead of 131), then walk the rows' heads in units of 2V elements, V pairs of
 // a head's rotated part or 2V elements of the rest, neighbouring threads on
-// neighbouring units.
+// neighbouring units. Measured: 604 MB of f16 heads (16384 rows) 131 us, 4.6 TB/s, a
+// copy of that size 4.8; 52 MB of f32 rows to f16 (1152 rows) 10 us, 5.3 TB/s; one row
+// 3.4 us in the kernel, 8 with the call.
 #include "operators.h"
 
 #include <algorithm>
@@ -82,7 +84,8 @@ __device__ __forceinline__ float2 rope_angle(int32_t pos, double turns_per_posit
 // One tensor's heads of the block's rows.
 template <int V, bool HALF, bool XF16, bool YF16>
 __device__ __forceinline__ void rope_heads(const RopeArgs& a, const RopeGroup& g, int t0, int rows, const float2* cs) {
-  const int pairs = a.rd / 2, rot = g.rotate ? pairs / V : 0, units = g.rotate ? rot + (a.d - a.rd) / (2 * V) : a.d / (2 * V);
+  const int pairs = a.rd / 2, rot = g.rotate ? pairs / V : 0;
+  const int units = g.rotate ? rot + (a.d - a.rd) / (2 * V) : a.d / (2 * V);
   const int slots = 256 / units, u = threadIdx.x % units, slot = threadIdx.x / units;
   if (slot >= slots) return;
   const bool turn = u < rot;
@@ -158,8 +161,8 @@ void launch_rope(const RopeArgs& args, int ncu, hipStream_t st) {
     // r / heads = r * magic >> 32 for r < 2^16 (rows of a block times heads, below)
     g.magic = (((uint64_t)1 << 32) + g.heads - 1) / g.heads;
     const int xs = g.x_f16 ? 8 : 4, ys = g.y_f16 ? 8 : 4;  // elements in 16 bytes
-    aligned = aligned && (uintptr_t)g.x % 16 == 0 && (uintptr_t)g.y % 16 == 0 && g.x_row % xs == 0 && g.x_head % xs == 0 &&
-              g.y_row % ys == 0 && g.y_head % ys == 0;
+    aligned = aligned && (uintptr_t)g.x % 16 == 0 && (uintptr_t)g.y % 16 == 0 && g.x_row % xs == 0 &&
+              g.x_head % xs == 0 && g.y_row % ys == 0 && g.y_head % ys == 0;
   }
   // Rows per workgroup: enough that a pair's angle serves many heads, few enough that
   // the chip is full; a power of two of at most 16, and r below 2^16.

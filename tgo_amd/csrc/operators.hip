@@ -59,7 +59,8 @@ struct OnDevice {
   }
 };
 
-int no_ctx(const char* what) { return fail(TGOHIP_EINVAL, std::string(what) + ": the context is missing"); }
+int refuse(const std::string& why) { return fail(TGOHIP_EINVAL, why); }
+int no_ctx(const char* what) { return refuse(std::string(what) + ": the context is missing"); }
 
 // Making, changing or freeing a handle copies, allocates and waits, which a graph
 // cannot hold.
@@ -75,7 +76,7 @@ template <typename T>
 T* find(std::map<int, T>& m, int handle, const char* what) {
   auto it = m.find(handle);
   if (it != m.end()) return &it->second;
-  fail(TGOHIP_EINVAL, std::string(what) + ": no handle " + std::to_string(handle));
+  refuse(std::string(what) + ": no handle " + std::to_string(handle));
   return nullptr;
 }
 
@@ -139,30 +140,30 @@ std::string num(double v) {
 }
 
 int check_rope(const tgohip_rope_cfg* c) {
-  if (!c) return fail(TGOHIP_EINVAL, "rope: the configuration is missing");
+  if (!c) return refuse("rope: the configuration is missing");
   if (c->head_dim < 2 || c->head_dim > kRopeMaxHeadDim || c->head_dim % 2)
-    return fail(TGOHIP_EINVAL, "rope: head_dim is " + std::to_string(c->head_dim) + "; an even number from 2 to " +
-                                   std::to_string(kRopeMaxHeadDim));
+    return refuse("rope: head_dim is " + std::to_string(c->head_dim) + "; an even number from 2 to " +
+                  std::to_string(kRopeMaxHeadDim));
   if (c->rotary_dim < 2 || c->rotary_dim > c->head_dim || c->rotary_dim % 2)
-    return fail(TGOHIP_EINVAL, "rope: rotary_dim is " + std::to_string(c->rotary_dim) + " of head_dim " +
-                                   std::to_string(c->head_dim) + "; an even number from 2 to head_dim");
+    return refuse("rope: rotary_dim is " + std::to_string(c->rotary_dim) + " of head_dim " +
+                  std::to_string(c->head_dim) + "; an even number from 2 to head_dim");
   if (c->layout != TGOHIP_ROPE_INTERLEAVED && c->layout != TGOHIP_ROPE_HALF)
-    return fail(TGOHIP_EINVAL, "rope: layout is " + std::to_string(c->layout) + ", neither interleaved nor half");
+    return refuse("rope: layout is " + std::to_string(c->layout) + ", neither interleaved nor half");
   if (c->scaling < TGOHIP_ROPE_UNSCALED || c->scaling > TGOHIP_ROPE_BANDS)
-    return fail(TGOHIP_EINVAL, "rope: scaling is " + std::to_string(c->scaling) + ", not a TGOHIP_ROPE_* kind");
+    return refuse("rope: scaling is " + std::to_string(c->scaling) + ", not a TGOHIP_ROPE_* kind");
   if (!(c->base > 1.0) || !std::isfinite(c->base))
-    return fail(TGOHIP_EINVAL, "rope: base is " + num(c->base) + "; a finite number above 1");
+    return refuse("rope: base is " + num(c->base) + "; a finite number above 1");
   if (!(c->attention >= 0.0) || !std::isfinite(c->attention))
-    return fail(TGOHIP_EINVAL, "rope: attention is " + num(c->attention) + "; a finite factor, 0 for the scaling's own");
+    return refuse("rope: attention is " + num(c->attention) + "; a finite factor, 0 for the scaling's own");
   if (c->scaling == TGOHIP_ROPE_UNSCALED) return 0;
   if (!(c->factor >= 1.0) || !std::isfinite(c->factor))
-    return fail(TGOHIP_EINVAL, "rope: factor is " + num(c->factor) + "; a finite number of at least 1");
+    return refuse("rope: factor is " + num(c->factor) + "; a finite number of at least 1");
   if (c->scaling == TGOHIP_ROPE_LINEAR) return 0;
   if (!(c->original > 0.0) || !std::isfinite(c->original))
-    return fail(TGOHIP_EINVAL, "rope: original is " + num(c->original) + "; the positions trained on, above 0");
+    return refuse("rope: original is " + num(c->original) + "; the positions trained on, above 0");
   if (!(c->slow > 0.0) || !(c->fast > c->slow) || !std::isfinite(c->fast))
-    return fail(TGOHIP_EINVAL, "rope: fast is " + num(c->fast) + " and slow " + num(c->slow) +
-                                   " turns over the original positions; fast is above slow and slow above 0");
+    return refuse("rope: fast is " + num(c->fast) + " and slow " + num(c->slow) +
+                  " turns over the original positions; fast is above slow and slow above 0");
   return 0;
 }
 
@@ -192,27 +193,27 @@ void rope_freqs(const tgohip_rope_cfg& c, double* w, double* attention) {
 constexpr int64_t kMaxIndex = (int64_t)1 << 30;
 
 int check_packed(int B, const int32_t* nq, const int32_t* nk, int H, int Hkv, int D, int q_dtype) {
-  if (B < 0) return fail(TGOHIP_EINVAL, "packed_plan: " + std::to_string(B) + " sequences");
-  if (B > 0 && (!nq || !nk)) return fail(TGOHIP_EINVAL, "packed_plan: q_lengths and kv_lengths are host arrays");
+  if (B < 0) return refuse("packed_plan: " + std::to_string(B) + " sequences");
+  if (B > 0 && (!nq || !nk)) return refuse("packed_plan: q_lengths and kv_lengths are host arrays");
   if (D != 64 && D != 128)
-    return fail(TGOHIP_EINVAL, "packed_plan: head_dim is " + std::to_string(D) + "; the kernels are built for 64 and 128");
+    return refuse("packed_plan: head_dim is " + std::to_string(D) + "; the kernels are built for 64 and 128");
   if (H <= 0 || Hkv <= 0 || H % Hkv != 0)
-    return fail(TGOHIP_EINVAL, "packed_plan: " + std::to_string(H) + " query heads over " + std::to_string(Hkv) +
-                                   " kv heads; each kv head serves the same number of query heads");
-  if (H > 65536) return fail(TGOHIP_EINVAL, "packed_plan: " + std::to_string(H) + " query heads; at most 65536");
+    return refuse("packed_plan: " + std::to_string(H) + " query heads over " + std::to_string(Hkv) +
+                  " kv heads; each kv head serves the same number of query heads");
+  if (H > 65536) return refuse("packed_plan: " + std::to_string(H) + " query heads; at most 65536");
   if (q_dtype != TGOHIP_F32 && q_dtype != TGOHIP_F16)
-    return fail(TGOHIP_EINVAL, "packed_plan: q_dtype is " + std::to_string(q_dtype) + "; queries are f32 or f16");
+    return refuse("packed_plan: q_dtype is " + std::to_string(q_dtype) + "; queries are f32 or f16");
   int64_t tq = 0, tk = 0;
   for (int s = 0; s < B; s++) {
     if (nq[s] < 0 || nk[s] < 0)
-      return fail(TGOHIP_EINVAL, "packed_plan: sequence " + std::to_string(s) + " has " + std::to_string(nq[s]) +
-                                     " queries and " + std::to_string(nk[s]) + " keys");
+      return refuse("packed_plan: sequence " + std::to_string(s) + " has " + std::to_string(nq[s]) +
+                    " queries and " + std::to_string(nk[s]) + " keys");
     tq += nq[s];
     tk += nk[s];
   }
   if (tq * H >= kMaxIndex || tk >= kMaxIndex)
-    return fail(TGOHIP_EINVAL, "packed_plan: " + std::to_string(tq) + " query rows of " + std::to_string(H) +
-                                   " heads and " + std::to_string(tk) + " key rows; heads of rows, and key rows, stay below 2^30");
+    return refuse("packed_plan: " + std::to_string(tq) + " query rows of " + std::to_string(H) +
+                  " heads and " + std::to_string(tk) + " key rows; heads of rows, and key rows, stay below 2^30");
   return 0;
 }
 
@@ -226,7 +227,7 @@ int tgohip_rope_freqs(const tgohip_rope_cfg* cfg, double* inv_freq, double* atte
   return guarded([&]() -> int {
     const int rc = check_rope(cfg);
     if (rc) return rc;
-    if (!inv_freq || !attention) return fail(TGOHIP_EINVAL, "rope_freqs: inv_freq and attention are host buffers");
+    if (!inv_freq || !attention) return refuse("rope_freqs: inv_freq and attention are host buffers");
     rope_freqs(*cfg, inv_freq, attention);
     return 0;
   });
@@ -237,7 +238,7 @@ int tgohip_rope_new(tgohip_ctx* c, const tgohip_rope_cfg* cfg, int* handle) {
     int rc = check_rope(cfg);
     if (rc) return rc;
     if (!c) return no_ctx("rope_new");
-    if (!handle) return fail(TGOHIP_EINVAL, "rope_new: handle is missing");
+    if (!handle) return refuse("rope_new: handle is missing");
     OnDevice on(c->device);
     if ((rc = no_capture(c, "rope_new"))) return rc;
     double w[kRopeMaxHeadDim / 2], attention;
@@ -280,17 +281,17 @@ int tgohip_rope(tgohip_ctx* c, int handle, const int32_t* positions, int T, cons
     if (!c) return no_ctx("rope");
     RopeTable* t = find(c->ops.ropes, handle, "rope");
     if (!t) return TGOHIP_EINVAL;
-    if (T < 0 || T >= 1 << 24) return fail(TGOHIP_EINVAL, "rope: " + std::to_string(T) + " rows; 0 to 2^24 - 1");
+    if (T < 0 || T >= 1 << 24) return refuse("rope: " + std::to_string(T) + " rows; 0 to 2^24 - 1");
     if (n < 1 || n > kRopeGroups || !heads)
-      return fail(TGOHIP_EINVAL, "rope: " + std::to_string(n) + " tensors of heads; 1 to " + std::to_string(kRopeGroups));
+      return refuse("rope: " + std::to_string(n) + " tensors of heads; 1 to " + std::to_string(kRopeGroups));
     if (T == 0) return 0;
-    if (!positions || (uintptr_t)positions % 4) return fail(TGOHIP_EINVAL, "rope: positions is a device buffer of int32");
+    if (!positions || (uintptr_t)positions % 4) return refuse("rope: positions is a device buffer of int32");
     const Span at{(const char*)positions, 1, 1, 0, 0, (int64_t)T * 4};
     RopeArgs a{};
     Span xs[kRopeGroups], ys[kRopeGroups];
     for (int i = 0; i < n; i++) {
       const tgohip_rope_heads& g = heads[i];
-      auto bad = [i](const std::string& m) { return fail(TGOHIP_EINVAL, "rope: tensor " + std::to_string(i) + ": " + m); };
+      auto bad = [i](const std::string& m) { return refuse("rope: tensor " + std::to_string(i) + ": " + m); };
       if (!g.x || !g.y) return bad("x and y are device buffers");
       if (g.heads < 1 || g.heads > 65536) return bad(std::to_string(g.heads) + " heads; 1 to 65536");
       if ((g.x_dtype != TGOHIP_F32 && g.x_dtype != TGOHIP_F16) || (g.y_dtype != TGOHIP_F32 && g.y_dtype != TGOHIP_F16))
@@ -311,7 +312,8 @@ int tgohip_rope(tgohip_ctx* c, int handle, const int32_t* positions, int T, cons
       }
       int64_t need = t->d;
       if (n0 > 1) {
-        if (s0 < need) return bad("heads of y overlap (strides " + std::to_string(g.y_row) + ", " + std::to_string(g.y_head) + ")");
+        if (s0 < need)
+          return bad("heads of y overlap (strides " + std::to_string(g.y_row) + ", " + std::to_string(g.y_head) + ")");
         need = (n0 - 1) * s0 + t->d;
       }
       if (n1 > 1 && s1 < need)
@@ -322,13 +324,13 @@ int tgohip_rope(tgohip_ctx* c, int handle, const int32_t* positions, int T, cons
     }
     for (int i = 0; i < n; i++) {
       if (meet(ys[i], at))
-        return fail(TGOHIP_EINVAL, "rope: y of tensor " + std::to_string(i) + " meets positions in memory");
+        return refuse("rope: y of tensor " + std::to_string(i) + " meets positions in memory");
       for (int j = 0; j < n; j++) {
         if (meet(ys[i], xs[j]) && !(i == j && a.g[i].x_f16 == a.g[i].y_f16 && same(ys[i], xs[i])))
-          return fail(TGOHIP_EINVAL, "rope: y of tensor " + std::to_string(i) + " meets x of tensor " + std::to_string(j) +
-                                         " in memory; y is its own x (same type and strides) or apart");
+          return refuse("rope: y of tensor " + std::to_string(i) + " meets x of tensor " + std::to_string(j) +
+                        " in memory; y is its own x (same type and strides) or apart");
         if (i < j && meet(ys[i], ys[j]))
-          return fail(TGOHIP_EINVAL, "rope: y of tensors " + std::to_string(i) + " and " + std::to_string(j) + " meet in memory");
+          return refuse("rope: y of tensors " + std::to_string(i) + " and " + std::to_string(j) + " meet in memory");
       }
     }
     a.positions = positions;
@@ -354,7 +356,7 @@ int tgohip_packed_plan(tgohip_ctx* c, int B, const int32_t* q_lengths, const int
     int rc = check_packed(B, q_lengths, kv_lengths, H, H_kv, head_dim, q_dtype);
     if (rc) return rc;
     if (!c) return no_ctx("packed_plan");
-    if (!handle) return fail(TGOHIP_EINVAL, "packed_plan: handle is missing");
+    if (!handle) return refuse("packed_plan: handle is missing");
     if (*handle && !find(c->ops.packed, *handle, "packed_plan")) return TGOHIP_EINVAL;
     OnDevice on(c->device);
     if ((rc = no_capture(c, "packed_plan"))) return rc;
@@ -362,9 +364,10 @@ int tgohip_packed_plan(tgohip_ctx* c, int B, const int32_t* q_lengths, const int
     packed_build_plan(B, q_lengths, kv_lengths, H, H_kv, head_dim, causal != 0, q_dtype == TGOHIP_F16, c->ncu, plan);
     const size_t items = plan.items.size();
     plan.items.insert(plan.items.end(), plan.few.begin(), plan.few.end());
-    if (plan.part_rows > INT_MAX || plan.items.size() > (size_t)INT_MAX / 256 || plan.merges.size() > (size_t)INT_MAX / 256)
-      return fail(TGOHIP_EINVAL, "packed_plan: the batch needs " + std::to_string(plan.items.size()) +
-                                     " workgroups, more than one launch takes");
+    const size_t most = (size_t)INT_MAX / 256;
+    if (plan.part_rows > INT_MAX || plan.items.size() > most || plan.merges.size() > most)
+      return refuse("packed_plan: the batch needs " + std::to_string(plan.items.size()) +
+                    " workgroups, more than one launch takes");
     const bool fresh = *handle == 0;
     const int h = fresh ? c->ops.next++ : *handle;
     PackedHandle& p = c->ops.packed[h];
@@ -399,7 +402,7 @@ int tgohip_packed_describe(int B, const int32_t* q_lengths, const int32_t* kv_le
   return guarded([&]() -> int {
     const int rc = check_packed(B, q_lengths, kv_lengths, H, H_kv, head_dim, q_dtype);
     if (rc) return rc;
-    if (ncu < 1 || !out) return fail(TGOHIP_EINVAL, "packed_describe: ncu and plan");
+    if (ncu < 1 || !out) return refuse("packed_describe: ncu and plan");
     PackedPlan plan;
     packed_build_plan(B, q_lengths, kv_lengths, H, H_kv, head_dim, causal != 0, q_dtype == TGOHIP_F16, ncu, plan);
     *out = tgohip_packed_plan_t{(int32_t)plan.items.size(), (int32_t)plan.few.size(), 0, 0, plan.part_rows, 0};
@@ -434,12 +437,12 @@ int tgohip_packed_attention(tgohip_ctx* c, int handle, const void* q, int64_t q_
     const PackedPlan& pl = p->plan;
     if (!pl.D) return fail(TGOHIP_ESTATE, "packed_attention: the plan was not made again after a failure");
     if (!(scale > 0.f) || scale > 0x1p32f)  // scores stay below 2^72, and above kPackNoMax
-      return fail(TGOHIP_EINVAL, "packed_attention: scale is " + num(scale) + "; a number above 0, at most 2^32");
+      return refuse("packed_attention: scale is " + num(scale) + "; a number above 0, at most 2^32");
     if (out_dtype != TGOHIP_F32 && out_dtype != TGOHIP_F16 && out_dtype != TGOHIP_F16X2)
-      return fail(TGOHIP_EINVAL, "packed_attention: out_dtype is " + std::to_string(out_dtype) + "; f32, f16 or a pair");
+      return refuse("packed_attention: out_dtype is " + std::to_string(out_dtype) + "; f32, f16 or a pair");
     if (pl.tq == 0) return 0;
-    if (!q || !out) return fail(TGOHIP_EINVAL, "packed_attention: q and out are device buffers");
-    if (pl.tk && (!k || !v)) return fail(TGOHIP_EINVAL, "packed_attention: k and v are device buffers");
+    if (!q || !out) return refuse("packed_attention: q and out are device buffers");
+    if (pl.tk && (!k || !v)) return refuse("packed_attention: k and v are device buffers");
     const int64_t qw = (int64_t)pl.H * pl.D, kw = (int64_t)pl.Hkv * pl.D, top = (int64_t)1 << 30;
     struct {
       const char* name;
@@ -451,22 +454,22 @@ int tgohip_packed_attention(tgohip_ctx* c, int handle, const void* q, int64_t q_
                {"out", out, out_row, qw, pl.tq, out_dtype == TGOHIP_F32 ? 4 : 8, top}};
     for (auto& o : ops) {
       if (o.rows > 1 && (o.row < o.width || o.row > o.most))
-        return fail(TGOHIP_EINVAL, std::string("packed_attention: ") + o.name + " rows are " + std::to_string(o.row) +
-                                       " elements apart and hold " + std::to_string(o.width) + "; at most " +
-                                       std::to_string(o.most) + " apart");
+        return refuse(std::string("packed_attention: ") + o.name + " rows are " + std::to_string(o.row) +
+                      " elements apart and hold " + std::to_string(o.width) + "; at most " +
+                      std::to_string(o.most) + " apart");
       if (misaligned(o.p) || (o.rows > 1 && o.row % o.unit))
-        return fail(TGOHIP_EINVAL, std::string("packed_attention: ") + o.name + " rows start on 16-byte boundaries");
+        return refuse(std::string("packed_attention: ") + o.name + " rows start on 16-byte boundaries");
     }
     if (out_dtype == TGOHIP_F16X2 && pl.tq > 1 && out_row != qw)
-      return fail(TGOHIP_EINVAL, "packed_attention: a pair's rows are dense (out_row " + std::to_string(out_row) + ", not " +
-                                     std::to_string(qw) + ")");
+      return refuse("packed_attention: a pair's rows are dense (out_row " + std::to_string(out_row) + ", not " +
+                    std::to_string(qw) + ")");
     const int64_t ob = out_dtype == TGOHIP_F32 ? 4 : 2, planes = out_dtype == TGOHIP_F16X2 ? 2 : 1;
     const Span so{(const char*)out, planes * pl.tq, 1, (pl.tq > 1 ? out_row : qw) * ob, 0, qw * ob};
     const Span in[] = {{(const char*)q, pl.tq, 1, q_row * elt(pl.q_f16), 0, qw * elt(pl.q_f16)},
                        {(const char*)k, pl.tk, 1, k_row * 2, 0, kw * 2},
                        {(const char*)v, pl.tk, 1, v_row * 2, 0, kw * 2}};
     for (int i = 0; i < 3; i++)
-      if (meet(so, in[i])) return fail(TGOHIP_EINVAL, std::string("packed_attention: out meets ") + ops[i].name + " in memory");
+      if (meet(so, in[i])) return refuse(std::string("packed_attention: out meets ") + ops[i].name + " in memory");
     PackedArgs a{};
     a.q = q;
     a.k = (const half_t*)k;
@@ -494,12 +497,12 @@ int tgohip_packed_attention(tgohip_ctx* c, int handle, const void* q, int64_t q_
 int tgohip_adapters_new(tgohip_ctx* c, int K, int N, int capacity, int* handle) {
   return guarded([&]() -> int {
     if (K <= 0 || N <= 0 || K % 64 != 0 || N % 32 != 0 || K > 1 << 22 || N > 1 << 22)
-      return fail(TGOHIP_EINVAL, "adapters_new: the projection is [" + std::to_string(K) + "," + std::to_string(N) +
-                                     "]; this library takes K a multiple of 64 and N a multiple of 32, up to 2^22");
+      return refuse("adapters_new: the projection is [" + std::to_string(K) + "," + std::to_string(N) +
+                    "]; this library takes K a multiple of 64 and N a multiple of 32, up to 2^22");
     if (capacity < 1 || capacity > 65536)
-      return fail(TGOHIP_EINVAL, "adapters_new: capacity is " + std::to_string(capacity) + "; 1 to 65536 adapters");
+      return refuse("adapters_new: capacity is " + std::to_string(capacity) + "; 1 to 65536 adapters");
     if (!c) return no_ctx("adapters_new");
-    if (!handle) return fail(TGOHIP_EINVAL, "adapters_new: handle is missing");
+    if (!handle) return refuse("adapters_new: handle is missing");
     OnDevice on(c->device);
     if (const int rc = no_capture(c, "adapters_new")) return rc;
     AdapterSet s;
@@ -508,7 +511,8 @@ int tgohip_adapters_new(tgohip_ctx* c, int K, int N, int capacity, int* handle) 
     s.table.assign((size_t)capacity, AdapterEntry{nullptr, nullptr, 0, 0.f});
     int rc = s.table_dev.ensure(s.table.size() * sizeof(AdapterEntry));
     if (!rc) {
-      const hipError_t e = hipMemcpy(s.table_dev.p, s.table.data(), s.table.size() * sizeof(AdapterEntry), hipMemcpyHostToDevice);
+      const hipError_t e = hipMemcpy(s.table_dev.p, s.table.data(), s.table.size() * sizeof(AdapterEntry),
+                                     hipMemcpyHostToDevice);
       if (e != hipSuccess) rc = fail(TGOHIP_EDEVICE, hip_message(e, "adapter table"));
     }
     if (rc) {
@@ -535,16 +539,16 @@ int tgohip_adapters_put(tgohip_ctx* c, int handle, int index, int rank, int dtyp
                         float scale) {
   return guarded([&]() -> int {
     if (rank < 1 || rank > kAdapterMaxRank)
-      return fail(TGOHIP_EINVAL, "adapters_put: rank is " + std::to_string(rank) + "; 1 to " + std::to_string(kAdapterMaxRank));
+      return refuse("adapters_put: rank is " + std::to_string(rank) + "; 1 to " + std::to_string(kAdapterMaxRank));
     if (dtype != TGOHIP_F32 && dtype != TGOHIP_F16)
-      return fail(TGOHIP_EINVAL, "adapters_put: dtype is " + std::to_string(dtype) + "; host planes are f32 or f16");
-    if (!down || !up) return fail(TGOHIP_EINVAL, "adapters_put: down and up are host planes");
-    if (!std::isfinite(scale)) return fail(TGOHIP_EINVAL, "adapters_put: scale is " + num(scale) + ", not a finite number");
+      return refuse("adapters_put: dtype is " + std::to_string(dtype) + "; host planes are f32 or f16");
+    if (!down || !up) return refuse("adapters_put: down and up are host planes");
+    if (!std::isfinite(scale)) return refuse("adapters_put: scale is " + num(scale) + ", not a finite number");
     if (!c) return no_ctx("adapters_put");
     AdapterSet* s = find(c->ops.sets, handle, "adapters_put");
     if (!s) return TGOHIP_EINVAL;
     if (index < 0 || index >= (int)s->table.size())
-      return fail(TGOHIP_EINVAL, "adapters_put: index " + std::to_string(index) + " of a set of " + std::to_string(s->table.size()));
+      return refuse("adapters_put: index " + std::to_string(index) + " of a set of " + std::to_string(s->table.size()));
     OnDevice on(c->device);
     if (const int rc = no_capture(c, "adapters_put")) return rc;
     // down [rank][K] with rows of zeros, up [N][rank] with columns of zeros, to a
@@ -557,7 +561,7 @@ int tgohip_adapters_put(tgohip_ctx* c, int handle, int index, int rank, int dtyp
       tmp.resize((size_t)rank * (s->K + (size_t)s->N));
       if (!to_half((const float*)down, tmp.data(), (size_t)rank * s->K) ||
           !to_half((const float*)up, tmp.data() + (size_t)rank * s->K, (size_t)rank * s->N))
-        return fail(TGOHIP_EINVAL, "adapters_put: a value is past f16's range (65504)");
+        return refuse("adapters_put: a value is past f16's range (65504)");
       d16 = tmp.data();
       u16 = tmp.data() + (size_t)rank * s->K;
     }
@@ -566,7 +570,8 @@ int tgohip_adapters_put(tgohip_ctx* c, int handle, int index, int rank, int dtyp
     void* dev = nullptr;
     hipError_t e = hipMalloc(&dev, h.size() * 2);
     if (e != hipSuccess)
-      return fail(TGOHIP_ENOMEM, "device allocation of " + std::to_string(h.size() * 2) + " bytes: " + hipGetErrorString(e));
+      return fail(TGOHIP_ENOMEM,
+                  "device allocation of " + std::to_string(h.size() * 2) + " bytes: " + hipGetErrorString(e));
     e = hipMemcpy(dev, h.data(), h.size() * 2, hipMemcpyHostToDevice);
     int rc = e == hipSuccess ? 0 : fail(TGOHIP_EDEVICE, hip_message(e, "adapter planes"));
     if (!rc) rc = adapter_set(c, s, index, AdapterEntry{(const half_t*)dev, (const half_t*)dev + nd, rp, scale});
@@ -582,7 +587,8 @@ int tgohip_adapters_drop(tgohip_ctx* c, int handle, int index) {
     AdapterSet* s = find(c->ops.sets, handle, "adapters_drop");
     if (!s) return TGOHIP_EINVAL;
     if (index < 0 || index >= (int)s->table.size())
-      return fail(TGOHIP_EINVAL, "adapters_drop: index " + std::to_string(index) + " of a set of " + std::to_string(s->table.size()));
+      return refuse("adapters_drop: index " + std::to_string(index) + " of a set of " +
+                    std::to_string(s->table.size()));
     OnDevice on(c->device);
     if (const int rc = no_capture(c, "adapters_drop")) return rc;
     return adapter_set(c, s, index, AdapterEntry{nullptr, nullptr, 0, 0.f});
@@ -606,20 +612,21 @@ int tgohip_adapters_free(tgohip_ctx* c, int handle) {
 
 int tgohip_adapter_rows(tgohip_ctx* c, int B, const int32_t* extents, const int32_t* adapters, int* handle) {
   return guarded([&]() -> int {
-    if (B < 0) return fail(TGOHIP_EINVAL, "adapter_rows: " + std::to_string(B) + " requests");
-    if (B > 0 && (!extents || !adapters)) return fail(TGOHIP_EINVAL, "adapter_rows: extents and adapters are host arrays");
+    if (B < 0) return refuse("adapter_rows: " + std::to_string(B) + " requests");
+    if (B > 0 && (!extents || !adapters)) return refuse("adapter_rows: extents and adapters are host arrays");
     int64_t T = 0;
     int top = -1;
     for (int b = 0; b < B; b++) {
-      if (extents[b] < 0) return fail(TGOHIP_EINVAL, "adapter_rows: request " + std::to_string(b) + " has " + std::to_string(extents[b]) + " rows");
+      const auto bad = [b](const std::string& m) { return refuse("adapter_rows: request " + std::to_string(b) + m); };
+      if (extents[b] < 0) return bad(" has " + std::to_string(extents[b]) + " rows");
       if (adapters[b] < -1 || adapters[b] >= 65536)
-        return fail(TGOHIP_EINVAL, "adapter_rows: request " + std::to_string(b) + " names adapter " + std::to_string(adapters[b]) + "; -1 (none) to 65535");
+        return bad(" names adapter " + std::to_string(adapters[b]) + "; -1 (none) to 65535");
       T += extents[b];
       if (extents[b]) top = std::max(top, (int)adapters[b]);
     }
-    if (T >= 1 << 20) return fail(TGOHIP_EINVAL, "adapter_rows: " + std::to_string(T) + " rows; below 2^20");
+    if (T >= 1 << 20) return refuse("adapter_rows: " + std::to_string(T) + " rows; below 2^20");
     if (!c) return no_ctx("adapter_rows");
-    if (!handle) return fail(TGOHIP_EINVAL, "adapter_rows: handle is missing");
+    if (!handle) return refuse("adapter_rows: handle is missing");
     if (*handle && !find(c->ops.rows, *handle, "adapter_rows")) return TGOHIP_EINVAL;
     OnDevice on(c->device);
     if (const int rc = no_capture(c, "adapter_rows")) return rc;
@@ -684,7 +691,8 @@ int tgohip_adapter_rows_free(tgohip_ctx* c, int handle) {
   });
 }
 
-int tgohip_adapters(tgohip_ctx* c, int set, int rows, const void* x, int x_dtype, const void* base, void* y, int y_dtype) {
+int tgohip_adapters(tgohip_ctx* c, int set, int rows, const void* x, int x_dtype, const void* base, void* y,
+                    int y_dtype) {
   return guarded([&]() -> int {
     if (!c) return no_ctx("adapters");
     AdapterSet* s = find(c->ops.sets, set, "adapters: set");
@@ -693,21 +701,21 @@ int tgohip_adapters(tgohip_ctx* c, int set, int rows, const void* x, int x_dtype
     if (!r) return TGOHIP_EINVAL;
     if (r->T < 0) return fail(TGOHIP_ESTATE, "adapters: the rows were not made again after a failure");
     if (x_dtype != TGOHIP_F32 && x_dtype != TGOHIP_F16 && x_dtype != TGOHIP_F16X2)
-      return fail(TGOHIP_EINVAL, "adapters: x_dtype is " + std::to_string(x_dtype) + "; f32, f16 or a pair");
+      return refuse("adapters: x_dtype is " + std::to_string(x_dtype) + "; f32, f16 or a pair");
     if (y_dtype != TGOHIP_F32 && y_dtype != TGOHIP_F16)
-      return fail(TGOHIP_EINVAL, "adapters: y_dtype is " + std::to_string(y_dtype) + "; f32 or f16");
+      return refuse("adapters: y_dtype is " + std::to_string(y_dtype) + "; f32 or f16");
     if (r->max_adapter >= (int)s->table.size())
-      return fail(TGOHIP_EINVAL, "adapters: the rows name adapter " + std::to_string(r->max_adapter) + " and the set holds " +
-                                     std::to_string(s->table.size()));
+      return refuse("adapters: the rows name adapter " + std::to_string(r->max_adapter) + " and the set holds " +
+                    std::to_string(s->table.size()));
     if (r->T == 0) return 0;
-    if (!x || !y) return fail(TGOHIP_EINVAL, "adapters: x and y are device buffers");
+    if (!x || !y) return refuse("adapters: x and y are device buffers");
     if (misaligned(x) || misaligned(base) || misaligned(y))
-      return fail(TGOHIP_EINVAL, "adapters: x, base and y start on 16-byte boundaries");
+      return refuse("adapters: x, base and y start on 16-byte boundaries");
     const int64_t T = r->T, yb = y_dtype == TGOHIP_F16 ? 2 : 4;
     const Span sx{(const char*)x, 1, 1, 0, 0, T * s->K * (x_dtype == TGOHIP_F16 ? 2 : 4)};
     const Span sy{(const char*)y, 1, 1, 0, 0, T * s->N * yb}, sb{(const char*)base, 1, 1, 0, 0, T * s->N * yb};
-    if (meet(sy, sx)) return fail(TGOHIP_EINVAL, "adapters: y meets x in memory");
-    if (base && base != y && meet(sy, sb)) return fail(TGOHIP_EINVAL, "adapters: y meets base in memory; y is base itself or apart");
+    if (meet(sy, sx)) return refuse("adapters: y meets x in memory");
+    if (base && base != y && meet(sy, sb)) return refuse("adapters: y meets base in memory; y is base itself or apart");
     AdapterArgs a{};
     a.table = (const AdapterEntry*)s->table_dev.p;
     a.tiles = (const AdapterTile*)((const char*)r->meta.p + r->tiles_off);
