@@ -313,7 +313,9 @@ int tgohip_dequant_f16(tgohip_ctx* ctx, int handle, uint16_t* y);
  * layer's calls then only launch kernels on the context's stream. Such calls
  * can be captured into a HIP graph; making, changing or freeing a handle is
  * refused then (TGOHIP_ESTATE), and a handle that a graph was captured with is not
- * replaced or freed while the graph is used (its memory may move). No counterpart
+ * replaced or freed while the graph is used (its memory may move). How a batch is cut
+ * depends on the whole of it, and the order of a row's f32 sums on the cut; one plan
+ * gives the same bits at every call. No counterpart
  * in the reference, whose step has one unscaled rotary layout, no adapters, and
  * attention over the block pool only. */
 

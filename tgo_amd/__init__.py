@@ -226,13 +226,19 @@ def ptr(a):
     return ctypes.c_void_p(a.data_ptr())
 
 
-def _addr(t):
-    """A contiguous device tensor's address (or None)."""
+def _elsewhere(t, what, device):
+    at = t.get_device()
+    return TgoError(EINVAL, "%s is a tensor of %s; operands are tensors of device %d" %
+                    (what, "the host" if at < 0 else "device %d" % at, device))
+
+
+def _addr(t, what, device):
+    """A contiguous tensor's address (or None), of the context's device."""
     if t is None:
         return None
     assert t.is_contiguous(), "tensors passed to the C ABI are contiguous"
-    if not t.is_cuda:
-        raise TgoError(EINVAL, "a %s tensor of the host; operands are device tensors" % t.dtype)
+    if t.get_device() != device:
+        raise _elsewhere(t, what, device)
     return t.data_ptr()
 
 
@@ -340,7 +346,7 @@ def _kind(t):
     return k
 
 
-def _heads_view(t, what):
+def _heads_view(t, what, device):
     """(address, row stride, head stride, dtype code) of a device tensor [rows, heads, head_dim]."""
     s = t.stride()
     if len(s) != 3 or (s[2] != 1 and t.shape[2] > 1):
@@ -348,14 +354,14 @@ def _heads_view(t, what):
     kind = _kind(t)
     if kind is None:
         raise TgoError(EINVAL, "%s is %s; float32 or float16" % (what, t.dtype))
-    if not t.is_cuda:
-        raise TgoError(EINVAL, "%s is a tensor of the host; operands are device tensors" % what)
+    if t.get_device() != device:
+        raise _elsewhere(t, what, device)
     return t.data_ptr(), s[0], s[1], kind
 
 
-def _packed_rows(t, what, rows, heads, d, kind):
+def _packed_rows(t, what, device, rows, heads, d, kind):
     """(address, row stride, dtype code) of a packed operand [rows, heads, d] whose heads are dense."""
-    at, row, head, dt = _heads_view(t, what)
+    at, row, head, dt = _heads_view(t, what, device)
     if tuple(t.shape) != (rows, heads, d) or (heads > 1 and head != d):
         raise TgoError(EINVAL, "%s is [%d, %d, %d] with dense heads" % (what, rows, heads, d))
     if kind is not None and dt != kind:
@@ -559,6 +565,7 @@ class Context:
         if not self.h:
             raise TgoError(EDEVICE, last_error())
         self.cfg = None
+        self.device = device
         self._ropes, self._packed, self._sets, self._rows = {}, {}, {}, {}  # what this binding checks shapes by
 
     def close(self):
@@ -751,11 +758,12 @@ class Context:
             if shape != y.shape or shape[0] != T or (d is not None and shape[2] != d):
                 raise TgoError(EINVAL, "rope: tensor %d is %s and %s for %d positions and heads of %s" %
                                (i, tuple(shape), tuple(y.shape), T, d))
-            xa, xr, xh, xd = _heads_view(x, "rope: x")
-            ya, yr, yh, yd = _heads_view(y, "rope: y")
+            xa, xr, xh, xd = _heads_view(x, "rope: x", self.device)
+            ya, yr, yh, yd = _heads_view(y, "rope: y", self.device)
             f += xa, ya, xr, xh, yr, yh, shape[1], xd, yd, (1 if turn[0] else 0) if turn else 1
         n = len(heads)
-        check(_lib.tgohip_rope(self.h, handle, _addr(positions), T, _ROPE_HEADS[n].pack(*f) if n < 4 else None, n))
+        check(_lib.tgohip_rope(self.h, handle, _addr(positions, "positions", self.device), T,
+                               _ROPE_HEADS[n].pack(*f) if n < 4 else None, n))
 
     def packed_plan(self, q_lengths, kv_lengths, H, Hkv, head_dim=128, causal=True, q_dtype=F32, plan=0):
         """Decomposes a batch for packed_attention; returns the plan's handle. plan: a handle whose plan
@@ -777,15 +785,15 @@ class Context:
         float16 device tensors (any row stride); out float32, float16, or [2, rows, H, head_dim] float16
         for the hi and lo planes of a pair."""
         tq, tk, H, Hkv, d, qd = self._packed.get(plan, (0, 0, 1, 1, 64, F32))
-        qa, qr, _ = _packed_rows(q, "q", tq, H, d, qd)
-        ka, kr, _ = _packed_rows(k, "k", tk, Hkv, d, F16)
-        va, vr, _ = _packed_rows(v, "v", tk, Hkv, d, F16)
+        qa, qr, _ = _packed_rows(q, "q", self.device, tq, H, d, qd)
+        ka, kr, _ = _packed_rows(k, "k", self.device, tk, Hkv, d, F16)
+        va, vr, _ = _packed_rows(v, "v", self.device, tk, Hkv, d, F16)
         if out.dim() == 4:
             if tuple(out.shape) != (2, tq, H, d) or not out.is_contiguous() or _kind(out) != F16:
                 raise TgoError(EINVAL, "out as a pair is a dense float16 [2, %d, %d, %d]" % (tq, H, d))
-            oa, orow, od = _addr(out), H * d, F16X2
+            oa, orow, od = _addr(out, "out", self.device), H * d, F16X2
         else:
-            oa, orow, od = _packed_rows(out, "out", tq, H, d, None)
+            oa, orow, od = _packed_rows(out, "out", self.device, tq, H, d, None)
         check(_lib.tgohip_packed_attention(self.h, plan, qa, qr, ka, kr, va, vr, scale, oa, orow, od))
 
     def adapters_new(self, K, N, capacity):
@@ -837,7 +845,9 @@ class Context:
                 or (base is not None and (base.numel() < T * N or _kind(base) != y_dtype))):
             raise TgoError(EINVAL, "adapters: x %s, base and y %s of %d rows of [%d, %d]; x_dtype %d, y_dtype %d" %
                            (tuple(x.shape), tuple(y.shape), T, K, N, x_dtype, y_dtype))
-        check(_lib.tgohip_adapters(self.h, handle, rows, _addr(x), x_dtype, _addr(base), _addr(y), y_dtype))
+        at = self.device
+        check(_lib.tgohip_adapters(self.h, handle, rows, _addr(x, "x", at), x_dtype, _addr(base, "base", at),
+                                   _addr(y, "y", at), y_dtype))
 
     def greedy(self, logits, B, V, ids, margins=None):
         """sample argmax (first strict maximum) and TopTwoMargin over device rows."""

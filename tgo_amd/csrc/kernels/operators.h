@@ -39,7 +39,7 @@ struct PackedItem {
   int32_t shift;    // token t sees keys 0 .. min(t + shift, nk - 1)
   int32_t r0, nr;
   int32_t kv_lo, kv_hi;
-  int32_t kvh;      // -1: an empty slot of the launch order
+  int32_t kvh;
   int32_t part;     // first row of its partial result, -1 when it writes out
 };
 // Rows [r0, r0 + nr) of a (sequence, kv head): `parts` partial results, row i of

@@ -587,96 +587,94 @@ __device__ __forceinline__ void pack_values(PackRows<D, QF16>& w, const float16_
   if (!QF16) w.l += (l[0] + l[1]) + (l[2] + l[3]);
 }
 
-// Rows [w0, w0 + 32 blocks) of an item again, for a workgroup that met an infinite
+// Rows [w0, w0 + 32) of an item again, for a workgroup that met an infinite
 // or NaN value in a tile some of its rows see only part of: a masked key's
 // probability is 0, but 0 times such a value is not. The products take those
 // values as 0 (the same sums, to the bit, where none is seen); a product of
 // visibility and occurrence then tells which outputs see +inf and which -inf, NaN
 // being both. Rare: a plain loop behind the kernel's own.
 template <int D, bool QF16>
-__device__ __forceinline__ void packed_redo(const PackedArgs* ap, int item, int w0, int blocks, lds_t K, lds_t V,
+__device__ __forceinline__ void packed_redo(const PackedArgs* ap, int item, int w0, lds_t K, lds_t V,
                                             lds_t buf) {
   const PackedArgs& a = *ap;
   const PackedItem it = a.items[item];
   const int tid = threadIdx.x, lane = tid & 63, kh = lane >> 5;
   const int kat = pack_k_at<D>(lane & 31, kh), vat = pack_v_at<D>(lane);
-  for (int b = 0; b < blocks; b++) {
-    PackRows<D, QF16> w;
-    w.init(a, it, w0 + 32 * b, lane);
+  PackRows<D, QF16> w;
+  w.init(a, it, w0, lane);
 #pragma unroll 1
-    for (int pass = 0; pass < 3; pass++) {
-      float16_t seen[D / 32];
+  for (int pass = 0; pass < 3; pass++) {
+    float16_t seen[D / 32];
 #pragma unroll
-      for (int db = 0; db < D / 32; db++) seen[db] = float16_t{};
+    for (int db = 0; db < D / 32; db++) seen[db] = float16_t{};
 #pragma unroll 1
-      for (int t0 = it.kv_lo; t0 < it.kv_hi; t0 += kPackTile) {
-        __syncthreads();
-        for (int i = tid; i < kPackTile * (D / 8); i += blockDim.x) {
-          const int p = i / (D / 8), c = i % (D / 8);
-          const int64_t row = it.k0 + min(t0 + p, it.kv_hi - 1);
-          *(__attribute__((address_space(3))) half8_t*)(K + p * 2 * D + 16 * (c ^ pack_k_swz<D>(p))) =
-              *(const half8_t*)(a.k + row * a.k_row + it.kvh * D + c * 8);
-          *(__attribute__((address_space(3))) half8_t*)(V + p * 2 * D + 16 * (c ^ pack_v_swz<D>(p))) =
-              *(const half8_t*)(a.v + row * a.v_row + it.kvh * D + c * 8);
-        }
-        __syncthreads();
-        float16_t sc[2];
-        half8_t ps[4];
-        const int left = min(w.lim, it.kv_hi - 1) - t0 - 4 * kh;
-        if (pass == 0) {
-          pack_scores<D, QF16>(w, K, kat, sc);
-          bool any = false;
-#pragma unroll
-          for (int pb = 0; pb < 2; pb++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-              const bool vis = pack_visible(left, pb, i);
-              any |= vis;
-              if (!vis) sc[pb][i] = -INFINITY;
-            }
-          if (!__builtin_amdgcn_ballot_w64(any)) continue;  // as the kernel skips it
-          if constexpr (QF16) pack_probs_f16<D>(w, sc, a.qscale, ps);
-          else pack_maximum<D>(w, sc, a.qscale);
-        }
-        float l[4] = {};
-#pragma unroll
-        for (int u = 0; u < 4; u++) {
-          half8_t ph = ps[u], pl;
-          if (pass == 0) {
-            if (!QF16) pack_probs<QF16>(sc, u, a.qscale, w.m, l[u], ph, pl);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-              ph[e] = (half_t)(pack_visible(left, u >> 1, (u & 1) * 8 + e) ? 1.f : 0.f);
-          }
-#pragma unroll
-          for (int db = 0; db < D / 32; db++) {
-            half8_t va = pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-              const float f = (float)va[e];
-              if (pass == 0) va[e] = fabsf(f) < INFINITY ? va[e] : (half_t)0.f;
-              else va[e] = (half_t)(f != f || f == (pass == 1 ? INFINITY : -INFINITY) ? 1.f : 0.f);
-            }
-            if (pass == 0) {
-              w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, w.o[db], 0, 0, 0);
-              if (!QF16) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl, w.o[db], 0, 0, 0);
-            } else {
-              seen[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, seen[db], 0, 0, 0);
-            }
-          }
-        }
-        w.l += (l[0] + l[1]) + (l[2] + l[3]);
+    for (int t0 = it.kv_lo; t0 < it.kv_hi; t0 += kPackTile) {
+      __syncthreads();
+      for (int i = tid; i < kPackTile * (D / 8); i += blockDim.x) {
+        const int p = i / (D / 8), c = i % (D / 8);
+        const int64_t row = it.k0 + min(t0 + p, it.kv_hi - 1);
+        *(__attribute__((address_space(3))) half8_t*)(K + p * 2 * D + 16 * (c ^ pack_k_swz<D>(p))) =
+            *(const half8_t*)(a.k + row * a.k_row + it.kvh * D + c * 8);
+        *(__attribute__((address_space(3))) half8_t*)(V + p * 2 * D + 16 * (c ^ pack_v_swz<D>(p))) =
+            *(const half8_t*)(a.v + row * a.v_row + it.kvh * D + c * 8);
       }
+      __syncthreads();
+      float16_t sc[2];
+      half8_t ps[4];
+      const int left = min(w.lim, it.kv_hi - 1) - t0 - 4 * kh;
+      if (pass == 0) {
+        pack_scores<D, QF16>(w, K, kat, sc);
+        bool any = false;
 #pragma unroll
-      for (int db = 0; db < D / 32; db++)
+        for (int pb = 0; pb < 2; pb++)
 #pragma unroll
-        for (int i = 0; i < 16; i++)
-          if (seen[db][i] > 0.f) w.o[db][i] += pass == 1 ? INFINITY : -INFINITY;
+          for (int i = 0; i < 16; i++) {
+            const bool vis = pack_visible(left, pb, i);
+            any |= vis;
+            if (!vis) sc[pb][i] = -INFINITY;
+          }
+        if (!__builtin_amdgcn_ballot_w64(any)) continue;  // as the kernel skips it
+        if constexpr (QF16) pack_probs_f16<D>(w, sc, a.qscale, ps);
+        else pack_maximum<D>(w, sc, a.qscale);
+      }
+      float l[4] = {};
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        half8_t ph = ps[u], pl;
+        if (pass == 0) {
+          if (!QF16) pack_probs<QF16>(sc, u, a.qscale, w.m, l[u], ph, pl);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            ph[e] = (half_t)(pack_visible(left, u >> 1, (u & 1) * 8 + e) ? 1.f : 0.f);
+        }
+#pragma unroll
+        for (int db = 0; db < D / 32; db++) {
+          half8_t va = pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u);
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const float f = (float)va[e];
+            if (pass == 0) va[e] = fabsf(f) < INFINITY ? va[e] : (half_t)0.f;
+            else va[e] = (half_t)(f != f || f == (pass == 1 ? INFINITY : -INFINITY) ? 1.f : 0.f);
+          }
+          if (pass == 0) {
+            w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, w.o[db], 0, 0, 0);
+            if (!QF16) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl, w.o[db], 0, 0, 0);
+          } else {
+            seen[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, seen[db], 0, 0, 0);
+          }
+        }
+      }
+      w.l += (l[0] + l[1]) + (l[2] + l[3]);
     }
-    __syncthreads();
-    w.write(a, it, lane, buf);
+#pragma unroll
+    for (int db = 0; db < D / 32; db++)
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        if (seen[db][i] > 0.f) w.o[db][i] += pass == 1 ? INFINITY : -INFINITY;
   }
+  __syncthreads();
+  w.write(a, it, lane, buf);
 }
 
 // The workgroup's share of a tile by DMA (global_load_lds_dwordx4): lane i of wave v's
@@ -772,8 +770,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_kernel(PackedArgs a) {
   const int per = TB / (128 * D);
   lds_t buf = (lds_t)(wave < per ? K0 : wave < 2 * per ? V0 : wave < 3 * per ? K1 : V1) + wave % per * 128 * D;
   if (__syncthreads_or(bad)) {
-    packed_redo<D, QF16>((const PackedArgs*)__builtin_amdgcn_kernarg_segment_ptr(), blockIdx.x, w0, 1, (lds_t)K0,
-                         (lds_t)V0, buf);
+    packed_redo<D, QF16>((const PackedArgs*)__builtin_amdgcn_kernarg_segment_ptr(), blockIdx.x, w0, (lds_t)K0, (lds_t)V0,
+                         buf);
     return;
   }
   w.write(a, it, lane, buf);

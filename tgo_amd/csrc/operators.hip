@@ -35,11 +35,14 @@ void OpHandles::release() {
 
 namespace {
 
-// Entry points do not throw across the C ABI.
+// Entry points do not throw across the C ABI, and a refused call leaves no error behind
+// that the next launch would report as its own.
 template <typename F>
 int guarded(F f) {
   try {
-    return f();
+    const int rc = f();
+    if (rc) (void)hipGetLastError();
+    return rc;
   } catch (const std::bad_alloc&) {
     return fail(TGOHIP_ENOMEM, "host allocation failed");
   } catch (const std::exception& e) {
