@@ -194,6 +194,23 @@ def test_packed_parts_cover_every_key_once(seed):
         assert one.tiles + one.few <= p.tiles + p.few
 
 
+def test_a_batch_is_cut_where_that_ends_sooner():
+    """On 256 compute units of two workgroups: a batch that fills them evenly stays whole, one that a few
+    workgroups outlast is cut, and a short batch of long contexts goes over the whole chip."""
+    def plan(nq, nk, **kw):
+        return tgo_amd.packed_describe(nq, nk, 32, 8, **kw)
+    p = plan([1] * 64, [4096] * 64)  # 512 workgroups of one length
+    assert (p.few, p.longest_few, p.part_rows) == (512, 4096, 0)
+    p = plan([1] * 66, [4096] * 66)  # 16 more than run at a time
+    assert p.few > 528 and p.longest_few == 4096 and 0 < p.merged_rows < 66 * 32
+    p = plan([1], [32768])  # 8 kv heads over every compute unit, in pieces of one size
+    assert (p.few, p.longest_few, p.part_rows, p.merged_rows) == (512, 512, 2048, 32)
+    p = plan([100, 20], [2300, 2700])
+    assert p.tiles == 256 and p.longest_tile < 2300 / 4 and p.merged_rows == 120 * 32
+    p = plan([2048], [2048], q_dtype=tgo_amd.F16)  # the long rows beside the short ones
+    assert (p.tiles, p.part_rows) == (512, 0)
+
+
 def test_packed_describe_refusals():
     for kw in (dict(head_dim=80), dict(ncu=0), dict(q_dtype=2)):
         with pytest.raises(TgoError):

@@ -626,6 +626,16 @@ def test_adapters_many_rows(ctx, torch_gpu, extents):
     check_adapters(ctx, torch_gpu, 1024, 1536, [8 + i for i in range(39)], extents, who, "x2", "f32")
 
 
+@pytest.mark.parametrize("xk,yk", [("f32", "f32"), ("x2", "f32"), ("f16", "f16"), ("f32", "f16"), ("f16", "f32")])
+@pytest.mark.parametrize("K,N,ranks", [(64, 32, [3, 16]), (192, 96, [30, 9]), (1088, 160, [64, 17, 50]), (4096, 2080, [128, 5, 70])])
+def test_adapters_of_large_tiles(ctx, torch_gpu, K, N, ranks, xk, yk):
+    """Beyond 512 rows tiles hold up to 64: full ones and ones of 1, 16, 17, 33, 48 and 63 rows, requests
+    without an adapter between them, odd numbers of 64-element units in a share of K."""
+    extents = [200, 1, 64, 81, 33, 16, 65, 112, 3]
+    who = [0, 1, -1, 1, 0, len(ranks) - 1, -1, len(ranks) - 1, 0]
+    check_adapters(ctx, torch_gpu, K, N, ranks, extents, who, xk, yk, base="same" if K == 192 else "apart")
+
+
 def test_adapters_are_replaced_and_dropped(ctx, torch_gpu):
     torch = torch_gpu
     K, N = 256, 128
