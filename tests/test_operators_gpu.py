@@ -893,6 +893,48 @@ def test_captured_adapters_and_split_attention_replay(ctx, torch_gpu):
             f(a)
 
 
+def test_rotary_and_adapter_offsets_past_32_bits(ctx, torch_gpu):
+    """More than 2^31 elements of heads, of x and of y: the last rows are right, and the first ones too."""
+    torch = torch_gpu
+    T, K, r = 140000, 16384, 4
+    assert T * K > 2 ** 31
+    buf = torch.zeros(T, K, device="cuda", dtype=torch.float16)
+    x = torch.zeros_like(buf)
+    at = torch.tensor([0, 1, 77777, T - 65, T - 2, T - 1], device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x[at] = torch.randn(len(at), K, device="cuda", generator=g).half()
+    buf[at] = torch.randn(len(at), K, device="cuda", generator=g).half()
+    base = buf[at].double()
+    down, up = make_adapter(torch, K, K, r, 5)
+    s, rows, h = ctx.adapters_new(K, K, 1), ctx.adapter_rows([T], [0]), ctx.rope_new(128, 1e4, layout=tgo_amd.ROPE_HALF)
+    try:
+        ctx.adapters_put(s, 0, down.cpu().numpy(), up.cpu().numpy(), 1.5)
+        print("adapters: %d rows of [%d, %d]" % (T, K, K), flush=True)
+        ctx.adapters(s, rows, x, buf, buf, x_dtype=tgo_amd.F16, y_dtype=tgo_amd.F16)
+        torch.cuda.synchronize()
+        loaded = {0: (down.double(), up.double(), 1.5)}
+        want, tol = adapters64(torch, x[at].double(), base, [len(at)], [0], loaded, K, K, False)
+        assert bool(((buf[at].double() - want).abs() <= tol + f16_step(want)).all())
+        assert float(buf.abs().sum(1, dtype=torch.float32).count_nonzero()) == len(at)  # no row but these
+        print("rope: %d rows of %d heads" % (T, K // 128), flush=True)
+        positions = torch.arange(T, device="cuda", dtype=torch.int32)
+        before = x[at].double().reshape(len(at), K // 128, 128)
+        heads = x.view(T, K // 128, 128)
+        ctx.rope(h, positions, [(heads, heads)])
+        torch.cuda.synchronize()
+        w, _ = tgo_amd.rope_freqs(128, 1e4, layout=tgo_amd.ROPE_HALF)
+        angle = at.double()[:, None] * torch.tensor(w, device="cuda")[None]
+        c, sn = angle.cos()[:, None], angle.sin()[:, None]
+        a, b = before[..., :64], before[..., 64:]
+        want = torch.cat([a * c - b * sn, a * sn + b * c], 2)
+        # cos and sin within 2 ulp of 1, two f32 operations, one f16 rounding
+        tol = 8 * U * (a.abs() + b.abs()).repeat(1, 1, 2) + f16_step(want)
+        assert bool(((heads[at].double() - want).abs() <= tol).all())
+    finally:
+        for f, a in ((ctx.rope_free, h), (ctx.adapters_free, s), (ctx.adapter_rows_free, rows)):
+            f(a)
+
+
 def test_one_row_of_strange_strides_and_its_refusals(ctx, torch_gpu):
     """A single row's stride says nothing: the pair's lo plane is a row's width behind the hi plane, and the
     check of what it meets goes by that. A scale past 2^32 is refused."""
