@@ -374,12 +374,13 @@ int tgohip_rope(tgohip_ctx* ctx, int handle, const int32_t* positions, int T,
 /* Attention over packed sequences. Sequence s has q_lengths[s] query rows and
  * kv_lengths[s] key rows, each packed one sequence behind the other (either may
  * be 0). causal: query i of n_q sits at position n_kv - n_q + i and sees the keys
- * up to it; otherwise every key. A query that sees no key gives zeros, and no
- * key or value that a query does not see (another sequence's, a later token's)
- * reaches its output, infinities and NaN included (an infinite value that it does
- * see may give NaN in place of the infinity: its f16 probability, or the lo part of
- * a pair's, may be 0). Each kv head serves H / H_kv neighbouring query heads, H at
- * most 65536. head_dim 64 or 128.
+ * up to it; otherwise every key. A query that sees no key gives zeros (one whose
+ * scores are all -inf gives NaN, as their softmax is), and no key or value that a
+ * query does not see (another sequence's, a later token's) reaches its output,
+ * infinities and NaN included (an infinite key or value that it does see may give
+ * NaN in place of the infinity: its f16 probability, or the lo part of a pair's or
+ * of an f32 query's, may be 0). Each kv head serves H / H_kv neighbouring query
+ * heads, H at most 65536. head_dim 64 or 128.
  * packed_plan decomposes the batch under *handle (host arrays; *handle 0: a new
  * one; a plan's handle: that plan is replaced in stream order, its memory
  * reused). It holds the partial results of contexts split over several
@@ -402,7 +403,9 @@ int tgohip_packed_describe(int B, const int32_t* q_lengths, const int32_t* kv_le
  * plan's q_dtype, k and v [key rows, H_kv, head_dim] f16, out like q in f32, f16
  * or as a pair (TGOHIP_F16X2, dense rows, the lo plane behind the hi plane). Rows
  * are *_row elements apart (k's and v's at most 2^24, q's and out's 2^30), heads
- * dense; rows start on 16-byte boundaries. scale is above 0 and at most 2^32. With
+ * dense; rows start on 16-byte boundaries. scale is above 0 and at most 2^32, and every
+ * finite score is right to the error of its own products, the steps of f32 at its size
+ * (scores past 2^22 in log2 units take a slower path). With
  * f32 queries the products are those of tgohip_paged_attention's f32 form (q and
  * the probabilities as f16 hi + lo pairs, so |q| < 65504); with f16 queries the
  * probabilities are rounded to f16. Sums, maxima and partial results are f32.

@@ -1046,3 +1046,171 @@ def test_handles_are_not_made_or_changed_under_capture(ctx, torch_gpu):
     finally:
         for f, a in ((ctx.rope_free, h), (ctx.adapters_free, s), (ctx.adapter_rows_free, rows), (ctx.packed_free, plan)):
             f(a)
+
+
+# ---------------------------------------------------------------------------
+# scores past the steps of f32
+# ---------------------------------------------------------------------------
+
+def exact_scores(torch, nq, nk, H, Hkv, d, f16, bases, seed=1):
+    """q, k, v whose products are whole numbers below 2^24, exact in f32 in every order: a key's first dim
+    (`bases`, of the position in its sequence) sets the size, a small second one the order of the keys, with
+    many ties. f32 queries have a lo part."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.zeros(sum(nq), H, d, device="cuda")
+    q[..., 0] = 2048 if f16 else 2049
+    q[..., 1] = torch.randint(-3, 4, (sum(nq), H), device="cuda", generator=g).float()
+    k = torch.zeros(sum(nk), Hkv, d, device="cuda")
+    k[..., 0] = torch.cat([bases(m) for m in nk])[:, None]
+    k[..., 1] = torch.randint(0, 40, (sum(nk), Hkv), device="cuda", generator=g).float()
+    v = torch.randn(sum(nk), Hkv, d, device="cuda", generator=g).half()
+    return (q.half() if f16 else q), k.half(), v
+
+
+def check_exact_scores(torch, got, q, k, v, nq, nk, scale, causal):
+    H, d = q.shape[1:]
+    G, f16 = H // k.shape[1], q.dtype == torch.float16
+    tq = tk = 0
+    for n, m in zip(nq, nk):
+        for h in range(H):
+            s = scale * (q[tq:tq + n, h].double() @ k[tk:tk + m, h // G].double().t())
+            seen = torch.ones_like(s, dtype=torch.bool)
+            if causal:
+                seen = torch.arange(m, device="cuda")[None] <= torch.arange(m - n, m, device="cuda")[:, None]
+            s = s.masked_fill(~seen, -math.inf)
+            live, top = seen.any(1, keepdim=True), s.amax(1, keepdim=True)
+            gap = torch.where(seen, top - s, 0.0)
+            p = torch.where(seen, (-gap).exp(), 0.0)
+            l = p.sum(1, keepdim=True).clamp_min(1e-300)
+            vh = v[tk:tk + m, h // G].double()
+            want = torch.where(live, p @ vh / l, 0.0)
+            # An exponent is the exact score less the reference: log2(e) scale is rounded twice (2 U of the gap),
+            # the difference and its rest once each (U of themselves, the rest at most U |top|), as often as the
+            # reference moves or parts are merged; past 2^32 two scores are equal or 2^9 apart and more, and the
+            # rest is the same for equal ones. exp2 and few more steps: 64 U.
+            rest = torch.where(top.abs() < 2.0 ** 32, 16 * U * U * 1.45 * top.abs(), 0.0)
+            e = p * (8 * U * gap.clamp_max(200.0) + torch.where(live, rest, 0.0) + 64 * U + (HALF if f16 else 2.0 ** -22)
+                     + 4 * math.sqrt(m) * U) + seen * (p < 1) * 2.0 ** -25
+            tol = (e @ vh.abs() + (e.sum(1, keepdim=True) / l) * (p @ vh.abs())) / l
+            out = got[tq:tq + n, h].double()
+            tol = tol + (f16_step(want) if got.dtype == torch.float16 else U * want.abs())
+            err = (out - want).abs()
+            assert bool((err <= torch.where(live, tol, 0.0)).all()), (n, m, h, scale, int((~(err <= tol)).any(1).sum()),
+                                                                      int(out.isnan().any(1).sum()), int((out == 0).all(1).sum()))
+        tq, tk = tq + n, tk + m
+
+
+LARGE = {"few": ([1, 1, 2], [64, 700, 131]), "tiles": ([200, 64, 33], [200, 300, 33]), "merged": ([1, 3], [30000, 9000]),
+         "cut": ([100], [12000])}
+
+
+@pytest.mark.parametrize("form", sorted(LARGE))
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("f16", [False, True])
+def test_packed_attention_with_scores_past_f32_steps(ctx, torch_gpu, f16, d, form):
+    """Scores of 2^20 to 2^54 in log2 units, where neighbouring f32 are up to 2^31 apart: the largest key,
+    and the keys that tie with it, take all there is. Constant size, rising and falling along the context,
+    and far below 0."""
+    torch = torch_gpu
+    nq, nk = LARGE[form]
+    flat = lambda m: torch.full((m,), 2048.0, device="cuda")
+    steps = lambda m: (torch.arange(m, device="cuda") * 8 // m).float() * 256
+    for bases in (flat, lambda m: -flat(m), steps, lambda m: steps(m).flip(0), lambda m: steps(m) - 2048):
+        q, k, v = exact_scores(torch, nq, nk, 4, 2, d, f16, bases)
+        for bits in (20, 23, 25, 27, 28, 29, 31, 36, 46, 54):
+            scale = float(np.float32(2.0 ** (bits - 22) / 1.44))
+            out = attend(ctx, torch, q, k, v, nq, nk, True, out=torch.full(q.shape, float("nan"), device="cuda"), scale=scale)
+            check_exact_scores(torch, out, q, k, v, nq, nk, scale, True)
+
+
+@pytest.mark.parametrize("form", sorted(LARGE))
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("size,scale", [(1.0, 2.0 ** 24), (1.0, 2.0 ** 28), (60000.0, 128 ** -0.5), (60000.0, 2.0 ** 32)])
+def test_packed_attention_over_the_whole_range_of_scores(ctx, torch_gpu, size, scale, f16, form):
+    """Whatever the size of finite queries, keys and scale, a row is the value of its leading key where that
+    leads by more than the products' own error, and lies among its values where it does not."""
+    torch = torch_gpu
+    nq, nk = LARGE[form]
+    d, H, Hkv = 128, 4, 2
+    g = torch.Generator(device="cuda").manual_seed(9)
+    make = (lambda *s: torch.randn(*s, device="cuda", generator=g)) if size == 1 else (
+        lambda *s: (torch.rand(*s, device="cuda", generator=g) * 2 - 1) * size)
+    q, k, v = make(sum(nq), H, d), make(sum(nk), Hkv, d).half(), torch.randn(sum(nk), Hkv, d, device="cuda", generator=g).half()
+    q = q.half() if f16 else q
+    out = attend(ctx, torch, q, k, v, nq, nk, True, out=torch.full(q.shape, float("nan"), device="cuda"), scale=scale)
+    led = tq = tk = 0
+    for n, m in zip(nq, nk):
+        seen = torch.arange(m, device="cuda")[None] <= torch.arange(m - n, m, device="cuda")[:, None]
+        for h in range(H):
+            qh, kh, vh = q[tq:tq + n, h].double(), k[tk:tk + m, h // 2].double(), v[tk:tk + m, h // 2].double()
+            s = (qh @ kh.t()).masked_fill(~seen, -math.inf)
+            off = (2.0 ** -22 + 4 * math.sqrt(d) * U) * (qh.abs() @ kh.abs().t()).amax(1)
+            two = s.topk(min(2, m), 1).values
+            got = out[tq:tq + n, h].double()
+            lead = (two[:, 0] - two[:, -1] > 2 * off + 60 / scale) | (seen.sum(1) == 1)
+            want = vh[s.argmax(1)]
+            # the probability and its sum as pairs, or as the same f16, and the division
+            assert bool(((got - want).abs() <= 2.0 ** -20 * want.abs() + 2.0 ** -30)[lead].all()), (n, m, h)
+            lo = torch.where(seen[:, :, None], vh[None], math.inf).amin(1) if n * m < 1 << 16 else vh.amin(0)
+            hi = torch.where(seen[:, :, None], vh[None], -math.inf).amax(1) if n * m < 1 << 16 else vh.amax(0)
+            assert bool(((got >= lo - 2.0 ** -8) & (got <= hi + 2.0 ** -8)).all()), (n, m, h)
+            led += int(lead.sum())
+        tq, tk = tq + n, tk + m
+    assert led > 0.8 * sum(nq) * H
+
+
+@pytest.mark.parametrize("form", sorted(LARGE))
+@pytest.mark.parametrize("f16", [False, True])
+def test_rows_whose_keys_all_score_minus_infinity(ctx, torch_gpu, f16, form):
+    """The softmax of scores that are all -inf is NaN, that of no scores is a row of zeros, and some of -inf
+    count nothing beside finite ones."""
+    torch = torch_gpu
+    nq, nk = LARGE[form]
+    nq, nk = nq + [5], nk + [3]  # two queries that see no key
+    q, k, v = inputs(torch, nq, nk, 4, 2, 64, f16)
+    q[..., 0] = 1 if f16 else 1 + 2.0 ** -12  # the lo part is not 0: 0 times -inf would be NaN
+    part, rest = k.clone(), torch.ones(len(k), dtype=torch.bool, device="cuda")
+    at = 0
+    for m in nk:
+        part[at + m // 3:at + m, :, 0] = float("-inf")
+        rest[at + m // 3:at + m] = False
+        at += m
+    whole = k.clone()
+    whole[..., 0] = float("-inf")
+    out = attend(ctx, torch, q, whole, v, nq, nk)
+    none = torch.zeros(len(q), dtype=torch.bool, device="cuda")
+    none[sum(nq) - 5:sum(nq) - 3] = True
+    assert bool((out[none] == 0).all()) and bool(out[~none].isnan().all())
+    # the same rows over the keys that are left: as many as each query sees of them
+    out = attend(ctx, torch, q, part, v, nq, nk, False)
+    want = [m // 3 for m in nk]
+    short = attend(ctx, torch, q, k[rest].contiguous(), v[rest].contiguous(), nq, want, False)
+    live = torch.cat([torch.full((n,), m > 0, device="cuda") for n, m in zip(nq, want)])
+    both = 2.0 ** -9 if f16 else 2.0 ** -18  # other tiles and cuts: a few roundings of probabilities and sums each
+    assert bool(((out - short).abs()[live] <= both * v.abs().max()).all())
+
+
+@pytest.mark.parametrize("form", sorted(LARGE))
+@pytest.mark.parametrize("f16", [False, True])
+def test_rows_of_large_scores_leave_the_rows_beside_them_alone(ctx, torch_gpu, f16, form):
+    """Every other row's scores are of 2^30, those of the rows between are ordinary, and keep their bits; so do
+    all of them beside a value that is not finite and that they do not see."""
+    torch = torch_gpu
+    nq, nk = LARGE[form]
+    q, k, v = inputs(torch, nq, nk, 6, 2, 128, f16)
+    q[..., 0] = 0
+    k[:, :, 0] = torch.randint(1, 9, k.shape[:2], device="cuda").half() * 4096
+    large = q.clone()
+    large[:, ::2, 0] = 32768.0
+    small = attend(ctx, torch, q, k, v, nq, nk)
+    mixed = attend(ctx, torch, large, k, v, nq, nk)
+    torch.cuda.synchronize()
+    assert torch.equal(mixed[:, 1::2], small[:, 1::2])
+    assert not bool(mixed.isnan().any())
+    # the first sequence's last key, which its last query sees, and the last one's first, which all of it see
+    for at, first, last in ((nk[0] - 1, nq[0] - 1, nq[0]), (sum(nk) - nk[-1], sum(nq) - nq[-1], sum(nq))):
+        bad = v.clone()
+        bad[at] = float("inf")
+        out = attend(ctx, torch, large, k, bad, nq, nk)
+        torch.cuda.synchronize()
+        assert torch.equal(out[:first], mixed[:first]) and torch.equal(out[last:], mixed[last:])

@@ -66,7 +66,7 @@ struct PackedArgs {
   const half_t* v;
   void* out;
   float* part_o;   // [part_rows][D]
-  float* part_ml;  // [part_rows][2]: the reference maximum (log2) and the sum
+  float* part_ml;  // [part_rows][4]: the reference m, e (log2) and the sum
   const PackedItem* items;
   const PackedMerge* merges;
   int64_t q_row, k_row, v_row, out_row, out_lo;  // elements

@@ -40,12 +40,21 @@ constexpr int kFewTile = 32;    // keys of a wave's tile there
 constexpr int kFewWaves = 2;
 constexpr int kPackWaves = 4;
 constexpr int kPackRows = 32 * kPackWaves;  // rows of an item of packed_kernel
-// Online softmax with a lazy reference m (log2 units): it starts at kPackNoMax, a
-// row's probabilities are 2^(s - m), and m moves to the row's maximum - kPackLift
-// once that passes m + kPackTop. They so stay below 2^kPackTop (f16 ends at 2^16),
-// and the largest is at least 2^kPackLift: an f16 probability keeps an absolute
-// error of 2^(-25 - kPackLift) of it, its normal range reaching 2^-21 of it.
+// Online softmax with a lazy reference m + e (log2 units): it starts at kPackNoMax, a
+// row's probabilities are 2^(s - m - e), and it moves to the row's maximum - kPackLift
+// once that passes it by more than kPackTop. They so stay below 2^kPackTop (f16 ends at
+// 2^16), and the largest is at least about 2^kPackLift: an f16 probability keeps an
+// absolute error of 2^(-25 - kPackLift) of it, its normal range reaching 2^-21 of it.
+// The multiply-add that scales a score subtracts m in the same rounding, so the one thing
+// lost in m is its distance from the maximum: half a step of f32, up to 1/4 while |m| is
+// at most kPackFar, and there e is 0. Past that (a step is 16 at 2^28, and probabilities
+// would pass f16 or all be 0) m is the rounded maximum and e what it lacks, kPackLift
+// less; the lift itself is lost in e from 2^48 on, where two scores are equal or a step
+// of 2^25 apart. The kernels' loops keep no e, nor its check in every tile: where a row's
+// reference goes past kPackFar, its workgroup takes its keys again with one, as it does
+// for values that are not finite.
 constexpr float kPackNoMax = -1.0e30f;
+constexpr float kPackFar = 4194304.f;  // 2^22
 constexpr float kPackLift = 7.f;
 constexpr float kPackTop = 15.f;
 constexpr float kPackSum = 32768.f;  // 2^kPackTop
@@ -392,15 +401,32 @@ __device__ __forceinline__ void pack_load_q(const void* q, int64_t off, half8_t&
   }
 }
 
+// Four neighbouring values of a result, `off` elements from its start.
+__device__ __forceinline__ void pack_store4(const PackedArgs& a, int64_t off, float4_t v) {
+  if (a.out_form == OUT_F32) {
+    *(float4_t*)((float*)a.out + off) = v;
+    return;
+  }
+  half4_t hv, lv;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    hv[e] = (half_t)v[e];
+    lv[e] = (half_t)(v[e] - (float)hv[e]);
+  }
+  *(half4_t*)((half_t*)a.out + off) = hv;
+  if (a.out_form == OUT_X2) *(half4_t*)((half_t*)a.out + a.out_lo + off) = lv;
+}
+
 // One 32-row block of a wave: where its rows are, what they have seen. Lane (r, kh)
 // = (lane % 32, lane / 32) holds row r: its query's dims 16s + 8kh + [0,8), its
-// maximum and (its half of the keys') sum, and of O^T dims 32db + 8g + 4kh + [0,4).
-template <int D, bool QF16>
+// reference and (its half of the keys') sum, and of O^T dims 32db + 8g + 4kh + [0,4),
+// db below NB.
+template <int D, bool QF16, int NB = D / 32>
 struct PackRows {
   int r, lim;  // row of the item and its last visible key
   half8_t qh[D / 16], ql[QF16 ? 1 : D / 16];
-  float m, l;
-  float16_t o[D / 32];
+  float m, e, l;
+  float16_t o[NB];
 
   // Rows past the item's repeat its first one; nothing of them is stored.
   __device__ __forceinline__ void init(const PackedArgs& a, const PackedItem& it, int r0, int lane) {
@@ -414,9 +440,19 @@ struct PackRows {
   }
   __device__ __forceinline__ void clear() {
     m = kPackNoMax;
+    e = 0.f;
     l = 0.f;
 #pragma unroll
-    for (int db = 0; db < D / 32; db++) o[db] = float16_t{};
+    for (int db = 0; db < NB; db++) o[db] = float16_t{};
+  }
+  // 1 over a row's sum, and what a sum of 0 gives: 0 where the row sees no key, NaN where
+  // its scores are all -inf. A part keeps its sum, and says the latter in m's place.
+  __device__ __forceinline__ float2 finish(const PackedArgs& a, const PackedItem& it, int lane) {
+    l += __shfl_xor(l, 32, 64);
+    const bool part = it.part >= 0, blank = l == 0.f && lim >= it.kv_lo;
+    if (part && lane < 32 && r < it.nr)
+      *(float4_t*)(a.part_ml + ((int64_t)it.part + r) * 4) = float4_t{blank ? NAN : m, e, l, 0.f};
+    return float2{part ? 1.f : 1.f / l, blank && !part ? NAN : 0.f};
   }
   // The rows' results, through 128 D bytes of LDS that are the wave's own: a lane
   // holds four dims of its row at a time, and stores leave in whole rows. Stored as
@@ -424,24 +460,19 @@ struct PackRows {
   // a tile (8192 items of 128 rows, f16).
   __device__ __forceinline__ void write(const PackedArgs& a, const PackedItem& it, int lane, lds_t buf) {
     typedef __attribute__((address_space(3))) float4_t* f4;
-    l += __shfl_xor(l, 32, 64);
+    const float2 fin = finish(a, it, lane);
     const int l32 = lane & 31, kh = lane >> 5;
     const bool part = it.part >= 0;
-    const float inv = part ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int db = 0; db < D / 32; db++)
 #pragma unroll
       for (int g = 0; g < 4; g++) {
         float4_t v;
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = l == 0.f ? 0.f : o[db][4 * g + e] * inv;
+        for (int e = 0; e < 4; e++) v[e] = l == 0.f ? fin.y : o[db][4 * g + e] * fin.x;
         const int c = db * 8 + 2 * g + kh;  // chunk of four dims
         *(f4)(buf + l32 * 4 * D + 16 * (c ^ (l32 & 7))) = v;
       }
-    if (part && kh == 0 && r < it.nr) {
-      a.part_ml[((int64_t)it.part + r) * 2] = m;
-      a.part_ml[((int64_t)it.part + r) * 2 + 1] = l;
-    }
     pack_wave_sync();
     const int r0 = r - l32;
     if (part || a.out_form == OUT_F32) {
@@ -483,8 +514,8 @@ struct PackRows {
 
 // S^T = K . Q^T on v_mfma_f32_32x32x16_f16: lane (r, kh) gets row r's scores at keys
 // 32pb + 8(i/4) + 4kh + i%4 of the tile.
-template <int D, bool QF16>
-__device__ __forceinline__ void pack_scores(const PackRows<D, QF16>& w, lds_t K, int at, float16_t (&sc)[2]) {
+template <int D, bool QF16, int NB>
+__device__ __forceinline__ void pack_scores(const PackRows<D, QF16, NB>& w, lds_t K, int at, float16_t (&sc)[2]) {
   sc[0] = sc[1] = float16_t{};
 #pragma unroll
   for (int s = 0; s < D / 16; s++)
@@ -501,8 +532,8 @@ __device__ __forceinline__ void pack_scores(const PackRows<D, QF16>& w, lds_t K,
 __device__ __forceinline__ bool pack_visible(int left, int pb, int i) {
   return pb * 32 + 8 * (i >> 2) + (i & 3) <= left;
 }
-// A row's largest score of a tile, scaled.
-__device__ __forceinline__ float pack_top(const float16_t (&sc)[2], float qs) {
+// A row's largest score of a tile, not scaled.
+__device__ __forceinline__ float pack_top(const float16_t (&sc)[2]) {
   // one chain: the compiler makes it 16 three-way maxima (of pairs, it quiets every
   // score first, 32 instructions more)
   float t = -INFINITY;
@@ -510,32 +541,47 @@ __device__ __forceinline__ float pack_top(const float16_t (&sc)[2], float qs) {
   for (int pb = 0; pb < 2; pb++)
 #pragma unroll
     for (int i = 0; i < 16; i++) t = fmaxf(t, sc[pb][i]);
-  return fmaxf(t, __shfl_xor(t, 32, 64)) * qs;
+  return fmaxf(t, __shfl_xor(t, 32, 64));
 }
-// Moves the reference maximum of the rows that need it to their tile's largest score
-// t. A row's own scores alone decide: its result does not depend on the rows beside it.
-template <int D, bool QF16>
-__device__ __forceinline__ void pack_raise(PackRows<D, QF16>& w, float t, bool need) {
-  const float mnew = need ? t - kPackLift : w.m;
-  const float alpha = __builtin_amdgcn_exp2f(w.m - mnew);
+// Moves the reference of the rows that need it to their tile's largest score `top`. A
+// row's own scores alone decide: its result does not depend on the rows beside it. Without
+// an e (FAR false), past: a row's reference should have one.
+template <bool FAR, int D, bool QF16, int NB>
+__device__ __forceinline__ void pack_raise(PackRows<D, QF16, NB>& w, float top, float qs, bool need, bool& past) {
+#pragma clang fp contract(off)  // the same bits in every kernel
+  const float t = top * qs;
+  const bool far = fabsf(t) > kPackFar;
+  const float mnew = need ? (FAR && far ? t : fmaf(top, qs, -kPackLift)) : w.m;
+  float alpha = w.m - mnew;
+  if constexpr (FAR) {
+    const float enew = need ? (far ? fmaf(top, qs, -t) - kPackLift : 0.f) : w.e;
+    alpha += w.e - enew;
+    w.e = enew;
+  } else {
+    past |= need && far;
+  }
+  alpha = __builtin_amdgcn_exp2f(alpha);
   w.l *= alpha;
 #pragma unroll
-  for (int db = 0; db < D / 32; db++) w.o[db] *= alpha;
+  for (int db = 0; db < NB; db++) w.o[db] *= alpha;
   w.m = mnew;
 }
 // Scores 8u .. 8u + 7 of the lane to probabilities, their sum on l, as f16 (or a
 // pair) where the second product's B operand wants them: its k index 8kh + e of
 // step u is key 16u + (e < 4 ? 4kh + e : 8 + 4kh + e - 4), the lane's own score e.
 // f16 probabilities are summed as rounded, two to an instruction, in f32.
-template <bool QF16>
+template <bool QF16, bool FAR>
 __device__ __forceinline__ void pack_probs(const float16_t (&sc)[2], int u, float qs, float m, float& l, half8_t& ph,
-                                           half8_t& pl) {
+                                           half8_t& pl, float below) {
   typedef float float2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
   for (int e = 0; e < 8; e += 2) {
     float2_t p;
 #pragma unroll
-    for (int g = 0; g < 2; g++) p[g] = __builtin_amdgcn_exp2f(fmaf(sc[u >> 1][8 * (u & 1) + e + g], qs, -m));
+    for (int g = 0; g < 2; g++) {
+      const float x = fmaf(sc[u >> 1][8 * (u & 1) + e + g], qs, -m);
+      p[g] = __builtin_amdgcn_exp2f(FAR ? x - below : x);
+    }
     const half2_t h = __builtin_convertvector(p, half2_t);
     ph[e] = h[0];
     ph[e + 1] = h[1];
@@ -555,49 +601,51 @@ __device__ __forceinline__ void pack_probs(const float16_t (&sc)[2], int u, floa
 // key far above the ones before): only then is the tile's maximum looked for, and
 // the probabilities taken again. That saves the search, 25 of 165 VALU
 // instructions a tile.
-template <int D>
-__device__ __forceinline__ void pack_probs_f16(PackRows<D, true>& w, const float16_t (&sc)[2], float qs,
-                                               half8_t (&ph)[4]) {
+template <bool FAR, int D, int NB>
+__device__ __forceinline__ void pack_probs_f16(PackRows<D, true, NB>& w, const float16_t (&sc)[2], float qs,
+                                               half8_t (&ph)[4], bool& past) {
   float l[4] = {};
   half8_t none;
 #pragma unroll
-  for (int u = 0; u < 4; u++) pack_probs<true>(sc, u, qs, w.m, l[u], ph[u], none);
+  for (int u = 0; u < 4; u++) pack_probs<true, FAR>(sc, u, qs, w.m, l[u], ph[u], none, w.e);
   const bool over = (l[0] + l[1]) + (l[2] + l[3]) > kPackSum;
   if (__builtin_amdgcn_ballot_w64(over)) {  // uniform across the wave
     const bool other = __shfl_xor((int)over, 32, 64);  // the row's other half of the keys
-    pack_raise<D, true>(w, pack_top(sc, qs), over | other);
+    pack_raise<FAR>(w, pack_top(sc), qs, over | other, past);
 #pragma unroll
     for (int u = 0; u < 4; u++) {
       l[u] = 0.f;
-      pack_probs<true>(sc, u, qs, w.m, l[u], ph[u], none);
+      pack_probs<true, FAR>(sc, u, qs, w.m, l[u], ph[u], none, w.e);
     }
   }
   w.l += (l[0] + l[1]) + (l[2] + l[3]);
 }
 // A tile's maximum, before its pairs of probabilities.
-template <int D>
-__device__ __forceinline__ void pack_maximum(PackRows<D, false>& w, const float16_t (&sc)[2], float qs) {
-  const float t = pack_top(sc, qs);
-  const bool grow = t > w.m + kPackTop;
-  if (__builtin_amdgcn_ballot_w64(grow)) pack_raise<D, false>(w, t, grow);
+template <bool FAR, int D, bool QF16, int NB>
+__device__ __forceinline__ void pack_maximum(PackRows<D, QF16, NB>& w, const float16_t (&sc)[2], float qs, bool& past) {
+  const float top = pack_top(sc);
+  bool grow = top * qs > w.m + kPackTop;  // as without an e where the row has none
+  if (FAR && fabsf(w.m) > kPackFar + kPackLift) grow = fmaf(top, qs, -w.m) - w.e > kPackTop;
+  if (__builtin_amdgcn_ballot_w64(grow)) pack_raise<FAR>(w, top, qs, grow, past);
 }
 // A tile's probabilities and O^T += V^T . P^T. f16 probabilities all come first: the
 // other wave of the SIMD fills the matrix unit meanwhile. Pairs come step by step,
 // or they would not fit the registers beside q's pairs.
 template <int D, bool QF16>
-__device__ __forceinline__ void pack_values(PackRows<D, QF16>& w, const float16_t (&sc)[2], float qs, lds_t V, int at) {
+__device__ __forceinline__ void pack_values(PackRows<D, QF16>& w, const float16_t (&sc)[2], float qs, lds_t V, int at,
+                                            bool& past) {
   half8_t ph[4], pl, first[D / 32];
   if (QF16) {
     // the first products' operands come from LDS under the exponentials
 #pragma unroll
     for (int db = 0; db < D / 32; db++) first[db] = pack_v_frag<D>(V, at ^ (64 * db));
   }
-  if constexpr (QF16) pack_probs_f16<D>(w, sc, qs, ph);
-  else pack_maximum<D>(w, sc, qs);
+  if constexpr (QF16) pack_probs_f16<false>(w, sc, qs, ph, past);
+  else pack_maximum<false>(w, sc, qs, past);
   float l[4] = {};  // a chain of adds per step
 #pragma unroll
   for (int u = 0; u < 4; u++) {
-    if (!QF16) pack_probs<QF16>(sc, u, qs, w.m, l[u], ph[u], pl);
+    if (!QF16) pack_probs<QF16, false>(sc, u, qs, w.m, l[u], ph[u], pl, 0.f);
 #pragma unroll
     for (int db = 0; db < D / 32; db++) {
       const half8_t va = QF16 && u == 0 ? first[db] : pack_v_frag<D>(V, (at ^ (64 * db)) + 32 * D * u);
@@ -609,70 +657,70 @@ __device__ __forceinline__ void pack_values(PackRows<D, QF16>& w, const float16_
   if (!QF16) w.l += (l[0] + l[1]) + (l[2] + l[3]);
 }
 
-// Rows [w0, w0 + 32) of an item again, for a workgroup that met an infinite
-// or NaN value in a tile some of its rows see only part of: a masked key's
+// Rows [w0, w0 + 32) of an item again, for a workgroup whose references need an e or that
+// met an infinite or NaN value in a tile some of its rows see only part of: a masked key's
 // probability is 0, but 0 times such a value is not. The products take those
 // values as 0 (the same sums, to the bit, where none is seen); a product of
 // visibility and occurrence then tells which outputs see +inf and which -inf, NaN
-// being both. Rare: a plain loop behind the kernel's own.
+// being both. Rare: a plain loop behind the kernel's own, 32 dims of the result at a
+// time, so that it needs no more registers than the kernel (with all dims at once the
+// 128-dim kernels kept 102 to 111 registers in memory around it).
 template <int D, bool QF16>
-__device__ __forceinline__ void packed_redo(const PackedArgs* ap, int item, int w0, lds_t K, lds_t V,
-                                            lds_t buf) {
+__device__ __forceinline__ void packed_redo(const PackedArgs* ap, int item, int w0, lds_t K, lds_t V) {
   const PackedArgs& a = *ap;
   const PackedItem it = a.items[item];
   const int tid = threadIdx.x, lane = tid & 63, kh = lane >> 5;
-  const int kat = pack_k_at<D>(lane & 31, kh), vat = pack_v_at<D>(lane);
-  PackRows<D, QF16> w;
-  w.init(a, it, w0, lane);
+  const int kat = pack_k_at<D>(lane & 31, kh);
+  PackRows<D, QF16, 1> w;
 #pragma unroll 1
-  for (int pass = 0; pass < 3; pass++) {
-    float16_t seen[D / 32];
-#pragma unroll
-    for (int db = 0; db < D / 32; db++) seen[db] = float16_t{};
+  for (int db = 0; db < D / 32; db++) {
+    const int vat = pack_v_at<D>(lane) ^ (64 * db);
+    w.init(a, it, w0, lane);
+    bool past = false;
 #pragma unroll 1
-    for (int t0 = it.kv_lo; t0 < it.kv_hi; t0 += kPackTile) {
-      __syncthreads();
-      for (int i = tid; i < kPackTile * (D / 8); i += blockDim.x) {
-        const int p = i / (D / 8), c = i % (D / 8);
-        const int64_t row = it.k0 + min(t0 + p, it.kv_hi - 1);
-        *(__attribute__((address_space(3))) half8_t*)(K + p * 2 * D + 16 * (c ^ pack_k_swz<D>(p))) =
-            *(const half8_t*)(a.k + row * a.k_row + it.kvh * D + c * 8);
-        *(__attribute__((address_space(3))) half8_t*)(V + p * 2 * D + 16 * (c ^ pack_v_swz<D>(p))) =
-            *(const half8_t*)(a.v + row * a.v_row + it.kvh * D + c * 8);
-      }
-      __syncthreads();
-      float16_t sc[2];
-      half8_t ps[4];
-      const int left = min(w.lim, it.kv_hi - 1) - t0 - 4 * kh;
-      if (pass == 0) {
-        pack_scores<D, QF16>(w, K, kat, sc);
-        bool any = false;
-#pragma unroll
-        for (int pb = 0; pb < 2; pb++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const bool vis = pack_visible(left, pb, i);
-            any |= vis;
-            if (!vis) sc[pb][i] = -INFINITY;
-          }
-        if (!__builtin_amdgcn_ballot_w64(any)) continue;  // as the kernel skips it
-        if constexpr (QF16) pack_probs_f16<D>(w, sc, a.qscale, ps);
-        else pack_maximum<D>(w, sc, a.qscale);
-      }
-      float l[4] = {};
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        half8_t ph = ps[u], pl;
-        if (pass == 0) {
-          if (!QF16) pack_probs<QF16>(sc, u, a.qscale, w.m, l[u], ph, pl);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; e++)
-            ph[e] = (half_t)(pack_visible(left, u >> 1, (u & 1) * 8 + e) ? 1.f : 0.f);
+    for (int pass = 0; pass < 3; pass++) {
+      float16_t seen = {};
+#pragma unroll 1
+      for (int t0 = it.kv_lo; t0 < it.kv_hi; t0 += kPackTile) {
+        __syncthreads();
+        for (int i = tid; i < kPackTile * (D / 8); i += blockDim.x) {
+          const int p = i / (D / 8), c = i % (D / 8);
+          const int64_t row = it.k0 + min(t0 + p, it.kv_hi - 1);
+          *(__attribute__((address_space(3))) half8_t*)(K + p * 2 * D + 16 * (c ^ pack_k_swz<D>(p))) =
+              *(const half8_t*)(a.k + row * a.k_row + it.kvh * D + c * 8);
+          *(__attribute__((address_space(3))) half8_t*)(V + p * 2 * D + 16 * (c ^ pack_v_swz<D>(p))) =
+              *(const half8_t*)(a.v + row * a.v_row + it.kvh * D + c * 8);
         }
+        __syncthreads();
+        float16_t sc[2];
+        half8_t ps[4];
+        const int left = min(w.lim, it.kv_hi - 1) - t0 - 4 * kh;
+        if (pass == 0) {
+          pack_scores(w, K, kat, sc);
+          bool any = false;
 #pragma unroll
-        for (int db = 0; db < D / 32; db++) {
-          half8_t va = pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u);
+          for (int pb = 0; pb < 2; pb++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const bool vis = pack_visible(left, pb, i);
+              any |= vis;
+              if (!vis) sc[pb][i] = -INFINITY;
+            }
+          if (!__builtin_amdgcn_ballot_w64(any)) continue;  // as the kernel skips it
+          if constexpr (QF16) pack_probs_f16<true>(w, sc, a.qscale, ps, past);
+          else pack_maximum<true>(w, sc, a.qscale, past);
+        }
+        float l[4] = {};
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          half8_t ph = ps[u], pl, va = pack_v_frag<D>(V, vat + 32 * D * u);
+          if (pass == 0) {
+            if (!QF16) pack_probs<QF16, true>(sc, u, a.qscale, w.m, l[u], ph, pl, w.e);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+              ph[e] = (half_t)(pack_visible(left, u >> 1, (u & 1) * 8 + e) ? 1.f : 0.f);
+          }
 #pragma unroll
           for (int e = 0; e < 8; e++) {
             const float f = (float)va[e];
@@ -680,23 +728,32 @@ __device__ __forceinline__ void packed_redo(const PackedArgs* ap, int item, int 
             else va[e] = (half_t)(f != f || f == (pass == 1 ? INFINITY : -INFINITY) ? 1.f : 0.f);
           }
           if (pass == 0) {
-            w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, w.o[db], 0, 0, 0);
-            if (!QF16) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl, w.o[db], 0, 0, 0);
+            w.o[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, w.o[0], 0, 0, 0);
+            if (!QF16) w.o[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl, w.o[0], 0, 0, 0);
           } else {
-            seen[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, seen[db], 0, 0, 0);
+            seen = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, seen, 0, 0, 0);
           }
         }
+        w.l += (l[0] + l[1]) + (l[2] + l[3]);
       }
-      w.l += (l[0] + l[1]) + (l[2] + l[3]);
-    }
-#pragma unroll
-    for (int db = 0; db < D / 32; db++)
 #pragma unroll
       for (int i = 0; i < 16; i++)
-        if (seen[db][i] > 0.f) w.o[db][i] += pass == 1 ? INFINITY : -INFINITY;
+        if (seen[i] > 0.f) w.o[0][i] += pass == 1 ? INFINITY : -INFINITY;
+    }
+    const float2 fin = w.finish(a, it, lane);
+    const int row = it.r0 + w.r;
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      float4_t v;
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = w.l == 0.f ? fin.y : w.o[0][4 * g + e] * fin.x;
+      const int d = 32 * db + 8 * g + 4 * kh;
+      if (w.r < it.nr) {
+        if (it.part >= 0) *(float4_t*)(a.part_o + ((int64_t)it.part + w.r) * D + d) = v;
+        else pack_store4(a, (it.q0 + row / a.G) * a.out_row + (it.kvh * a.G + row % a.G) * D + d, v);
+      }
+    }
   }
-  __syncthreads();
-  w.write(a, it, lane, buf);
 }
 
 // The workgroup's share of a tile by DMA (global_load_lds_dwordx4): lane i of wave v's
@@ -768,7 +825,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_kernel(PackedArgs a) {
     dma(t0 + kPackTile, Kn, Vn);
     if (t0 > whi) return;  // no row of this wave sees the tile
     float16_t sc[2];
-    pack_scores<D, QF16>(w, K, kat, sc);
+    pack_scores(w, K, kat, sc);
     if (t0 + kPackTile - 1 > wlo || t0 + kPackTile > it.kv_hi) {
       const int left = min(w.lim, it.kv_hi - 1) - t0 - 4 * kh;
 #pragma unroll
@@ -781,7 +838,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_kernel(PackedArgs a) {
 #pragma unroll
         for (int db = 0; db < D / 32; db++) bad |= half8_nonfinite(pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u));
     }
-    pack_values<D, QF16>(w, sc, a.qscale, V, vat);
+    pack_values<D, QF16>(w, sc, a.qscale, V, vat, bad);
   };
   for (int t0 = it.kv_lo; t0 < it.kv_hi; t0 += 2 * kPackTile) {
     tile(t0, (lds_t)K0, (lds_t)V0, (lds_t)K1, (lds_t)V1);
@@ -792,8 +849,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_kernel(PackedArgs a) {
   const int per = TB / (128 * D);
   lds_t buf = (lds_t)(wave < per ? K0 : wave < 2 * per ? V0 : wave < 3 * per ? K1 : V1) + wave % per * 128 * D;
   if (__syncthreads_or(bad)) {
-    packed_redo<D, QF16>((const PackedArgs*)__builtin_amdgcn_kernarg_segment_ptr(), blockIdx.x, w0, (lds_t)K0, (lds_t)V0,
-                         buf);
+    packed_redo<D, QF16>((const PackedArgs*)__builtin_amdgcn_kernarg_segment_ptr(), blockIdx.x, w0, (lds_t)K0, (lds_t)V0);
     return;
   }
   w.write(a, it, lane, buf);
@@ -851,9 +907,9 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void packed_few_kernel(PackedArg
   const int wlo = min(it.r0 / a.G + it.shift, it.nk - 1);
   const int whi = min((it.r0 + it.nr - 1) / a.G + it.shift, it.nk - 1);
 
-  // MODE 0: the attention. Where a masked tile holds a value that is not finite, the
-  // keys run again as packed_redo does: MODE 1 with such values as 0, then 2 and 3
-  // for what the rows see of +inf and -inf.
+  // MODE 0: the attention. Where a masked tile holds a value that is not finite, or a
+  // reference needs its e, the keys run again as packed_redo does: MODE 1 with one and
+  // such values as 0, then 2 and 3 for what the rows see of +inf and -inf.
   bool bad = false;
   float16_t seen[D / 32];
   auto run = [&](auto mode) {
@@ -881,12 +937,11 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void packed_few_kernel(PackedArg
         }
 #pragma unroll
         for (int i = 0; i < 16; i++) sc[1][i] = -INFINITY;
-        const float t = pack_top(sc, a.qscale);
-        const bool grow = t > w.m + kPackTop;
-        if (__builtin_amdgcn_ballot_w64(grow)) pack_raise<D, QF16>(w, t, grow);
+        pack_maximum<MODE == 1>(w, sc, a.qscale, bad);
         float l[2] = {};
 #pragma unroll
-        for (int u = 0; u < 2; u++) pack_probs<QF16>(sc, u, a.qscale, w.m, l[u], ph[u], pl[u]);
+        for (int u = 0; u < 2; u++)
+          pack_probs<QF16, MODE == 1>(sc, u, a.qscale, w.m, l[u], ph[u], pl[u], w.e);
         w.l += l[0] + l[1];
       } else {
 #pragma unroll
@@ -946,23 +1001,24 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void packed_few_kernel(PackedArg
     add(-INFINITY);
     __syncthreads();
   }
-  // The second wave's rows to the first one's maximum, through LDS.
+  // The two waves' rows to the higher one's reference, through LDS.
   static_assert(kFewWaves == 2 && 2 * TB >= 128 * D, "a buffer holds a wave's rows");
   typedef __attribute__((address_space(3))) float16_t* f16p;
-  typedef __attribute__((address_space(3))) float* fp;
+  typedef __attribute__((address_space(3))) float4_t* f4;
   if (wave == 1) {
 #pragma unroll
     for (int db = 0; db < D / 32; db++) *(f16p)((lds_t)K0 + (db * 64 + lane) * 64) = w.o[db];
-    *(fp)((lds_t)V0 + lane * 8) = w.m;
-    *(fp)((lds_t)V0 + lane * 8 + 4) = w.l;
+    *(f4)((lds_t)V0 + lane * 16) = float4_t{w.m, w.e, w.l, 0.f};
   }
   __syncthreads();
   if (wave == 1) return;
-  const float m1 = *(fp)((lds_t)V0 + lane * 8), l1 = *(fp)((lds_t)V0 + lane * 8 + 4);
-  const float m = fmaxf(w.m, m1);
-  const float x0 = __builtin_amdgcn_exp2f(w.m - m), x1 = __builtin_amdgcn_exp2f(m1 - m);
-  w.l = x0 * w.l + x1 * l1;
-  w.m = m;
+  const float4_t other = *(f4)((lds_t)V0 + lane * 16);
+  const float up = (other[0] - w.m) + (other[1] - w.e);
+  const bool higher = up > 0.f;
+  const float x0 = higher ? __builtin_amdgcn_exp2f(-up) : 1.f, x1 = higher ? 1.f : __builtin_amdgcn_exp2f(up);
+  w.l = x0 * w.l + x1 * other[2];
+  w.m = higher ? other[0] : w.m;
+  w.e = higher ? other[1] : w.e;
 #pragma unroll
   for (int db = 0; db < D / 32; db++) {
     const float16_t o1 = *(f16p)((lds_t)K0 + (db * 64 + lane) * 64);
@@ -972,70 +1028,75 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void packed_few_kernel(PackedArg
   w.write(a, it, lane, (lds_t)K1);
 }
 
-// Merges the parts of up to eight rows: sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p.
+// Merges the parts of up to eight rows: sum_p 2^(m_p - M) o_p / sum_p 2^(m_p - M) l_p, m_p
+// and M being references, m + e.
 // D / 4 lanes hold a row, four dims each; with fewer rows the lane groups share a
 // row's parts and meet in LDS, in their order.
 template <int D>
 __global__ __launch_bounds__(256) void packed_merge_kernel(PackedArgs a) {
   constexpr int LR = D / 4, GR = 256 / LR;  // lanes per row, groups of them
   __shared__ float4_t so[GR][LR];
-  __shared__ float sl[GR], sm[GR];
+  __shared__ float sl[GR], sm[GR], se[GR];
   const PackedMerge g = a.merges[blockIdx.x];
   const int grp = threadIdx.x / LR, d = threadIdx.x % LR * 4;
   const int slices = GR / (g.nr > 4 ? 8 : g.nr > 2 ? 4 : g.nr), i = grp / slices, sl0 = grp % slices;
   float4_t v = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f, m = kPackNoMax;
+  float l = 0.f, M = kPackNoMax, E = 0.f;
+  bool blank = false;  // a part with a sum of 0 whose keys all score -inf
   if (i < g.nr) {
-    // eight parts' loads in flight, the reference maximum moving with them
-    float M = kPackNoMax;
+    // eight parts' loads in flight, the reference moving with them
     for (int p0 = sl0; p0 < g.parts; p0 += 8 * slices) {
-      float2 ml[8];
+      float3 ml[8];
       float4_t po[8];
 #pragma unroll
       for (int u = 0; u < 8; u++) {
         const int p = min(p0 + u * slices, g.parts - 1);
         const int64_t pr = (int64_t)g.part + i + (int64_t)p * g.step;
-        ml[u] = *(const float2*)(a.part_ml + pr * 2);
+        ml[u] = *(const float3*)(a.part_ml + pr * 4);
         po[u] = *(const float4_t*)(a.part_o + pr * D + d);
       }
-      float top = M;
+      float tm = M, te = E;
 #pragma unroll
       for (int u = 0; u < 8; u++) {
-        if (p0 + u * slices >= g.parts) ml[u].y = 0.f;
-        if (ml[u].y != 0.f) top = fmaxf(top, ml[u].x);  // 0: the part shows this row no key
+        blank |= ml[u].z == 0.f && ml[u].x != ml[u].x;  // past the parts: the last one again
+        if (p0 + u * slices >= g.parts) ml[u].z = 0.f;
+        if (ml[u].z != 0.f && (ml[u].x - tm) + (ml[u].y - te) > 0.f) tm = ml[u].x, te = ml[u].y;
       }
-      const float old = __builtin_amdgcn_exp2f(M - top);
-      M = top;
+      const float old = __builtin_amdgcn_exp2f((M - tm) + (E - te));
+      M = tm;
+      E = te;
       l *= old;
       v *= old;
 #pragma unroll
       for (int u = 0; u < 8; u++) {
-        if (ml[u].y == 0.f) continue;
-        const float w = __builtin_amdgcn_exp2f(ml[u].x - M);
-        l += w * ml[u].y;
+        if (ml[u].z == 0.f) continue;  // the part shows this row no key, or none that counts
+        const float w = __builtin_amdgcn_exp2f((ml[u].x - M) + (ml[u].y - E));
+        l += w * ml[u].z;
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] += w * po[u][e];
       }
     }
-    m = M;
   }
   if (slices > 1) {
     so[grp][d / 4] = v;
     if (d == 0) {
       sl[grp] = l;
-      sm[grp] = m;
+      sm[grp] = l == 0.f && blank ? NAN : M;
+      se[grp] = E;
     }
     __syncthreads();
     if (sl0 == 0) {
-      float top = m;
-      for (int s = 1; s < slices; s++)
-        if (sl[grp + s] != 0.f) top = fmaxf(top, sm[grp + s]);
-      float w = __builtin_amdgcn_exp2f(m - top);
+      float tm = M, te = E;
+      for (int s = 1; s < slices; s++) {
+        if (sl[grp + s] == 0.f) blank |= sm[grp + s] != sm[grp + s];
+        else if ((sm[grp + s] - tm) + (se[grp + s] - te) > 0.f) tm = sm[grp + s], te = se[grp + s];
+      }
+      float w = __builtin_amdgcn_exp2f((M - tm) + (E - te));
       l *= w;
       v *= w;
       for (int s = 1; s < slices; s++) {
         if (sl[grp + s] == 0.f) continue;
-        w = __builtin_amdgcn_exp2f(sm[grp + s] - top);
+        w = __builtin_amdgcn_exp2f((sm[grp + s] - tm) + (se[grp + s] - te));
         l += w * sl[grp + s];
 #pragma unroll
         for (int e = 0; e < 4; e++) v[e] += w * so[grp + s][d / 4][e];
@@ -1046,19 +1107,8 @@ __global__ __launch_bounds__(256) void packed_merge_kernel(PackedArgs a) {
   const int row = g.r0 + i, tok = row / a.G, head = g.kvh * a.G + row % a.G;
   const int64_t off = (g.q0 + tok) * a.out_row + head * D + d;
 #pragma unroll
-  for (int e = 0; e < 4; e++) v[e] = l == 0.f ? 0.f : v[e] / l;
-  if (a.out_form == OUT_F32) {
-    *(float4_t*)((float*)a.out + off) = v;
-    return;
-  }
-  half4_t hv, lv;
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    hv[e] = (half_t)v[e];
-    lv[e] = (half_t)(v[e] - (float)hv[e]);
-  }
-  *(half4_t*)((half_t*)a.out + off) = hv;
-  if (a.out_form == OUT_X2) *(half4_t*)((half_t*)a.out + a.out_lo + off) = lv;
+  for (int e = 0; e < 4; e++) v[e] = l == 0.f ? (blank ? NAN : 0.f) : v[e] / l;
+  pack_store4(a, off, v);
 }
 
 template <int D, bool QF16>

@@ -379,7 +379,7 @@ int tgohip_packed_plan(tgohip_ctx* c, int B, const int32_t* q_lengths, const int
     Stager sg;
     sg.add(plan.items.data(), plan.items.size() * sizeof(PackedItem));
     const size_t off = sg.add(plan.merges.data(), plan.merges.size() * sizeof(PackedMerge));
-    if (plan.part_rows) rc = p.part.ensure((size_t)plan.part_rows * (head_dim + 2) * sizeof(float));
+    if (plan.part_rows) rc = p.part.ensure((size_t)plan.part_rows * (head_dim + 4) * sizeof(float));
     if (!rc) rc = sg.upload(c, p.meta);
     if (rc) {
       if (fresh) {
