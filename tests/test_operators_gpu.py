@@ -1214,3 +1214,29 @@ def test_rows_of_large_scores_leave_the_rows_beside_them_alone(ctx, torch_gpu, f
         out = attend(ctx, torch, large, k, bad, nq, nk)
         torch.cuda.synchronize()
         assert torch.equal(out[:first], mixed[:first]) and torch.equal(out[last:], mixed[last:])
+
+
+@pytest.mark.parametrize("q_f16", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_few_rows_again_over_every_number_of_tiles(ctx, torch_gpu, q_f16, d):
+    """The few-row kernel's repeats for values that are not finite, over contexts of one to eight tiles a wave:
+    each run over the keys starts in the buffer that the one before may have ended in."""
+    torch = torch_gpu
+    nk = [5, 32, 33, 64, 65, 96, 97, 130, 161, 200, 260, 330, 420, 500]
+    nq = [5] * len(nk)
+    q, k, v = inputs(torch, nq, nk, 4, 1, d, q_f16)
+    clean = attend(ctx, torch, q, k, v, nq, nk)
+    last = torch.tensor(nk, device="cuda").cumsum(0) - 1
+    sees = (torch.arange(1, len(nk) + 1, device="cuda") * 5) - 1
+    for value in (float("nan"), float("inf"), float("-inf")):
+        bad = v.clone()
+        bad[last, :, 7] = value
+        for _ in range(3):
+            out = attend(ctx, torch, q, k, bad, nq, nk)
+            torch.cuda.synchronize()
+            keep = torch.ones(len(q), dtype=torch.bool, device="cuda")
+            keep[sees] = False
+            assert torch.equal(out[keep], clean[keep])
+            rest = [j for j in range(d) if j != 7]
+            assert torch.equal(out[sees][..., rest], clean[sees][..., rest])
+            assert not bool(out[sees][..., 7].isfinite().any())

@@ -317,9 +317,13 @@ void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int H
 // kernels
 // ---------------------------------------------------------------------------
 
-// s_waitcnt vmcnt(0) lgkmcnt(0): the wave's DMA has landed, and its LDS reads have
-// returned, before other data goes where they read.
-constexpr int kPackWait = 0x0070;
+// s_waitcnt vmcnt(0) lgkmcnt(0), and no memory access moves across it: the wave's DMA has
+// landed, and its LDS reads have returned, before other data goes where they read.
+__device__ __forceinline__ void pack_wait() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  asm volatile("" ::: "memory");
+}
 // A barrier without a memory fence, which would wait for every DMA in flight; no
 // memory access moves across it.
 __device__ __forceinline__ void pack_barrier() {
@@ -820,7 +824,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_kernel(PackedArgs a) {
   auto tile = [&](int t0, lds_t K, lds_t V, lds_t Kn, lds_t Vn) {
     // this wave's DMA of the tile has landed, every wave's has, and every wave is
     // done with the other buffer
-    __builtin_amdgcn_s_waitcnt(kPackWait);
+    pack_wait();
     pack_barrier();
     dma(t0 + kPackTile, Kn, Vn);
     if (t0 > whi) return;  // no row of this wave sees the tile
@@ -915,8 +919,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void packed_few_kernel(PackedArg
   auto run = [&](auto mode) {
     constexpr int MODE = decltype(mode)::value;
     auto tile = [&](int t0, lds_t K, lds_t V, lds_t Kn, lds_t Vn) {
-      __builtin_amdgcn_s_waitcnt(kPackWait);
-      asm volatile("" ::: "memory");
+      pack_wait();
       dma(t0 + step, Kn, Vn);
       if (t0 > whi) return;
       const int left = min(w.lim, it.kv_hi - 1) - t0 - 4 * kh;
@@ -972,7 +975,10 @@ __global__ __launch_bounds__(64 * kFewWaves, 1) void packed_few_kernel(PackedArg
           }
         }
     };
-    if (MODE != 0) dma(first, Kw[0], Vw[0]);
+    if (MODE != 0) {
+      pack_wait();  // the run before may still be reading the buffer
+      dma(first, Kw[0], Vw[0]);
+    }
     for (int t0 = first; t0 < it.kv_hi; t0 += 2 * step) {
       tile(t0, Kw[0], Vw[0], Kw[1], Vw[1]);
       if (t0 + step < it.kv_hi) tile(t0 + step, Kw[1], Vw[1], Kw[0], Vw[0]);
