@@ -424,9 +424,10 @@ int tgohip_packed_attention(tgohip_ctx* ctx, int handle, const void* q, int64_t 
  * to the nearest f16, refused past its range) or f16, rank 1 to 128. adapters_drop
  * empties an index. An empty index is no adapter. put, drop and free wait for the
  * context's stream; a graph of other streams that uses the set is waited for by its
- * owner. A captured call sees later puts and drops; it is captured for the largest
- * rank loaded so far (of 16, 32, 64 and 128), and rows of an adapter put later
- * beyond that are NaN in its replays. */
+ * owner. A call's kernels are those of the largest rank that the set holds then (of
+ * 16, 32, 64 and 128), whichever adapters its rows name. A captured call sees later
+ * puts and drops; rows of an adapter put later whose rank is beyond the largest at
+ * the capture are NaN in its replays. */
 int tgohip_adapters_new(tgohip_ctx* ctx, int K, int N, int capacity, int* handle);
 int tgohip_adapters_put(tgohip_ctx* ctx, int handle, int index, int rank, int dtype,
                         const void* down, const void* up, float scale);

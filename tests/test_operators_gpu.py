@@ -1240,3 +1240,45 @@ def test_few_rows_again_over_every_number_of_tiles(ctx, torch_gpu, q_f16, d):
             rest = [j for j in range(d) if j != 7]
             assert torch.equal(out[sees][..., rest], clean[sees][..., rest])
             assert not bool(out[sees][..., 7].isfinite().any())
+
+
+def test_a_set_is_what_it_holds(ctx, torch_gpu):
+    """An adapter of a large rank that was dropped or replaced leaves no trace: the bits of a set that never
+    held it, and a call that is captured then is captured for the ranks loaded then."""
+    torch = torch_gpu
+    K, N, extents, who = 4096, 256, [600, 70, 3], [0, 1, 0]
+    x, base = torch.randn(sum(extents), K, device="cuda").half(), torch.randn(sum(extents), N, device="cuda")
+    fresh, used, rows = ctx.adapters_new(K, N, 3), ctx.adapters_new(K, N, 3), ctx.adapter_rows(extents, who)
+    try:
+        def put(h, i, r, seed):
+            down, up = make_adapter(torch, K, N, r, seed)
+            ctx.adapters_put(h, i, down.cpu().numpy(), up.cpu().numpy(), 1.0)
+
+        def run(h):
+            y = torch.full_like(base, float("nan"))
+            ctx.adapters(h, rows, x, base, y, x_dtype=tgo_amd.F16)
+            torch.cuda.synchronize()
+            return y
+        put(used, 2, 128, 9)
+        put(used, 1, 100, 8)
+        for h in (fresh, used):
+            put(h, 0, 16, 1)
+            put(h, 1, 8, 2)
+        ctx.adapters_drop(used, 2)
+        assert torch.equal(run(used), run(fresh))
+        graph, side, y = torch.cuda.CUDAGraph(), torch.cuda.Stream(), torch.zeros_like(base)
+        ctx.set_stream(side.cuda_stream)
+        try:
+            with torch.cuda.graph(graph, stream=side):
+                ctx.adapters(used, rows, x, base, y, x_dtype=tgo_amd.F16)
+        finally:
+            ctx.set_stream(torch.cuda.current_stream().cuda_stream)
+        put(used, 1, 33, 3)
+        for _ in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert bool(y[600:670].isnan().all())
+            assert torch.equal(y[:600], run(fresh)[:600]) and torch.equal(y[670:], run(fresh)[670:])
+    finally:
+        for f, a in ((ctx.adapters_free, fresh), (ctx.adapters_free, used), (ctx.adapter_rows_free, rows)):
+            f(a)

@@ -535,6 +535,8 @@ static int adapter_set(tgohip_ctx* c, AdapterSet* s, int index, const AdapterEnt
   TGOHIP_HIP(hipMemcpy((AdapterEntry*)s->table_dev.p + index, &e, sizeof e, hipMemcpyHostToDevice));
   (void)hipFree((void*)s->table[index].down);
   s->table[index] = e;
+  s->rank_pad = 0;
+  for (const AdapterEntry& a : s->table) s->rank_pad = std::max(s->rank_pad, a.rank_pad);
   return 0;
 }
 
@@ -579,7 +581,6 @@ int tgohip_adapters_put(tgohip_ctx* c, int handle, int index, int rank, int dtyp
     int rc = e == hipSuccess ? 0 : fail(TGOHIP_EDEVICE, hip_message(e, "adapter planes"));
     if (!rc) rc = adapter_set(c, s, index, AdapterEntry{(const half_t*)dev, (const half_t*)dev + nd, rp, scale});
     if (rc) (void)hipFree(dev);
-    else s->rank_pad = std::max(s->rank_pad, rp);
     return rc;
   });
 }

@@ -88,7 +88,7 @@ struct PackedHandle {
 };
 struct AdapterSet {
   int K = 0, N = 0;
-  int rank_pad = 0;  // the largest loaded so far
+  int rank_pad = 0;  // the largest loaded
   std::vector<AdapterEntry> table;
   DevBuf table_dev;
 };
