@@ -399,6 +399,23 @@ typedef struct {
 } tgohip_packed_plan_t;
 int tgohip_packed_describe(int B, const int32_t* q_lengths, const int32_t* kv_lengths, int H, int H_kv,
                            int head_dim, int causal, int q_dtype, int ncu, tgohip_packed_plan_t* plan);
+/* The same decomposition piece by piece. A workgroup takes rows [row, row + rows) of
+ * the sequence whose first packed query is q0 and kv head kv_head, row r being query
+ * r / (H / H_kv), and keys [kv_lo, kv_hi) of those from k0 on; query i sees keys up to
+ * i + shift. part: its first row of partial results, -1 when it writes its rows
+ * itself. A merge joins rows [row, row + rows): part p's are at partial rows
+ * part + p step on. pieces holds the tile kernel's, then the few-row kernel's;
+ * *n_pieces and *n_merges are the arrays' sizes going in (both 0: counted only) and
+ * what the batch has coming out. */
+typedef struct {
+  int32_t q0, k0, kv_head, row, rows, kv_lo, kv_hi, shift, part;
+} tgohip_packed_piece_t;
+typedef struct {
+  int32_t q0, kv_head, row, rows, part, parts, step;
+} tgohip_packed_merge_t;
+int tgohip_packed_pieces(int B, const int32_t* q_lengths, const int32_t* kv_lengths, int H, int H_kv,
+                         int head_dim, int causal, int q_dtype, int ncu, tgohip_packed_piece_t* pieces,
+                         int* n_pieces, tgohip_packed_merge_t* merges, int* n_merges);
 /* out = softmax(scale q k^T) v over a plan's rows. q [rows, H, head_dim] in the
  * plan's q_dtype, k and v [key rows, H_kv, head_dim] f16, out like q in f32, f16
  * or as a pair (TGOHIP_F16X2, dense rows, the lo plane behind the hi plane). Rows

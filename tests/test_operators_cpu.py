@@ -215,3 +215,88 @@ def test_packed_describe_refusals():
     for kw in (dict(head_dim=80), dict(ncu=0), dict(q_dtype=2)):
         with pytest.raises(TgoError):
             tgo_amd.packed_describe([1], [1], 8, 2, **kw)
+
+
+def check_pieces(nq, nk, H, Hkv, causal, **kw):
+    """Every row of every kv head is in one block of rows; a block's pieces hold its keys, each once; cut blocks
+    have partial rows of their own and merges that join each row once."""
+    pieces, merges = tgo_amd.packed_pieces(nq, nk, H, Hkv, causal=causal, **kw)
+    p = tgo_amd.packed_describe(nq, nk, H, Hkv, causal=causal, **kw)
+    assert len(pieces) == p.tiles + p.few
+    G, q0, k0 = H // Hkv, np.concatenate([[0], np.cumsum(nq)]), np.concatenate([[0], np.cumsum(nk)])
+    by = {}
+    for i, t in enumerate(pieces):
+        by.setdefault((int(t["q0"]), int(t["kv_head"]), int(t["row"]), int(t["rows"])), []).append((t, i >= p.tiles))
+    blocks = {}
+    for (at, head, row, rows) in by:
+        blocks.setdefault((at, head), []).append((row, rows))
+    used, joined = np.zeros(p.part_rows, np.int32), {}
+    for m in merges:
+        for i in range(m["rows"]):
+            key = (int(m["q0"]), int(m["kv_head"]), int(m["row"]) + i)
+            assert key not in joined
+            joined[key] = (int(m["part"]) + i, int(m["parts"]), int(m["step"]))
+        assert 1 <= m["rows"] <= 8
+    for s, (n, k) in enumerate(zip(nq, nk)):
+        for head in range(Hkv if n else 0):
+            end = 0
+            for row, rows in sorted(blocks.pop((int(q0[s]), head))):
+                assert row == end and 1 <= rows <= 128
+                end = row + rows
+                cut = sorted(by[int(q0[s]), head, row, rows], key=lambda c: c[0]["kv_lo"])
+                last = (end - 1) // G  # the block's last query, which sees the most
+                hi = max(0, min(k, last + k - n + 1)) if causal else k
+                at = 0
+                for t, few in cut:
+                    assert t["k0"] == k0[s] and t["kv_lo"] == at and (t["kv_hi"] > at or hi == 0)
+                    assert t["kv_lo"] % 64 == 0 and (not few or n * G <= 32)
+                    # queries see up to their own position, or everything
+                    assert all(min(i + int(t["shift"]), k - 1) == (min(i + k - n, k - 1) if causal else k - 1)
+                               for i in (row // G, last))
+                    at = t["kv_hi"]
+                assert at == hi and len({few for _, few in cut}) == 1
+                if len(cut) == 1:
+                    assert cut[0][0]["part"] == -1 and (int(q0[s]), head, row) not in joined
+                    continue
+                base = min(int(t["part"]) for t, _ in cut)
+                for j, (t, _) in enumerate(cut):  # the merge adds them in the keys' order
+                    assert t["part"] == base + j * rows
+                    used[t["part"]:t["part"] + rows] += 1
+                for i in range(rows):
+                    assert joined.pop((int(q0[s]), head, row + i)) == (base + i, len(cut), rows)
+            assert end == n * G
+    assert not blocks and not joined and (used == 1).all()
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_packed_pieces_hold_every_row_and_key_once(seed):
+    r = np.random.default_rng(1000 + seed)
+    n = int(r.integers(1, 24))
+    top = int(np.exp(r.uniform(0, math.log(40000))))
+    nk = np.exp(r.uniform(0, math.log(top + 1), n)).astype(int) - (r.random(n) < 0.1)
+    kind = r.integers(0, 4)
+    nq = [np.ones(n, int), r.integers(0, 9, n), r.integers(0, 500, n), np.minimum(nk, 3000)][kind]
+    H, Hkv = [(32, 8), (7, 1), (4, 4), (64, 4), (160, 1)][seed % 5]
+    for causal in (True, False):
+        for ncu in (256, 1, 40, 2048):
+            check_pieces(nq.tolist(), nk.tolist(), H, Hkv, causal, ncu=ncu, head_dim=[64, 128][seed % 2],
+                         q_dtype=[tgo_amd.F32, tgo_amd.F16][seed // 2 % 2])
+
+
+def test_packed_pieces_of_batches_that_are_cut():
+    for nq, nk in (([1], [32768]), ([1] * 66, [4096] * 66), ([100, 20], [2300, 2700]), ([128], [32768]), ([7], [0]),
+                   ([0, 0], [3, 0]), ([], []), ([1, 20], [5000, 20]), ([1] * 300, list(range(1, 30001, 100)))):
+        check_pieces(nq, nk, 32, 8, True)
+        check_pieces(nq, nk, 32, 8, False)
+
+
+def test_packed_pieces_refusals():
+    with pytest.raises(TgoError, match="head_dim is 80"):
+        tgo_amd.packed_pieces([1], [1], 8, 2, head_dim=80)
+    with pytest.raises(TgoError, match="ncu"):
+        tgo_amd.packed_pieces([1], [1], 8, 2, ncu=0)
+    a, n, m = tgo_amd.i32([5]), ctypes.c_int(1), ctypes.c_int(0)
+    one = np.zeros(1, tgo_amd.PIECE)
+    assert tgo_amd.lib().tgohip_packed_pieces(1, tgo_amd.ptr(a), tgo_amd.ptr(a), 8, 2, 128, 1, 0, 256, tgo_amd.ptr(one),
+                                              ctypes.byref(n), None, ctypes.byref(m)) == tgo_amd.EINVAL
+    assert "hold 1 pieces" in tgo_amd.last_error() and (n.value, m.value) == (2, 0)

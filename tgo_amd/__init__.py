@@ -130,6 +130,7 @@ def lib():
         "tgohip_rope": (I, [P, I, P, I, P, I]),
         "tgohip_packed_plan": (I, [P, I, P, P, I, I, I, I, I, P]),
         "tgohip_packed_describe": (I, [I, P, P, I, I, I, I, I, I, ctypes.POINTER(PackedPlan)]),
+        "tgohip_packed_pieces": (I, [I, P, P, I, I, I, I, I, I, P, P, P, P]),
         "tgohip_packed_free": (I, [P, I]),
         "tgohip_packed_attention": (I, [P, I, P, I64, P, I64, P, I64, F, P, I64, I]),
         "tgohip_adapters_new": (I, [P, I, I, I, P]),
@@ -334,6 +335,25 @@ def packed_describe(q_lengths, kv_lengths, H, Hkv, head_dim=128, causal=True, q_
     check(lib().tgohip_packed_describe(len(nq), ptr(nq), ptr(nk), H, Hkv, head_dim, int(causal), q_dtype, ncu,
                                        ctypes.byref(p)))
     return p
+
+
+PIECE = np.dtype([(n, np.int32) for n in ("q0", "k0", "kv_head", "row", "rows", "kv_lo", "kv_hi", "shift", "part")])
+MERGE = np.dtype([(n, np.int32) for n in ("q0", "kv_head", "row", "rows", "part", "parts", "step")])
+
+
+def packed_pieces(q_lengths, kv_lengths, H, Hkv, head_dim=128, causal=True, q_dtype=F32, ncu=256):
+    """A packed batch's decomposition piece by piece, without a GPU: arrays of PIECE and MERGE records."""
+    nq, nk, n, m = i32(q_lengths), i32(kv_lengths), ctypes.c_int(), ctypes.c_int()
+    if len(nq) != len(nk):
+        raise TgoError(EINVAL, "packed_pieces: %d query lengths and %d key lengths" % (len(nq), len(nk)))
+    pieces, merges = np.zeros(0, PIECE), np.zeros(0, MERGE)
+    for _ in range(2):  # counted, then filled
+        check(lib().tgohip_packed_pieces(len(nq), ptr(nq), ptr(nk), H, Hkv, head_dim, int(causal), q_dtype, ncu,
+                                         ptr(pieces), ctypes.byref(n), ptr(merges), ctypes.byref(m)))
+        if len(pieces) == n.value and len(merges) == m.value:
+            break
+        pieces, merges = np.zeros(n.value, PIECE), np.zeros(m.value, MERGE)
+    return pieces, merges
 
 
 _KINDS = {}  # a torch dtype's code: F32, F16, or None for one the operators do not take

@@ -416,6 +416,35 @@ int tgohip_packed_describe(int B, const int32_t* q_lengths, const int32_t* kv_le
   });
 }
 
+int tgohip_packed_pieces(int B, const int32_t* q_lengths, const int32_t* kv_lengths, int H, int H_kv, int head_dim,
+                         int causal, int q_dtype, int ncu, tgohip_packed_piece_t* pieces, int* n_pieces,
+                         tgohip_packed_merge_t* merges, int* n_merges) {
+  return guarded([&]() -> int {
+    const int rc = check_packed(B, q_lengths, kv_lengths, H, H_kv, head_dim, q_dtype);
+    if (rc) return rc;
+    if (ncu < 1 || !n_pieces || !n_merges) return refuse("packed_pieces: ncu, n_pieces and n_merges");
+    PackedPlan plan;
+    packed_build_plan(B, q_lengths, kv_lengths, H, H_kv, head_dim, causal != 0, q_dtype == TGOHIP_F16, ncu, plan);
+    plan.items.insert(plan.items.end(), plan.few.begin(), plan.few.end());
+    const int np = (int)plan.items.size(), nm = (int)plan.merges.size(), mp = *n_pieces, mm = *n_merges;
+    *n_pieces = np;
+    *n_merges = nm;
+    if (mp == 0 && mm == 0) return 0;
+    if (mp < np || mm < nm || (np && !pieces) || (nm && !merges))
+      return refuse("packed_pieces: the arrays hold " + std::to_string(mp) + " pieces and " + std::to_string(mm) +
+                    " merges; the batch has " + std::to_string(np) + " and " + std::to_string(nm));
+    for (int i = 0; i < np; i++) {
+      const PackedItem& it = plan.items[i];
+      pieces[i] = tgohip_packed_piece_t{it.q0, it.k0, it.kvh, it.r0, it.nr, it.kv_lo, it.kv_hi, it.shift, it.part};
+    }
+    for (int i = 0; i < nm; i++) {
+      const PackedMerge& m = plan.merges[i];
+      merges[i] = tgohip_packed_merge_t{m.q0, m.kvh, m.r0, m.nr, m.part, m.parts, m.step};
+    }
+    return 0;
+  });
+}
+
 int tgohip_packed_free(tgohip_ctx* c, int handle) {
   return guarded([&]() -> int {
     if (!c) return no_ctx("packed_free");
