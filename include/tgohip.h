@@ -385,7 +385,8 @@ int tgohip_rope(tgohip_ctx* ctx, int handle, const int32_t* positions, int T,
  * one; a plan's handle: that plan is replaced in stream order, its memory
  * reused). It holds the partial results of contexts split over several
  * workgroups, so calls that use one plan run in stream order, not at once: two
- * streams, or two graphs replayed at once, take a plan each. */
+ * streams, or two graphs replayed at once, take a plan each. A batch of more than
+ * 2^23 - 1 workgroups (128 rows of a sequence and kv head each) is refused. */
 int tgohip_packed_plan(tgohip_ctx* ctx, int B, const int32_t* q_lengths, const int32_t* kv_lengths,
                        int H, int H_kv, int head_dim, int causal, int q_dtype, int* handle);
 int tgohip_packed_free(tgohip_ctx* ctx, int handle);

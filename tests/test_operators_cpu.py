@@ -300,3 +300,20 @@ def test_packed_pieces_refusals():
     assert tgo_amd.lib().tgohip_packed_pieces(1, tgo_amd.ptr(a), tgo_amd.ptr(a), 8, 2, 128, 1, 0, 256, tgo_amd.ptr(one),
                                               ctypes.byref(n), None, ctypes.byref(m)) == tgo_amd.EINVAL
     assert "hold 1 pieces" in tgo_amd.last_error() and (n.value, m.value) == (2, 0)
+
+
+def test_batches_of_more_workgroups_than_a_launch_takes_are_refused():
+    """Before anything is decomposed: these have 8.5 and 65 million blocks of rows, the last would fill the
+    host's memory."""
+    for B in (130, 1000, 16000):
+        for call in (tgo_amd.packed_describe, tgo_amd.packed_pieces):
+            with pytest.raises(TgoError, match="workgroups, more than one launch takes"):
+                call([1] * B, [1] * B, 65536, 65536)
+        rc, msg = plan([1] * B, [1] * B, H=65536, Hkv=65536)
+        assert rc == tgo_amd.EINVAL and "more than one launch takes" in msg
+    p = tgo_amd.packed_describe([1] * 100, [1] * 100, 65536, 8192, head_dim=64)
+    assert p.tiles + p.few == 100 * 8192
+    for ncu in (0, -1, 65537, 2 ** 31 - 1):
+        for call in (tgo_amd.packed_describe, tgo_amd.packed_pieces):
+            with pytest.raises(TgoError, match="ncu"):
+                call([1], [9000], 8, 2, ncu=ncu)

@@ -55,6 +55,7 @@ struct PackedPlan {
   std::vector<PackedMerge> merges;
   int64_t part_rows = 0;
 };
+constexpr int kPackRows = 128;  // the most rows of an item
 // Decomposes a call (host only). nq, nk: [B], checked by the caller.
 void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int Hkv, int D, bool causal,
                        bool q_f16, int ncu, PackedPlan& plan);

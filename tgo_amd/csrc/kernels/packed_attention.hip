@@ -39,7 +39,7 @@ constexpr int kPackFew = 32;    // rows of a sequence and kv head up to which pa
 constexpr int kFewTile = 32;    // keys of a wave's tile there
 constexpr int kFewWaves = 2;
 constexpr int kPackWaves = 4;
-constexpr int kPackRows = 32 * kPackWaves;  // rows of an item of packed_kernel
+static_assert(kPackRows == 32 * kPackWaves, "packed_kernel takes an item's rows");
 // Online softmax with a lazy reference m + e (log2 units): it starts at kPackNoMax, a
 // row's probabilities are 2^(s - m - e), and it moves to the row's maximum - kPackLift
 // once that passes it by more than kPackTop. They so stay below 2^kPackTop (f16 ends at

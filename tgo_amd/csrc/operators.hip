@@ -195,6 +195,13 @@ void rope_freqs(const tgohip_rope_cfg& c, double* w, double* attention) {
 // Packed rows and head counts stay below this, so that every index fits 32 bits.
 constexpr int64_t kMaxIndex = (int64_t)1 << 30;
 
+// Items and merges are one launch each, of at most 256 threads a workgroup.
+int packed_fits(int64_t items, int64_t merges) {
+  const int64_t most = INT_MAX / 256, n = std::max(items, merges);
+  if (n <= most) return 0;
+  return refuse("packed_plan: the batch needs " + std::to_string(n) + " workgroups, more than one launch takes");
+}
+
 int check_packed(int B, const int32_t* nq, const int32_t* nk, int H, int Hkv, int D, int q_dtype) {
   if (B < 0) return refuse("packed_plan: " + std::to_string(B) + " sequences");
   if (B > 0 && (!nq || !nk)) return refuse("packed_plan: q_lengths and kv_lengths are host arrays");
@@ -206,18 +213,27 @@ int check_packed(int B, const int32_t* nq, const int32_t* nk, int H, int Hkv, in
   if (H > 65536) return refuse("packed_plan: " + std::to_string(H) + " query heads; at most 65536");
   if (q_dtype != TGOHIP_F32 && q_dtype != TGOHIP_F16)
     return refuse("packed_plan: q_dtype is " + std::to_string(q_dtype) + "; queries are f32 or f16");
-  int64_t tq = 0, tk = 0;
+  int64_t tq = 0, tk = 0, blocks = 0;
   for (int s = 0; s < B; s++) {
     if (nq[s] < 0 || nk[s] < 0)
       return refuse("packed_plan: sequence " + std::to_string(s) + " has " + std::to_string(nq[s]) +
                     " queries and " + std::to_string(nk[s]) + " keys");
     tq += nq[s];
     tk += nk[s];
+    blocks += ((int64_t)nq[s] * (H / Hkv) + kPackRows - 1) / kPackRows * Hkv;
   }
   if (tq * H >= kMaxIndex || tk >= kMaxIndex)
     return refuse("packed_plan: " + std::to_string(tq) + " query rows of " + std::to_string(H) +
                   " heads and " + std::to_string(tk) + " key rows; heads of rows, and key rows, stay below 2^30");
-  return 0;
+  return packed_fits(blocks, blocks);
+}
+
+// A checked batch's decomposition on `ncu` compute units.
+int packed_decompose(int B, const int32_t* nq, const int32_t* nk, int H, int Hkv, int D, int causal, int q_dtype, int ncu,
+                     PackedPlan& plan) {
+  packed_build_plan(B, nq, nk, H, Hkv, D, causal != 0, q_dtype == TGOHIP_F16, ncu, plan);
+  if (plan.part_rows > INT_MAX) return refuse("packed_plan: the batch has more rows of partial results than 2^31 - 1");
+  return packed_fits((int64_t)(plan.items.size() + plan.few.size()), (int64_t)plan.merges.size());
 }
 
 }  // namespace
@@ -364,13 +380,9 @@ int tgohip_packed_plan(tgohip_ctx* c, int B, const int32_t* q_lengths, const int
     OnDevice on(c->device);
     if ((rc = no_capture(c, "packed_plan"))) return rc;
     PackedPlan plan;
-    packed_build_plan(B, q_lengths, kv_lengths, H, H_kv, head_dim, causal != 0, q_dtype == TGOHIP_F16, c->ncu, plan);
+    if ((rc = packed_decompose(B, q_lengths, kv_lengths, H, H_kv, head_dim, causal, q_dtype, c->ncu, plan))) return rc;
     const size_t items = plan.items.size();
     plan.items.insert(plan.items.end(), plan.few.begin(), plan.few.end());
-    const size_t most = (size_t)INT_MAX / 256;
-    if (plan.part_rows > INT_MAX || plan.items.size() > most || plan.merges.size() > most)
-      return refuse("packed_plan: the batch needs " + std::to_string(plan.items.size()) +
-                    " workgroups, more than one launch takes");
     const bool fresh = *handle == 0;
     const int h = fresh ? c->ops.next++ : *handle;
     PackedHandle& p = c->ops.packed[h];
@@ -403,11 +415,11 @@ int tgohip_packed_plan(tgohip_ctx* c, int B, const int32_t* q_lengths, const int
 int tgohip_packed_describe(int B, const int32_t* q_lengths, const int32_t* kv_lengths, int H, int H_kv, int head_dim,
                            int causal, int q_dtype, int ncu, tgohip_packed_plan_t* out) {
   return guarded([&]() -> int {
-    const int rc = check_packed(B, q_lengths, kv_lengths, H, H_kv, head_dim, q_dtype);
+    int rc = check_packed(B, q_lengths, kv_lengths, H, H_kv, head_dim, q_dtype);
     if (rc) return rc;
-    if (ncu < 1 || !out) return refuse("packed_describe: ncu and plan");
+    if (ncu < 1 || ncu > 65536 || !out) return refuse("packed_describe: ncu (1 to 65536) and plan");
     PackedPlan plan;
-    packed_build_plan(B, q_lengths, kv_lengths, H, H_kv, head_dim, causal != 0, q_dtype == TGOHIP_F16, ncu, plan);
+    if ((rc = packed_decompose(B, q_lengths, kv_lengths, H, H_kv, head_dim, causal, q_dtype, ncu, plan))) return rc;
     *out = tgohip_packed_plan_t{(int32_t)plan.items.size(), (int32_t)plan.few.size(), 0, 0, plan.part_rows, 0};
     for (const PackedItem& it : plan.items) out->longest_tile = std::max(out->longest_tile, it.kv_hi - it.kv_lo);
     for (const PackedItem& it : plan.few) out->longest_few = std::max(out->longest_few, it.kv_hi - it.kv_lo);
@@ -420,11 +432,12 @@ int tgohip_packed_pieces(int B, const int32_t* q_lengths, const int32_t* kv_leng
                          int causal, int q_dtype, int ncu, tgohip_packed_piece_t* pieces, int* n_pieces,
                          tgohip_packed_merge_t* merges, int* n_merges) {
   return guarded([&]() -> int {
-    const int rc = check_packed(B, q_lengths, kv_lengths, H, H_kv, head_dim, q_dtype);
+    int rc = check_packed(B, q_lengths, kv_lengths, H, H_kv, head_dim, q_dtype);
     if (rc) return rc;
-    if (ncu < 1 || !n_pieces || !n_merges) return refuse("packed_pieces: ncu, n_pieces and n_merges");
+    if (ncu < 1 || ncu > 65536 || !n_pieces || !n_merges)
+      return refuse("packed_pieces: ncu (1 to 65536), n_pieces and n_merges");
     PackedPlan plan;
-    packed_build_plan(B, q_lengths, kv_lengths, H, H_kv, head_dim, causal != 0, q_dtype == TGOHIP_F16, ncu, plan);
+    if ((rc = packed_decompose(B, q_lengths, kv_lengths, H, H_kv, head_dim, causal, q_dtype, ncu, plan))) return rc;
     plan.items.insert(plan.items.end(), plan.few.begin(), plan.few.end());
     const int np = (int)plan.items.size(), nm = (int)plan.merges.size(), mp = *n_pieces, mm = *n_merges;
     *n_pieces = np;
