@@ -425,7 +425,8 @@ int tgohip_packed_pieces(int B, const int32_t* q_lengths, const int32_t* kv_leng
  * finite score is right to the error of its own products, the steps of f32 at its size
  * (scores past 2^22 in log2 units take a slower path). With
  * f32 queries the products are those of tgohip_paged_attention's f32 form (q and
- * the probabilities as f16 hi + lo pairs, so |q| < 65504); with f16 queries the
+ * the probabilities as f16 hi + lo pairs, so |q| < 65504, and each q is carried to
+ * 2^-22 of itself or to 2^-25, whichever is more); with f16 queries the
  * probabilities are rounded to f16. Sums, maxima and partial results are f32.
  * Memory behind the last row stays as it is; out meets none of q, k and v. */
 int tgohip_packed_attention(tgohip_ctx* ctx, int handle, const void* q, int64_t q_row, const void* k,
@@ -460,8 +461,10 @@ int tgohip_adapter_rows(tgohip_ctx* ctx, int B, const int32_t* extents, const in
 int tgohip_adapter_rows_free(tgohip_ctx* ctx, int handle);
 /* x [rows,K] f32, f16 or a pair; base (or NULL: zeros) and y [rows,N] in y_dtype
  * (f32 or f16), y may be base. 16-byte aligned. Both products are f32 sums over
- * f16 adapters; f32 and pair activations are carried as hi + lo (|x| < 65504),
- * x . down^T as a pair scaled by a power of two per row. Rows behind the last
+ * f16 adapters; f32 and pair activations are carried as hi + lo (|x| < 65504, and
+ * an f32 x to 2^-22 of itself or to 2^-25, whichever is more: rows far below 2^-3
+ * lose bits as they do in tgohip_linear), x . down^T as a pair scaled by a power of
+ * two per row. Rows behind the last
  * request stay as they are. */
 int tgohip_adapters(tgohip_ctx* ctx, int set, int rows, const void* x, int x_dtype,
                     const void* base, void* y, int y_dtype);

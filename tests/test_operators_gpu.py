@@ -1282,3 +1282,53 @@ def test_a_set_is_what_it_holds(ctx, torch_gpu):
     finally:
         for f, a in ((ctx.adapters_free, fresh), (ctx.adapters_free, used), (ctx.adapter_rows_free, rows)):
             f(a)
+
+
+@pytest.mark.parametrize("extents", [[1, 5, 9], [300, 1, 280]])
+def test_adapters_of_small_activations(ctx, torch_gpu, extents):
+    """f32 rows of 1, 1e-3, 1e-4 and 1e-6, and of all of them mixed: each x is carried as hi + lo, to 2^-22 of
+    itself or to half of f16's smallest step, 2^-25."""
+    torch = torch_gpu
+    K, N, who = 1024, 192, [0, 1, 0]
+    T = sum(extents)
+    g = torch.Generator(device="cuda").manual_seed(12)
+    sizes = torch.tensor([1.0, 1e-3, 1e-4, 1e-6], device="cuda")
+    x = torch.randn(T, K, device="cuda", generator=g)
+    row = torch.arange(T, device="cuda") % 5
+    mixed = sizes[torch.randint(0, 4, (T, K), device="cuda", generator=g)]
+    x *= torch.where(row[:, None] < 4, sizes[row.clamp_max(3)][:, None], mixed)
+    s, rows = ctx.adapters_new(K, N, 2), ctx.adapter_rows(extents, who)
+    try:
+        loaded = {}
+        for i, r in enumerate((16, 40)):
+            down, up = make_adapter(torch, K, N, r, i)
+            ctx.adapters_put(s, i, down.cpu().numpy(), up.cpu().numpy(), 1.0)
+            loaded[i] = (down.double(), up.double(), 1.0)
+        y = torch.full((T, N), float("nan"), device="cuda")
+        ctx.adapters(s, rows, x, None, y)
+        torch.cuda.synchronize()
+        want, tol = adapters64(torch, x.double(), None, extents, who, loaded, K, N, True)
+        at = 0
+        for n, a in zip(extents, who):  # the floor of every x through both products
+            down, up, _ = loaded[a]
+            tol[at:at + n] += (2.0 ** -25 * down.abs().sum(1)) @ up.abs().t() * (1 + 2.0 ** -20)
+            at += n
+        assert bool(((y.double() - want).abs() <= tol).all())
+    finally:
+        ctx.adapter_rows_free(rows)
+        ctx.adapters_free(s)
+
+
+@pytest.mark.parametrize("nq,nk", [([1, 2], [900, 64]), ([150, 40], [150, 300])])
+def test_packed_attention_of_small_queries(ctx, torch_gpu, nq, nk):
+    """f32 queries of 1e-4 over keys of some hundreds: each q is carried to 2^-25 at worst."""
+    torch = torch_gpu
+    q, k, v = inputs(torch, nq, nk, 4, 2, 128, False, seed=6)
+    q, k = q * 1e-4, (k * 200).half()
+    out = attend(ctx, torch, q, k, v, nq, nk, scale=0.25)
+    torch.cuda.synchronize()
+    want, tol = attention64(torch, q, k, v, nq, nk, 0.25, True)
+    # a score is off by that of every dim; a probability and its sum by e^ds - 1 < 1.1 ds each
+    ds = 0.25 * 2.0 ** -25 * float(k.abs().double().sum(-1).max())
+    assert ds < 0.01
+    assert bool(((out.double() - want).abs() <= tol + 2.2 * ds * float(v.abs().max()) + U * want.abs()).all())

@@ -27,7 +27,8 @@
 
 namespace tgohip {
 
-// Eight f32 as f16 hi + lo.
+// Eight f32 as f16 hi + lo: to 2^-22 of each, or to 2^-25 (half of f16's smallest step)
+// where that is more, as the projection that y's base comes from carries them.
 __device__ __forceinline__ void adapter_split(float4_t u, float4_t v, half8_t& hi, half8_t& lo) {
 #pragma unroll
   for (int j = 0; j < 8; j++) {
