@@ -317,3 +317,11 @@ def test_batches_of_more_workgroups_than_a_launch_takes_are_refused():
         for call in (tgo_amd.packed_describe, tgo_amd.packed_pieces):
             with pytest.raises(TgoError, match="ncu"):
                 call([1], [9000], 8, 2, ncu=ncu)
+
+
+@pytest.mark.parametrize("attention", [1e39, 3.5e38, 1e300])
+def test_rope_factors_past_f32_are_refused(attention):
+    """cos and sin are multiplied in f32: a factor past its range would make every output infinite or NaN."""
+    with pytest.raises(TgoError, match="attention is"):
+        tgo_amd.rope_freqs(128, 1e6, attention=attention)
+    assert tgo_amd.rope_freqs(128, 1e6, attention=3.4e38)[1] == 3.4e38

@@ -156,8 +156,8 @@ int check_rope(const tgohip_rope_cfg* c) {
     return refuse("rope: scaling is " + std::to_string(c->scaling) + ", not a TGOHIP_ROPE_* kind");
   if (!(c->base > 1.0) || !std::isfinite(c->base))
     return refuse("rope: base is " + num(c->base) + "; a finite number above 1");
-  if (!(c->attention >= 0.0) || !std::isfinite(c->attention))
-    return refuse("rope: attention is " + num(c->attention) + "; a finite factor, 0 for the scaling's own");
+  if (!(c->attention >= 0.0) || !std::isfinite((float)c->attention))
+    return refuse("rope: attention is " + num(c->attention) + "; a finite factor of f32, 0 for the scaling's own");
   if (c->scaling == TGOHIP_ROPE_UNSCALED) return 0;
   if (!(c->factor >= 1.0) || !std::isfinite(c->factor))
     return refuse("rope: factor is " + num(c->factor) + "; a finite number of at least 1");
