@@ -1332,3 +1332,24 @@ def test_packed_attention_of_small_queries(ctx, torch_gpu, nq, nk):
     ds = 0.25 * 2.0 ** -25 * float(k.abs().double().sum(-1).max())
     assert ds < 0.01
     assert bool(((out.double() - want).abs() <= tol + 2.2 * ds * float(v.abs().max()) + U * want.abs()).all())
+
+
+def test_tensors_of_other_ranks_are_refused(ctx, torch_gpu):
+    """Operands without the axes that the call needs, with the binding's own error."""
+    torch = torch_gpu
+    h, plan = ctx.rope_new(64, 1e4), ctx.packed_plan([2], [2], 1, 1, head_dim=64)
+    try:
+        x, pos = torch.zeros(2, 1, 64, device="cuda"), torch.zeros(2, device="cuda", dtype=torch.int32)
+        for shape in ((2, 64), (128,), (2, 1, 64, 1), ()):
+            flat = torch.zeros(shape, device="cuda")
+            with pytest.raises(TgoError, match="tensor 0 is"):
+                ctx.rope(h, pos, [(flat, flat)])
+            with pytest.raises(TgoError, match="\\[rows, heads, head_dim\\]"):
+                ctx.packed_attention(plan, flat, x.half(), x.half(), torch.zeros_like(x), 0.1)
+        with pytest.raises(TgoError, match="tensors of heads"):
+            ctx.rope(h, pos, [])
+        with pytest.raises(TgoError, match="tensors of heads"):
+            ctx.rope(h, pos, [(x, torch.zeros_like(x))] * 4)
+    finally:
+        ctx.rope_free(h)
+        ctx.packed_free(plan)

@@ -775,7 +775,7 @@ class Context:
         f = []
         for i, (x, y, *turn) in enumerate(heads):
             shape = x.shape
-            if shape != y.shape or shape[0] != T or (d is not None and shape[2] != d):
+            if len(shape) != 3 or shape != y.shape or shape[0] != T or (d is not None and shape[2] != d):
                 raise TgoError(EINVAL, "rope: tensor %d is %s and %s for %d positions and heads of %s" %
                                (i, tuple(shape), tuple(y.shape), T, d))
             xa, xr, xh, xd = _heads_view(x, "rope: x", self.device)
