@@ -667,33 +667,39 @@ __device__ __forceinline__ void pack_values(PackRows<D, QF16>& w, const float16_
 // values as 0 (the same sums, to the bit, where none is seen); a product of
 // visibility and occurrence then tells which outputs see +inf and which -inf, NaN
 // being both. Rare: a plain loop behind the kernel's own, 32 dims of the result at a
-// time, so that it needs no more registers than the kernel (with all dims at once the
-// 128-dim kernels kept 102 to 111 registers in memory around it).
+// time where there are 128, so that the kernel keeps next to none of its registers in
+// memory around it (with all dims 102 to 111, with 64 of them 30 and 83, 1% on the kernel's
+// own time). Measured, us: 4 f32 chunks of 2116 to 8176 keys 125, an infinity in the last
+// value 1570, scores of 2^28 927; 32 full f32 sequences, 16 heads of 64, 52, 156, 156.
 template <int D, bool QF16>
 __device__ __forceinline__ void packed_redo(const PackedArgs* ap, int item, int w0, lds_t K, lds_t V) {
   const PackedArgs& a = *ap;
   const PackedItem it = a.items[item];
   const int tid = threadIdx.x, lane = tid & 63, kh = lane >> 5;
   const int kat = pack_k_at<D>(lane & 31, kh);
-  PackRows<D, QF16, 1> w;
+  constexpr int NB = D == 64 ? 2 : 1;  // blocks of 32 dims at a time
+  PackRows<D, QF16, NB> w;
 #pragma unroll 1
-  for (int db = 0; db < D / 32; db++) {
-    const int vat = pack_v_at<D>(lane) ^ (64 * db);
+  for (int d0 = 0; d0 < D; d0 += 32 * NB) {
+    const int vat = pack_v_at<D>(lane) ^ (2 * d0);
     w.init(a, it, w0, lane);
-    bool past = false;
+    bool past = false, odd = false;
 #pragma unroll 1
     for (int pass = 0; pass < 3; pass++) {
-      float16_t seen = {};
+      if (pass == 1 && !__syncthreads_or(odd)) break;  // every value is finite
+      float16_t seen[NB] = {};
 #pragma unroll 1
       for (int t0 = it.kv_lo; t0 < it.kv_hi; t0 += kPackTile) {
         __syncthreads();
         for (int i = tid; i < kPackTile * (D / 8); i += blockDim.x) {
           const int p = i / (D / 8), c = i % (D / 8);
           const int64_t row = it.k0 + min(t0 + p, it.kv_hi - 1);
-          *(__attribute__((address_space(3))) half8_t*)(K + p * 2 * D + 16 * (c ^ pack_k_swz<D>(p))) =
-              *(const half8_t*)(a.k + row * a.k_row + it.kvh * D + c * 8);
-          *(__attribute__((address_space(3))) half8_t*)(V + p * 2 * D + 16 * (c ^ pack_v_swz<D>(p))) =
-              *(const half8_t*)(a.v + row * a.v_row + it.kvh * D + c * 8);
+          if (pass == 0)
+            *(__attribute__((address_space(3))) half8_t*)(K + p * 2 * D + 16 * (c ^ pack_k_swz<D>(p))) =
+                *(const half8_t*)(a.k + row * a.k_row + it.kvh * D + c * 8);
+          const half8_t vv = *(const half8_t*)(a.v + row * a.v_row + it.kvh * D + c * 8);
+          *(__attribute__((address_space(3))) half8_t*)(V + p * 2 * D + 16 * (c ^ pack_v_swz<D>(p))) = vv;
+          odd |= half8_nonfinite(vv);
         }
         __syncthreads();
         float16_t sc[2];
@@ -717,7 +723,7 @@ __device__ __forceinline__ void packed_redo(const PackedArgs* ap, int item, int 
         float l[4] = {};
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-          half8_t ph = ps[u], pl, va = pack_v_frag<D>(V, vat + 32 * D * u);
+          half8_t ph = ps[u], pl;
           if (pass == 0) {
             if (!QF16) pack_probs<QF16, true>(sc, u, a.qscale, w.m, l[u], ph, pl, w.e);
           } else {
@@ -726,37 +732,45 @@ __device__ __forceinline__ void packed_redo(const PackedArgs* ap, int item, int 
               ph[e] = (half_t)(pack_visible(left, u >> 1, (u & 1) * 8 + e) ? 1.f : 0.f);
           }
 #pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const float f = (float)va[e];
-            if (pass == 0) va[e] = fabsf(f) < INFINITY ? va[e] : (half_t)0.f;
-            else va[e] = (half_t)(f != f || f == (pass == 1 ? INFINITY : -INFINITY) ? 1.f : 0.f);
-          }
-          if (pass == 0) {
-            w.o[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, w.o[0], 0, 0, 0);
-            if (!QF16) w.o[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl, w.o[0], 0, 0, 0);
-          } else {
-            seen = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, seen, 0, 0, 0);
+          for (int db = 0; db < NB; db++) {
+            half8_t va = pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const float f = (float)va[e];
+              if (pass == 0) va[e] = fabsf(f) < INFINITY ? va[e] : (half_t)0.f;
+              else va[e] = (half_t)(f != f || f == (pass == 1 ? INFINITY : -INFINITY) ? 1.f : 0.f);
+            }
+            if (pass == 0) {
+              w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, w.o[db], 0, 0, 0);
+              if (!QF16) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl, w.o[db], 0, 0, 0);
+            } else {
+              seen[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, seen[db], 0, 0, 0);
+            }
           }
         }
         w.l += (l[0] + l[1]) + (l[2] + l[3]);
       }
 #pragma unroll
-      for (int i = 0; i < 16; i++)
-        if (seen[i] > 0.f) w.o[0][i] += pass == 1 ? INFINITY : -INFINITY;
+      for (int db = 0; db < NB; db++)
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+          if (seen[db][i] > 0.f) w.o[db][i] += pass == 1 ? INFINITY : -INFINITY;
     }
     const float2 fin = w.finish(a, it, lane);
     const int row = it.r0 + w.r;
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
-      float4_t v;
+    for (int db = 0; db < NB; db++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = w.l == 0.f ? fin.y : w.o[0][4 * g + e] * fin.x;
-      const int d = 32 * db + 8 * g + 4 * kh;
-      if (w.r < it.nr) {
-        if (it.part >= 0) *(float4_t*)(a.part_o + ((int64_t)it.part + w.r) * D + d) = v;
-        else pack_store4(a, (it.q0 + row / a.G) * a.out_row + (it.kvh * a.G + row % a.G) * D + d, v);
+      for (int g = 0; g < 4; g++) {
+        float4_t v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = w.l == 0.f ? fin.y : w.o[db][4 * g + e] * fin.x;
+        const int d = d0 + 32 * db + 8 * g + 4 * kh;
+        if (w.r < it.nr) {
+          if (it.part >= 0) *(float4_t*)(a.part_o + ((int64_t)it.part + w.r) * D + d) = v;
+          else pack_store4(a, (it.q0 + row / a.G) * a.out_row + (it.kvh * a.G + row % a.G) * D + d, v);
+        }
       }
-    }
   }
 }
 
