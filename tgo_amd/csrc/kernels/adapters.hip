@@ -11,10 +11,14 @@
 //   adapter_up_kernel    y = base + s u . up^T; with tiles of 16 rows it sums the
 //                        planes itself, a launch less
 // Measured, the three together (us; bytes are x, base, y and each adapter once):
-//   1 row, rank 16, [4096, 4096]                7.5, 3.3 and 3.6 of them the kernels
-//   128 rows of 32 adapters, [4096, 6144]       10.8, 1.7 TB/s
-//   1152 rows, rank 64, [4096, 24576]           96, 3.7 TB/s: 15, 5 and 76
-//   8000 f16 rows, rank 24, [12288, 4096]       79, 3.9 TB/s: 38, 5 and 34
+//   1 row, rank 16, [4096, 4096]                8.6, 3.7 and 4.1 of them the kernels
+//   128 rows of 32 adapters, [4096, 6144]       10.6, 1.8 TB/s
+//   1152 rows, rank 64, [4096, 24576]           95, 3.7 TB/s: 15, 5 and 77
+//   8000 f16 rows, rank 24, [12288, 4096]       77, 4.0 TB/s: 39, 5 and 33
+// The kernels are built for the set's largest rank, RB blocks of 16: a tile of a smaller
+// one loads its last rows again and multiplies them for nothing. Two adapters of rank 16
+// over [4096, 6144], alone in their set and beside one of rank 128: 128 f32 rows 7.5 and
+// 13.1, 1152 f32 rows 24 and 36, 8000 f16 rows 105 and 143.
 // Both products in one launch, each workgroup computing its tile's u, was slower for
 // all but the smallest K: one row of [4096, 4096] 9.4 us for 8.0, 128 rows of
 // [12288, 4096] 27.9 for 12.0, 16 rows of [1024, 4096] 6.1 for 6.9.
@@ -92,7 +96,8 @@ __device__ __forceinline__ void adapter_wait() {
 // each with its buffer on its way, keep the memory busy; no wave waits for another.
 // 7000 f16 rows of K = 12288 and a rank of 24: 37 us, 4.6 TB/s; loaded to registers as
 // half lines 56 us, as the unit above 43 (L1 holds half of what is in flight); without
-// the nt bit 40.
+// the nt bit 40. At rank 128 f16 rows and pairs take more than 256 registers with their
+// sums, and a CU holds four waves.
 template <int XK, int RB>
 __device__ __forceinline__ void adapter_down_64(const AdapterArgs& a, const AdapterTile& t, const AdapterEntry& e, int s0,
                                                 int s1, int wave, adapter_lds buf, float4_t (&acc)[4][RB]) {
@@ -451,7 +456,8 @@ __global__ __launch_bounds__(256) void adapter_up_kernel(AdapterArgs a) {
   if constexpr (TB == 1) {
     for (int i = tid; i < 16 * RB * 16; i += 256) {
       const int m = i / (RB * 16), r = i - m * (RB * 16);
-      // every plane's load in flight, summed in their order
+      // every plane's load in flight, summed in their order: as many loads as there may be
+      // planes, the last one again where a batch has fewer
       float s = 0.f, v[kAdapterMaxSplits];
       const bool in = m < t.n && r < e.rank_pad;
       const float* u = a.u + ((int64_t)t.start + (in ? m : 0)) * kAdapterMaxRank + (in ? r : 0);

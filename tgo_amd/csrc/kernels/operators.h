@@ -82,7 +82,14 @@ int packed_enqueue(const PackedArgs& a, int D, int q_f16, const PackedCounts& n,
 
 // ---- adapters (adapters.hip) --------------------------------------------------
 constexpr int kAdapterMaxRank = 128;
-constexpr int kAdapterFewRows = 512;  // rows up to which a batch's tiles hold 16 rows
+// Rows up to which a batch's tiles hold 16 rows, 64 beyond. Tiles of 16 / of 64, us:
+//   [4096, 6144], rank 16, 8 adapters: 128 rows 7.5 / 11.2, 512 11.8 / 16.9, 1024 18.8 /
+//       21.9, 2048 31.5 / 31.9; 256 adapters: 256 rows 29.2 / 27.6, 1024 33.3 / 32.9
+//   [4096, 4096], rank 64, 8 adapters: 256 rows 11.6 / 17.0, 512 17.0 / 21.6, 768 22.2 /
+//       24.6, 1024 28.0 / 25.8; 256 adapters: 256 rows 64.1 / 55.5, 1024 78.2 / 70.7
+// Rows alone decide: with many rows of a small rank 16 would do a little longer, with
+// many adapters of a large one less long.
+constexpr int kAdapterFewRows = 512;
 struct AdapterEntry {
   const half_t* down;  // [rank_pad][K]
   const half_t* up;    // [N][rank_pad]
@@ -113,6 +120,10 @@ struct AdapterArgs {
 // The shares of K for a batch of `tiles` tiles (their planes are the workspace): up to
 // two workgroups a CU, all on the chip at once. With 1, 2, 3 or 4 per CU, us: 8000 f16
 // rows of [12288, 4096] 86, 81, 92, 86; 1152 pairs of [4096, 24576] 104, 103, 107, 106.
+// Tiles without an adapter count too, though their workgroups return at once. Counting
+// all / only those with one, us: an adapter for 1000 of 8000 f32 rows of [12288, 4096] 53 /
+// 32, for half of 1056 of [4096, 24576] 57 / 55, for a third of 48 tiles of [12288, 4096]
+// 35 / 37.
 constexpr int kAdapterMaxSplits = 16;
 inline int adapter_splits(int tiles, int ncu) {
   return tiles > 0 ? std::min(kAdapterMaxSplits, std::max(1, 2 * ncu / tiles)) : 1;

@@ -14,17 +14,19 @@
 //                        group's heads side by side), tiles of 64 keys: MFMA-bound
 //   packed_few_kernel    up to 32 such rows (decoding): bound by the keys' bytes
 //   packed_merge_kernel  rows whose keys were cut into pieces
-// Measured (us, 32 heads over 8 of 128 dims unless said):
-//   one causal prompt of 16384 f16 rows           2140, 1.03 PFLOP/s, the matrix unit
-//       busy 53% at 1.93 GHz (all four SIMDs' power holds the clock), VALU 41%
-//   16 f16 prompts of 1 to 1384 rows              53, 0.64 PFLOP/s
-//   4 f32 chunks of 82 to 354 rows, 2116 to 8176 keys   122, 0.42 PFLOP/s, twice that executed
-//   32 full f32 sequences of 22 to 763 rows, 16 heads of 64   51, 0.30 PFLOP/s
+// Measured (us a call, averages back to back, 32 heads over 8 of 128 dims unless said):
+//   one causal prompt of 16384 f16 rows           2190 (2120 to 2230 by the card), 1.00
+//       PFLOP/s, the matrix unit busy 53% at 1.90 GHz (all four SIMDs' power holds the
+//       clock), VALU 40%
+//   16 f16 prompts of 1 to 1384 rows              54, 0.63 PFLOP/s
+//   4 f32 chunks of 82 to 354 rows, 2116 to 8176 keys   125, 0.41 PFLOP/s, twice that executed
+//   32 full f32 sequences of 22 to 763 rows, 16 heads of 64   52, 0.30 PFLOP/s
 //   64 decoders of 16 to 8192 keys                73, 5.3 TB/s
-//   64 decoders of 4096 keys                      163, 6.6 TB/s
+//   64 decoders of 4096 keys                      165, 6.5 TB/s
 // Tried and slower or no faster in packed_kernel, for that prompt (2240 us then): the
 // next tile's scores beside this one's softmax 2252; eight waves on four LDS buffers
-// 2666; 64 rows a wave spills; the waves' priorities by phase 2240.
+// 2666; the waves' priorities by phase 2240. 64 rows a wave spilled, with packed_redo's
+// registers in the kernel, more than now: not tried since.
 #include "operators.h"
 
 #include <algorithm>
@@ -801,8 +803,9 @@ __device__ __forceinline__ void pack_dma_end(const char* base, int p, int c, int
 }
 
 // WAVES waves of 32 rows each; tiles of 64 keys go through two LDS buffers, the next
-// one's DMA in flight while one is used. Two workgroups a CU (64 KiB of LDS and 256
-// registers each), so that one's products run under the other's softmax: without the
+// one's DMA in flight while one is used. Two workgroups a CU (128 dims: 64 KiB of LDS and
+// 251 or 256 registers each; 64 dims: 33 KiB, and 221 or 244 registers, of which the loop
+// alone would leave room for a third workgroup and packed_redo does not), so that one's products run under the other's softmax: without the
 // softmax the 16384-row prompt took 12% less, without the DMA 14%.
 template <int D, bool QF16, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void packed_kernel(PackedArgs a) {
@@ -881,7 +884,7 @@ constexpr int kNonTemporal = 2;  // the nt bit: keys of few rows are read once
 // 64 KiB and two waves a workgroup, two workgroups a CU: at any time about 64 KiB of
 // K and V are on their way to each CU, and one workgroup's start and end lie under
 // the other's stream.
-// 64 decoders of 4096 keys: 162 us, 6.6 TB/s of the 7.0 that a plain read reaches here,
+// 64 decoders of 4096 keys: 165 us, 6.5 TB/s of the 7.0 that a plain read reaches here,
 // 190 in packed_kernel; of 16 to 8192 keys 73 us, 5.3 TB/s, and 84.
 template <int D, bool QF16>
 __global__ __launch_bounds__(64 * kFewWaves, 1) void packed_few_kernel(PackedArgs a) {

@@ -164,11 +164,15 @@ void launch_rope(const RopeArgs& args, int ncu, hipStream_t st) {
     aligned = aligned && (uintptr_t)g.x % 16 == 0 && (uintptr_t)g.y % 16 == 0 && g.x_row % xs == 0 &&
               g.x_head % xs == 0 && g.y_row % ys == 0 && g.y_head % ys == 0;
   }
-  // Rows per workgroup: enough that a pair's angle serves many heads, few enough that
-  // the chip is full; a power of two of at most 16, and r below 2^16.
+  // Rows per workgroup: enough that its few heads fill it, few enough that the chip is
+  // full; a power of two of at most 16, and r below 2^16. At most 1 / 4 / 16 / 64 rows, us,
+  // f16 heads of 128 dims: 65536 rows of one head 48.8 / 17.2 / 12.9 / 14.5, 16384 of 8
+  // heads 16.9 / 12.3 / 12.4 / 12.3, of 72 heads 108 / 118 / 123 / 123.
   a.rows = 1;
   while (a.rows < 16 && 2 * a.rows * heads <= 65535 && (int64_t)a.n * a.T / (2 * a.rows) >= 4 * ncu) a.rows *= 2;
-  // Units of 16 bytes and more: V pairs need runs of V (half) or 2V elements.
+  // Units of 16 bytes and more: V pairs need runs of V (half) or 2V elements. Such units /
+  // single elements, us: 16384 rows of 72 f16 heads 123 / 241, 4096 of 40 14.1 / 22.9,
+  // 1152 f32 rows of 40 heads 10.2 / 10.0.
   const auto fits = [&](int v) { return aligned && a.rd % (2 * v) == 0 && a.d % (2 * v) == 0 && a.d / (2 * v) <= 256; };
   if (a.half) {
     if (fits(8)) rope_launch<8, true>(a, st);
