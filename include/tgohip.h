@@ -469,6 +469,94 @@ int tgohip_adapter_rows_free(tgohip_ctx* ctx, int handle);
 int tgohip_adapters(tgohip_ctx* ctx, int set, int rows, const void* x, int x_dtype,
                     const void* base, void* y, int y_dtype);
 
+/* ---- an 8-bit paged cache for a caller's own layer --------------------------
+ * The caller's device buffers: K and V codes [layers, pages, kv_heads, block, head_dim], one
+ * byte each, and one f32 scale for each row of head_dim, [layers, pages, kv_heads, block].
+ * Slot s of the pool is position s % block of page s / block, as in the f16 pool. A row
+ * stands for code * scale: int8 codes of -127 to 127, or e4m3 ones (no NaN: 0x7f and 0xff do
+ * not occur), its scale the row's largest magnitude over 127 or 448, at least 2^-40 (so the
+ * smallest differences are 2^-40); codes are the nearest to value / scale, ties to even. A
+ * row that holds a value that is not finite, or past 2^40, stands for NaN throughout (its
+ * scale is NaN, its codes 0). Other writers keep scales at 0 (a row of zeros: memory as it is
+ * cleared), from 2^-40 to 2^40, or NaN. Buffers are apart from each other and from every other
+ * operand of a call, and codes start on 16-byte boundaries. head_dim 64 or 128, block a power of two up to 1024,
+ * kv_heads at most 4096, a layer's rows (pages * block * kv_heads) below 2^31. No counterpart
+ * in the reference, whose pool is f16. */
+#define TGOHIP_CACHE_I8 0
+#define TGOHIP_CACHE_F8 1
+typedef struct {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int32_t form, layers, pages, kv_heads, block, head_dim;
+} tgohip_cache;
+
+/* What a projection leaves for one layer: T rows of heads, element j of head h of row t at
+ * x[t x_row + h x_head + j] (strides in elements, at most 2^36; 0 reads one row or head for
+ * all). heads query heads (0: q and q_out unused), k and v of the cache's kv_heads. */
+typedef struct {
+  const void *q, *k, *v; /* x_dtype: TGOHIP_F32 or TGOHIP_F16 */
+  void* q_out;           /* out_dtype: the same two */
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  const float *q_gain, *k_gain; /* device [head_dim]; NULL: that tensor is not normed */
+  float eps;
+  int32_t heads, x_dtype, out_dtype;
+} tgohip_cache_rows;
+/* Queries and keys normed per head (x / sqrt(mean x^2 + eps) * gain, RMSNorm of
+ * nn/attention.go:196-201), rotated to their positions (device int32 [T]) by a rotary handle
+ * (0: neither; positions is then unused), keys and values quantised into their slots
+ * (device int32 [T]) of a layer, queries to q_out, in one launch. Sums, angles' products and
+ * the rows before quantisation are f32. A slot below 0 or at or past pages * block is a
+ * dropped write (plan.go:182-192): the row's query is written, its key and value go nowhere.
+ * Slots of the pool that a call names twice hold a mix of those rows. q_out may be q itself (same
+ * type and strides) or apart from every input. Can be captured. */
+int tgohip_cache_store(tgohip_ctx* ctx, const tgohip_cache* cache, int layer, int rope,
+                       const int32_t* positions, const int32_t* slots, int T,
+                       const tgohip_cache_rows* rows);
+
+/* Rows of slots (device int32 [T]) of a layer back as values: K's to k_out, V's to v_out
+ * (either may be NULL), [T, kv_heads, head_dim] with the strides given, f32 (exact but for the
+ * product's rounding) or f16 (rounded once more, past its range infinite). A slot outside the
+ * pool reads as zeros. Can be captured. */
+int tgohip_cache_read(tgohip_ctx* ctx, const tgohip_cache* cache, int layer, const int32_t* slots, int T,
+                      void* k_out, int64_t k_row, int64_t k_head, void* v_out, int64_t v_row,
+                      int64_t v_head, int out_dtype);
+
+/* Rows of slots from[i] to slots to[i] (host arrays, n of them), K and V of every head and
+ * every layer: after drafted tokens have been verified, those accepted to the positions they
+ * now have. Every row is read before it is written over, so the moves act at once, whatever
+ * their order; `to` names no slot twice. Permutations are made in cycles of up to 64 rows,
+ * longer ones are refused. Not under capture (TGOHIP_ESTATE). */
+int tgohip_cache_move(tgohip_ctx* ctx, const tgohip_cache* cache, const int32_t* from, const int32_t* to, int n);
+
+/* Attention over such a cache. Sequence b has extents[b] new tokens, the last of its
+ * lengths[b] positions, whose keys and values the store has written; position p is in slot
+ * pages[b * max_pages + p / block] * block + p % block (host arrays). Each new token sees every
+ * position before the new ones, and of those itself and its ancestors: parents (host, one for
+ * each new token in order, NULL: all in order) holds each token's parent, an earlier token of
+ * its sequence, or -1 for one that follows the context directly. A sequence whose parents
+ * are -1, 0, 1, ... is a chunk in causal order, of any extent; others, trees, have up to 64
+ * tokens. (A drafted token's rotary position is lengths - extents + its depth: positions
+ * and slots are the caller's.) H query heads, each kv head serves H / kv_heads neighbouring ones,
+ * H at most 65536. cache gives the geometry only.
+ * cache_plan decomposes the batch under *handle as tgohip_packed_plan does (0: a new one; a
+ * plan's: replaced in stream order), for every layer; calls that use one plan run in stream
+ * order, not at once. */
+int tgohip_cache_plan(tgohip_ctx* ctx, const tgohip_cache* cache, int B, const int32_t* extents,
+                      const int32_t* lengths, const uint32_t* pages, int max_pages,
+                      const int32_t* parents, int H, int q_dtype, int* handle);
+int tgohip_cache_plan_free(tgohip_ctx* ctx, int handle);
+/* out = softmax(scale q k^T) v over a plan's rows: q [sum of extents, H, head_dim] in the plan's
+ * q_dtype, out like q in f32, f16 or as a pair (TGOHIP_F16X2, dense rows). Rows are *_row
+ * elements apart (at most 2^30), heads dense, 16-byte aligned; scale is above 0 and at most
+ * 2^32. Both products take the codes as they are, scales are f32 in the softmax; f32 queries go
+ * as f16 hi + lo pairs and so do their probabilities (|q| < 65504, carried to 2^-22 of
+ * itself or 2^-25), f16 queries take f16 probabilities. Scores, sums and partial results are
+ * f32. A row that sees a key or value standing for NaN is NaN; nothing that it does not see
+ * reaches it. Memory behind the last row stays as it is; out meets neither q nor the cache. Can
+ * be captured. */
+int tgohip_cache_attention(tgohip_ctx* ctx, int handle, const tgohip_cache* cache, int layer, const void* q,
+                           int64_t q_row, float scale, void* out, int64_t out_row, int out_dtype);
+
 /* ---- host-side mirrors of the reference's batched path ------------------ */
 
 /* model.NewBatchStep (model/batch.go:66-152). Members are given as

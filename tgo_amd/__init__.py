@@ -20,6 +20,7 @@ F32, F16, F16X2 = 0, 1, 2
 LINEAR_ROWS, LINEAR_PIPE, LINEAR_GEMV, LINEAR_TILES = range(4)  # LinearPlan.kernel
 ROPE_INTERLEAVED, ROPE_HALF = 0, 1
 ROPE_UNSCALED, ROPE_LINEAR, ROPE_YARN, ROPE_BANDS = range(4)
+CACHE_I8, CACHE_F8 = 0, 1
 PROF_ATTN, PROF_QKV, PROF_O, PROF_GATEUP, PROF_DOWN, PROF_LMHEAD = range(6)
 PROF_NAMES = ("attention", "qkv", "o", "gateup", "down", "lm_head")
 
@@ -61,6 +62,18 @@ class RopeHeads(ctypes.Structure):
 class PackedPlan(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("tiles", "few", "longest_tile", "longest_few")] + [
         (n, ctypes.c_int64) for n in ("part_rows", "merged_rows")]
+
+
+class CacheC(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [
+        (n, ctypes.c_int32) for n in ("form", "layers", "pages", "kv_heads", "block", "head_dim")]
+
+
+class CacheRows(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out")] + [
+        (n, ctypes.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "out_row", "out_head")] + [
+        ("q_gain", ctypes.c_void_p), ("k_gain", ctypes.c_void_p), ("eps", ctypes.c_float)] + [
+        (n, ctypes.c_int32) for n in ("heads", "x_dtype", "out_dtype")]
 
 
 class LinearPlan(ctypes.Structure):
@@ -140,6 +153,12 @@ def lib():
         "tgohip_adapter_rows": (I, [P, I, P, P, P]),
         "tgohip_adapter_rows_free": (I, [P, I]),
         "tgohip_adapters": (I, [P, I, I, P, I, P, P, I]),
+        "tgohip_cache_store": (I, [P, P, I, I, P, P, I, P]),
+        "tgohip_cache_read": (I, [P, P, I, P, I, P, I64, I64, P, I64, I64, I]),
+        "tgohip_cache_move": (I, [P, P, P, P, I]),
+        "tgohip_cache_plan": (I, [P, P, I, P, P, P, I, P, I, I, P]),
+        "tgohip_cache_plan_free": (I, [P, I]),
+        "tgohip_cache_attention": (I, [P, I, P, I, P, I64, F, P, I64, I]),
         "tgohip_new_batch_step": (I, [I, I, I, I, I, P, P, P, P, P, I, I, I, P, P, P, P, P, P, P]),
         "tgohip_next_step": (I, [I, P, P, P, I, I, P, P, P, P, P, P]),
         "tgohip_victim": (I, [I, P, P, P, P]),
@@ -394,6 +413,37 @@ _INT32 = {}  # the int32 dtype, once met
 _ROPE_HEADS = [struct.Struct("=" + n * "QQqqqqiiii") for n in range(4)]
 
 
+# tgohip_cache_rows
+_CACHE_ROWS = struct.Struct("=QQQQqqqqqqqqQQfiii")
+
+
+class Cache:
+    """An 8-bit paged cache over the caller's device tensors: k, v [layers, pages, kv_heads, block, head_dim]
+    int8 or float8_e4m3fn, k_scale, v_scale [layers, pages, kv_heads, block] float32, all contiguous."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        form = {"torch.int8": CACHE_I8, "torch.float8_e4m3fn": CACHE_F8}.get(str(k.dtype))
+        shape = tuple(k.shape)
+        if form is None or v.dtype != k.dtype:
+            raise TgoError(EINVAL, "cache: k and v are %s and %s; both int8 or both float8_e4m3fn" % (k.dtype, v.dtype))
+        if len(shape) != 5 or tuple(v.shape) != shape:
+            raise TgoError(EINVAL, "cache: k and v are %s and %s; [layers, pages, kv_heads, block, head_dim]" %
+                           (shape, tuple(v.shape)))
+        self.device = k.get_device()
+        for t, what in ((k, "k"), (v, "v"), (k_scale, "k_scale"), (v_scale, "v_scale")):
+            if not t.is_contiguous():
+                raise TgoError(EINVAL, "cache: %s is not contiguous" % what)
+            if t.get_device() != self.device:
+                raise TgoError(EINVAL, "cache: %s is on another device than k" % what)
+        for t, what in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+            if _kind(t) != F32 or tuple(t.shape) != shape[:4]:
+                raise TgoError(EINVAL, "cache: %s is %s of %s; float32 %s" % (what, tuple(t.shape), t.dtype, shape[:4]))
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.layers, self.pages, self.kv_heads, self.block, self.head_dim = shape
+        self.c = CacheC(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), form, *shape)
+        self.at = ctypes.addressof(self.c)
+
+
 def sha256(data: bytes):
     buf = np.frombuffer(data, dtype=np.uint8).copy() if data else np.zeros(1, np.uint8)
     out = np.zeros(32, np.uint8)
@@ -586,7 +636,8 @@ class Context:
             raise TgoError(EDEVICE, last_error())
         self.cfg = None
         self.device = device
-        self._ropes, self._packed, self._sets, self._rows = {}, {}, {}, {}  # what this binding checks shapes by
+        # what this binding checks shapes by
+        self._ropes, self._packed, self._sets, self._rows, self._plans = {}, {}, {}, {}, {}
 
     def close(self):
         if self.h:
@@ -868,6 +919,111 @@ class Context:
         at = self.device
         check(_lib.tgohip_adapters(self.h, handle, rows, _addr(x, "x", at), x_dtype, _addr(base, "base", at),
                                    _addr(y, "y", at), y_dtype))
+
+    # ---- an 8-bit paged cache ----
+    def _cache(self, cache):
+        if cache.device != self.device:
+            raise _elsewhere(cache.k, "the cache", self.device)
+        return cache.at
+
+    def _slots(self, t, what):
+        if _INT32.get(t.dtype) is None:
+            if str(t.dtype) != "torch.int32":
+                raise TgoError(EINVAL, "%s is int32, not %s" % (what, t.dtype))
+            _INT32[t.dtype] = True
+        return _addr(t, what, self.device)
+
+    def cache_store(self, cache, layer, slots, k, v, q=None, q_out=None, positions=None, rope=0, q_gain=None,
+                    k_gain=None, eps=1e-6):
+        """Writes T rows of one layer: k, v [T, kv_heads, head_dim] quantised into slots (int32 [T]), q
+        [T, heads, head_dim] to q_out; q and k normed by q_gain, k_gain (float32 [head_dim]) and turned to
+        positions (int32 [T]) by a rotary handle, where those are given. Any row and head strides."""
+        T, d = slots.numel(), cache.head_dim
+        at = self._cache(cache)
+        ka, kr, kh, kd = _heads_view(k, "cache_store: k", self.device)
+        va, vr, vh, vd = _heads_view(v, "cache_store: v", self.device)
+        want = (T, cache.kv_heads, d)
+        if tuple(k.shape) != want or tuple(v.shape) != want:
+            raise TgoError(EINVAL, "cache_store: k and v are %s and %s for %d slots and heads of the cache; %s" %
+                           (tuple(k.shape), tuple(v.shape), T, want))
+        qa = qr = qh = oa = orow = oh = heads = 0
+        qd, od = kd, F32
+        if q is not None:
+            if q_out is None or q.shape != q_out.shape or q.dim() != 3 or q.shape[0] != T or q.shape[2] != d:
+                raise TgoError(EINVAL, "cache_store: q and q_out are [%d, heads, %d] both" % (T, d))
+            qa, qr, qh, qd = _heads_view(q, "cache_store: q", self.device)
+            oa, orow, oh, od = _heads_view(q_out, "cache_store: q_out", self.device)
+            heads = q.shape[1]
+        if kd != vd or kd != qd:
+            raise TgoError(EINVAL, "cache_store: q, k and v are of one type")
+        for g, what in ((q_gain, "q_gain"), (k_gain, "k_gain")):
+            if g is not None and (_kind(g) != F32 or g.numel() != d):
+                raise TgoError(EINVAL, "cache_store: %s is float32 [%d]" % (what, d))
+        pa = 0
+        if rope:
+            if positions is None or positions.numel() != T:
+                raise TgoError(EINVAL, "cache_store: positions is int32 [%d]" % T)
+            pa = self._slots(positions, "positions")
+        check(_lib.tgohip_cache_store(self.h, at, layer, rope, pa, self._slots(slots, "slots"), T, _CACHE_ROWS.pack(
+            qa, ka, va, oa, qr, qh, kr, kh, vr, vh, orow, oh, _addr(q_gain, "q_gain", self.device) or 0,
+            _addr(k_gain, "k_gain", self.device) or 0, eps, heads, kd, od)))
+
+    def cache_read(self, cache, layer, slots, k_out=None, v_out=None):
+        """Rows of slots (int32 [T]) of one layer as values: K's to k_out, V's to v_out ([T, kv_heads, head_dim],
+        float32 or float16, any row and head strides), where given. Zeros for slots outside the pool."""
+        T, f, kind = slots.numel(), [], None
+        for y, what in ((k_out, "k_out"), (v_out, "v_out")):
+            if y is None:
+                f += 0, 0, 0
+                continue
+            a, row, head, dt = _heads_view(y, "cache_read: " + what, self.device)
+            if tuple(y.shape) != (T, cache.kv_heads, cache.head_dim) or (kind is not None and dt != kind):
+                raise TgoError(EINVAL, "cache_read: %s is [%d, %d, %d], both of one type" %
+                               (what, T, cache.kv_heads, cache.head_dim))
+            kind = dt
+            f += a, row, head
+        check(_lib.tgohip_cache_read(self.h, self._cache(cache), layer, self._slots(slots, "slots"), T, *f,
+                                     F32 if kind is None else kind))
+
+    def cache_move(self, cache, src, dst):
+        """Rows of slots src[i] to slots dst[i] (host arrays) in every layer and head, all at once."""
+        a, b = i32(src), i32(dst)
+        if a.shape != b.shape or a.ndim != 1:
+            raise TgoError(EINVAL, "cache_move: %d slots to %d slots" % (a.size, b.size))
+        check(_lib.tgohip_cache_move(self.h, self._cache(cache), a.ctypes.data, b.ctypes.data, a.size))
+
+    def cache_plan(self, cache, extents, lengths, pages, H, parents=None, q_dtype=F32, plan=0):
+        """Decomposes a batch for cache_attention; returns the plan's handle. extents[b] new tokens end
+        lengths[b] positions, pages [B, max_pages] their page table, parents (one per new token) their trees'.
+        plan: a handle whose plan this one replaces."""
+        n, l, h = i32(extents), i32(lengths), ctypes.c_int(plan)
+        t = u32(pages)
+        if t.ndim != 2 or not len(n) == len(l) == len(t):
+            raise TgoError(EINVAL, "cache_plan: %d extents, %d lengths and a page table of %s" % (len(n), len(l), t.shape))
+        up = None if parents is None else i32(parents)
+        if up is not None and up.size != int(n.sum(dtype=np.int64)):
+            raise TgoError(EINVAL, "cache_plan: %d parents for %d new tokens" % (up.size, int(n.sum(dtype=np.int64))))
+        check(lib().tgohip_cache_plan(self.h, cache.at, len(n), ptr(n), ptr(l), ptr(t), t.shape[1], ptr(up), H, q_dtype,
+                                      ctypes.byref(h)))
+        self._plans[h.value] = (int(n.sum(dtype=np.int64)), H, cache.head_dim, q_dtype)
+        return h.value
+
+    def cache_plan_free(self, plan):
+        check(lib().tgohip_cache_plan_free(self.h, plan))
+        self._plans.pop(plan, None)
+
+    def cache_attention(self, plan, cache, layer, q, out, scale):
+        """Attention of a plan's new tokens over one layer: q, out [tokens, H, head_dim] (any row stride); out
+        float32, float16, or [2, tokens, H, head_dim] float16 for the hi and lo planes of a pair."""
+        t, H, d, qd = self._plans.get(plan, (0, 1, 64, F32))
+        qa, qr, _ = _packed_rows(q, "q", self.device, t, H, d, qd)
+        if out.dim() == 4:
+            if tuple(out.shape) != (2, t, H, d) or not out.is_contiguous() or _kind(out) != F16:
+                raise TgoError(EINVAL, "out as a pair is a dense float16 [2, %d, %d, %d]" % (t, H, d))
+            oa, orow, od = _addr(out, "out", self.device), H * d, F16X2
+        else:
+            oa, orow, od = _packed_rows(out, "out", self.device, t, H, d, None)
+        check(_lib.tgohip_cache_attention(self.h, plan, self._cache(cache), layer, qa, qr, scale, oa, orow, od))
 
     def greedy(self, logits, B, V, ids, margins=None):
         """sample argmax (first strict maximum) and TopTwoMargin over device rows."""

@@ -14,7 +14,8 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 HIP_SOURCES = ["runtime.hip", "kernels/attention.hip", "kernels/gemm.hip", "kernels/gemm_rows.hip",
                "kernels/elementwise.hip", "kernels/probe.hip", "operators.hip", "kernels/rope.hip",
-               "kernels/packed_attention.hip", "kernels/adapters.hip"]
+               "kernels/packed_attention.hip", "kernels/adapters.hip", "cache.hip", "kernels/cache_rows.hip",
+               "kernels/cache_attention.hip"]
 CXX_SOURCES = ["host/hostlogic.cpp", "host/checkpoint.cpp"]
 
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Wall",

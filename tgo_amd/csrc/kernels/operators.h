@@ -1,6 +1,7 @@
 // operators.h -- the op-level operators beside the projections and paged
-// attention: rotary positions, packed attention, the adapters of many requests.
-// Arguments and launches of kernels/rope.hip, packed_attention.hip, adapters.hip.
+// attention: rotary positions, packed attention, the adapters of many requests, the
+// 8-bit cache. Arguments and launches of kernels/rope.hip, packed_attention.hip,
+// adapters.hip, cache_rows.hip, cache_attention.hip.
 #pragma once
 
 #include "../common.h"
@@ -56,6 +57,15 @@ struct PackedPlan {
   int64_t part_rows = 0;
 };
 constexpr int kPackRows = 128;  // the most rows of an item
+// What a kernel's tiles of 64 keys cost: us of one whose workgroup has its CU alone, and
+// the part of that rate each of two workgroups on a CU reaches.
+struct PackRate {
+  double tile, shared;
+};
+// Items, longest first, cut along their keys at multiples of `tile` (pieces of at least
+// `least` tiles) as ends soonest; plan gets the merges and rows of partial results.
+void pack_cut(const std::vector<PackedItem>& whole, int tile, int least, int ncu, const PackRate& rate,
+              std::vector<PackedItem>& out, PackedPlan& plan);
 // Decomposes a call (host only). nq, nk: [B], checked by the caller.
 void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int Hkv, int D, bool causal,
                        bool q_f16, int ncu, PackedPlan& plan);
@@ -79,6 +89,8 @@ struct PackedCounts {
   int items = 0, few = 0, merges = 0;
 };
 int packed_enqueue(const PackedArgs& a, int D, int q_f16, const PackedCounts& n, hipStream_t st);
+// The merges alone, of partial results that other kernels left (a.q, k, v and items unused).
+void packed_merge_enqueue(const PackedArgs& a, int D, int merges, hipStream_t st);
 
 // ---- adapters (adapters.hip) --------------------------------------------------
 constexpr int kAdapterMaxRank = 128;
@@ -130,5 +142,92 @@ inline int adapter_splits(int tiles, int ncu) {
 }
 // tile_rows: 16 or 64, the most rows of a tile.
 void launch_adapters(const AdapterArgs& a, int tile_rows, int ncu, hipStream_t st);
+
+// ---- 8-bit cache (cache_rows.hip, cache_attention.hip) ------------------------------
+// One layer: codes [pages][kv_heads][block][d], scales [pages][kv_heads][block]. A row is
+// one position of one kv head; the rows of a layer number below 2^31.
+struct CacheLayer {
+  uint8_t *k, *v;
+  float *ks, *vs;
+  int32_t capacity, bshift, Hkv, d, f8;  // pages * block; log2(block)
+  // the row of a slot and head
+  __host__ __device__ int64_t row(int32_t slot, int h) const {
+    return ((((int64_t)(slot >> bshift) * Hkv) + h) << bshift) + (slot & ((1 << bshift) - 1));
+  }
+};
+constexpr int kCacheMaxHeads = 4096;
+struct CacheStoreArgs {
+  CacheLayer c;
+  const int32_t *positions, *slots;
+  const double* inv_freq;  // as RopeArgs's
+  float attention;
+  int T, rd, half;  // rd 0: nothing is rotated
+  const void *q, *k, *v;
+  void* q_out;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
+  const float *q_gain, *k_gain;  // null: not normed
+  float eps;
+  int H, x_f16, out_f16;
+  int rows, slice;  // rows and heads of a workgroup, set by launch_cache_store
+  uint64_t magic;
+};
+void launch_cache_store(const CacheStoreArgs& a, int ncu, hipStream_t st);
+struct CacheReadArgs {
+  CacheLayer c;
+  const int32_t* slots;
+  int T, f16;
+  void* out[2];  // k's, v's; null: not read
+  int64_t row[2], head[2];
+};
+void launch_cache_read(const CacheReadArgs& a, int ncu, hipStream_t st);
+// Rows src[i] to dst[i] (slots) of every layer and head; a workgroup takes moves
+// [start, start + n) of one (layer, head, K or V), kCacheMoveSeg of them read before any
+// is written.
+constexpr int kCacheMoveSeg = 64;
+struct CacheMoveBatch {
+  int32_t start, n;
+};
+struct CacheMoveArgs {
+  CacheLayer c;  // of layer 0
+  int layers, batches;
+  int64_t layer_rows;
+  const int32_t *src, *dst;
+  const CacheMoveBatch* batch;
+};
+void launch_cache_move(const CacheMoveArgs& a, hipStream_t st);
+
+// A work item: rows [r0, r0 + nr) of a sequence and kv head (as PackedItem's) against
+// positions [kv_lo, kv_hi). tree 0: token t sees positions up to t + shift; 1: those
+// below shift, and shift + j where bit j of its mask is set.
+struct CacheItem {
+  int32_t q0, seq, nk, shift, r0, nr, kv_lo, kv_hi, kvh, part, tree, pad;
+};
+struct CachePlan {
+  int H = 0;
+  int64_t tq = 0;
+  std::vector<CacheItem> items;  // of the tile kernel, then of the few-row kernel
+  int tiles = 0;
+  std::vector<PackedMerge> merges;
+  int64_t part_rows = 0;
+};
+constexpr int kCacheMaxTree = 64;  // tokens of a tree: the bits of a mask
+// tree: [B], whether a sequence's new tokens are one (null: none is).
+void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, const uint8_t* tree, int H, int Hkv, int D,
+                      bool q_f16, int ncu, CachePlan& plan);
+struct CacheAttnArgs {
+  CacheLayer c;
+  const void* q;
+  void* out;
+  const CacheItem* items;
+  const PackedMerge* merges;
+  const uint32_t* pages;
+  const uint64_t* masks;
+  float *part_o, *part_ml;
+  int64_t q_row, out_row, out_lo;
+  int max_pages, G, out_form, q_f16;
+  int tiles, few, nmerges;
+  float qscale;  // scale * log2(e)
+};
+int cache_attention_enqueue(const CacheAttnArgs& a, hipStream_t st);
 
 }  // namespace tgohip

@@ -28,6 +28,7 @@
 // 2666; the waves' priorities by phase 2240. 64 rows a wave spilled, with packed_redo's
 // registers in the kernel, more than now: not tried since.
 #include "operators.h"
+#include "waits.h"
 
 #include <algorithm>
 #include <climits>
@@ -88,11 +89,6 @@ static std::vector<int> pack_order(const std::vector<int>& lengths) {
   return order;
 }
 
-// What a kernel's tiles of 64 keys cost: us of one whose workgroup has its CU alone, and
-// the part of that rate each of two workgroups on a CU reaches.
-struct PackRate {
-  double tile, shared;
-};
 constexpr int kPackFixed = 3;  // tiles that a piece costs beside its own: its start and its result
 
 // us until the last piece has ended and the rows of cut items are merged. Pieces are
@@ -204,8 +200,8 @@ static PackCut pack_even(const std::vector<int>& tiles, int slots, int longest, 
 // keys 249, -, -, 175; 4 chunks of 82 to 354 f32 queries over 2116 to 8176 keys 237, 226,
 // 130, 136; 2 of 23 and 114 over 2300 and 2700 87, 39, 41, 43; one prompt of 2048 f16
 // queries 61, -, -, 68; 3 prompts of 600 to 900 f32 queries 52, -, -, 59.
-static void pack_cut(const std::vector<PackedItem>& whole, int tile, int least, int ncu, const PackRate& rate,
-                     std::vector<PackedItem>& out, PackedPlan& plan) {
+void pack_cut(const std::vector<PackedItem>& whole, int tile, int least, int ncu, const PackRate& rate,
+              std::vector<PackedItem>& out, PackedPlan& plan) {
   PackCut cut;
   cut.pieces.assign(whole.size(), 1);
   cut.tiles.reserve(whole.size());
@@ -318,27 +314,6 @@ void packed_build_plan(int B, const int32_t* nq, const int32_t* nk, int H, int H
 // ---------------------------------------------------------------------------
 // kernels
 // ---------------------------------------------------------------------------
-
-// s_waitcnt vmcnt(0) lgkmcnt(0), and no memory access moves across it: the wave's DMA has
-// landed, and its LDS reads have returned, before other data goes where they read.
-__device__ __forceinline__ void pack_wait() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0070);
-  asm volatile("" ::: "memory");
-}
-// A barrier without a memory fence, which would wait for every DMA in flight; no
-// memory access moves across it.
-__device__ __forceinline__ void pack_barrier() {
-  asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-}
-// Orders a wave's own LDS writes before its other lanes' reads (and back).
-__device__ __forceinline__ void pack_wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
 
 // A tile of kPackTile keys in LDS: rows of D f16, their 16-byte chunks XOR-swizzled.
 // K's chunks by the row, so that 32 lanes reading one chunk of 32 rows touch
@@ -1140,6 +1115,12 @@ static void packed_launch(PackedArgs a, const PackedCounts& n, hipStream_t st) {
   a.items += n.items;
   if (n.few) hipLaunchKernelGGL((packed_few_kernel<D, QF16>), dim3(n.few), dim3(64 * kFewWaves), 0, st, a);
   if (n.merges) hipLaunchKernelGGL((packed_merge_kernel<D>), dim3(n.merges), dim3(256), 0, st, a);
+}
+
+void packed_merge_enqueue(const PackedArgs& a, int D, int merges, hipStream_t st) {
+  if (!merges) return;
+  if (D == 128) hipLaunchKernelGGL((packed_merge_kernel<128>), dim3(merges), dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((packed_merge_kernel<64>), dim3(merges), dim3(256), 0, st, a);
 }
 
 int packed_enqueue(const PackedArgs& a, int D, int q_f16, const PackedCounts& n, hipStream_t st) {

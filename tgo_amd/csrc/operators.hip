@@ -2,12 +2,11 @@
 // paged attention: rotary positions, packed attention, the adapters of many
 // requests. A program makes their handles once (per model, per batch) and each
 // call then only launches kernels on the context's stream.
-#include "runtime.h"
+#include "operators_abi.h"
 
 #include <algorithm>
 #include <climits>
 #include <cmath>
-#include <new>
 
 namespace tgohip {
 
@@ -25,89 +24,20 @@ void OpHandles::release() {
     r.second.meta.release();
     r.second.u.release();
   }
+  for (auto& p : caches) {
+    p.second.meta.release();
+    p.second.part.release();
+  }
   ropes.clear();
   packed.clear();
   sets.clear();
   rows.clear();
+  caches.clear();
 }
 
 }  // namespace tgohip
 
 namespace {
-
-// Entry points do not throw across the C ABI, and a refused call leaves no error behind
-// that the next launch would report as its own.
-template <typename F>
-int guarded(F f) {
-  try {
-    const int rc = f();
-    if (rc) (void)hipGetLastError();
-    return rc;
-  } catch (const std::bad_alloc&) {
-    return fail(TGOHIP_ENOMEM, "host allocation failed");
-  } catch (const std::exception& e) {
-    return fail(TGOHIP_EDEVICE, std::string("internal: ") + e.what());
-  }
-}
-
-// Makes the context's device current for a call, and the caller's again after it.
-struct OnDevice {
-  int prev = -1;
-  bool moved = false;
-  explicit OnDevice(int device) {
-    if (hipGetDevice(&prev) == hipSuccess && prev != device) moved = hipSetDevice(device) == hipSuccess;
-  }
-  ~OnDevice() {
-    if (moved) (void)hipSetDevice(prev);
-  }
-};
-
-int refuse(const std::string& why) { return fail(TGOHIP_EINVAL, why); }
-int no_ctx(const char* what) { return refuse(std::string(what) + ": the context is missing"); }
-
-// Making, changing or freeing a handle copies, allocates and waits, which a graph
-// cannot hold.
-int no_capture(tgohip_ctx* c, const char* what) {
-  hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-  const hipError_t e = hipStreamIsCapturing(c->stream, &st);
-  if (e != hipSuccess) return fail(TGOHIP_EDEVICE, hip_message(e, what));
-  if (st == hipStreamCaptureStatusNone) return 0;
-  return fail(TGOHIP_ESTATE, std::string(what) + ": the context's stream is being captured");
-}
-
-template <typename T>
-T* find(std::map<int, T>& m, int handle, const char* what) {
-  auto it = m.find(handle);
-  if (it != m.end()) return &it->second;
-  refuse(std::string(what) + ": no handle " + std::to_string(handle));
-  return nullptr;
-}
-
-bool misaligned(const void* p) { return ((uintptr_t)p & 15) != 0; }
-int64_t elt(int f16) { return f16 ? 2 : 4; }
-
-// A device operand: `rows` rows of `heads` heads of d elements, strides in bytes.
-struct Span {
-  const char* p;
-  int64_t rows, heads, row, head, d;
-  int64_t width() const { return (heads - 1) * head + d; }  // of one row
-  int64_t end() const { return rows ? (rows - 1) * row + width() : 0; }
-};
-// Whether two operands may share memory: apart, or columns of the same rows that
-// do not meet.
-bool meet(const Span& a, const Span& b) {
-  if (!a.rows || !b.rows) return false;
-  if (a.p + a.end() <= b.p || b.p + b.end() <= a.p) return false;
-  if (a.row == b.row && a.row > 0 && a.width() <= a.row && b.width() <= a.row) {
-    int64_t off = (b.p - a.p) % a.row;
-    if (off < 0) off += a.row;
-    if (off >= a.width() && off + b.width() <= a.row) return false;
-  }
-  return true;
-}
-bool same(const Span& a, const Span& b) {
-  return a.p == b.p && a.d == b.d && (a.rows <= 1 || a.row == b.row) && (a.heads <= 1 || a.head == b.head);
-}
 
 // Rounds to the nearest f16 (ties to even), subnormal ones included: an adapter's
 // values sit near the bottom of f16's range, where the loader's rule
@@ -134,12 +64,6 @@ bool to_half(const float* src, uint16_t* dst, size_t n) {
     dst[i] = (uint16_t)(h | ((w >> 16) & 0x8000u));
   }
   return !past;
-}
-
-std::string num(double v) {
-  char b[64];
-  snprintf(b, sizeof b, "%g", v);
-  return b;
 }
 
 int check_rope(const tgohip_rope_cfg* c) {

@@ -97,12 +97,20 @@ struct AdapterRows {
   size_t tiles_off = 0;
   DevBuf meta, u;
 };
+struct CacheHandle {
+  CachePlan plan;  // its vectors empty: they are in meta
+  int items = 0, nmerges = 0, max_pages = 0, q_f16 = 0;
+  int pages = 0, Hkv = 0, block = 0, D = 0;  // the cache's geometry; D 0: no plan
+  size_t merges_off = 0, pages_off = 0, masks_off = 0;
+  DevBuf meta, part;
+};
 struct OpHandles {
   int next = 1;
   std::map<int, RopeTable> ropes;
   std::map<int, PackedHandle> packed;
   std::map<int, AdapterSet> sets;
   std::map<int, AdapterRows> rows;
+  std::map<int, CacheHandle> caches;
   void release();  // frees the device memory of every handle
 };
 
