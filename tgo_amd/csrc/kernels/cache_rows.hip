@@ -39,25 +39,39 @@ __device__ __forceinline__ void cache_values4(uint32_t w, float s, float* v) {
   }
 }
 
-// One head of one row, by D / 8 neighbouring lanes: lane j holds 4 / V units of 2V
-// elements, unit u = j + D / 8 i. A unit of the rotated part is V pairs, in the half layout two runs of V,
-// others 2V neighbouring elements from 2V u on.
-template <int V, bool HALF, int D, bool F8, bool XF16>
-__device__ __forceinline__ void cache_store_head(const CacheStoreArgs& a, int t, int h, int j, const float2* cs) {
+// Sum and maximum over LPH (8 or 16) neighbouring lanes, in all of them: DPP moves within
+// a row of 16 lanes (exchanges of 1 and 2 lanes, then mirrors of 8 and 16).
+template <int CTRL>
+__device__ __forceinline__ float cache_dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int LPH, typename F>
+__device__ __forceinline__ float cache_over_lanes(float v, F f) {
+  v = f(v, cache_dpp<0xb1>(v));
+  v = f(v, cache_dpp<0x4e>(v));
+  v = f(v, cache_dpp<0x141>(v));
+  if (LPH == 16) v = f(v, cache_dpp<0x140>(v));
+  return v;
+}
+
+// Elements of one head of one row in D / 8 neighbouring lanes: lane j holds 4 / V units of
+// 2V, unit u = j + D / 8 i. A unit of the rotated part is V pairs, in the half layout two runs
+// of V; others are 2V neighbouring elements from 2V u on.
+template <int V>
+struct HeadRow {
+  float A[4 / V][V], B[4 / V][V];
+};
+
+// Rows [t0, t0 + rows) of head h, row t0 + phase, then every P-th. What belongs to the head
+// (its tensor, gains, places) is taken once, a row is loaded while the one before is worked on.
+template <int KIND, int V, bool HALF, int D, bool F8, bool XF16>
+__device__ __forceinline__ void cache_store_rows(const CacheStoreArgs& a, int t0, int rows, int h, int phase, int P, int j,
+                                                 const float2* cs) {
   constexpr int LPH = D / 8, NU = 4 / V;
-  const int kind = h < a.H ? 0 : h < a.H + a.c.Hkv ? 1 : 2;
-  const int hh = kind == 0 ? h : kind == 1 ? h - a.H : h - a.H - a.c.Hkv;
-  int32_t slot = 0;
-  if (kind) {
-    slot = a.slots[t];
-    if ((uint32_t)slot >= (uint32_t)a.c.capacity) return;  // all lanes of the head alike
-  }
-  const void* src = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-  const int64_t off = kind == 0   ? t * a.q_row + hh * a.q_head
-                      : kind == 1 ? t * a.k_row + hh * a.k_head
-                                  : t * a.v_row + hh * a.v_head;
-  const int turned = kind < 2 ? a.rd / (2 * V) : 0, pairs = a.rd / 2;
-  float A[NU][V], B[NU][V];
+  const int turned = KIND < 2 ? a.rd / (2 * V) : 0, pairs = a.rd / 2;
+  const void* src = KIND == 0 ? a.q : KIND == 1 ? a.k : a.v;
+  const int64_t row = KIND == 0 ? a.q_row : KIND == 1 ? a.k_row : a.v_row;
+  const int64_t head = KIND == 0 ? a.q_head : KIND == 1 ? a.k_head : a.v_head;
   int ja[NU], jb[NU];
 #pragma unroll
   for (int i = 0; i < NU; i++) {
@@ -65,100 +79,119 @@ __device__ __forceinline__ void cache_store_head(const CacheStoreArgs& a, int t,
     const bool split = HALF && u < turned;
     ja[i] = split ? V * u : 2 * V * u;
     jb[i] = split ? pairs + V * u : ja[i] + V;
-    rope_load<V, XF16>(src, off + ja[i], A[i]);
-    rope_load<V, XF16>(src, off + jb[i], B[i]);
   }
-  const float* gain = kind == 0 ? a.q_gain : kind == 1 ? a.k_gain : nullptr;
+  const float* gain = KIND == 0 ? a.q_gain : KIND == 1 ? a.k_gain : nullptr;
+  HeadRow<V> g;
   if (gain) {
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < NU; i++)
-#pragma unroll
-      for (int e = 0; e < V; e++) ss += A[i][e] * A[i][e] + B[i][e] * B[i][e];
-#pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-    const float sc = 1.0f / sqrtf(ss / (float)D + a.eps);
 #pragma unroll
     for (int i = 0; i < NU; i++) {
-      float ga[V], gb[V];
-      rope_load<V, false>(gain, ja[i], ga);
-      rope_load<V, false>(gain, jb[i], gb);
+      rope_load<V, false>(gain, ja[i], g.A[i]);
+      rope_load<V, false>(gain, jb[i], g.B[i]);
+    }
+  }
+  const auto load = [&](int t, HeadRow<V>& x, int32_t& slot) {
+    const int64_t off = t * row + h * head;
+#pragma unroll
+    for (int i = 0; i < NU; i++) {
+      rope_load<V, XF16>(src, off + ja[i], x.A[i]);
+      rope_load<V, XF16>(src, off + jb[i], x.B[i]);
+    }
+    if (KIND) slot = a.slots[t];
+  };
+  HeadRow<V> x, next;
+  int32_t slot = 0, next_slot = 0;
+  if (phase < rows) load(t0 + phase, next, next_slot);
+  for (int t = phase; t < rows; t += P) {
+    x = next;
+    slot = next_slot;
+    load(t0 + min(t + P, rows - 1), next, next_slot);
+    if (gain) {
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < NU; i++)
+#pragma unroll
+        for (int e = 0; e < V; e++) ss += x.A[i][e] * x.A[i][e] + x.B[i][e] * x.B[i][e];
+      ss = cache_over_lanes<LPH>(ss, [](float p, float q) { return p + q; });
+      const float sc = __builtin_amdgcn_rsqf(ss * (1.f / D) + a.eps);
+#pragma unroll
+      for (int i = 0; i < NU; i++)
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          x.A[i][e] = x.A[i][e] * sc * g.A[i][e];
+          x.B[i][e] = x.B[i][e] * sc * g.B[i][e];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NU; i++) {
+      const int u = j + LPH * i;
+      if (u >= turned) continue;
+      float p[2 * V];
 #pragma unroll
       for (int e = 0; e < V; e++) {
-        A[i][e] = A[i][e] * sc * ga[e];
-        B[i][e] = B[i][e] * sc * gb[e];
+        p[e] = x.A[i][e];
+        p[V + e] = x.B[i][e];
+      }
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        const float2 w = cs[t * pairs + V * u + e];
+        const int m = HALF ? e : 2 * e, n = HALF ? V + e : 2 * e + 1;
+        const float f = p[m], r = p[n];
+        p[m] = fmaf(f, w.x, -(r * w.y));
+        p[n] = fmaf(f, w.y, r * w.x);
+      }
+#pragma unroll
+      for (int e = 0; e < V; e++) {
+        x.A[i][e] = p[e];
+        x.B[i][e] = p[V + e];
       }
     }
-  }
+    if constexpr (KIND == 0) {
+      const int64_t to = (t0 + t) * a.out_row + h * a.out_head;
 #pragma unroll
-  for (int i = 0; i < NU; i++) {
-    const int u = j + LPH * i;
-    if (u >= turned) continue;
-    float p[2 * V];
-#pragma unroll
-    for (int e = 0; e < V; e++) {
-      p[e] = A[i][e];
-      p[V + e] = B[i][e];
-    }
-#pragma unroll
-    for (int e = 0; e < V; e++) {
-      const float2 w = cs[V * u + e];
-      const int x = HALF ? e : 2 * e, y = HALF ? V + e : 2 * e + 1;
-      const float f = p[x], g = p[y];
-      p[x] = fmaf(f, w.x, -(g * w.y));
-      p[y] = fmaf(f, w.y, g * w.x);
-    }
-#pragma unroll
-    for (int e = 0; e < V; e++) {
-      A[i][e] = p[e];
-      B[i][e] = p[V + e];
-    }
-  }
-  if (kind == 0) {
-    const int64_t to = t * a.out_row + hh * a.out_head;
-#pragma unroll
-    for (int i = 0; i < NU; i++) {
-      if (a.out_f16) {
-        rope_store<V, true>(a.q_out, to + ja[i], A[i]);
-        rope_store<V, true>(a.q_out, to + jb[i], B[i]);
-      } else {
-        rope_store<V, false>(a.q_out, to + ja[i], A[i]);
-        rope_store<V, false>(a.q_out, to + jb[i], B[i]);
+      for (int i = 0; i < NU; i++) {
+        if (a.out_f16) {
+          rope_store<V, true>(a.q_out, to + ja[i], x.A[i]);
+          rope_store<V, true>(a.q_out, to + jb[i], x.B[i]);
+        } else {
+          rope_store<V, false>(a.q_out, to + ja[i], x.A[i]);
+          rope_store<V, false>(a.q_out, to + jb[i], x.B[i]);
+        }
       }
-    }
-    return;
-  }
-  float peak = 0.f;  // infinite where a value is past kCacheMost or NaN
-#pragma unroll
-  for (int i = 0; i < NU; i++)
-#pragma unroll
-    for (int e = 0; e < V; e++) {
-      const float x = fabsf(A[i][e]), y = fabsf(B[i][e]);
-      peak = fmaxf(peak, x <= kCacheMost ? x : INFINITY);
-      peak = fmaxf(peak, y <= kCacheMost ? y : INFINITY);
-    }
-#pragma unroll
-  for (int o = LPH / 2; o > 0; o >>= 1) peak = fmaxf(peak, __shfl_xor(peak, o, 64));
-  const bool bad = peak == INFINITY;
-  const float scale = fmaxf(peak / (F8 ? 448.f : 127.f), kCacheLeast), inv = 1.0f / scale;
-  const int64_t row = a.c.row(slot, hh);
-  uint8_t* to = (kind == 1 ? a.c.k : a.c.v) + row * D;
-  if (j == 0) (kind == 1 ? a.c.ks : a.c.vs)[row] = bad ? NAN : scale;
-#pragma unroll
-  for (int i = 0; i < NU; i++) {
-    float x[4], y[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      x[e] = bad ? 0.f : A[i][e % V] * inv;
-      y[e] = bad ? 0.f : B[i][e % V] * inv;
-    }
-    const uint32_t w0 = cache_codes4<F8>(x[0], x[1], x[2], x[3]), w1 = cache_codes4<F8>(y[0], y[1], y[2], y[3]);
-    if constexpr (V == 4) {
-      *(uint32_t*)(to + ja[i]) = w0;
-      *(uint32_t*)(to + jb[i]) = w1;
     } else {
-      to[ja[i]] = (uint8_t)w0;
-      to[jb[i]] = (uint8_t)w1;
+      float peak = 0.f;  // infinite where a value is past kCacheMost or NaN
+#pragma unroll
+      for (int i = 0; i < NU; i++)
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          const float m = fabsf(x.A[i][e]), n = fabsf(x.B[i][e]);
+          peak = fmaxf(peak, m <= kCacheMost ? m : INFINITY);
+          peak = fmaxf(peak, n <= kCacheMost ? n : INFINITY);
+        }
+      peak = cache_over_lanes<LPH>(peak, [](float p, float q) { return fmaxf(p, q); });
+      const bool bad = peak == INFINITY;
+      const float scale = fmaxf(peak / (F8 ? 448.f : 127.f), kCacheLeast);
+      const float inv = __builtin_amdgcn_rcpf(scale);
+      if ((uint32_t)slot >= (uint32_t)a.c.capacity) continue;  // all lanes of the head alike
+      const int64_t at = a.c.row(slot, h);
+      uint8_t* to = (KIND == 1 ? a.c.k : a.c.v) + at * D;
+      if (j == 0) (KIND == 1 ? a.c.ks : a.c.vs)[at] = bad ? NAN : scale;
+#pragma unroll
+      for (int i = 0; i < NU; i++) {
+        float m[4], n[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          m[e] = bad ? 0.f : x.A[i][e % V] * inv;
+          n[e] = bad ? 0.f : x.B[i][e % V] * inv;
+        }
+        const uint32_t w0 = cache_codes4<F8>(m[0], m[1], m[2], m[3]), w1 = cache_codes4<F8>(n[0], n[1], n[2], n[3]);
+        if constexpr (V == 4) {
+          *(uint32_t*)(to + ja[i]) = w0;
+          *(uint32_t*)(to + jb[i]) = w1;
+        } else {
+          to[ja[i]] = (uint8_t)w0;
+          to[jb[i]] = (uint8_t)w1;
+        }
+      }
     }
   }
 }
@@ -166,8 +199,8 @@ __device__ __forceinline__ void cache_store_head(const CacheStoreArgs& a, int t,
 template <int V, bool HALF, int D, bool F8, bool XF16>
 __global__ __launch_bounds__(256) void cache_store_kernel(CacheStoreArgs a) {
   extern __shared__ float2 cs[];  // [rows][pairs]
-  constexpr int LPH = D / 8;
-  const int heads = a.H + 2 * a.c.Hkv, h0 = blockIdx.y * a.slice, n = min(a.slice, heads - h0);
+  constexpr int LPH = D / 8, GR = 256 / LPH;
+  const int heads = a.H + 2 * a.c.Hkv, h0 = blockIdx.y * a.slice, hn = min(h0 + a.slice, heads);
   const int t0 = blockIdx.x * a.rows, rows = min(a.rows, a.T - t0), pairs = a.rd / 2;
   if (pairs && h0 < a.H + a.c.Hkv) {
     for (int i = threadIdx.x; i < rows * pairs; i += 256) {
@@ -176,9 +209,14 @@ __global__ __launch_bounds__(256) void cache_store_kernel(CacheStoreArgs a) {
     }
     __syncthreads();
   }
-  for (int r = threadIdx.x / LPH; r < rows * a.slice; r += 256 / LPH) {
-    const int t = (int)(((uint64_t)r * a.magic) >> 32), h = r - t * a.slice;
-    if (h < n) cache_store_head<V, HALF, D, F8, XF16>(a, t0 + t, h0 + h, threadIdx.x % LPH, cs + t * pairs);
+  // GR heads at a time, the last few of the slice with their rows shared by several groups of lanes
+  const int g = threadIdx.x / LPH, j = threadIdx.x % LPH;
+  for (int h = h0; h < hn; h += GR) {
+    const int n = min(GR, hn - h), P = GR / n, phase = g / n, mine = h + g % n;
+    if (phase >= P) continue;
+    if (mine < a.H) cache_store_rows<0, V, HALF, D, F8, XF16>(a, t0, rows, mine, phase, P, j, cs);
+    else if (mine < a.H + a.c.Hkv) cache_store_rows<1, V, HALF, D, F8, XF16>(a, t0, rows, mine - a.H, phase, P, j, cs);
+    else cache_store_rows<2, V, HALF, D, F8, XF16>(a, t0, rows, mine - a.H - a.c.Hkv, phase, P, j, cs);
   }
 }
 
@@ -206,7 +244,6 @@ void launch_cache_store(const CacheStoreArgs& args, int ncu, hipStream_t st) {
     a.slice = std::max(at_once, (a.slice + 1) / 2);
   a.rows = 1;
   while (a.rows < 16 && (int64_t)a.T * ((heads + a.slice - 1) / a.slice) / (2 * a.rows) >= 4 * ncu) a.rows *= 2;
-  a.magic = (((uint64_t)1 << 32) + a.slice - 1) / a.slice;
   const auto fits = [](const void* p, int64_t row, int64_t head, int f16) {
     const int n = f16 ? 8 : 4;
     return (uintptr_t)p % 16 == 0 && row % n == 0 && head % n == 0;

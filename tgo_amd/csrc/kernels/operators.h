@@ -169,7 +169,6 @@ struct CacheStoreArgs {
   float eps;
   int H, x_f16, out_f16;
   int rows, slice;  // rows and heads of a workgroup, set by launch_cache_store
-  uint64_t magic;
 };
 void launch_cache_store(const CacheStoreArgs& a, int ncu, hipStream_t st);
 struct CacheReadArgs {
