@@ -98,18 +98,26 @@ __device__ __forceinline__ void cache_out4(const CacheAttnArgs& a, int64_t off, 
   if (a.out_form == OUT_X2) *(half4_t*)((half_t*)a.out + a.out_lo + off) = lv;
 }
 
-// Which of the 64 keys from position t0 on a token sees, as bits. mask: its tree's.
-__device__ __forceinline__ uint64_t cache_visible(const CacheItem& it, int tok, uint64_t mask, int t0) {
-  const int end = it.kv_hi - t0;  // at least 1
-  uint64_t v;
+// Which of the 32 keys from position t0 on a token sees, as bits. mask: its tree's.
+// 64-bit shifts here go by amounts of the whole wave only: with a lane's amount in the last
+// register that the wave has allocated, v_lshlrev_b64 has shifted by the lane's v0 instead
+// (one register pair is read where one register is the amount, and the second lies past
+// the allocation), on gfx950 and with the compiler none the wiser.
+__device__ __forceinline__ uint32_t cache_ones(int n) {  // the lowest n bits, all from 32 on
+  return n >= 32 ? ~0u : n > 0 ? (1u << n) - 1 : 0u;
+}
+__device__ __forceinline__ uint32_t cache_visible(const CacheItem& it, int tok, uint64_t mask, int t0) {
+  uint32_t v;
   if (it.tree) {
     const int off = it.shift - t0;  // keys before the tree's
-    v = off >= 64 ? ~0ull : off > 0 ? (mask << off) | ((1ull << off) - 1) : off > -64 ? mask >> -off : 0ull;
+    v = off >= 32  ? ~0u
+        : off > 0  ? ((uint32_t)mask << off) | cache_ones(off)
+        : off > -64 ? (uint32_t)(mask >> -off)
+                    : 0u;
   } else {
-    const int n = tok + it.shift + 1 - t0;
-    v = n >= 64 ? ~0ull : n > 0 ? (1ull << n) - 1 : 0ull;
+    v = cache_ones(tok + it.shift + 1 - t0);
   }
-  return end >= 64 ? v : v & ((1ull << end) - 1);
+  return v & cache_ones(it.kv_hi - t0);
 }
 
 // LDS tiles hold rows of D bytes, their 16-byte chunks XOR-swizzled: K's so that the 16
@@ -129,13 +137,18 @@ __device__ __forceinline__ int cache_v_swz(int r) {
 // LDS. S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16: lane (l16, g) holds row
 // l16 of each block of 16 rows, its scores at keys 16 kb + 4g + i, and of O^T dims
 // 16 db + 4g + i.
+template <int D>
+struct CacheLds {
+  char tiles[kFewWaves * 4 * kFewTile * D] __attribute__((aligned(1024)));
+  float4_t scales[kFewWaves][3 * kFewTile / 4];
+  float2 refs[kFewWaves][kFewRows];
+};
+
 template <int D, bool QF16, bool F8, int RB>
-__global__ __launch_bounds__(64 * kFewWaves, 2) void cache_few_kernel(CacheAttnArgs a) {
+__device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, CacheLds<D>& lds) {
   constexpr int TB = kFewTile * D, RPI = 1024 / D, NI = kFewTile / RPI, NS = D / 32, ND = D / 16;
-  __shared__ __attribute__((aligned(1024))) char tiles[kFewWaves * 4 * TB];
-  __shared__ float4_t scales[kFewWaves][3 * kFewTile / 4];
-  __shared__ float2 refs[kFewWaves][RB][16];
-  static_assert(kFewWaves * 4 * TB >= kFewWaves * RB * ND * 1024, "the tiles hold the waves' results");
+  auto& tiles = lds.tiles;
+  auto& scales = lds.scales;
   const CacheItem it = a.items[blockIdx.x];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
@@ -241,7 +254,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void cache_few_kernel(CacheAttnA
     half8_t ph[RB], pl[RB];
 #pragma unroll
     for (int b = 0; b < RB; b++) {
-      const uint32_t vis = masked ? (uint32_t)cache_visible(it, tok[b], mask[b], t0) >> (4 * g) : ~0u;
+      const uint32_t vis = masked ? cache_visible(it, tok[b], mask[b], t0) >> (4 * g) : ~0u;
       float top = -INFINITY;
 #pragma unroll
       for (int kb = 0; kb < 2; kb++) {
@@ -302,46 +315,43 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void cache_few_kernel(CacheAttnA
   }
 
   // The waves' rows meet: each brings its own to the largest reference, then every wave
-  // adds a share of the dims.
+  // adds a share of the dims, a block of rows at a time.
 #pragma unroll
   for (int b = 0; b < RB; b++) {
     l[b] += __shfl_xor(l[b], 16, 64);
     l[b] += __shfl_xor(l[b], 32, 64);
-    if (lane < 16) refs[wave][b][lane] = float2{m[b], l[b]};
+    if (lane < 16) lds.refs[wave][16 * b + lane] = float2{m[b], l[b]};
   }
   __syncthreads();
   typedef __attribute__((address_space(3))) float4_t* f4p;
-  float M[RB], L[RB];
+  static_assert(4 * TB >= 2 * ND * 1024, "the tiles hold two blocks of the waves' results");
 #pragma unroll
   for (int b = 0; b < RB; b++) {
-    M[b] = refs[0][b][l16].x;
+    float M = lds.refs[0][16 * b + l16].x, L = 0.f;
 #pragma unroll
-    for (int w = 1; w < kFewWaves; w++) M[b] = fmaxf(M[b], refs[w][b][l16].x);
-    L[b] = 0.f;
+    for (int w = 1; w < kFewWaves; w++) M = fmaxf(M, lds.refs[w][16 * b + l16].x);
 #pragma unroll
     for (int w = 0; w < kFewWaves; w++) {
-      const float2 r = refs[w][b][l16];
-      L[b] += r.y * __builtin_amdgcn_exp2f(r.x - M[b]);
+      const float2 r = lds.refs[w][16 * b + l16];
+      L += r.y * __builtin_amdgcn_exp2f(r.x - M);
     }
-    const float mul = __builtin_amdgcn_exp2f(m[b] - M[b]);
+    const lds_t buf = (lds_t)tiles + (b & 1) * (kFewWaves * ND * 1024) + lane * 16;
+    const float own = __builtin_amdgcn_exp2f(m[b] - M);
 #pragma unroll
-    for (int d = 0; d < ND; d++) *(f4p)((lds_t)tiles + (((wave * RB + b) * ND + d) * 64 + lane) * 16) = o[b][d] * mul;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int b = 0; b < RB; b++) {
+    for (int d = 0; d < ND; d++) *(f4p)(buf + (wave * ND + d) * 1024) = o[b][d] * own;
+    __syncthreads();
     const int r = 16 * b + l16;
     const bool live = r < it.nr, part = it.part >= 0;
     const int row = it.r0 + r, t = row / a.G, head = it.kvh * a.G + row % a.G;
     if (part && live && wave == 0 && g == 0)
-      *(float4_t*)(a.part_ml + ((int64_t)it.part + r) * 4) = float4_t{M[b], 0.f, L[b], 0.f};
-    const float mul = part ? 1.f : L[b] == 0.f ? 0.f : 1.f / L[b];
+      *(float4_t*)(a.part_ml + ((int64_t)it.part + r) * 4) = float4_t{M, 0.f, L, 0.f};
+    const float mul = part ? 1.f : L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
     for (int x = 0; x < ND / kFewWaves; x++) {
       const int d = wave * (ND / kFewWaves) + x;
       float4_t v = float4_t{};
 #pragma unroll
-      for (int w = 0; w < kFewWaves; w++) v += *(f4p)((lds_t)tiles + (((w * RB + b) * ND + d) * 64 + lane) * 16);
+      for (int w = 0; w < kFewWaves; w++) v += *(f4p)(buf + (w * ND + d) * 1024);
       if (!live) continue;
       v *= mul;
       if (part) *(float4_t*)(a.part_o + ((int64_t)it.part + r) * D + 16 * d + 4 * g) = v;
@@ -350,6 +360,13 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void cache_few_kernel(CacheAttnA
   }
 }
 
+// Up to kFewRows rows: 16 or 32, two workgroups a CU.
+template <int D, bool QF16, bool F8>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void cache_few_kernel(CacheAttnArgs a) {
+  __shared__ CacheLds<D> lds;
+  if (a.items[blockIdx.x].nr <= 16) cache_rows_body<D, QF16, F8, 1>(a, lds);
+  else cache_rows_body<D, QF16, F8, 2>(a, lds);
+}
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
@@ -360,7 +377,6 @@ void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, con
   plan.H = H;
   const int G = H / Hkv;
   std::vector<PackedItem> whole, cut;
-  std::vector<int32_t> starts((size_t)B);
   int64_t q0 = 0;
   for (int s = 0; s < B; s++) {
     const int64_t rows = (int64_t)extents[s] * G;
@@ -385,8 +401,8 @@ void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, con
 }
 
 template <int D, bool QF16, bool F8>
-static void cache_attention_launch(const CacheAttnArgs& a, hipStream_t st) {
-  if (a.few) hipLaunchKernelGGL((cache_few_kernel<D, QF16, F8, kFewRows / 16>), dim3(a.few), dim3(64 * kFewWaves), 0, st, a);
+static void cache_attention_launch(CacheAttnArgs a, hipStream_t st) {
+  if (a.few) hipLaunchKernelGGL((cache_few_kernel<D, QF16, F8>), dim3(a.few), dim3(64 * kFewWaves), 0, st, a);
 }
 template <int D>
 static void cache_attention_form(const CacheAttnArgs& a, hipStream_t st) {
