@@ -9,14 +9,13 @@
 // product takes hold their value's scale, so that their largest is near 1 whatever the
 // scales are, and the sum takes it out again. m moves along (online softmax), and only
 // when a probability would leave its range.
-#include "operators.h"
-#include "waits.h"
+#include "pack_rows.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tgohip {
 
-typedef __attribute__((address_space(3))) char* lds_t;
 constexpr int kNonTemporal = 2;  // the nt bit: a context's rows are read once
 // The reference starts at kCacheNoMax; where a term passes it by more than 2^kCacheTop (f16
 // ends at 2^16) it moves to the row's largest, kCacheLift less, so that small terms
@@ -137,23 +136,15 @@ __device__ __forceinline__ int cache_v_swz(int r) {
 // LDS. S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16: lane (l16, g) holds row
 // l16 of each block of 16 rows, its scores at keys 16 kb + 4g + i, and of O^T dims
 // 16 db + 4g + i.
-template <int D>
-struct CacheLds {
-  char tiles[kFewWaves * 4 * kFewTile * D] __attribute__((aligned(1024)));
-  float4_t scales[kFewWaves][3 * kFewTile / 4];
-  float2 refs[kFewWaves][kFewRows];
-};
-
 template <int D, bool QF16, bool F8, int RB>
-__device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, CacheLds<D>& lds) {
+__device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, lds_t K0, lds_t V0, lds_t K1, lds_t V1,
+                                                float* scales, float2* refs) {
   constexpr int TB = kFewTile * D, RPI = 1024 / D, NI = kFewTile / RPI, NS = D / 32, ND = D / 16;
-  auto& tiles = lds.tiles;
-  auto& scales = lds.scales;
   const CacheItem it = a.items[blockIdx.x];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
-  const lds_t base = (lds_t)tiles + wave * 4 * TB;  // K and V of the even tiles, then of the odd ones
-  float* mine = (float*)scales[wave];
+  const lds_t Kw[2] = {K0 + wave * TB, K1 + wave * TB}, Vw[2] = {V0 + wave * TB, V1 + wave * TB};
+  float* mine = scales + wave * 3 * kFewTile;
   const uint32_t* table = a.pages + (int64_t)it.seq * a.max_pages;
   const int first = it.kv_lo + wave * kFewTile, step = kFewWaves * kFewTile;
 
@@ -182,7 +173,7 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, CacheLds
   uint32_t page = 0;
   if (first < it.kv_hi) {
     const int row = key_row(first, key_page(first));
-    dma(row, base, base + TB);
+    dma(row, Kw[0], Vw[0]);
     ks = a.c.ks[row];
     vs = a.c.vs[row];
     if (first + step < it.kv_hi) page = key_page(first + step);
@@ -310,8 +301,8 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, CacheLds
     }
   };
   for (int t0 = first; t0 < it.kv_hi; t0 += 2 * step) {
-    tile(t0, base, base + TB, base + 2 * TB, base + 3 * TB);
-    if (t0 + step < it.kv_hi) tile(t0 + step, base + 2 * TB, base + 3 * TB, base, base + TB);
+    tile(t0, Kw[0], Vw[0], Kw[1], Vw[1]);
+    if (t0 + step < it.kv_hi) tile(t0 + step, Kw[1], Vw[1], Kw[0], Vw[0]);
   }
 
   // The waves' rows meet: each brings its own to the largest reference, then every wave
@@ -320,25 +311,26 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, CacheLds
   for (int b = 0; b < RB; b++) {
     l[b] += __shfl_xor(l[b], 16, 64);
     l[b] += __shfl_xor(l[b], 32, 64);
-    if (lane < 16) lds.refs[wave][16 * b + lane] = float2{m[b], l[b]};
+    if (lane < 16) refs[wave * kFewRows + 16 * b + lane] = float2{m[b], l[b]};
   }
   __syncthreads();
   typedef __attribute__((address_space(3))) float4_t* f4p;
-  static_assert(4 * TB >= 2 * ND * 1024, "the tiles hold two blocks of the waves' results");
+  static_assert(2 * TB == ND * 1024, "a K and a V tile hold a block of a wave's results");
+  const auto merge = [&](auto block) {
+    constexpr int b = decltype(block)::value;
+    float M = refs[16 * b + l16].x, L = 0.f;
 #pragma unroll
-  for (int b = 0; b < RB; b++) {
-    float M = lds.refs[0][16 * b + l16].x, L = 0.f;
-#pragma unroll
-    for (int w = 1; w < kFewWaves; w++) M = fmaxf(M, lds.refs[w][16 * b + l16].x);
+    for (int w = 1; w < kFewWaves; w++) M = fmaxf(M, refs[w * kFewRows + 16 * b + l16].x);
 #pragma unroll
     for (int w = 0; w < kFewWaves; w++) {
-      const float2 r = lds.refs[w][16 * b + l16];
+      const float2 r = refs[w * kFewRows + 16 * b + l16];
       L += r.y * __builtin_amdgcn_exp2f(r.x - M);
     }
-    const lds_t buf = (lds_t)tiles + (b & 1) * (kFewWaves * ND * 1024) + lane * 16;
+    const lds_t lo = b ? K1 : K0, hi = b ? V1 : V0;
+    const auto at = [&](int w, int d) { return (d < ND / 2 ? lo : hi) + w * TB + d % (ND / 2) * 1024 + lane * 16; };
     const float own = __builtin_amdgcn_exp2f(m[b] - M);
 #pragma unroll
-    for (int d = 0; d < ND; d++) *(f4p)(buf + (wave * ND + d) * 1024) = o[b][d] * own;
+    for (int d = 0; d < ND; d++) *(f4p)at(wave, d) = o[b][d] * own;
     __syncthreads();
     const int r = 16 * b + l16;
     const bool live = r < it.nr, part = it.part >= 0;
@@ -351,22 +343,191 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, CacheLds
       const int d = wave * (ND / kFewWaves) + x;
       float4_t v = float4_t{};
 #pragma unroll
-      for (int w = 0; w < kFewWaves; w++) v += *(f4p)(buf + (w * ND + d) * 1024);
+      for (int w = 0; w < kFewWaves; w++) v += *(f4p)at(w, d);
       if (!live) continue;
       v *= mul;
       if (part) *(float4_t*)(a.part_o + ((int64_t)it.part + r) * D + 16 * d + 4 * g) = v;
       else cache_out4(a, (int64_t)(it.q0 + t) * a.out_row + head * D + 16 * d + 4 * g, v);
     }
-  }
+  };
+  static_assert(RB <= 2, "a pair of buffers for each block");
+  merge(std::integral_constant<int, 0>{});
+  if constexpr (RB == 2) merge(std::integral_constant<int, 1>{});
 }
 
 // Up to kFewRows rows: 16 or 32, two workgroups a CU.
 template <int D, bool QF16, bool F8>
 __global__ __launch_bounds__(64 * kFewWaves, 2) void cache_few_kernel(CacheAttnArgs a) {
-  __shared__ CacheLds<D> lds;
-  if (a.items[blockIdx.x].nr <= 16) cache_rows_body<D, QF16, F8, 1>(a, lds);
-  else cache_rows_body<D, QF16, F8, 2>(a, lds);
+  // an array for each buffer: a read of one does not wait for the DMA into another
+  __shared__ __attribute__((aligned(1024))) char K0[kFewWaves * kFewTile * D], V0[kFewWaves * kFewTile * D];
+  __shared__ __attribute__((aligned(1024))) char K1[kFewWaves * kFewTile * D], V1[kFewWaves * kFewTile * D];
+  __shared__ __attribute__((aligned(16))) float scales[kFewWaves * 3 * kFewTile];
+  __shared__ float2 refs[kFewWaves * kFewRows];
+  if (a.items[blockIdx.x].nr <= 16)
+    cache_rows_body<D, QF16, F8, 1>(a, (lds_t)K0, (lds_t)V0, (lds_t)K1, (lds_t)V1, scales, refs);
+  else
+    cache_rows_body<D, QF16, F8, 2>(a, (lds_t)K0, (lds_t)V0, (lds_t)K1, (lds_t)V1, scales, refs);
 }
+
+// Items of up to 128 rows, 32 a wave: chunks, and trees of more rows. Tiles of 64 keys as f16 in
+// LDS, converted once for all rows: the next tile's codes come through registers while this
+// one is used, and go into the other buffer behind it. Products as packed_kernel's.
+template <int D, bool QF16, bool F8>
+__global__ __launch_bounds__(256, 2) void cache_tile_kernel(CacheAttnArgs a) {
+  constexpr int TB = kPackTile * D * 2, CH = D / 16, RPI = 256 / CH, NI = kPackTile / RPI;
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  __shared__ __attribute__((aligned(1024))) char K0[TB], V0[TB], K1[TB], V1[TB];
+  __shared__ __attribute__((aligned(16))) float S0[3 * kPackTile], S1[3 * kPackTile];
+  const CacheItem it = a.items[blockIdx.x];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kh = lane >> 5, w0 = 32 * wave;
+  PackedArgs pa{};
+  pa.q = a.q;
+  pa.out = a.out;
+  pa.part_o = a.part_o;
+  pa.part_ml = a.part_ml;
+  pa.q_row = a.q_row;
+  pa.out_row = a.out_row;
+  pa.out_lo = a.out_lo;
+  pa.G = a.G;
+  pa.out_form = a.out_form;
+  const PackedItem pit{it.q0, 0, it.nk, it.shift, it.r0, it.nr, it.kv_lo, it.kv_hi, it.kvh, it.part};
+  const uint32_t* table = a.pages + (int64_t)it.seq * a.max_pages;
+  const int kat = pack_k_at<D>(lane & 31, kh), vat = pack_v_at<D>(lane);
+
+  // A thread's chunk of 16 codes of rows p, p + RPI of a tile; the first wave's key for scales.
+  const int p = tid / CH, c = tid % CH;
+  u4 rk[NI], rv[NI];
+  uint32_t page[NI], key_page = 0;
+  float ks = 0.f, vs = 1.f;
+  const auto row_of = [&](int pos, uint32_t pg) {
+    return (int64_t)(((pg * (uint32_t)a.c.Hkv + (uint32_t)it.kvh) << a.c.bshift) + (uint32_t)(pos & ((1 << a.c.bshift) - 1)));
+  };
+  const auto pages = [&](int t0) {
+#pragma unroll
+    for (int n = 0; n < NI; n++) page[n] = table[min(t0 + n * RPI + p, it.kv_hi - 1) >> a.c.bshift];
+    if (tid < kPackTile) key_page = table[min(t0 + tid, it.kv_hi - 1) >> a.c.bshift];
+  };
+  // Past the item's keys: its last one.
+  const auto fetch = [&](int t0) {
+#pragma unroll
+    for (int n = 0; n < NI; n++) {
+      const int64_t at = row_of(min(t0 + n * RPI + p, it.kv_hi - 1), page[n]) * D + 16 * c;
+      rk[n] = *(const u4*)(a.c.k + at);
+      rv[n] = *(const u4*)(a.c.v + at);
+    }
+    if (tid < kPackTile) {
+      const int64_t at = row_of(min(t0 + tid, it.kv_hi - 1), key_page);
+      ks = a.c.ks[at];
+      vs = a.c.vs[at];
+    }
+  };
+  const auto put = [&](lds_t K, lds_t V, float* S) {
+    typedef __attribute__((address_space(3))) half8_t* h8;
+#pragma unroll
+    for (int n = 0; n < NI; n++) {
+      const int r = n * RPI + p;
+      *(h8)(K + r * 2 * D + 16 * ((2 * c) ^ pack_k_swz<D>(r))) = cache_half8<F8>(rk[n][0], rk[n][1]);
+      *(h8)(K + r * 2 * D + 16 * ((2 * c + 1) ^ pack_k_swz<D>(r))) = cache_half8<F8>(rk[n][2], rk[n][3]);
+      *(h8)(V + r * 2 * D + 16 * ((2 * c) ^ pack_v_swz<D>(r))) = cache_half8<F8>(rv[n][0], rv[n][1]);
+      *(h8)(V + r * 2 * D + 16 * ((2 * c + 1) ^ pack_v_swz<D>(r))) = cache_half8<F8>(rv[n][2], rv[n][3]);
+    }
+    if (tid < kPackTile) {
+      const KeyScales s = cache_scales(ks, vs, a.qscale);
+      S[tid] = s.a;
+      S[kPackTile + tid] = s.b;
+      S[2 * kPackTile + tid] = s.inv;
+    }
+  };
+  pages(it.kv_lo);
+  fetch(it.kv_lo);
+  if (it.kv_lo + kPackTile < it.kv_hi) pages(it.kv_lo + kPackTile);
+  PackRows<D, QF16> w;
+  w.init(pa, pit, w0, lane);
+  const int tok = (it.r0 + (w.r < it.nr ? w.r : 0)) / a.G;
+  const uint64_t mask = it.tree ? a.masks[it.q0 + tok] : 0;
+  // the first position that some row of the wave may not see, the last that some row may
+  const int partly = it.tree ? it.shift : (it.r0 + w0) / a.G + it.shift + 1;
+  const int whi = w0 < it.nr ? (it.r0 + min(w0 + 32, it.nr) - 1) / a.G + it.shift : -1;
+  put((lds_t)K0, (lds_t)V0, S0);
+  __syncthreads();
+
+  const auto tile = [&](int t0, lds_t K, lds_t V, const float* S, lds_t Kn, lds_t Vn, float* Sn) {
+    const bool more = t0 + kPackTile < it.kv_hi;
+    if (more) {
+      fetch(t0 + kPackTile);
+      if (t0 + 2 * kPackTile < it.kv_hi) pages(t0 + 2 * kPackTile);
+    }
+    if (t0 <= whi) {
+      float16_t sc[2];
+      pack_scores(w, K, kat, sc);
+#pragma unroll
+      for (int x = 0; x < 8; x++) {
+        const float4_t ka = *(const float4_t*)(S + 8 * x + 4 * kh);
+        const float4_t kb = *(const float4_t*)(S + kPackTile + 8 * x + 4 * kh);
+#pragma unroll
+        for (int e = 0; e < 4; e++) sc[x >> 2][4 * (x & 3) + e] = fmaf(sc[x >> 2][4 * (x & 3) + e], ka[e], kb[e]);
+      }
+      if (t0 + kPackTile > partly || t0 + kPackTile > it.kv_hi) {
+#pragma unroll
+        for (int pb = 0; pb < 2; pb++) {
+          const uint32_t vis = cache_visible(it, tok, mask, t0 + 32 * pb) >> (4 * kh);
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            if (!(vis >> (8 * (i >> 2) + (i & 3)) & 1)) sc[pb][i] = -INFINITY;
+        }
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int pb = 0; pb < 2; pb++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) top = fmaxf(top, sc[pb][i]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const bool need = top > w.m + kCacheTop;
+      if (__builtin_amdgcn_ballot_w64(need)) {
+        const float mnew = need ? (fabsf(top) > kCacheFar ? top : top - kCacheLift) : w.m;
+        const float alpha = __builtin_amdgcn_exp2f(w.m - mnew);
+        w.l *= alpha;
+#pragma unroll
+        for (int db = 0; db < D / 32; db++) w.o[db] *= alpha;
+        w.m = mnew;
+      }
+      float l[2] = {};
+#pragma unroll
+      for (int u = 0; u < 4; u++) {
+        half8_t ph, pl;
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+          const float4_t inv = *(const float4_t*)(S + 2 * kPackTile + 16 * u + 8 * y + 4 * kh);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float x = __builtin_amdgcn_exp2f(sc[u >> 1][8 * (u & 1) + 4 * y + e] - w.m);
+            const half_t h = (half_t)x;
+            ph[4 * y + e] = h;
+            if (!QF16) pl[4 * y + e] = (half_t)(x - (float)h);
+            l[y] = fmaf(x, inv[e], l[y]);
+          }
+        }
+#pragma unroll
+        for (int db = 0; db < D / 32; db++) {
+          const half8_t va = pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u);
+          w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, w.o[db], 0, 0, 0);
+          if (!QF16) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl, w.o[db], 0, 0, 0);
+        }
+      }
+      w.l += l[0] + l[1];
+    }
+    if (more) put(Kn, Vn, Sn);
+    __syncthreads();
+  };
+  for (int t0 = it.kv_lo; t0 < it.kv_hi; t0 += 2 * kPackTile) {
+    tile(t0, (lds_t)K0, (lds_t)V0, S0, (lds_t)K1, (lds_t)V1, S1);
+    if (t0 + kPackTile < it.kv_hi) tile(t0 + kPackTile, (lds_t)K1, (lds_t)V1, S1, (lds_t)K0, (lds_t)V0, S0);
+  }
+  static_assert(TB == 128 * D, "a tile holds a wave's rows");
+  w.write(pa, pit, lane, (lds_t)(wave == 0 ? K0 : wave == 1 ? V0 : wave == 2 ? K1 : V1));
+}
+
 // ---------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------
@@ -376,32 +537,40 @@ void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, con
   plan = CachePlan();
   plan.H = H;
   const int G = H / Hkv;
-  std::vector<PackedItem> whole, cut;
+  std::vector<PackedItem> whole[2], cut[2];  // tiles, few rows
   int64_t q0 = 0;
   for (int s = 0; s < B; s++) {
     const int64_t rows = (int64_t)extents[s] * G;
     const int shift = lengths[s] - extents[s];
-    for (int64_t r0 = 0; r0 < rows; r0 += kFewRows) {
-      const int nr = (int)std::min<int64_t>(kFewRows, rows - r0);
+    const bool few = rows <= kFewRows;
+    const int most = few ? kFewRows : kPackRows;
+    for (int64_t r0 = 0; r0 < rows; r0 += most) {
+      const int nr = (int)std::min<int64_t>(most, rows - r0);
       const int hi = (int)std::min<int64_t>(lengths[s], (r0 + nr - 1) / G + shift + 1);
       for (int h = 0; h < Hkv; h++)  // k0: the sequence
-        whole.push_back(PackedItem{(int32_t)q0, s, lengths[s], shift, (int32_t)r0, nr, 0, hi, h, -1});
+        whole[few].push_back(PackedItem{(int32_t)q0, s, lengths[s], shift, (int32_t)r0, nr, 0, hi, h, -1});
     }
     q0 += extents[s];
   }
   plan.tq = q0;
   PackedPlan merges;
-  pack_cut(whole, kFewTile * kFewWaves, 2, ncu, PackRate{1.8 * D / 128.0, 0.7}, cut, merges);
+  const double dims = D / 128.0;
+  pack_cut(whole[0], kPackTile, 4, ncu, q_f16 ? PackRate{1.6 * dims, 0.6} : PackRate{2.2 * dims, 0.55}, cut[0], merges);
+  pack_cut(whole[1], kFewTile * kFewWaves, 2, ncu, PackRate{1.8 * dims, 0.7}, cut[1], merges);
   plan.merges = std::move(merges.merges);
   plan.part_rows = merges.part_rows;
-  plan.items.reserve(cut.size());
-  for (const PackedItem& p : cut)
-    plan.items.push_back(CacheItem{p.q0, p.k0, p.nk, p.shift, p.r0, p.nr, p.kv_lo, p.kv_hi, p.kvh, p.part,
-                                   tree && tree[p.k0] ? 1 : 0, 0});
+  plan.tiles = (int)cut[0].size();
+  plan.items.reserve(cut[0].size() + cut[1].size());
+  for (const auto& c : cut)
+    for (const PackedItem& p : c)
+      plan.items.push_back(CacheItem{p.q0, p.k0, p.nk, p.shift, p.r0, p.nr, p.kv_lo, p.kv_hi, p.kvh, p.part,
+                                     tree && tree[p.k0] ? 1 : 0, 0});
 }
 
 template <int D, bool QF16, bool F8>
 static void cache_attention_launch(CacheAttnArgs a, hipStream_t st) {
+  if (a.tiles) hipLaunchKernelGGL((cache_tile_kernel<D, QF16, F8>), dim3(a.tiles), dim3(256), 0, st, a);
+  a.items += a.tiles;
   if (a.few) hipLaunchKernelGGL((cache_few_kernel<D, QF16, F8>), dim3(a.few), dim3(64 * kFewWaves), 0, st, a);
 }
 template <int D>
