@@ -412,7 +412,10 @@ int tgohip_cache_plan(tgohip_ctx* c, const tgohip_cache* cache, int B, const int
     Stager sg;
     sg.add(plan.items.data(), plan.items.size() * sizeof(CacheItem));
     p.merges_off = sg.add(plan.merges.data(), plan.merges.size() * sizeof(PackedMerge));
-    p.pages_off = sg.add(pages, (size_t)B * max_pages * sizeof(uint32_t));
+    // the kernels' table: the row, in a layer, of a page's first position of head 0
+    std::vector<uint32_t> rows(pages, pages + (size_t)B * max_pages);
+    for (uint32_t& x : rows) x *= (uint32_t)(Hkv * cache->block);
+    p.pages_off = sg.add(rows.data(), rows.size() * sizeof(uint32_t));
     p.masks_off = sg.add(masks.data(), masks.size() * sizeof(uint64_t));
     if (plan.part_rows) rc = p.part.ensure((size_t)plan.part_rows * (cache->head_dim + 4) * sizeof(float));
     if (!rc) rc = sg.upload(c, p.meta);
@@ -507,6 +510,7 @@ int tgohip_cache_attention(tgohip_ctx* c, int handle, const tgohip_cache* cache,
     a.out_form = out_dtype == TGOHIP_F32 ? OUT_F32 : out_dtype == TGOHIP_F16 ? OUT_F16 : OUT_X2;
     a.q_f16 = p->q_f16;
     a.tiles = pl.tiles;
+    a.tile_rows = pl.tile_rows;
     a.few = p->items - pl.tiles;
     a.nmerges = p->nmerges;
     a.qscale = scale * 1.4426950408889634f;

@@ -53,18 +53,30 @@ __device__ __forceinline__ half8_t cache_half8(uint32_t a, uint32_t b) {
   return half8_t{r[0][0], r[0][1], r[1][0], r[1][1], r[2][0], r[2][1], r[3][0], r[3][1]};
 }
 
-// What a key's scales are in the softmax: a_k, b_k and 1 / v_scale_k. A value row that
-// stands for NaN makes its key's score NaN.
+// What a key's scales are in the softmax: a_k, b_k / a_k and 1 / v_scale_k. The products
+// accumulate onto b_k / a_k, so that one multiply-add makes a term's exponent of them,
+// a_k (b_k / a_k + S_k) - m. A row that stands for NaN makes its key's start NaN, not a_k:
+// a masked score, -inf by then, stays so.
 struct KeyScales {
-  float a, b, inv;
+  float a, start, inv;
 };
 __device__ __forceinline__ KeyScales cache_scales(float ks, float vs, float qscale) {
   KeyScales r;
   const float v = fminf(fmaxf(vs, kScaleLeast), kScaleMost);
-  r.a = vs == vs ? ks * qscale : NAN;
-  r.b = __builtin_amdgcn_logf(v);
-  r.inv = 1.0f / v;
+  r.a = fminf(fmaxf(ks, kScaleLeast), kScaleMost) * qscale;
+  r.start = ks == ks && vs == vs ? __builtin_amdgcn_logf(v) * __builtin_amdgcn_rcpf(r.a) : NAN;
+  r.inv = __builtin_amdgcn_rcpf(v);
   return r;
+}
+
+// What two terms lack as f16: an exact difference each (one instruction that reads the half
+// as it is; the compiler makes it a conversion and a subtraction), rounded.
+typedef float float2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ half2_t cache_rest2(float2_t p, half2_t h) {
+  float2_t r;
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(r[0]) : "v"(h), "v"(p[0]));
+  asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r[1]) : "v"(h), "v"(p[1]));
+  return __builtin_convertvector(r, half2_t);
 }
 
 template <bool QF16>
@@ -146,13 +158,14 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, lds_t K0
   const lds_t Kw[2] = {K0 + wave * TB, K1 + wave * TB}, Vw[2] = {V0 + wave * TB, V1 + wave * TB};
   float* mine = scales + wave * 3 * kFewTile;
   const uint32_t* table = a.pages + (int64_t)it.seq * a.max_pages;
+  const uint32_t head_row = (uint32_t)it.kvh << a.c.bshift;
   const int first = it.kv_lo + wave * kFewTile, step = kFewWaves * kFewTile;
 
   // The row of the lane's key (lane % 32) of the tile at t0; past the item's keys its last one.
   const auto key_page = [&](int t0) { return table[min(t0 + (lane & 31), it.kv_hi - 1) >> a.c.bshift]; };
   const auto key_row = [&](int t0, uint32_t page) {
     const int p = min(t0 + (lane & 31), it.kv_hi - 1);
-    return (int)(((page * (uint32_t)a.c.Hkv + (uint32_t)it.kvh) << a.c.bshift) + (uint32_t)(p & ((1 << a.c.bshift) - 1)));
+    return (int)(page + head_row + (uint32_t)(p & ((1 << a.c.bshift) - 1)));
   };
   const auto dma = [&](int row, lds_t K, lds_t V) {
 #pragma unroll
@@ -208,7 +221,7 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, lds_t K0
     const KeyScales sk = cache_scales(ks, vs, a.qscale);
     if (lane < 32) {
       mine[lane] = sk.a;
-      mine[kFewTile + lane] = sk.b;
+      mine[kFewTile + lane] = sk.start;
       mine[2 * kFewTile + lane] = sk.inv;
     }
     if (t0 + step < it.kv_hi) {
@@ -224,7 +237,7 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, lds_t K0
 #pragma unroll
     for (int kb = 0; kb < 2; kb++) {
 #pragma unroll
-      for (int b = 0; b < RB; b++) sc[b][kb] = float4_t{};
+      for (int b = 0; b < RB; b++) sc[b][kb] = *(const float4_t*)(mine + kFewTile + 16 * kb + 4 * g);
       const int r = 16 * kb + l16;
 #pragma unroll
       for (int h = 0; h < D / 64; h++) {
@@ -245,20 +258,25 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, lds_t K0
     half8_t ph[RB], pl[RB];
 #pragma unroll
     for (int b = 0; b < RB; b++) {
-      const uint32_t vis = masked ? cache_visible(it, tok[b], mask[b], t0) >> (4 * g) : ~0u;
-      float top = -INFINITY;
+      float4_t ka[2];
 #pragma unroll
       for (int kb = 0; kb < 2; kb++) {
-        const float4_t ka = *(const float4_t*)(mine + 16 * kb + 4 * g);
-        const float4_t kv = *(const float4_t*)(mine + kFewTile + 16 * kb + 4 * g);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          float t = fmaf(sc[b][kb][i], ka[i], kv[i]);
-          if (masked && !(vis >> (16 * kb + i) & 1)) t = -INFINITY;
-          sc[b][kb][i] = t;
-          top = fmaxf(top, t);
-        }
+        ka[kb] = *(const float4_t*)(mine + 16 * kb + 4 * g);
+        sc[b][kb] *= ka[kb];
       }
+      if (masked) {
+        const uint32_t vis = cache_visible(it, tok[b], mask[b], t0) >> (4 * g);
+#pragma unroll
+        for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (!(vis >> (16 * kb + i) & 1)) sc[b][kb][i] = -INFINITY;
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) top = fmaxf(top, sc[b][kb][i]);
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
       const bool need = top > m[b] + kCacheTop;
@@ -274,12 +292,18 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, lds_t K0
       for (int kb = 0; kb < 2; kb++) {
         const float4_t inv = *(const float4_t*)(mine + 2 * kFewTile + 16 * kb + 4 * g);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float p = __builtin_amdgcn_exp2f(sc[b][kb][i] - m[b]);
-          const half_t h = (half_t)p;
-          ph[b][4 * kb + i] = h;
-          if (!QF16) pl[b][4 * kb + i] = (half_t)(p - (float)h);
-          l[b] = fmaf(p, inv[i], l[b]);
+        for (int i = 0; i < 4; i += 2) {
+          const float2_t p = {__builtin_amdgcn_exp2f(sc[b][kb][i] - m[b]), __builtin_amdgcn_exp2f(sc[b][kb][i + 1] - m[b])};
+          const half2_t h = __builtin_convertvector(p, half2_t);
+          ph[b][4 * kb + i] = h[0];
+          ph[b][4 * kb + i + 1] = h[1];
+          if (!QF16) {
+            const half2_t r = cache_rest2(p, h);
+            pl[b][4 * kb + i] = r[0];
+            pl[b][4 * kb + i + 1] = r[1];
+          }
+          l[b] = fmaf(p[0], inv[i], l[b]);
+          l[b] = fmaf(p[1], inv[i + 1], l[b]);
         }
       }
     }
@@ -369,12 +393,13 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void cache_few_kernel(CacheAttnA
     cache_rows_body<D, QF16, F8, 2>(a, (lds_t)K0, (lds_t)V0, (lds_t)K1, (lds_t)V1, scales, refs);
 }
 
-// Items of up to 128 rows, 32 a wave: chunks, and trees of more rows. Tiles of 64 keys as f16 in
-// LDS, converted once for all rows: the next tile's codes come through registers while this
-// one is used, and go into the other buffer behind it. Products as packed_kernel's.
-template <int D, bool QF16, bool F8>
-__global__ __launch_bounds__(256, 2) void cache_tile_kernel(CacheAttnArgs a) {
-  constexpr int TB = kPackTile * D * 2, CH = D / 16, RPI = 256 / CH, NI = kPackTile / RPI;
+// Items of up to 32 WAVES rows, 32 a wave: chunks, and trees of more rows. Tiles of 64 keys as
+// f16 in LDS, converted once for all rows: the next tile's codes come through registers while
+// this one is used, and go into the other buffer behind it. Products as packed_kernel's.
+template <int D, bool QF16, bool F8, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void cache_tile_kernel(CacheAttnArgs a) {
+  constexpr int TB = kPackTile * D * 2, CH = D / 16, ROWS = 64 * WAVES / CH;
+  constexpr int RPI = ROWS < kPackTile ? ROWS : kPackTile, NI = kPackTile / RPI;  // with D 64 and 8 waves some idle
   typedef uint32_t u4 __attribute__((ext_vector_type(4)));
   __shared__ __attribute__((aligned(1024))) char K0[TB], V0[TB], K1[TB], V1[TB];
   __shared__ __attribute__((aligned(16))) float S0[3 * kPackTile], S1[3 * kPackTile];
@@ -393,15 +418,16 @@ __global__ __launch_bounds__(256, 2) void cache_tile_kernel(CacheAttnArgs a) {
   pa.out_form = a.out_form;
   const PackedItem pit{it.q0, 0, it.nk, it.shift, it.r0, it.nr, it.kv_lo, it.kv_hi, it.kvh, it.part};
   const uint32_t* table = a.pages + (int64_t)it.seq * a.max_pages;
+  const uint32_t head_row = (uint32_t)it.kvh << a.c.bshift;
   const int kat = pack_k_at<D>(lane & 31, kh), vat = pack_v_at<D>(lane);
 
   // A thread's chunk of 16 codes of rows p, p + RPI of a tile; the first wave's key for scales.
-  const int p = tid / CH, c = tid % CH;
+  const int p = min(tid / CH, kPackTile - 1), c = tid % CH;
   u4 rk[NI], rv[NI];
   uint32_t page[NI], key_page = 0;
   float ks = 0.f, vs = 1.f;
   const auto row_of = [&](int pos, uint32_t pg) {
-    return (int64_t)(((pg * (uint32_t)a.c.Hkv + (uint32_t)it.kvh) << a.c.bshift) + (uint32_t)(pos & ((1 << a.c.bshift) - 1)));
+    return (int64_t)(pg + head_row + (uint32_t)(pos & ((1 << a.c.bshift) - 1)));
   };
   const auto pages = [&](int t0) {
 #pragma unroll
@@ -435,7 +461,7 @@ __global__ __launch_bounds__(256, 2) void cache_tile_kernel(CacheAttnArgs a) {
     if (tid < kPackTile) {
       const KeyScales s = cache_scales(ks, vs, a.qscale);
       S[tid] = s.a;
-      S[kPackTile + tid] = s.b;
+      S[kPackTile + tid] = s.start;
       S[2 * kPackTile + tid] = s.inv;
     }
   };
@@ -459,63 +485,130 @@ __global__ __launch_bounds__(256, 2) void cache_tile_kernel(CacheAttnArgs a) {
       if (t0 + 2 * kPackTile < it.kv_hi) pages(t0 + 2 * kPackTile);
     }
     if (t0 <= whi) {
+      // S^T onto where each key's starts, in the lane's order of keys: 32 pb + 8 (i / 4) + 4 kh + i % 4
       float16_t sc[2];
-      pack_scores(w, K, kat, sc);
+      const auto scores = [&] {
 #pragma unroll
-      for (int x = 0; x < 8; x++) {
-        const float4_t ka = *(const float4_t*)(S + 8 * x + 4 * kh);
-        const float4_t kb = *(const float4_t*)(S + kPackTile + 8 * x + 4 * kh);
+        for (int x = 0; x < 8; x++) {
+          const float4_t st = *(const float4_t*)(S + kPackTile + 8 * x + 4 * kh);
 #pragma unroll
-        for (int e = 0; e < 4; e++) sc[x >> 2][4 * (x & 3) + e] = fmaf(sc[x >> 2][4 * (x & 3) + e], ka[e], kb[e]);
-      }
-      if (t0 + kPackTile > partly || t0 + kPackTile > it.kv_hi) {
-#pragma unroll
-        for (int pb = 0; pb < 2; pb++) {
-          const uint32_t vis = cache_visible(it, tok, mask, t0 + 32 * pb) >> (4 * kh);
-#pragma unroll
-          for (int i = 0; i < 16; i++)
-            if (!(vis >> (8 * (i >> 2) + (i & 3)) & 1)) sc[pb][i] = -INFINITY;
+          for (int e = 0; e < 4; e++) sc[x >> 2][4 * (x & 3) + e] = st[e];
         }
-      }
-      float top = -INFINITY;
 #pragma unroll
-      for (int pb = 0; pb < 2; pb++)
+        for (int s = 0; s < D / 16; s++) {
+          half8_t ka[2];
 #pragma unroll
-        for (int i = 0; i < 16; i++) top = fmaxf(top, sc[pb][i]);
-      top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const bool need = top > w.m + kCacheTop;
-      if (__builtin_amdgcn_ballot_w64(need)) {
+          for (int pb = 0; pb < 2; pb++) ka[pb] = pack_k_frag(K, (kat ^ (32 * s)) + 64 * D * pb);
+#pragma unroll
+          for (int pb = 0; pb < 2; pb++) sc[pb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[pb], w.qh[s], sc[pb], 0, 0, 0);
+          if (!QF16) {
+#pragma unroll
+            for (int pb = 0; pb < 2; pb++)
+              sc[pb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[pb], w.ql[QF16 ? 0 : s], sc[pb], 0, 0, 0);
+            if (s % 2) __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+        if (t0 + kPackTile > partly || t0 + kPackTile > it.kv_hi) {
+#pragma unroll
+          for (int pb = 0; pb < 2; pb++) {
+            const uint32_t vis = cache_visible(it, tok, mask, t0 + 32 * pb) >> (4 * kh);
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+              if (!(vis >> (8 * (i >> 2) + (i & 3)) & 1)) sc[pb][i] = -INFINITY;
+          }
+        }
+      };
+      scores();
+      __builtin_amdgcn_sched_barrier(0);
+      const auto largest = [&] {  // of the row, not yet scaled scores in sc
+        float top = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+          const float4_t ka = *(const float4_t*)(S + 8 * x + 4 * kh);
+#pragma unroll
+          for (int e = 0; e < 4; e++) top = fmaxf(top, sc[x >> 2][4 * (x & 3) + e] * ka[e]);
+        }
+        return fmaxf(top, __shfl_xor(top, 32, 64));
+      };
+      const auto raise = [&](float top, bool need) {
         const float mnew = need ? (fabsf(top) > kCacheFar ? top : top - kCacheLift) : w.m;
         const float alpha = __builtin_amdgcn_exp2f(w.m - mnew);
         w.l *= alpha;
 #pragma unroll
         for (int db = 0; db < D / 32; db++) w.o[db] *= alpha;
         w.m = mnew;
-      }
-      float l[2] = {};
-#pragma unroll
-      for (int u = 0; u < 4; u++) {
-        half8_t ph, pl;
+      };
+      // Step u's eight terms, their share of the sum on l.
+      const auto terms = [&](int u, half8_t& ph, half8_t& pl, float& l, float& most) {
 #pragma unroll
         for (int y = 0; y < 2; y++) {
+          const float4_t ka = *(const float4_t*)(S + 16 * u + 8 * y + 4 * kh);
           const float4_t inv = *(const float4_t*)(S + 2 * kPackTile + 16 * u + 8 * y + 4 * kh);
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float x = __builtin_amdgcn_exp2f(sc[u >> 1][8 * (u & 1) + 4 * y + e] - w.m);
-            const half_t h = (half_t)x;
-            ph[4 * y + e] = h;
-            if (!QF16) pl[4 * y + e] = (half_t)(x - (float)h);
-            l[y] = fmaf(x, inv[e], l[y]);
+          for (int e = 0; e < 4; e += 2) {
+            const int i = 8 * (u & 1) + 4 * y + e;
+            float2_t x;
+#pragma unroll
+            for (int f = 0; f < 2; f++) x[f] = __builtin_amdgcn_exp2f(fmaf(sc[u >> 1][i + f], ka[e + f], -w.m));
+            const half2_t h = __builtin_convertvector(x, half2_t);
+            ph[4 * y + e] = h[0];
+            ph[4 * y + e + 1] = h[1];
+            if (QF16) {
+              most = fmaxf(fmaxf(most, x[0]), x[1]);
+            } else {
+              const half2_t r = cache_rest2(x, h);
+              pl[4 * y + e] = r[0];
+              pl[4 * y + e + 1] = r[1];
+            }
+            l = fmaf(x[0], inv[e], l);
+            l = fmaf(x[1], inv[e + 1], l);
+          }
+        }
+      };
+      if constexpr (QF16) {
+        // All terms by the reference as it is; only where one of a row's has passed f16's range (its
+        // first tile, or a key far above the ones before) is the row's largest looked for.
+        half8_t ph[4], none;
+        float l[4] = {}, most = 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; u++) terms(u, ph[u], none, l[u], most);
+        __builtin_amdgcn_sched_barrier(0);
+        const float limit = 32768.f;  // 2^kCacheTop
+        if (__builtin_amdgcn_ballot_w64(most > limit)) {
+          const bool need = fmaxf(most, __shfl_xor(most, 32, 64)) > limit;
+          raise(largest(), need);
+#pragma unroll
+          for (int u = 0; u < 4; u++) {
+            l[u] = 0.f;
+            terms(u, ph[u], none, l[u], most);
           }
         }
 #pragma unroll
-        for (int db = 0; db < D / 32; db++) {
-          const half8_t va = pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u);
-          w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, ph, w.o[db], 0, 0, 0);
-          if (!QF16) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pl, w.o[db], 0, 0, 0);
+        for (int u = 0; u < 4; u++)
+#pragma unroll
+          for (int db = 0; db < D / 32; db++)
+            w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u), ph[u], w.o[db], 0, 0, 0);
+        w.l += (l[0] + l[1]) + (l[2] + l[3]);
+      } else {
+        const float top = largest();
+        const bool need = top > w.m + kCacheTop;
+        if (__builtin_amdgcn_ballot_w64(need)) raise(top, need);
+        // pairs go step by step: all at once would not fit the registers beside the queries'
+        float l[2] = {}, most;
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+          half8_t ph, pl;
+          terms(u, ph, pl, l[u & 1], most);
+          half8_t va[D / 32];
+#pragma unroll
+          for (int db = 0; db < D / 32; db++) va[db] = pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u);
+#pragma unroll
+          for (int db = 0; db < D / 32; db++) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[db], ph, w.o[db], 0, 0, 0);
+#pragma unroll
+          for (int db = 0; db < D / 32; db++) w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[db], pl, w.o[db], 0, 0, 0);
         }
+        w.l += l[0] + l[1];
       }
-      w.l += l[0] + l[1];
     }
     if (more) put(Kn, Vn, Sn);
     __syncthreads();
@@ -525,7 +618,13 @@ __global__ __launch_bounds__(256, 2) void cache_tile_kernel(CacheAttnArgs a) {
     if (t0 + kPackTile < it.kv_hi) tile(t0 + kPackTile, (lds_t)K1, (lds_t)V1, S1, (lds_t)K0, (lds_t)V0, S0);
   }
   static_assert(TB == 128 * D, "a tile holds a wave's rows");
-  w.write(pa, pit, lane, (lds_t)(wave == 0 ? K0 : wave == 1 ? V0 : wave == 2 ? K1 : V1));
+  const int turn = wave % 4;
+  const lds_t buf = (lds_t)(turn == 0 ? K0 : turn == 1 ? V0 : turn == 2 ? K1 : V1);
+  if (wave < 4) w.write(pa, pit, lane, buf);
+  if (WAVES > 4) {
+    __syncthreads();
+    if (wave >= 4) w.write(pa, pit, lane, buf);
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -538,12 +637,21 @@ void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, con
   plan.H = H;
   const int G = H / Hkv;
   std::vector<PackedItem> whole[2], cut[2];  // tiles, few rows
+  // f16 queries in blocks of 256 rows where that pads little
+  int64_t narrow = 0, wide = 0;
+  for (int s = 0; s < B; s++) {
+    const int64_t rows = (int64_t)extents[s] * G;
+    if (rows <= kFewRows) continue;
+    narrow += (rows + 127) / 128 * 128 * lengths[s];
+    wide += (rows + 255) / 256 * 256 * lengths[s];
+  }
+  plan.tile_rows = q_f16 && 10 * wide <= 11 * narrow ? 256 : 128;
   int64_t q0 = 0;
   for (int s = 0; s < B; s++) {
     const int64_t rows = (int64_t)extents[s] * G;
     const int shift = lengths[s] - extents[s];
     const bool few = rows <= kFewRows;
-    const int most = few ? kFewRows : kPackRows;
+    const int most = few ? kFewRows : plan.tile_rows;
     for (int64_t r0 = 0; r0 < rows; r0 += most) {
       const int nr = (int)std::min<int64_t>(most, rows - r0);
       const int hi = (int)std::min<int64_t>(lengths[s], (r0 + nr - 1) / G + shift + 1);
@@ -555,7 +663,7 @@ void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, con
   plan.tq = q0;
   PackedPlan merges;
   const double dims = D / 128.0;
-  pack_cut(whole[0], kPackTile, 4, ncu, q_f16 ? PackRate{1.6 * dims, 0.6} : PackRate{2.2 * dims, 0.55}, cut[0], merges);
+  pack_cut(whole[0], kPackTile, 12, ncu, q_f16 ? PackRate{1.6 * dims, 0.6} : PackRate{2.2 * dims, 0.55}, cut[0], merges);
   pack_cut(whole[1], kFewTile * kFewWaves, 2, ncu, PackRate{1.8 * dims, 0.7}, cut[1], merges);
   plan.merges = std::move(merges.merges);
   plan.part_rows = merges.part_rows;
@@ -569,7 +677,11 @@ void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, con
 
 template <int D, bool QF16, bool F8>
 static void cache_attention_launch(CacheAttnArgs a, hipStream_t st) {
-  if (a.tiles) hipLaunchKernelGGL((cache_tile_kernel<D, QF16, F8>), dim3(a.tiles), dim3(256), 0, st, a);
+  if (a.tiles && a.tile_rows == 256) {
+    if constexpr (QF16) hipLaunchKernelGGL((cache_tile_kernel<D, QF16, F8, 8>), dim3(a.tiles), dim3(512), 0, st, a);
+  } else if (a.tiles) {
+    hipLaunchKernelGGL((cache_tile_kernel<D, QF16, F8, 4>), dim3(a.tiles), dim3(256), 0, st, a);
+  }
   a.items += a.tiles;
   if (a.few) hipLaunchKernelGGL((cache_few_kernel<D, QF16, F8>), dim3(a.few), dim3(64 * kFewWaves), 0, st, a);
 }

@@ -205,7 +205,7 @@ struct CachePlan {
   int H = 0;
   int64_t tq = 0;
   std::vector<CacheItem> items;  // of the tile kernel, then of the few-row kernel
-  int tiles = 0;
+  int tiles = 0, tile_rows = 0;   // rows of an item of the tile kernel: 128 or 256
   std::vector<PackedMerge> merges;
   int64_t part_rows = 0;
 };
@@ -219,12 +219,12 @@ struct CacheAttnArgs {
   void* out;
   const CacheItem* items;
   const PackedMerge* merges;
-  const uint32_t* pages;
+  const uint32_t* pages;  // the row of a page's first position (head 0)
   const uint64_t* masks;
   float *part_o, *part_ml;
   int64_t q_row, out_row, out_lo;
   int max_pages, G, out_form, q_f16;
-  int tiles, few, nmerges;
+  int tiles, tile_rows, few, nmerges;
   float qscale;  // scale * log2(e)
 };
 int cache_attention_enqueue(const CacheAttnArgs& a, hipStream_t st);
