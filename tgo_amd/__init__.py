@@ -6,6 +6,7 @@ path (model.NewBatchStep, nextStep/victim, prefix.Pool/Lease, Scheduler,
 nn.Linear, tensor.Attention). Every call goes through the C ABI; a missing or
 unbuilt library raises -- there is no CPU fallback.
 """
+import array
 import ctypes
 import os
 import struct
@@ -268,6 +269,21 @@ def u32(a):
 
 def i32(a):
     return np.ascontiguousarray(np.asarray(a, dtype=np.int32))
+
+
+def _host_slots(a):
+    """Slots as int32 on the host: what holds them, its address, their number. A list of ints goes through
+    array, 18 ns each; through numpy 28."""
+    if type(a) is list:
+        try:
+            a = array.array("i", a)
+            return (a,) + a.buffer_info()
+        except TypeError:  # no ints
+            pass
+    a = i32(a)
+    if a.ndim != 1:
+        raise TgoError(EINVAL, "slots are a list, not of shape %s" % (a.shape,))
+    return a, a.ctypes.data, a.size
 
 
 # ---------------------------------------------------------------------------
@@ -987,10 +1003,10 @@ class Context:
 
     def cache_move(self, cache, src, dst):
         """Rows of slots src[i] to slots dst[i] (host arrays) in every layer and head, all at once."""
-        a, b = i32(src), i32(dst)
-        if a.shape != b.shape or a.ndim != 1:
-            raise TgoError(EINVAL, "cache_move: %d slots to %d slots" % (a.size, b.size))
-        check(_lib.tgohip_cache_move(self.h, self._cache(cache), a.ctypes.data, b.ctypes.data, a.size))
+        (a, at, n), (b, to, m) = _host_slots(src), _host_slots(dst)
+        if n != m:
+            raise TgoError(EINVAL, "cache_move: %d slots to %d slots" % (n, m))
+        check(_lib.tgohip_cache_move(self.h, self._cache(cache), at, to, n))
 
     def cache_plan(self, cache, extents, lengths, pages, H, parents=None, q_dtype=F32, plan=0):
         """Decomposes a batch for cache_attention; returns the plan's handle. extents[b] new tokens end

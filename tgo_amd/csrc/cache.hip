@@ -100,70 +100,127 @@ bool overlap(int64_t rows, int64_t row, int64_t heads, int64_t head, int64_t d) 
   return n1 > 1 && s1 < need;
 }
 
-// The moves without those onto themselves, in an order in which a row is read before, or
-// in the same 64 as, it is written over; batches of them for a workgroup each.
+// What a slot is written by: open addressing over a power of two of at least twice the moves.
+struct Writers {
+  std::vector<int32_t> slot, move;
+  uint32_t mask;
+  explicit Writers(int n) {
+    uint32_t size = 16;
+    while (size < 2 * (uint32_t)n) size *= 2;
+    mask = size - 1;
+    slot.assign(size, -1);
+    move.resize(size);
+  }
+  uint32_t at(int32_t s) const {  // the slot's place, or the free one it would take
+    uint32_t i = (uint32_t)s * 0x9e3779b1u >> 7 & mask;
+    while (slot[i] >= 0 && slot[i] != s) i = (i + 1) & mask;
+    return i;
+  }
+};
+
+// One component's moves in an order in which a row is read before, or in the same 64 as, it
+// is written over; p: its moves, more than 64.
+int order_component(const int32_t* p, int n, const std::vector<int>& next, std::vector<int>& sorted) {
+  std::unordered_map<int, int> before;  // moves that come before one
+  for (int i = 0; i < n; i++)
+    if (next[p[i]] >= 0) before[next[p[i]]]++;
+  const auto waits = [&](int i) {
+    const auto b = before.find(i);
+    return b != before.end() && b->second > 0;
+  };
+  sorted.clear();
+  for (int i = 0; i < n; i++)
+    if (!waits(p[i])) sorted.push_back(p[i]);
+  for (size_t k = 0; k < sorted.size(); k++) {
+    const int m = next[sorted[k]];
+    if (m >= 0 && --before[m] == 0) sorted.push_back(m);
+  }
+  // What is left is the component's one cycle: it goes last, whole, in a segment of its
+  // own when it does not fit behind the others.
+  std::vector<int> cycle;
+  for (int i = 0; i < n; i++)
+    if (waits(p[i])) cycle.push_back(p[i]);
+  if (cycle.size() > (size_t)kCacheMoveSeg)
+    return refuse("cache_move: a cycle of " + str((int64_t)cycle.size()) + " slots; up to " + str(kCacheMoveSeg));
+  if (!cycle.empty())
+    while (sorted.size() % kCacheMoveSeg + cycle.size() > (size_t)kCacheMoveSeg)
+      sorted.push_back(sorted.back());  // again: reads what it read, writes what it wrote
+  sorted.insert(sorted.end(), cycle.begin(), cycle.end());
+  return 0;
+}
+
+// The moves without those onto themselves, in batches for a workgroup each: moves that
+// depend on each other stay in one. Up to 64 of a batch are all read before any is
+// written, in whatever order they stand.
 int order_moves(const int32_t* from, const int32_t* to, int n, std::vector<int32_t>& src, std::vector<int32_t>& dst,
                 std::vector<CacheMoveBatch>& batches) {
-  std::unordered_map<int32_t, int> writer;  // of a slot
-  writer.reserve((size_t)n * 2);
-  for (int i = 0; i < n; i++)
-    if (!writer.emplace(to[i], i).second)
-      return refuse("cache_move: two rows go to slot " + str(to[i]));
-  // next[i]: the move that writes what i reads, which i comes before
-  std::vector<int> next((size_t)n, -1), before((size_t)n, 0);
+  Writers w(n);
+  std::vector<int32_t> kept;
+  kept.reserve((size_t)n);
   for (int i = 0; i < n; i++) {
-    if (from[i] == to[i]) continue;
-    const auto w = writer.find(from[i]);
-    if (w == writer.end() || from[w->second] == to[w->second]) continue;
-    next[i] = w->second;
-    before[w->second]++;
+    const uint32_t at = w.at(to[i]);
+    if (w.slot[at] >= 0) return refuse("cache_move: two rows go to slot " + str(to[i]));
+    w.slot[at] = to[i];
+    w.move[at] = i;
+    if (from[i] != to[i]) kept.push_back(i);
   }
-  // Moves that depend on each other stay in one batch: components of the graph of next.
-  std::vector<int> root((size_t)n);
-  for (int i = 0; i < n; i++) root[i] = i;
+  if (kept.empty()) return 0;
+  src.reserve(kept.size());
+  dst.reserve(kept.size());
+  const auto put = [&](const int32_t* p, int count) {
+    if (batches.empty() || batches.back().n + count > kCacheMoveSeg)
+      batches.push_back(CacheMoveBatch{(int32_t)src.size(), 0});
+    batches.back().n += count;
+    for (int i = 0; i < count; i++) {
+      src.push_back(from[p[i]]);
+      dst.push_back(to[p[i]]);
+    }
+  };
+  if (kept.size() <= (size_t)kCacheMoveSeg) {
+    put(kept.data(), (int)kept.size());
+    return 0;
+  }
+  // next[i]: the move that writes what i reads, which i comes before. Its graph's components:
+  // root[i] is never behind i, so a component's root is its first move.
+  std::vector<int> next((size_t)n, -1), root((size_t)n);
+  for (const int i : kept) {
+    root[i] = i;
+    const uint32_t at = w.at(from[i]);
+    if (w.slot[at] < 0) continue;
+    const int m = w.move[at];
+    if (from[m] != to[m]) next[i] = m;
+  }
   const auto find_root = [&](int i) {
     while (root[i] != i) i = root[i] = root[root[i]];
     return i;
   };
-  for (int i = 0; i < n; i++)
-    if (next[i] >= 0) root[find_root(i)] = find_root(next[i]);
-  std::unordered_map<int, std::vector<int>> parts;
-  std::vector<int> order;  // roots as their first moves stand
-  for (int i = 0; i < n; i++) {
-    if (from[i] == to[i]) continue;
-    std::vector<int>& p = parts[find_root(i)];
-    if (p.empty()) order.push_back(find_root(i));
-    p.push_back(i);
+  for (const int i : kept) {
+    if (next[i] < 0) continue;
+    const int a = find_root(i), b = find_root(next[i]);
+    root[std::max(a, b)] = std::min(a, b);
   }
-  for (const int r : order) {
-    const std::vector<int>& p = parts[r];
-    std::vector<int> sorted;
-    sorted.reserve(p.size());
-    for (const int i : p)
-      if (!before[i]) sorted.push_back(i);
-    for (size_t k = 0; k < sorted.size(); k++) {
-      const int m = next[sorted[k]];
-      if (m >= 0 && --before[m] == 0) sorted.push_back(m);
+  // sorted by component, components as their first moves stand
+  std::vector<int32_t> count((size_t)n, 0), part(kept.size());
+  for (const int i : kept) count[find_root(i)]++;
+  int32_t sum = 0;
+  for (const int i : kept)
+    if (root[i] == i) {
+      const int32_t c = count[i];
+      count[i] = sum;
+      sum += c;
     }
-    // What is left is the component's one cycle: it goes last, whole, in a segment of its
-    // own when it does not fit behind the others.
-    std::vector<int> cycle;
-    for (const int i : p)
-      if (before[i] > 0) cycle.push_back(i);
-    if (cycle.size() > (size_t)kCacheMoveSeg)
-      return refuse("cache_move: a cycle of " + str((int64_t)cycle.size()) + " slots; up to " + str(kCacheMoveSeg));
-    if (!cycle.empty())
-      while (sorted.size() % kCacheMoveSeg + cycle.size() > (size_t)kCacheMoveSeg) {
-        sorted.push_back(sorted.back());  // again: reads what it read, writes what it wrote
-      }
-    sorted.insert(sorted.end(), cycle.begin(), cycle.end());
-    const bool fits = !batches.empty() && batches.back().n + sorted.size() <= (size_t)kCacheMoveSeg;
-    if (!fits) batches.push_back(CacheMoveBatch{(int32_t)src.size(), 0});
-    batches.back().n += (int32_t)sorted.size();
-    for (const int i : sorted) {
-      src.push_back(from[i]);
-      dst.push_back(to[i]);
+  for (const int i : kept) part[count[find_root(i)]++] = i;
+  std::vector<int> sorted;
+  for (size_t i = 0; i < part.size();) {
+    const size_t end = count[find_root(part[i])];
+    if (end - i <= (size_t)kCacheMoveSeg) {
+      put(&part[i], (int)(end - i));
+    } else {
+      const int rc = order_component(&part[i], (int)(end - i), next, sorted);
+      if (rc) return rc;
+      put(sorted.data(), (int)sorted.size());
     }
+    i = end;
   }
   return 0;
 }
@@ -324,19 +381,26 @@ int tgohip_cache_move(tgohip_ctx* c, const tgohip_cache* cache, const int32_t* f
     OnDevice on(c->device);
     if ((rc = no_capture(c, "cache_move"))) return rc;
     if (batches.empty()) return 0;
-    Stager sg;
-    const size_t o0 = sg.add(src.data(), src.size() * 4), o1 = sg.add(dst.data(), dst.size() * 4);
-    const size_t o2 = sg.add(batches.data(), batches.size() * sizeof(CacheMoveBatch));
-    if ((rc = sg.upload(c))) return rc;
     CacheMoveArgs a{};
     a.c = layer_of(cache, 0);
     a.layers = cache->layers;
     a.batches = (int)batches.size();
     a.layer_rows = layer_rows(cache);
-    a.src = sg.dev<int32_t>(c, o0);
-    a.dst = sg.dev<int32_t>(c, o1);
-    a.batch = sg.dev<CacheMoveBatch>(c, o2);
-    launch_cache_move(a, c->stream);
+    CacheMoveFew few{};
+    if (src.size() <= (size_t)kCacheMoveSeg) {
+      few.n = (int32_t)src.size();
+      std::copy(src.begin(), src.end(), few.src);
+      std::copy(dst.begin(), dst.end(), few.dst);
+    } else {
+      Stager sg;
+      const size_t o0 = sg.add(src.data(), src.size() * 4), o1 = sg.add(dst.data(), dst.size() * 4);
+      const size_t o2 = sg.add(batches.data(), batches.size() * sizeof(CacheMoveBatch));
+      if ((rc = sg.upload(c))) return rc;
+      a.src = sg.dev<int32_t>(c, o0);
+      a.dst = sg.dev<int32_t>(c, o1);
+      a.batch = sg.dev<CacheMoveBatch>(c, o2);
+    }
+    launch_cache_move(a, few, c->stream);
     TGOHIP_HIP(hipGetLastError());
     return 0;
   });

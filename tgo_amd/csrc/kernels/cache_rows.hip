@@ -332,44 +332,55 @@ void launch_cache_read(const CacheReadArgs& a, int ncu, hipStream_t st) {
 // moving
 // ---------------------------------------------------------------------------
 
-// D / 16 lanes a row, 16 bytes each.
-template <int D>
-__global__ __launch_bounds__(256) void cache_move_kernel(CacheMoveArgs a) {
-  constexpr int LPR = D / 16, PER = 256 / LPR, N = (kCacheMoveSeg + PER - 1) / PER;
-  const CacheMoveBatch b = a.batch[blockIdx.x];
+// D / 16 lanes a row, 16 bytes each, of K and of V.
+template <int D, bool INLINE>
+__global__ __launch_bounds__(256) void cache_move_kernel(CacheMoveArgs a, CacheMoveFew f) {
+  constexpr int LPR = D / 16, PER = 256 / LPR, N = kCacheMoveSeg / PER;
+  typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+  const CacheMoveBatch b = INLINE ? CacheMoveBatch{0, f.n} : a.batch[blockIdx.x];
   const int layer = blockIdx.y / a.c.Hkv, h = blockIdx.y % a.c.Hkv;
   const int64_t first = layer * a.layer_rows;
-  uint8_t* codes = (blockIdx.z ? a.c.v : a.c.k) + first * D;
-  float* scales = (blockIdx.z ? a.c.vs : a.c.ks) + first;
   const int j = threadIdx.x % LPR, g = threadIdx.x / LPR;
   for (int s0 = 0; s0 < b.n; s0 += kCacheMoveSeg) {
     const int n = min(kCacheMoveSeg, b.n - s0);
-    uint4 w[N];
-    float s[N];
+    u4 k[N], v[N];
+    float ks[N], vs[N];
     int64_t to[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
       const int m = b.start + s0 + min(g + i * PER, n - 1);
-      const int64_t from = a.c.row(a.src[m], h);
-      to[i] = a.c.row(a.dst[m], h);
-      w[i] = *(const uint4*)(codes + from * D + 16 * j);
-      s[i] = scales[from];
+      const int32_t src = INLINE ? f.src[m] : a.src[m], dst = INLINE ? f.dst[m] : a.dst[m];
+      const int64_t from = first + a.c.row(src, h);
+      to[i] = first + a.c.row(dst, h);
+      k[i] = *(const u4*)(a.c.k + from * D + 16 * j);
+      v[i] = *(const u4*)(a.c.v + from * D + 16 * j);
+      ks[i] = a.c.ks[from];
+      vs[i] = a.c.vs[from];
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; i++) {
       if (g + i * PER >= n) continue;
-      *(uint4*)(codes + to[i] * D + 16 * j) = w[i];
-      if (j == 0) scales[to[i]] = s[i];
+      *(u4*)(a.c.k + to[i] * D + 16 * j) = k[i];
+      *(u4*)(a.c.v + to[i] * D + 16 * j) = v[i];
+      if (j == 0) {
+        a.c.ks[to[i]] = ks[i];
+        a.c.vs[to[i]] = vs[i];
+      }
     }
     __syncthreads();
   }
 }
 
-void launch_cache_move(const CacheMoveArgs& a, hipStream_t st) {
-  const dim3 grid(a.batches, a.layers * a.c.Hkv, 2);
-  if (a.c.d == 128) hipLaunchKernelGGL((cache_move_kernel<128>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((cache_move_kernel<64>), grid, dim3(256), 0, st, a);
+template <int D>
+static void cache_move_launch(const CacheMoveArgs& a, const CacheMoveFew& f, hipStream_t st) {
+  if (f.n) hipLaunchKernelGGL((cache_move_kernel<D, true>), dim3(1, a.layers * a.c.Hkv), dim3(256), 0, st, a, f);
+  else hipLaunchKernelGGL((cache_move_kernel<D, false>), dim3(a.batches, a.layers * a.c.Hkv), dim3(256), 0, st, a, f);
+}
+
+void launch_cache_move(const CacheMoveArgs& a, const CacheMoveFew& f, hipStream_t st) {
+  if (a.c.d == 128) cache_move_launch<128>(a, f, st);
+  else cache_move_launch<64>(a, f, st);
 }
 
 }  // namespace tgohip

@@ -180,8 +180,7 @@ struct CacheReadArgs {
 };
 void launch_cache_read(const CacheReadArgs& a, int ncu, hipStream_t st);
 // Rows src[i] to dst[i] (slots) of every layer and head; a workgroup takes moves
-// [start, start + n) of one (layer, head, K or V), kCacheMoveSeg of them read before any
-// is written.
+// [start, start + n) of one (layer, head), kCacheMoveSeg of them read before any is written.
 constexpr int kCacheMoveSeg = 64;
 struct CacheMoveBatch {
   int32_t start, n;
@@ -193,7 +192,11 @@ struct CacheMoveArgs {
   const int32_t *src, *dst;
   const CacheMoveBatch* batch;
 };
-void launch_cache_move(const CacheMoveArgs& a, hipStream_t st);
+// Moves that fit one batch go with the kernel's arguments: n of them, 0: CacheMoveArgs's.
+struct CacheMoveFew {
+  int32_t n, src[kCacheMoveSeg], dst[kCacheMoveSeg];
+};
+void launch_cache_move(const CacheMoveArgs& a, const CacheMoveFew& f, hipStream_t st);
 
 // A work item: rows [r0, r0 + nr) of a sequence and kv head (as PackedItem's) against
 // positions [kv_lo, kv_hi). tree 0: token t sees positions up to t + shift; 1: those
