@@ -367,8 +367,8 @@ def moves(kind, n, r):
 
 
 @pytest.mark.parametrize("form,d", [("i8", 128), ("f8", 64)])
-@pytest.mark.parametrize("kind,n", [("apart", 1), ("apart", 333), ("down", 5), ("down", 64), ("down", 65), ("down", 1000),
-                                    ("up", 1000), ("up", 64), ("paths", 1), ("paths", 64), ("swaps", 100), ("spread", 200),
+@pytest.mark.parametrize("kind,n", [("apart", 1), ("apart", 333), ("apart", 480), ("apart", 481), ("down", 5), ("down", 64), ("down", 65), ("down", 1000),
+                                    ("up", 1000), ("up", 64), ("up", 65), ("paths", 1), ("paths", 64), ("paths", 200), ("swaps", 100), ("spread", 200),
                                     ("cycles", 3), ("cycle_behind_a_chain", 0), ("random", 40), ("random", 900)])
 def test_move(ctx, torch_gpu, kind, n, form, d):
     torch = torch_gpu

@@ -386,8 +386,10 @@ int tgohip_cache_move(tgohip_ctx* c, const tgohip_cache* cache, const int32_t* f
     a.layers = cache->layers;
     a.batches = (int)batches.size();
     a.layer_rows = layer_rows(cache);
-    CacheMoveFew few{};
-    if (src.size() <= (size_t)kCacheMoveSeg) {
+    CacheMoveFew few;
+    few.n = 0;
+    if (src.size() <= (size_t)kCacheMoveFew && batches.size() <= (size_t)kCacheMoveFewBatches) {
+      std::copy(batches.begin(), batches.end(), few.batch);
       few.n = (int32_t)src.size();
       std::copy(src.begin(), src.end(), few.src);
       std::copy(dst.begin(), dst.end(), few.dst);

@@ -192,10 +192,16 @@ struct CacheMoveArgs {
   const int32_t *src, *dst;
   const CacheMoveBatch* batch;
 };
-// Moves that fit one batch go with the kernel's arguments: n of them, 0: CacheMoveArgs's.
+// Up to this many moves and batches go with the kernel's arguments, which end at 4 KB; more are
+// fetched to the device first. By arguments / fetched, us a call: 448 moves of 36 layers
+// and 8 heads 16.2 / 25.0, 4 moves 5.2 / 12.
+constexpr int kCacheMoveFew = 480, kCacheMoveFewBatches = 16;
 struct CacheMoveFew {
-  int32_t n, src[kCacheMoveSeg], dst[kCacheMoveSeg];
+  int32_t n;  // 0: CacheMoveArgs's
+  CacheMoveBatch batch[kCacheMoveFewBatches];
+  int32_t src[kCacheMoveFew], dst[kCacheMoveFew];
 };
+static_assert(sizeof(CacheMoveArgs) + sizeof(CacheMoveFew) <= 4096, "a kernel's arguments");
 void launch_cache_move(const CacheMoveArgs& a, const CacheMoveFew& f, hipStream_t st);
 
 // A work item: rows [r0, r0 + nr) of a sequence and kv head (as PackedItem's) against
