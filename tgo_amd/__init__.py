@@ -949,40 +949,46 @@ class Context:
             _INT32[t.dtype] = True
         return _addr(t, what, self.device)
 
+    def _gain(self, g, what, d):
+        if _kind(g) != F32 or g.numel() != d:
+            raise TgoError(EINVAL, "cache_store: %s is float32 [%d]" % (what, d))
+        return _addr(g, what, self.device)
+
     def cache_store(self, cache, layer, slots, k, v, q=None, q_out=None, positions=None, rope=0, q_gain=None,
                     k_gain=None, eps=1e-6):
         """Writes T rows of one layer: k, v [T, kv_heads, head_dim] quantised into slots (int32 [T]), q
         [T, heads, head_dim] to q_out; q and k normed by q_gain, k_gain (float32 [head_dim]) and turned to
         positions (int32 [T]) by a rotary handle, where those are given. Any row and head strides."""
-        T, d = slots.numel(), cache.head_dim
+        T, d, dev = slots.numel(), cache.head_dim, self.device
         at = self._cache(cache)
-        ka, kr, kh, kd = _heads_view(k, "cache_store: k", self.device)
-        va, vr, vh, vd = _heads_view(v, "cache_store: v", self.device)
+        ka, kr, kh, kd = _heads_view(k, "cache_store: k", dev)
+        va, vr, vh, vd = _heads_view(v, "cache_store: v", dev)
         want = (T, cache.kv_heads, d)
-        if tuple(k.shape) != want or tuple(v.shape) != want:
+        if k.shape != want or v.shape != want:
             raise TgoError(EINVAL, "cache_store: k and v are %s and %s for %d slots and heads of the cache; %s" %
                            (tuple(k.shape), tuple(v.shape), T, want))
         qa = qr = qh = oa = orow = oh = heads = 0
         qd, od = kd, F32
         if q is not None:
-            if q_out is None or q.shape != q_out.shape or q.dim() != 3 or q.shape[0] != T or q.shape[2] != d:
+            shape = q.shape
+            if q_out is None or shape != q_out.shape or len(shape) != 3 or shape[0] != T or shape[2] != d:
                 raise TgoError(EINVAL, "cache_store: q and q_out are [%d, heads, %d] both" % (T, d))
-            qa, qr, qh, qd = _heads_view(q, "cache_store: q", self.device)
-            oa, orow, oh, od = _heads_view(q_out, "cache_store: q_out", self.device)
-            heads = q.shape[1]
+            heads = shape[1]
+            qa, qr, qh, qd = _heads_view(q, "cache_store: q", dev)
+            oa, orow, oh, od = _heads_view(q_out, "cache_store: q_out", dev)
         if kd != vd or kd != qd:
             raise TgoError(EINVAL, "cache_store: q, k and v are of one type")
-        for g, what in ((q_gain, "q_gain"), (k_gain, "k_gain")):
-            if g is not None and (_kind(g) != F32 or g.numel() != d):
-                raise TgoError(EINVAL, "cache_store: %s is float32 [%d]" % (what, d))
-        pa = 0
+        gq = gk = pa = 0
+        if q_gain is not None:
+            gq = self._gain(q_gain, "q_gain", d)
+        if k_gain is not None:
+            gk = self._gain(k_gain, "k_gain", d)
         if rope:
             if positions is None or positions.numel() != T:
                 raise TgoError(EINVAL, "cache_store: positions is int32 [%d]" % T)
             pa = self._slots(positions, "positions")
         check(_lib.tgohip_cache_store(self.h, at, layer, rope, pa, self._slots(slots, "slots"), T, _CACHE_ROWS.pack(
-            qa, ka, va, oa, qr, qh, kr, kh, vr, vh, orow, oh, _addr(q_gain, "q_gain", self.device) or 0,
-            _addr(k_gain, "k_gain", self.device) or 0, eps, heads, kd, od)))
+            qa, ka, va, oa, qr, qh, kr, kh, vr, vh, orow, oh, gq, gk, eps, heads, kd, od)))
 
     def cache_read(self, cache, layer, slots, k_out=None, v_out=None):
         """Rows of slots (int32 [T]) of one layer as values: K's to k_out, V's to v_out ([T, kv_heads, head_dim],
@@ -993,7 +999,7 @@ class Context:
                 f += 0, 0, 0
                 continue
             a, row, head, dt = _heads_view(y, "cache_read: " + what, self.device)
-            if tuple(y.shape) != (T, cache.kv_heads, cache.head_dim) or (kind is not None and dt != kind):
+            if y.shape != (T, cache.kv_heads, cache.head_dim) or (kind is not None and dt != kind):
                 raise TgoError(EINVAL, "cache_read: %s is [%d, %d, %d], both of one type" %
                                (what, T, cache.kv_heads, cache.head_dim))
             kind = dt
