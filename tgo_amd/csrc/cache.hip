@@ -575,9 +575,8 @@ int tgohip_cache_attention(tgohip_ctx* c, int handle, const tgohip_cache* cache,
     a.G = pl.H / p->Hkv;
     a.out_form = out_dtype == TGOHIP_F32 ? OUT_F32 : out_dtype == TGOHIP_F16 ? OUT_F16 : OUT_X2;
     a.q_f16 = p->q_f16;
-    a.tiles = pl.tiles;
-    a.tile_rows = pl.tile_rows;
-    a.few = p->items - pl.tiles;
+    a.nitems = p->items;
+    a.wide = pl.wide;
     a.nmerges = p->nmerges;
     a.qscale = scale * 1.4426950408889634f;
     OnDevice on(c->device);

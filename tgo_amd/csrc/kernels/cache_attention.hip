@@ -30,6 +30,7 @@ constexpr float kScaleLeast = 0x1p-40f, kScaleMost = 0x1p40f;
 constexpr int kFewTile = 32;   // keys of a wave's tile
 constexpr int kFewWaves = 4;
 constexpr int kFewRows = 32;   // rows of an item
+constexpr int kFewLast = 64;   // a (sequence, head)'s last rows, up to which they are such items
 
 // Eight codes as f16, exact. int8: 1024 + (c + 128) is the f16 whose low byte is c + 128.
 template <bool F8>
@@ -149,10 +150,9 @@ __device__ __forceinline__ int cache_v_swz(int r) {
 // l16 of each block of 16 rows, its scores at keys 16 kb + 4g + i, and of O^T dims
 // 16 db + 4g + i.
 template <int D, bool QF16, bool F8, int RB>
-__device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, lds_t K0, lds_t V0, lds_t K1, lds_t V1,
-                                                float* scales, float2* refs) {
+__device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, const CacheItem& it, lds_t K0, lds_t V0, lds_t K1,
+                                                lds_t V1, float* scales, float2* refs) {
   constexpr int TB = kFewTile * D, RPI = 1024 / D, NI = kFewTile / RPI, NS = D / 32, ND = D / 16;
-  const CacheItem it = a.items[blockIdx.x];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, g = lane >> 4;
   const lds_t Kw[2] = {K0 + wave * TB, K1 + wave * TB}, Vw[2] = {V0 + wave * TB, V1 + wave * TB};
@@ -379,31 +379,15 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, lds_t K0
   if constexpr (RB == 2) merge(std::integral_constant<int, 1>{});
 }
 
-// Up to kFewRows rows: 16 or 32, two workgroups a CU.
-template <int D, bool QF16, bool F8>
-__global__ __launch_bounds__(64 * kFewWaves, 2) void cache_few_kernel(CacheAttnArgs a) {
-  // an array for each buffer: a read of one does not wait for the DMA into another
-  __shared__ __attribute__((aligned(1024))) char K0[kFewWaves * kFewTile * D], V0[kFewWaves * kFewTile * D];
-  __shared__ __attribute__((aligned(1024))) char K1[kFewWaves * kFewTile * D], V1[kFewWaves * kFewTile * D];
-  __shared__ __attribute__((aligned(16))) float scales[kFewWaves * 3 * kFewTile];
-  __shared__ float2 refs[kFewWaves * kFewRows];
-  if (a.items[blockIdx.x].nr <= 16)
-    cache_rows_body<D, QF16, F8, 1>(a, (lds_t)K0, (lds_t)V0, (lds_t)K1, (lds_t)V1, scales, refs);
-  else
-    cache_rows_body<D, QF16, F8, 2>(a, (lds_t)K0, (lds_t)V0, (lds_t)K1, (lds_t)V1, scales, refs);
-}
-
 // Items of up to 32 WAVES rows, 32 a wave: chunks, and trees of more rows. Tiles of 64 keys as
 // f16 in LDS, converted once for all rows: the next tile's codes come through registers while
 // this one is used, and go into the other buffer behind it. Products as packed_kernel's.
 template <int D, bool QF16, bool F8, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void cache_tile_kernel(CacheAttnArgs a) {
+__device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const CacheItem& it, lds_t K0, lds_t V0, lds_t K1,
+                                                lds_t V1, float* S0, float* S1) {
   constexpr int TB = kPackTile * D * 2, CH = D / 16, ROWS = 64 * WAVES / CH;
   constexpr int RPI = ROWS < kPackTile ? ROWS : kPackTile, NI = kPackTile / RPI;  // with D 64 and 8 waves some idle
   typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-  __shared__ __attribute__((aligned(1024))) char K0[TB], V0[TB], K1[TB], V1[TB];
-  __shared__ __attribute__((aligned(16))) float S0[3 * kPackTile], S1[3 * kPackTile];
-  const CacheItem it = a.items[blockIdx.x];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kh = lane >> 5, w0 = 32 * wave;
   PackedArgs pa{};
@@ -475,7 +459,7 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void cache_tile_kernel(Cache
   // the first position that some row of the wave may not see, the last that some row may
   const int partly = it.tree ? it.shift : (it.r0 + w0) / a.G + it.shift + 1;
   const int whi = w0 < it.nr ? (it.r0 + min(w0 + 32, it.nr) - 1) / a.G + it.shift : -1;
-  put((lds_t)K0, (lds_t)V0, S0);
+  put(K0, V0, S0);
   __syncthreads();
 
   const auto tile = [&](int t0, lds_t K, lds_t V, const float* S, lds_t Kn, lds_t Vn, float* Sn) {
@@ -614,17 +598,41 @@ __global__ __launch_bounds__(64 * WAVES, 8 / WAVES) void cache_tile_kernel(Cache
     __syncthreads();
   };
   for (int t0 = it.kv_lo; t0 < it.kv_hi; t0 += 2 * kPackTile) {
-    tile(t0, (lds_t)K0, (lds_t)V0, S0, (lds_t)K1, (lds_t)V1, S1);
-    if (t0 + kPackTile < it.kv_hi) tile(t0 + kPackTile, (lds_t)K1, (lds_t)V1, S1, (lds_t)K0, (lds_t)V0, S0);
+    tile(t0, K0, V0, S0, K1, V1, S1);
+    if (t0 + kPackTile < it.kv_hi) tile(t0 + kPackTile, K1, V1, S1, K0, V0, S0);
   }
   static_assert(TB == 128 * D, "a tile holds a wave's rows");
   const int turn = wave % 4;
-  const lds_t buf = (lds_t)(turn == 0 ? K0 : turn == 1 ? V0 : turn == 2 ? K1 : V1);
+  const lds_t buf = turn == 0 ? K0 : turn == 1 ? V0 : turn == 2 ? K1 : V1;
   if (wave < 4) w.write(pa, pit, lane, buf);
   if (WAVES > 4) {
     __syncthreads();
     if (wave >= 4) w.write(pa, pit, lane, buf);
   }
+}
+
+// Items of all kinds, two workgroups a CU: chunks, trees and single tokens of a batch run
+// beside each other.
+template <int D, bool QF16, bool F8>
+__global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAttnArgs a) {
+  // an array for each buffer: a read of one does not wait for the DMA into another
+  __shared__ __attribute__((aligned(1024))) char K0[128 * D], V0[128 * D], K1[128 * D], V1[128 * D];
+  __shared__ __attribute__((aligned(16))) float S0[kFewWaves * 3 * kFewTile], S1[kFewWaves * 2 * kFewRows];
+  static_assert(kFewWaves * kFewTile == 128 && 2 * kPackTile == 128, "buffers of either body");
+  static_assert(3 * kPackTile <= kFewWaves * 2 * kFewRows && 3 * kPackTile <= kFewWaves * 3 * kFewTile, "scales of either");
+  const CacheItem it = a.items[blockIdx.x];
+  const lds_t k0 = (lds_t)K0, v0 = (lds_t)V0, k1 = (lds_t)K1, v1 = (lds_t)V1;
+  if (it.nr > kFewRows) cache_tile_body<D, QF16, F8, 4>(a, it, k0, v0, k1, v1, S0, S1);
+  else if (it.nr > 16) cache_rows_body<D, QF16, F8, 2>(a, it, k0, v0, k1, v1, S0, (float2*)S1);
+  else cache_rows_body<D, QF16, F8, 1>(a, it, k0, v0, k1, v1, S0, (float2*)S1);
+}
+// Items of 256 rows, one workgroup a CU.
+template <int D, bool F8>
+__global__ __launch_bounds__(512, 1) void cache_wide_kernel(CacheAttnArgs a) {
+  __shared__ __attribute__((aligned(1024))) char K0[128 * D], V0[128 * D], K1[128 * D], V1[128 * D];
+  __shared__ __attribute__((aligned(16))) float S0[3 * kPackTile], S1[3 * kPackTile];
+  const CacheItem it = a.items[blockIdx.x];
+  cache_tile_body<D, true, F8, 8>(a, it, (lds_t)K0, (lds_t)V0, (lds_t)K1, (lds_t)V1, S0, S1);
 }
 
 // ---------------------------------------------------------------------------
@@ -645,45 +653,60 @@ void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, con
     narrow += (rows + 127) / 128 * 128 * lengths[s];
     wide += (rows + 255) / 256 * 256 * lengths[s];
   }
-  plan.tile_rows = q_f16 && 10 * wide <= 11 * narrow ? 256 : 128;
+  const int most = q_f16 && 10 * wide <= 11 * narrow ? 256 : 128;  // rows of an item
   int64_t q0 = 0;
   for (int s = 0; s < B; s++) {
     const int64_t rows = (int64_t)extents[s] * G;
     const int shift = lengths[s] - extents[s];
-    const bool few = rows <= kFewRows;
-    const int most = few ? kFewRows : plan.tile_rows;
-    for (int64_t r0 = 0; r0 < rows; r0 += most) {
-      const int nr = (int)std::min<int64_t>(most, rows - r0);
+    for (int64_t r0 = 0, nr; r0 < rows; r0 += nr) {
+      const int64_t left = rows - r0;
+      nr = std::min<int64_t>(left, left <= kFewLast ? kFewRows : most);
       const int hi = (int)std::min<int64_t>(lengths[s], (r0 + nr - 1) / G + shift + 1);
       for (int h = 0; h < Hkv; h++)  // k0: the sequence
-        whole[few].push_back(PackedItem{(int32_t)q0, s, lengths[s], shift, (int32_t)r0, nr, 0, hi, h, -1});
+        whole[nr <= kFewRows].push_back(PackedItem{(int32_t)q0, s, lengths[s], shift, (int32_t)r0, (int)nr, 0, hi, h, -1});
     }
     q0 += extents[s];
   }
   plan.tq = q0;
-  PackedPlan merges;
+  // Each kind is cut for its share of the CUs, by what it costs: us of a key of an item alone on its CU
   const double dims = D / 128.0;
-  pack_cut(whole[0], kPackTile, 12, ncu, q_f16 ? PackRate{1.6 * dims, 0.6} : PackRate{2.2 * dims, 0.55}, cut[0], merges);
-  pack_cut(whole[1], kFewTile * kFewWaves, 2, ncu, PackRate{1.8 * dims, 0.7}, cut[1], merges);
+  const PackRate rate[2] = {most == 256 ? PackRate{2.2 * dims, 0.5} : q_f16 ? PackRate{1.6 * dims, 0.6} : PackRate{2.2 * dims, 0.55}, PackRate{1.8 * dims, 0.7}};
+  const int tile[2] = {kPackTile, kFewTile * kFewWaves}, least[2] = {12, 2};
+  double cost[2] = {}, key[2];
+  for (int f = 0; f < 2; f++) {
+    key[f] = rate[f].tile / rate[f].shared / tile[f];
+    for (const PackedItem& it : whole[f]) cost[f] += it.kv_hi * key[f];
+  }
+  PackedPlan merges;
+  for (int f = 0; f < 2; f++) {
+    const double share = most == 256 ? 1.0 : cost[f] / (cost[0] + cost[1]);
+    pack_cut(whole[f], tile[f], least[f], std::max(1, (int)(ncu * share + 0.5)), rate[f], cut[f], merges);
+  }
   plan.merges = std::move(merges.merges);
   plan.part_rows = merges.part_rows;
-  plan.tiles = (int)cut[0].size();
+  plan.wide = most == 256 ? (int)cut[0].size() : 0;
   plan.items.reserve(cut[0].size() + cut[1].size());
-  for (const auto& c : cut)
-    for (const PackedItem& p : c)
-      plan.items.push_back(CacheItem{p.q0, p.k0, p.nk, p.shift, p.r0, p.nr, p.kv_lo, p.kv_hi, p.kvh, p.part,
-                                     tree && tree[p.k0] ? 1 : 0, 0});
+  const auto take = [&](const PackedItem& p) {
+    plan.items.push_back(CacheItem{p.q0, p.k0, p.nk, p.shift, p.r0, p.nr, p.kv_lo, p.kv_hi, p.kvh, p.part,
+                                   tree && tree[p.k0] ? 1 : 0, 0});
+  };
+  // longest first, both kinds together where one kernel takes them
+  size_t f = 0;
+  for (const PackedItem& p : cut[0]) {
+    while (!plan.wide && f < cut[1].size() && (cut[1][f].kv_hi - cut[1][f].kv_lo) * key[1] > (p.kv_hi - p.kv_lo) * key[0])
+      take(cut[1][f++]);
+    take(p);
+  }
+  while (f < cut[1].size()) take(cut[1][f++]);
 }
 
 template <int D, bool QF16, bool F8>
 static void cache_attention_launch(CacheAttnArgs a, hipStream_t st) {
-  if (a.tiles && a.tile_rows == 256) {
-    if constexpr (QF16) hipLaunchKernelGGL((cache_tile_kernel<D, QF16, F8, 8>), dim3(a.tiles), dim3(512), 0, st, a);
-  } else if (a.tiles) {
-    hipLaunchKernelGGL((cache_tile_kernel<D, QF16, F8, 4>), dim3(a.tiles), dim3(256), 0, st, a);
-  }
-  a.items += a.tiles;
-  if (a.few) hipLaunchKernelGGL((cache_few_kernel<D, QF16, F8>), dim3(a.few), dim3(64 * kFewWaves), 0, st, a);
+  if constexpr (QF16)
+    if (a.wide) hipLaunchKernelGGL((cache_wide_kernel<D, F8>), dim3(a.wide), dim3(512), 0, st, a);
+  a.items += a.wide;
+  if (a.nitems > a.wide)
+    hipLaunchKernelGGL((cache_attention_kernel<D, QF16, F8>), dim3(a.nitems - a.wide), dim3(256), 0, st, a);
 }
 template <int D>
 static void cache_attention_form(const CacheAttnArgs& a, hipStream_t st) {

@@ -213,8 +213,8 @@ struct CacheItem {
 struct CachePlan {
   int H = 0;
   int64_t tq = 0;
-  std::vector<CacheItem> items;  // of the tile kernel, then of the few-row kernel
-  int tiles = 0, tile_rows = 0;   // rows of an item of the tile kernel: 128 or 256
+  std::vector<CacheItem> items;
+  int wide = 0;       // those of the kernel of 256 rows, which come first
   std::vector<PackedMerge> merges;
   int64_t part_rows = 0;
 };
@@ -233,7 +233,7 @@ struct CacheAttnArgs {
   float *part_o, *part_ml;
   int64_t q_row, out_row, out_lo;
   int max_pages, G, out_form, q_f16;
-  int tiles, tile_rows, few, nmerges;
+  int nitems, wide, nmerges;
   float qscale;  // scale * log2(e)
 };
 int cache_attention_enqueue(const CacheAttnArgs& a, hipStream_t st);
