@@ -547,7 +547,7 @@ int tgohip_cache_plan(tgohip_ctx* ctx, const tgohip_cache* cache, int B, const i
 int tgohip_cache_plan_free(tgohip_ctx* ctx, int handle);
 /* out = softmax(scale q k^T) v over a plan's rows: q [sum of extents, H, head_dim] in the plan's
  * q_dtype, out like q in f32, f16 or as a pair (TGOHIP_F16X2, dense rows). Rows are *_row
- * elements apart (at most 2^30), heads dense, 16-byte aligned; scale is above 0 and at most
+ * elements apart (at most 2^30), heads dense, 16-byte aligned; scale is from 2^-64 to
  * 2^32. Both products take the codes as they are, scales are f32 in the softmax; f32 queries go
  * as f16 hi + lo pairs and so do their probabilities (|q| < 65504, carried to 2^-22 of
  * itself or 2^-25), f16 queries take f16 probabilities. Scores, sums and partial results are

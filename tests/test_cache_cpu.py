@@ -161,7 +161,7 @@ def test_trees_have_as_many_tokens_as_a_mask_has_bits():
 
 @pytest.mark.parametrize("change,word", [
     (dict(layer=2), "layer 2 of 2"), (dict(scale=0.0), "scale is 0"), (dict(scale=-1.0), "scale is -1"), (dict(scale=NAN), "scale is nan"),
-    (dict(scale=2.0 ** 33), "at most 2\\^32"), (dict(dtype=3), "out_dtype is 3"), ({}, "context is missing"),
+    (dict(scale=2.0 ** 33), "at most 2\\^32"), (dict(scale=2.0 ** -65), "at least 2\\^-64"), (dict(dtype=3), "out_dtype is 3"), ({}, "context is missing"),
 ])
 def test_attention_refusals(change, word):
     a = dict(layer=0, scale=1.0, dtype=0)

@@ -610,6 +610,17 @@ def test_scales_far_apart(ctx, torch_gpu, f16, spread):
     b.check(b.run(ctx, out=torch.empty(b.q.shape, device="cuda")))  # past f16's range
 
 
+@pytest.mark.parametrize("f16", [False, True])
+def test_the_least_scale(ctx, torch_gpu, f16):
+    """Scores of next to nothing, beside value rows of 2^-40 to 2^38: all that is seen weighs the same."""
+    torch = torch_gpu
+    b = Batch(torch, [1, 40, 300], [700, 333, 700], 8, 2, 128, "i8", f16)
+    b.scale = 2.0 ** -64
+    b.pool.ks.fill_(2.0 ** -40)
+    b.pool.vs.copy_(torch.exp2(torch.randint(-40, 39, b.pool.vs.shape, device="cuda").float()))
+    b.check(b.run(ctx, out=torch.empty(b.q.shape, device="cuda")))  # past f16's range
+
+
 @pytest.mark.parametrize("size", [20.0, 400.0, 30000.0])
 @pytest.mark.parametrize("f16", [False, True])
 def test_peaked_scores(ctx, torch_gpu, size, f16):

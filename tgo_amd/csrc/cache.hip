@@ -357,7 +357,7 @@ int tgohip_cache_read(tgohip_ctx* c, const tgohip_cache* cache, int layer, const
     a.T = T;
     a.f16 = out_dtype == TGOHIP_F16;
     OnDevice on(c->device);
-    launch_cache_read(a, c->ncu, c->stream);
+    launch_cache_read(a, c->stream);
     TGOHIP_HIP(hipGetLastError());
     return 0;
   });
@@ -530,7 +530,8 @@ int tgohip_cache_attention(tgohip_ctx* c, int handle, const tgohip_cache* cache,
     int rc = check_cache("cache_attention", cache, layer);
     if (rc) return rc;
     const auto bad = [](const std::string& m) { return refuse("cache_attention: " + m); };
-    if (!(scale > 0.f) || scale > 0x1p32f) return bad("scale is " + num(scale) + "; a number above 0, at most 2^32");
+    // a key's scale times it, and log2 of a value's over that, stay in f32's range
+    if (!(scale >= 0x1p-64f && scale <= 0x1p32f)) return bad("scale is " + num(scale) + "; at least 2^-64 and at most 2^32");
     if (out_dtype != TGOHIP_F32 && out_dtype != TGOHIP_F16 && out_dtype != TGOHIP_F16X2)
       return bad("out_dtype is " + str(out_dtype) + "; f32, f16 or a pair");
     if (!c) return no_ctx("cache_attention");

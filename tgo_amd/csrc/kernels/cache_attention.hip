@@ -9,6 +9,14 @@
 // product takes hold their value's scale, so that their largest is near 1 whatever the
 // scales are, and the sum takes it out again. m moves along (online softmax), and only
 // when a probability would leave its range.
+//
+// What bounds it: few rows read the codes once, at HBM's rate; many are bound by the matrix
+// unit and the exponentials beside it. Measured (32 heads over 8 of 128 dims, us with the
+// merge): one f32 token over 8192 int8 keys 11.4 (two launches and chains of dependent loads);
+// 128 over 16 to 8192 keys 64, 5.9 TB/s in the kernel (a plain read here 6.6); 32 trees of
+// 17 to 60 tokens over 256 to 4096 keys 92; four f32 chunks of 187 to 405 over 2616 to 5417 e4m3
+// keys 135; 2048 f16 tokens, the last of 32768, 1112 to 1185 from card to card, 0.90 to 0.96 PFLOP/s (a large f16 matrix
+// product here 1.27).
 #include "pack_rows.h"
 
 #include <algorithm>
@@ -30,7 +38,10 @@ constexpr float kScaleLeast = 0x1p-40f, kScaleMost = 0x1p40f;
 constexpr int kFewTile = 32;   // keys of a wave's tile
 constexpr int kFewWaves = 4;
 constexpr int kFewRows = 32;   // rows of an item
-constexpr int kFewLast = 64;   // a (sequence, head)'s last rows, up to which they are such items
+// Up to so many rows at the end of a (sequence, head)'s go as such items. Up to 32 / 64 / 96 / 256,
+// us: 32 trees of 68 to 240 rows 97.6 / 94.4 / 95.0 / 100.8, four chunks of 748 to 1620
+// 141.5 / 141.5 / 141.4 / 144.1.
+constexpr int kFewLast = 64;
 
 // Eight codes as f16, exact. int8: 1024 + (c + 128) is the f16 whose low byte is c + 128.
 template <bool F8>
@@ -148,7 +159,10 @@ __device__ __forceinline__ int cache_v_swz(int r) {
 // two LDS buffers of its own, filled by DMA through the page table; their results meet in
 // LDS. S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16: lane (l16, g) holds row
 // l16 of each block of 16 rows, its scores at keys 16 kb + 4g + i, and of O^T dims
-// 16 db + 4g + i.
+// 16 db + 4g + i. A tile stays 8 bits in LDS and is converted by the wave that uses it, V by
+// the transposing read of bytes. Single tokens (4 rows of 16 used) by items of 16 / 32 rows, us: 128 of
+// 16 to 8192 keys 65 / 81, one of 8192 11.6 / 13.3. The next tile's loads before the wait for this
+// one (twice the bytes in flight): no faster, 64.7 beside 64.0.
 template <int D, bool QF16, bool F8, int RB>
 __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, const CacheItem& it, lds_t K0, lds_t V0, lds_t K1,
                                                 lds_t V1, float* scales, float2* refs) {
@@ -381,7 +395,9 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, const Ca
 
 // Items of up to 32 WAVES rows, 32 a wave: chunks, and trees of more rows. Tiles of 64 keys as
 // f16 in LDS, converted once for all rows: the next tile's codes come through registers while
-// this one is used, and go into the other buffer behind it. Products as packed_kernel's.
+// this one is used, and go into the other buffer behind it. Products as packed_kernel's. By
+// items of 32 rows alone (each converts for itself): 2048 f16 tokens behind 30720 positions 1941 us
+// beside 1235.
 template <int D, bool QF16, bool F8, int WAVES>
 __device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const CacheItem& it, lds_t K0, lds_t V0, lds_t K1,
                                                 lds_t V1, float* S0, float* S1) {
@@ -645,7 +661,9 @@ void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, con
   plan.H = H;
   const int G = H / Hkv;
   std::vector<PackedItem> whole[2], cut[2];  // tiles, few rows
-  // f16 queries in blocks of 256 rows where that pads little
+  // f16 queries in blocks of 256 rows (one workgroup a CU, half the tiles to convert) where that pads
+  // little. Of 128 / 256, us: 2048 tokens behind 30720 positions 1232 / 1134; the padding weighs
+  // as much as rows do. f32 queries' pairs leave no registers for it.
   int64_t narrow = 0, wide = 0;
   for (int s = 0; s < B; s++) {
     const int64_t rows = (int64_t)extents[s] * G;
@@ -668,7 +686,10 @@ void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, con
     q0 += extents[s];
   }
   plan.tq = q0;
-  // Each kind is cut for its share of the CUs, by what it costs: us of a key of an item alone on its CU
+  // Each kind is cut for its share of the CUs, by what it costs (key: us of an item's key). Both in
+  // one launch / one behind the other: 32 trees whose last rows are few 94 / 112 us. Pieces of many
+  // rows hold more keys than a tree has tokens, so that each row sees one of them; at least
+  // 4 / 12 tiles: 99 / 97.
   const double dims = D / 128.0;
   const PackRate rate[2] = {most == 256 ? PackRate{2.2 * dims, 0.5} : q_f16 ? PackRate{1.6 * dims, 0.6} : PackRate{2.2 * dims, 0.55}, PackRate{1.8 * dims, 0.7}};
   const int tile[2] = {kPackTile, kFewTile * kFewWaves}, least[2] = {12, 2};

@@ -178,7 +178,7 @@ struct CacheReadArgs {
   void* out[2];  // k's, v's; null: not read
   int64_t row[2], head[2];
 };
-void launch_cache_read(const CacheReadArgs& a, int ncu, hipStream_t st);
+void launch_cache_read(const CacheReadArgs& a, hipStream_t st);
 // Rows src[i] to dst[i] (slots) of every layer and head; a workgroup takes moves
 // [start, start + n) of one (layer, head), kCacheMoveSeg of them read before any is written.
 constexpr int kCacheMoveSeg = 64;
