@@ -97,7 +97,7 @@ def test_store_refusals(call, row, word):
 
 
 @pytest.mark.parametrize("change,word", [
-    (dict(layer=3), "layer 3 of 2"), (dict(T=-1), "-1 rows"), (dict(T=1 << 30), "below 2\\^31"), (dict(dtype=2), "out_dtype is 2"),
+    (dict(layer=3), "layer 3 of 2"), (dict(T=-1), "-1 rows"), (dict(T=1 << 29), "below 2\\^29"), (dict(dtype=2), "out_dtype is 2"),
     (dict(slots=None), "slots is a device buffer"), (dict(k=BASE + (10 << 20) + 2), "k_out is not aligned"),
     (dict(k_row=-4), "strides are not negative"), (dict(k_head=32), "heads of k_out overlap"), (dict(k=BASE + 64), "k_out meets the cache's k "),
     (dict(k=BASE + (3 << 20)), "k_out meets the cache's v_scale"), (dict(k=SLOTS), "k_out meets slots"),

@@ -397,6 +397,28 @@ def longest_cycle(src, dst):
     return best
 
 
+@pytest.mark.parametrize("n", [7, 400, 700])
+def test_moves_follow_each_other(ctx, torch_gpu, n):
+    """Moves of other rows without a wait between them: each acts on what the one before left."""
+    torch = torch_gpu
+    r = np.random.default_rng(n)
+    pool = Pool(torch, 2, (3 * n + 15) // 16, 2, 16, 64, "i8").fill(seed=n)
+    before = pool.bytes()
+    steps = []
+    for _ in range(6):
+        p = r.permutation(3 * n)
+        steps.append((p[:n], p[n:2 * n]))
+    host = [t.cpu().view(2, pool.k.shape[1], 2, 16, -1) for t in before]
+    for src, dst in steps:
+        ctx.cache_move(pool.cache, [int(x) for x in src], dst)
+    for i, t in enumerate(host):
+        for src, dst in steps:
+            t[:, dst // 16, :, dst % 16] = t[:, src // 16, :, src % 16].clone()
+    torch.cuda.synchronize()
+    for got, want in zip(pool.bytes(), host):
+        assert torch.equal(got.cpu().view(want.shape), want)
+
+
 def test_move_refusals(ctx, torch_gpu):
     torch = torch_gpu
     pool = Pool(torch, 2, 5, 2, 16, 64, "i8").fill()
@@ -554,6 +576,20 @@ def test_trees_of_drafted_tokens(ctx, torch_gpu, n, wide, ctx_len, H, Hkv, d, fo
     r = np.random.default_rng(n + ctx_len)
     b = Batch(torch_gpu, [n, 1, n], [ctx_len + n, 77, n + 3], H, Hkv, d, form, f16,
               trees=[random_tree(r, n, wide), None, [-1] * n])
+    b.check(b.run(ctx))
+
+
+@pytest.mark.parametrize("f16,d,form", [(False, 128, "i8"), (True, 128, "f8"), (False, 64, "f8"), (True, 64, "i8")])
+def test_last_rows_of_every_kind(ctx, torch_gpu, f16, d, form):
+    """Chunks that end in items of 128, 32 or fewer rows, beside single tokens and a tree; for f16 queries of many
+    rows, items of 256 with others behind them."""
+    sizes = [1, 16, 17, 96, 97, 127, 128, 129, 144, 160, 161, 191, 192, 193, 255, 256, 257, 1, 40]
+    r = np.random.default_rng(3)
+    lengths = [n + int(r.integers(0, 900)) for n in sizes]
+    trees = [None] * (len(sizes) - 1) + [random_tree(r, 40, 8)]
+    b = Batch(torch_gpu, sizes, lengths, 3, 3, d, form, f16, trees=trees)
+    b.check(b.run(ctx))
+    b = Batch(torch_gpu, [2580, 1, 5, 0], [3080, 3000, 70, 9], 2, 1, d, form, f16)
     b.check(b.run(ctx))
 
 

@@ -323,8 +323,8 @@ int tgohip_cache_read(tgohip_ctx* c, const tgohip_cache* cache, int layer, const
   return guarded([&]() -> int {
     int rc = check_cache("cache_read", cache, layer);
     if (rc) return rc;
-    if (T < 0 || (int64_t)T * cache->kv_heads > INT_MAX)
-      return refuse("cache_read: " + str(T) + " rows of " + str(cache->kv_heads) + " heads; heads of rows stay below 2^31");
+    if (T < 0 || (int64_t)T * cache->kv_heads >= 1 << 29)  // threads of a launch stay below 2^32
+      return refuse("cache_read: " + str(T) + " rows of " + str(cache->kv_heads) + " heads; heads of rows stay below 2^29");
     if (bad_type(out_dtype)) return refuse("cache_read: out_dtype is " + str(out_dtype) + "; f32 or f16");
     if (T == 0 || (!k_out && !v_out)) return c ? 0 : no_ctx("cache_read");
     if (!slots || (uintptr_t)slots % 4) return refuse("cache_read: slots is a device buffer of int32");
