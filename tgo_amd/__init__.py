@@ -406,12 +406,12 @@ def _heads_view(t, what, device):
     s = t.stride()
     if len(s) != 3 or (s[2] != 1 and t.shape[2] > 1):
         raise TgoError(EINVAL, "%s is a [rows, heads, head_dim] tensor with dense head rows" % what)
-    kind = _kind(t)
-    if kind is None:
+    kind = _KINDS.get(t.dtype)
+    if kind is None and _kind(t) is None:
         raise TgoError(EINVAL, "%s is %s; float32 or float16" % (what, t.dtype))
     if t.get_device() != device:
         raise _elsewhere(t, what, device)
-    return t.data_ptr(), s[0], s[1], kind
+    return t.data_ptr(), s[0], s[1], _kind(t) if kind is None else kind
 
 
 def _packed_rows(t, what, device, rows, heads, d, kind):
@@ -943,15 +943,19 @@ class Context:
         return cache.at
 
     def _slots(self, t, what):
-        if _INT32.get(t.dtype) is None:
+        if t.dtype not in _INT32:
             if str(t.dtype) != "torch.int32":
                 raise TgoError(EINVAL, "%s is int32, not %s" % (what, t.dtype))
             _INT32[t.dtype] = True
+        if t.get_device() == self.device and t.is_contiguous():
+            return t.data_ptr()
         return _addr(t, what, self.device)
 
     def _gain(self, g, what, d):
-        if _kind(g) != F32 or g.numel() != d:
+        if g.numel() != d or _kind(g) != F32:
             raise TgoError(EINVAL, "cache_store: %s is float32 [%d]" % (what, d))
+        if g.get_device() == self.device and g.is_contiguous():
+            return g.data_ptr()
         return _addr(g, what, self.device)
 
     def cache_store(self, cache, layer, slots, k, v, q=None, q_out=None, positions=None, rope=0, q_gain=None,
