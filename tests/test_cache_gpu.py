@@ -589,8 +589,10 @@ def test_last_rows_of_every_kind(ctx, torch_gpu, f16, d, form):
     trees = [None] * (len(sizes) - 1) + [random_tree(r, 40, 8)]
     b = Batch(torch_gpu, sizes, lengths, 3, 3, d, form, f16, trees=trees)
     b.check(b.run(ctx))
-    b = Batch(torch_gpu, [2580, 1, 5, 0], [3080, 3000, 70, 9], 2, 1, d, form, f16)
-    b.check(b.run(ctx))
+    for extents, lengths, H, Hkv in (([2580, 1, 5, 0], [3080, 3000, 70, 9], 2, 1), ([2048, 700], [2048, 1900], 2, 1),
+                                     ([2048, 1, 3], [27000, 700, 33], 8, 2)):
+        b = Batch(torch_gpu, extents, lengths, H, Hkv, d, form, f16)
+        b.check(b.run(ctx))
 
 
 def test_a_chain_of_parents_is_a_causal_chunk(ctx, torch_gpu):

@@ -661,17 +661,27 @@ void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, con
   plan.H = H;
   const int G = H / Hkv;
   std::vector<PackedItem> whole[2], cut[2];  // tiles, few rows
+  const double dims = D / 128.0;
+  const PackRate tiles = q_f16 ? PackRate{1.6 * dims, 0.6} : PackRate{2.2 * dims, 0.55};
   // f16 queries in blocks of 256 rows (one workgroup a CU, half the tiles to convert) where that pads
   // little. Of 128 / 256, us: 2048 tokens behind 30720 positions 1232 / 1134; the padding weighs
-  // as much as rows do. f32 queries' pairs leave no registers for it.
+  // as much as rows do. f32 queries' pairs leave no registers for it. Where few rows follow, they
+  // are a launch of their own behind it, which ends and starts for some 20 us of a CU's time: then
+  // only where blocks of 128 would take kWideLeast. 512 tokens behind 1536 and 64 decoders of 1024 to
+  // 4096 positions 84 / 106, a prompt of 2048 and 32 of 512 to 2048 74 / 97, 2048 behind 16384 and 128
+  // of 2048 to 8192 867 / 821.
+  constexpr double kWideLeast = 250.;  // us
   int64_t narrow = 0, wide = 0;
+  bool others = false;
   for (int s = 0; s < B; s++) {
     const int64_t rows = (int64_t)extents[s] * G;
+    others = others || (rows && (rows - 1) % 256 < kFewLast);
     if (rows <= kFewRows) continue;
     narrow += (rows + 127) / 128 * 128 * lengths[s];
     wide += (rows + 255) / 256 * 256 * lengths[s];
   }
-  const int most = q_f16 && 10 * wide <= 11 * narrow ? 256 : 128;  // rows of an item
+  const double time = (double)narrow / (128 * kPackTile) * Hkv * tiles.tile / tiles.shared / (2 * ncu);
+  const int most = q_f16 && 10 * wide <= 11 * narrow && (!others || time > kWideLeast) ? 256 : 128;  // rows of an item
   int64_t q0 = 0;
   for (int s = 0; s < B; s++) {
     const int64_t rows = (int64_t)extents[s] * G;
@@ -690,8 +700,7 @@ void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, con
   // one launch / one behind the other: 32 trees whose last rows are few 94 / 112 us. Pieces of many
   // rows hold more keys than a tree has tokens, so that each row sees one of them; at least
   // 4 / 12 tiles: 99 / 97.
-  const double dims = D / 128.0;
-  const PackRate rate[2] = {most == 256 ? PackRate{2.2 * dims, 0.5} : q_f16 ? PackRate{1.6 * dims, 0.6} : PackRate{2.2 * dims, 0.55}, PackRate{1.8 * dims, 0.7}};
+  const PackRate rate[2] = {most == 256 ? PackRate{2.2 * dims, 0.5} : tiles, PackRate{1.8 * dims, 0.7}};
   const int tile[2] = {kPackTile, kFewTile * kFewWaves}, least[2] = {12, 2};
   double cost[2] = {}, key[2];
   for (int f = 0; f < 2; f++) {
@@ -700,7 +709,7 @@ void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, con
   }
   PackedPlan merges;
   for (int f = 0; f < 2; f++) {
-    const double share = most == 256 ? 1.0 : cost[f] / (cost[0] + cost[1]);
+    const double share = most == 256 ? 1.0 : cost[f] / std::max(cost[0] + cost[1], 1e-9);
     pack_cut(whole[f], tile[f], least[f], std::max(1, (int)(ncu * share + 0.5)), rate[f], cut[f], merges);
   }
   plan.merges = std::move(merges.merges);
