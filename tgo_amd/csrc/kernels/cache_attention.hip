@@ -699,7 +699,7 @@ void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, con
   // Each kind is cut for its share of the CUs, by what it costs (key: us of an item's key). Both in
   // one launch / one behind the other: 32 trees whose last rows are few 94 / 112 us. Pieces of many
   // rows hold more keys than a tree has tokens, so that each row sees one of them; at least
-  // 4 / 12 tiles: 99 / 97.
+  // 8 / 12 / 20 tiles: 95.6 / 92.2 / 107.
   const PackRate rate[2] = {most == 256 ? PackRate{2.2 * dims, 0.5} : tiles, PackRate{1.8 * dims, 0.7}};
   const int tile[2] = {kPackTile, kFewTile * kFewWaves}, least[2] = {12, 2};
   double cost[2] = {}, key[2];
