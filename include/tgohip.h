@@ -475,7 +475,7 @@ int tgohip_adapters(tgohip_ctx* ctx, int set, int rows, const void* x, int x_dty
  * Slot s of the pool is position s % block of page s / block, as in the f16 pool. A row
  * stands for code * scale: int8 codes of -127 to 127, or e4m3 ones (no NaN: 0x7f and 0xff do
  * not occur), its scale the row's largest magnitude over 127 or 448, at least 2^-40 (so the
- * smallest differences are 2^-40); codes are the nearest to value / scale, ties to even. A
+ * smallest differences are 2^-40); codes are the nearest to value / scale as f32, ties to even. A
  * row that holds a value that is not finite, or past 2^40, stands for NaN throughout (its
  * scale is NaN, its codes 0). Other writers keep scales at 0 (a row of zeros: memory as it is
  * cleared), from 2^-40 to 2^40, or NaN. Buffers are apart from each other and from every other

@@ -1018,3 +1018,42 @@ def test_another_stream_and_the_device_of_the_context(ctx, torch_gpu):
     finally:
         ctx.set_stream(torch.cuda.current_stream().cuda_stream)
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("off", [0, 1])
+def test_codes_are_rounded_quotients(ctx, torch_gpu, off, f16, form):
+    """Rows neither normed nor rotated, in units of eight elements and of two: each code is value / scale as f32 gives
+    it, to the nearest, ties to even, and the scale the row's largest over 127 or 448, bit for bit. Half of the rows
+    consist of exact half steps."""
+    torch = torch_gpu
+    T, Hkv, d = 1024, 4, 128
+    r = np.random.default_rng(5)
+    x = r.standard_normal((T, Hkv, d)).astype(np.float32)
+    # a scale of few bits, times which the top and every half step are exact in the type
+    bits = 3 if f16 else 16
+    s = (2.0 ** (bits - 1) + r.integers(0, 2 ** (bits - 1), (T, Hkv, 1))) * 2.0 ** (1 - bits)
+    if form == "i8":
+        steps = np.arange(127) + 0.5
+    else:
+        grid = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).float().numpy()
+        steps = (grid[1:] + grid[:-1]) / 2
+    halves = r.choice(steps, (T, Hkv, d)) * r.choice([-1.0, 1.0], (T, Hkv, d))
+    halves[..., 77] = TOP[form]
+    x[::2] = (halves * s)[::2]
+    x = x.astype(np.float16 if f16 else np.float32)
+    y = x.astype(np.float32)
+    scale = np.maximum(np.abs(y).max(-1) / np.float32(TOP[form]), np.float32(2.0 ** -40))
+    q = y / scale[..., None]
+    want = np.rint(q) if form == "i8" else torch.from_numpy(q).to(torch.float8_e4m3fn).float().numpy()
+    buf = torch.zeros(off + x.size, device="cuda", dtype=torch.float16 if f16 else torch.float32)
+    buf[off:] = torch.from_numpy(x).cuda().flatten()
+    x = buf[off:].view(T, Hkv, d)
+    pool = Pool(torch, 1, T // 16, Hkv, 16, d, form)
+    store(ctx, torch, pool, 0, torch.arange(T, device="cuda", dtype=torch.int32), None, x, x)
+    torch.cuda.synchronize()
+    for codes, scales in ((pool.k, pool.ks), (pool.v, pool.vs)):
+        assert np.array_equal(scales[0].transpose(1, 2).reshape(T, Hkv).cpu().numpy(), scale)
+        got = codes[0].float().transpose(1, 2).reshape(T, Hkv, d).cpu().numpy()
+        assert np.array_equal(got, want), (float(np.abs(got - want).max()), int((got != want).sum()))
