@@ -1057,3 +1057,43 @@ def test_codes_are_rounded_quotients(ctx, torch_gpu, off, f16, form):
         assert np.array_equal(scales[0].transpose(1, 2).reshape(T, Hkv).cpu().numpy(), scale)
         got = codes[0].float().transpose(1, 2).reshape(T, Hkv, d).cpu().numpy()
         assert np.array_equal(got, want), (float(np.abs(got - want).max()), int((got != want).sum()))
+
+
+def log2_units(b):
+    """Makes a key's score q . code * k_scale in log2 units, to the bit."""
+    b.scale = next(float(x) for x in np.float32(math.log(2)) * (1 + np.arange(-8, 9, dtype=np.float32) * np.float32(2.0 ** -24))
+                   if np.float32(x) * np.float32(1.4426950408889634) == 1)
+
+
+# rows of one kv head that go as an item of up to 16, 32, 128 rows, and of 256 where queries are f16
+ITEMS = [5, 20, 100, 256]
+
+
+@pytest.mark.parametrize("n", ITEMS)
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("e", [10, 21, 23, 24, 25, 27])
+def test_a_key_sixteen_above_the_ones_before(ctx, torch_gpu, e, f16, n):
+    """Scores of 2^e, and in a later tile one of 16 more: every term is a power of two, so results are exact but for
+    the sums' roundings (4 sqrt(n) u and a quotient)."""
+    torch = torch_gpu
+    b = Batch(torch, [n], [700], 1, 1, 128, "i8", f16)
+    log2_units(b)
+    b.pool.k.zero_()
+    b.pool.k[..., 0] = 64
+    b.pool.ks.fill_(2.0 ** (e - 21))
+    b.pool.vs.fill_(1.0)
+    late = int(b.slots(0)[200])
+    b.pool.k[b.layer, late // 16, 0, late % 16, 1] = 16
+    b.q.zero_()
+    b.q[..., 0] = 2.0 ** 15
+    b.q[..., 1] = 2.0 ** (21 - e)
+    got = b.run(ctx)
+    v = b.pool.values(b.slots(0), b.layer)[1][:, 0]
+    w = torch.ones(700, device="cuda", dtype=torch.float64)
+    w[200] = 2.0 ** 16
+    for i in range(n):
+        m = 700 - n + i + 1
+        want = (w[:m] @ v[:m]) / w[:m].sum()
+        err = (got[i, 0].double() - want).abs()
+        tol = (4 * math.sqrt(700) + 2) * U * 127 + (f16_step(want) if f16 else 0)
+        assert bool((err <= tol).all()), (i, float(err.max()))

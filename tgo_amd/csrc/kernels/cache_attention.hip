@@ -28,7 +28,8 @@ constexpr int kNonTemporal = 2;  // the nt bit: a context's rows are read once
 // The reference starts at kCacheNoMax; where a term passes it by more than 2^kCacheTop (f16
 // ends at 2^16) it moves to the row's largest, kCacheLift less, so that small terms
 // keep an absolute error of 2^(-25 - kCacheLift) of that one's. Past kCacheFar a step of f32
-// is more than 1/4: the reference is then the largest itself, and differences stay exact.
+// is more than 1/4: the reference is then the largest itself. Whether a term passes it is asked of
+// their difference: of scores 16 apart at 2^24, where steps are 2, m + 15 may round to m + 16.
 constexpr float kCacheNoMax = -1.0e30f, kCacheFar = 4194304.f, kCacheLift = 7.f, kCacheTop = 15.f;
 // Scales as the store writes them: kept within these, so that a key's probability is lost
 // from the sum only where it is below 2^-46 of the largest (126 bits of f32's exponent
@@ -293,7 +294,7 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, const Ca
         for (int i = 0; i < 4; i++) top = fmaxf(top, sc[b][kb][i]);
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64));
-      const bool need = top > m[b] + kCacheTop;
+      const bool need = top - m[b] > kCacheTop;
       if (__builtin_amdgcn_ballot_w64(need)) {
         const float mnew = need ? (fabsf(top) > kCacheFar ? top : top - kCacheLift) : m[b];
         const float alpha = __builtin_amdgcn_exp2f(m[b] - mnew);
@@ -591,7 +592,7 @@ __device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const Ca
         w.l += (l[0] + l[1]) + (l[2] + l[3]);
       } else {
         const float top = largest();
-        const bool need = top > w.m + kCacheTop;
+        const bool need = top - w.m > kCacheTop;
         if (__builtin_amdgcn_ballot_w64(need)) raise(top, need);
         // pairs go step by step: all at once would not fit the registers beside the queries'
         float l[2] = {}, most;
