@@ -1097,3 +1097,25 @@ def test_a_key_sixteen_above_the_ones_before(ctx, torch_gpu, e, f16, n):
         err = (got[i, 0].double() - want).abs()
         tol = (4 * math.sqrt(700) + 2) * U * 127 + (f16_step(want) if f16 else 0)
         assert bool((err <= tol).all()), (i, float(err.max()))
+
+
+@pytest.mark.parametrize("n", ITEMS)
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("e", [16, 22, 26, 29, 33, 60])
+@pytest.mark.parametrize("form,d", [("i8", 128), ("f8", 64)])
+def test_keys_alike_far_from_zero(ctx, torch_gpu, form, d, e, f16, n):
+    """Keys that are all the same weigh the same, whatever their score (up to 2^e in size, of either sign): the mean
+    of the values seen, where the first row of a prompt sees one and a long context is cut and merged."""
+    torch = torch_gpu
+    for m in (n, 700, 9000):
+        b = Batch(torch, [n], [m], 1, 1, d, form, f16, size=1000.0)
+        b.pool.k.copy_(b.pool.k[0, 0, 0, 0].clone().expand_as(b.pool.k))
+        top = float(b.pool.k[0, 0, 0, 0].float().abs().sum()) * 5000 * b.scale * 1.4427
+        b.pool.ks.fill_(2.0 ** e / top)
+        b.pool.vs.fill_(0.37)
+        got = b.run(ctx).double()[:, 0]
+        v = b.pool.values(b.slots(0), b.layer)[1][:, 0]
+        want = (v.cumsum(0) / torch.arange(1, m + 1, device="cuda")[:, None])[m - n:]
+        # sums of m terms, 1 / v_scale, a quotient; f16 queries' terms, all alike, are rounded to f16
+        tol = (4 * math.sqrt(m) + 4) * U * v.abs().max() + (2 * f16_step(want) if f16 else 0)
+        assert bool(((got - want).abs() <= tol).all()), (m, float(((got - want).abs() / tol).max()))

@@ -28,8 +28,10 @@ constexpr int kNonTemporal = 2;  // the nt bit: a context's rows are read once
 // The reference starts at kCacheNoMax; where a term passes it by more than 2^kCacheTop (f16
 // ends at 2^16) it moves to the row's largest, kCacheLift less, so that small terms
 // keep an absolute error of 2^(-25 - kCacheLift) of that one's. Past kCacheFar a step of f32
-// is more than 1/4: the reference is then the largest itself. Whether a term passes it is asked of
-// their difference: of scores 16 apart at 2^24, where steps are 2, m + 15 may round to m + 16.
+// is more than 1/4: the reference is then the largest itself, and terms are taken from scores rounded to
+// f32 as it was (a multiply-add's would differ from it by what it lacks, at 2^28 up to 16). Whether a term
+// passes it is asked of their difference: of scores 16 apart at 2^24, where steps are 2, m + 15 may round to
+// m + 16.
 constexpr float kCacheNoMax = -1.0e30f, kCacheFar = 4194304.f, kCacheLift = 7.f, kCacheTop = 15.f;
 // Scales as the store writes them: kept within these, so that a key's probability is lost
 // from the sum only where it is below 2^-46 of the largest (126 bits of f32's exponent
@@ -232,6 +234,7 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, const Ca
   const int partly = it.tree ? it.shift : it.r0 / a.G + it.shift + 1;
 
   const auto tile = [&](int t0, lds_t K, lds_t V, lds_t Kn, lds_t Vn) {
+#pragma clang fp contract(off)  // a product fused into the subtraction would not be the score that m came from
     pack_wait();  // the tile has landed, and what was read of the other buffer has returned
     const KeyScales sk = cache_scales(ks, vs, a.qscale);
     if (lane < 32) {
@@ -476,6 +479,8 @@ __device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const Ca
   // the first position that some row of the wave may not see, the last that some row may
   const int partly = it.tree ? it.shift : (it.r0 + w0) / a.G + it.shift + 1;
   const int whi = w0 < it.nr ? (it.r0 + min(w0 + 32, it.nr) - 1) / a.G + it.shift : -1;
+  // f16 queries: above this a term has passed its range, 2^kCacheTop; below 0 where the row's reference is far
+  float limit = 32768.f;
   put(K0, V0, S0);
   __syncthreads();
 
@@ -521,13 +526,24 @@ __device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const Ca
       };
       scores();
       __builtin_amdgcn_sched_barrier(0);
-      const auto largest = [&] {  // of the row, not yet scaled scores in sc
+      // The scores as f32 rounds them, in place, and the row's largest.
+      const auto scale = [&] {
+#pragma clang fp contract(off)  // a product fused into what comes after would not be the score that m came from
+#pragma unroll
+        for (int x = 0; x < 8; x++) {
+          const float4_t ka = *(const float4_t*)(S + 8 * x + 4 * kh);
+#pragma unroll
+          for (int e = 0; e < 4; e++) sc[x >> 2][4 * (x & 3) + e] *= ka[e];
+        }
+      };
+      const auto largest = [&](bool scaled) {
+#pragma clang fp contract(off)
         float top = -INFINITY;
 #pragma unroll
         for (int x = 0; x < 8; x++) {
           const float4_t ka = *(const float4_t*)(S + 8 * x + 4 * kh);
 #pragma unroll
-          for (int e = 0; e < 4; e++) top = fmaxf(top, sc[x >> 2][4 * (x & 3) + e] * ka[e]);
+          for (int e = 0; e < 4; e++) top = fmaxf(top, sc[x >> 2][4 * (x & 3) + e] * (scaled ? 1.f : ka[e]));
         }
         return fmaxf(top, __shfl_xor(top, 32, 64));
       };
@@ -539,8 +555,9 @@ __device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const Ca
         for (int db = 0; db < D / 32; db++) w.o[db] *= alpha;
         w.m = mnew;
       };
-      // Step u's eight terms, their share of the sum on l.
-      const auto terms = [&](int u, half8_t& ph, half8_t& pl, float& l, float& most) {
+      // Step u's eight terms, their share of the sum on l; scaled: sc holds rounded scores.
+      const auto terms = [&](bool scaled, int u, half8_t& ph, half8_t& pl, float& l, float& most) {
+#pragma clang fp contract(off)
 #pragma unroll
         for (int y = 0; y < 2; y++) {
           const float4_t ka = *(const float4_t*)(S + 16 * u + 8 * y + 4 * kh);
@@ -550,7 +567,8 @@ __device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const Ca
             const int i = 8 * (u & 1) + 4 * y + e;
             float2_t x;
 #pragma unroll
-            for (int f = 0; f < 2; f++) x[f] = __builtin_amdgcn_exp2f(fmaf(sc[u >> 1][i + f], ka[e + f], -w.m));
+            for (int f = 0; f < 2; f++)
+              x[f] = __builtin_amdgcn_exp2f(fmaf(sc[u >> 1][i + f], scaled ? 1.f : ka[e + f], -w.m));
             const half2_t h = __builtin_convertvector(x, half2_t);
             ph[4 * y + e] = h[0];
             ph[4 * y + e + 1] = h[1];
@@ -568,20 +586,25 @@ __device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const Ca
       };
       if constexpr (QF16) {
         // All terms by the reference as it is; only where one of a row's has passed f16's range (its
-        // first tile, or a key far above the ones before) is the row's largest looked for.
+        // first tile, or a key far above the ones before), or its reference is far, is its largest looked
+        // for. Each row by itself: no bit of it depends on the wave's others. Scores rounded in every
+        // tile, as f32 queries' are: 1210 us beside 1177 for 2048 tokens behind 30720 positions.
         half8_t ph[4], none;
         float l[4] = {}, most = 0.f;
 #pragma unroll
-        for (int u = 0; u < 4; u++) terms(u, ph[u], none, l[u], most);
+        for (int u = 0; u < 4; u++) terms(false, u, ph[u], none, l[u], most);
         __builtin_amdgcn_sched_barrier(0);
-        const float limit = 32768.f;  // 2^kCacheTop
         if (__builtin_amdgcn_ballot_w64(most > limit)) {
-          const bool need = fmaxf(most, __shfl_xor(most, 32, 64)) > limit;
-          raise(largest(), need);
+          const bool passed = fmaxf(most, __shfl_xor(most, 32, 64)) > limit;
+          const float top = largest(false);
+          raise(top, limit < 0.f ? top - w.m > kCacheTop : passed);
+          const bool scaled = fabsf(w.m) > kCacheFar && w.m != kPackNoMax;
+          if (scaled) scale();
+          limit = scaled ? -1.f : 32768.f;
 #pragma unroll
           for (int u = 0; u < 4; u++) {
             l[u] = 0.f;
-            terms(u, ph[u], none, l[u], most);
+            terms(scaled, u, ph[u], none, l[u], most);
           }
         }
 #pragma unroll
@@ -591,7 +614,8 @@ __device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const Ca
             w.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u), ph[u], w.o[db], 0, 0, 0);
         w.l += (l[0] + l[1]) + (l[2] + l[3]);
       } else {
-        const float top = largest();
+        scale();
+        const float top = largest(true);
         const bool need = top - w.m > kCacheTop;
         if (__builtin_amdgcn_ballot_w64(need)) raise(top, need);
         // pairs go step by step: all at once would not fit the registers beside the queries'
@@ -599,7 +623,7 @@ __device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const Ca
 #pragma unroll
         for (int u = 0; u < 4; u++) {
           half8_t ph, pl;
-          terms(u, ph, pl, l[u & 1], most);
+          terms(true, u, ph, pl, l[u & 1], most);
           half8_t va[D / 32];
 #pragma unroll
           for (int db = 0; db < D / 32; db++) va[db] = pack_v_frag<D>(V, (vat ^ (64 * db)) + 32 * D * u);
