@@ -1119,3 +1119,24 @@ def test_keys_alike_far_from_zero(ctx, torch_gpu, form, d, e, f16, n):
         # sums of m terms, 1 / v_scale, a quotient; f16 queries' terms, all alike, are rounded to f16
         tol = (4 * math.sqrt(m) + 4) * U * v.abs().max() + (2 * f16_step(want) if f16 else 0)
         assert bool(((got - want).abs() <= tol).all()), (m, float(((got - want).abs() / tol).max()))
+
+
+@pytest.mark.parametrize("n", ITEMS)
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_the_largest_scores(ctx, torch_gpu, sign, f16, n):
+    """Queries, rows and the scale at the ends of their ranges: scores of 2^104 in size, where keys that are alike
+    weigh the same."""
+    torch = torch_gpu
+    for m in (n, 700, 9000):
+        b = Batch(torch, [n], [m], 1, 1, 128, "f8", f16)
+        b.scale = 2.0 ** 32
+        b.pool.k.copy_(torch.full(b.pool.k.shape, 448.0, device="cuda").to(b.pool.k.dtype))
+        b.pool.ks.fill_(2.0 ** 40)
+        b.pool.vs.fill_(0.37)
+        b.q.fill_(sign * 65472.0)
+        got = b.run(ctx).double()[:, 0]
+        v = b.pool.values(b.slots(0), b.layer)[1][:, 0]
+        want = (v.cumsum(0) / torch.arange(1, m + 1, device="cuda")[:, None])[m - n:]
+        tol = (4 * math.sqrt(m) + 4) * U * v.abs().max() + (f16_step(want) if f16 else 0)
+        assert bool(((got - want).abs() <= tol).all()), (m, float(((got - want).abs() / tol).max()))

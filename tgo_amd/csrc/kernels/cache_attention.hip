@@ -32,7 +32,7 @@ constexpr int kNonTemporal = 2;  // the nt bit: a context's rows are read once
 // f32 as it was (a multiply-add's would differ from it by what it lacks, at 2^28 up to 16). Whether a term
 // passes it is asked of their difference: of scores 16 apart at 2^24, where steps are 2, m + 15 may round to
 // m + 16.
-constexpr float kCacheNoMax = -1.0e30f, kCacheFar = 4194304.f, kCacheLift = 7.f, kCacheTop = 15.f;
+constexpr float kCacheNoMax = kPackLeast, kCacheFar = 4194304.f, kCacheLift = 7.f, kCacheTop = 15.f;
 // Scales as the store writes them: kept within these, so that a key's probability is lost
 // from the sum only where it is below 2^-46 of the largest (126 bits of f32's exponent
 // less the 80 between two scales).
@@ -474,6 +474,7 @@ __device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const Ca
   if (it.kv_lo + kPackTile < it.kv_hi) pages(it.kv_lo + kPackTile);
   PackRows<D, QF16> w;
   w.init(pa, pit, w0, lane);
+  w.m = kCacheNoMax;
   const int tok = (it.r0 + (w.r < it.nr ? w.r : 0)) / a.G;
   const uint64_t mask = it.tree ? a.masks[it.q0 + tok] : 0;
   // the first position that some row of the wave may not see, the last that some row may
@@ -598,7 +599,7 @@ __device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const Ca
           const bool passed = fmaxf(most, __shfl_xor(most, 32, 64)) > limit;
           const float top = largest(false);
           raise(top, limit < 0.f ? top - w.m > kCacheTop : passed);
-          const bool scaled = fabsf(w.m) > kCacheFar && w.m != kPackNoMax;
+          const bool scaled = fabsf(w.m) > kCacheFar && w.m != kCacheNoMax;
           if (scaled) scale();
           limit = scaled ? -1.f : 32768.f;
 #pragma unroll

@@ -10,6 +10,7 @@ namespace tgohip {
 
 constexpr int kPackTile = 64;            // keys staged in LDS per iteration
 constexpr float kPackNoMax = -1.0e30f;  // where a row's reference starts
+constexpr float kPackLeast = -3.0e38f;  // below every reference: the 8-bit cache's scores reach 2^105
 
 // A tile of kPackTile keys in LDS: rows of D f16, their 16-byte chunks XOR-swizzled.
 // K's chunks by the row, so that 32 lanes reading one chunk of 32 rows touch

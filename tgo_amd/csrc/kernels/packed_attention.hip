@@ -853,7 +853,7 @@ __global__ __launch_bounds__(256) void packed_merge_kernel(PackedArgs a) {
   const int grp = threadIdx.x / LR, d = threadIdx.x % LR * 4;
   const int slices = GR / (g.nr > 4 ? 8 : g.nr > 2 ? 4 : g.nr), i = grp / slices, sl0 = grp % slices;
   float4_t v = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f, M = kPackNoMax, E = 0.f;
+  float l = 0.f, M = kPackLeast, E = 0.f;
   bool blank = false;  // a part with a sum of 0 whose keys all score -inf
   if (i < g.nr) {
     // eight parts' loads in flight, the reference moving with them
