@@ -4,6 +4,7 @@ Tolerances count roundings, as in test_operators_gpu: u = 2^-24 for an f32 opera
 operand carried as an f16 hi + lo pair, half an ulp of f16 (2^-11 of the value, 2^-25 below its normal
 range) for an f16 result; a sum of n terms in f32 is off by 4 sqrt(n) u of their magnitudes. A code is
 off by half a step: 1/2 of an int8 row's scale, 2^-4 of an e4m3 value or 2^-10 of its scale."""
+import itertools
 import math
 
 import numpy as np
@@ -1140,3 +1141,24 @@ def test_the_largest_scores(ctx, torch_gpu, sign, f16, n):
         want = (v.cumsum(0) / torch.arange(1, m + 1, device="cuda")[:, None])[m - n:]
         tol = (4 * math.sqrt(m) + 4) * U * v.abs().max() + (f16_step(want) if f16 else 0)
         assert bool(((got - want).abs() <= tol).all()), (m, float(((got - want).abs() / tol).max()))
+
+
+@pytest.mark.parametrize("n", ITEMS)
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+def test_f16_queries_that_are_infinite(ctx, torch_gpu, value, n):
+    """Scores that are all infinite, of either sign or both, make their row NaN in every kind of item, whole or cut, a
+    tree's too, and no other row."""
+    torch = torch_gpu
+    for m, tree, signs in itertools.product((n, 700, 9000), (False, True), (1, 2)):
+        # a tree behind it keeps 256 rows out of one item
+        b = Batch(torch, [n] + tree * [4], [m] + tree * [m + 4], 1, 1, 128, "i8", True, trees=tree * [None, [-1, -1, 0, 1]])
+        b.pool.k[..., 3] = 5 if signs == 1 else torch.where(b.pool.k[..., 3] < 0, -7, 7).to(torch.int8)
+        clean = b.run(ctx)
+        assert bool(clean.isfinite().all())
+        rows = [0, n - 1] + tree * [n, n + 2]
+        b.q[rows, 0, 3] = value
+        got = b.run(ctx)
+        nan = torch.zeros_like(got, dtype=torch.bool)
+        nan[rows] = True
+        assert torch.equal(got.isnan(), nan), (m, tree, signs, int((got.isnan() != nan).sum()))
+        assert torch.equal(got[~nan], clean[~nan])

@@ -377,9 +377,12 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, const Ca
     const int r = 16 * b + l16;
     const bool live = r < it.nr, part = it.part >= 0;
     const int row = it.r0 + r, t = row / a.G, head = it.kvh * a.G + row % a.G;
+    // A sum of 0 is a row's whose scores are all -inf, which is NaN, or of a part that shows it no key. (A
+    // part of a tree's shows each row some: it holds more keys than a tree.)
+    const bool blank = L == 0.f && t + it.shift >= it.kv_lo;
     if (part && live && wave == 0 && g == 0)
-      *(float4_t*)(a.part_ml + ((int64_t)it.part + r) * 4) = float4_t{M, 0.f, L, 0.f};
-    const float mul = part ? 1.f : L == 0.f ? 0.f : 1.f / L;
+      *(float4_t*)(a.part_ml + ((int64_t)it.part + r) * 4) = float4_t{blank ? NAN : M, 0.f, L, 0.f};
+    const float mul = part ? 1.f : blank ? NAN : 1.f / L;
 #pragma unroll
     for (int x = 0; x < ND / kFewWaves; x++) {
       const int d = wave * (ND / kFewWaves) + x;
