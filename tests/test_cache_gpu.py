@@ -1162,3 +1162,24 @@ def test_f16_queries_that_are_infinite(ctx, torch_gpu, value, n):
         nan[rows] = True
         assert torch.equal(got.isnan(), nan), (m, tree, signs, int((got.isnan() != nan).sum()))
         assert torch.equal(got[~nan], clean[~nan])
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("size,eps", [(1e-30, 0.0), (1e-21, 1e-40), (1e-10, 0.0), (1e18, 1e-6), (1e25, 1e-6), (1e37, 1e30)])
+def test_norms_of_rows_of_every_size(ctx, torch_gpu, size, eps, form):
+    """f32 rows whose squares leave f32's range are normed like others, beside rows of ordinary size."""
+    torch = torch_gpu
+    T, H, Hkv, d = 37, 3, 2, 128
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(T, H + 2 * Hkv, d, device="cuda", generator=g)
+    x[::2, :H + Hkv] *= size
+    gains = [1 + 0.3 * torch.randn(d, device="cuda", generator=g) for _ in "qk"]
+    pool = Pool(torch, 1, 3, Hkv, 16, d, form)
+    slots = torch.arange(T, device="cuda", dtype=torch.int32)
+    q = store(ctx, torch, pool, 0, slots, x[:, :H], x[:, H:H + Hkv], x[:, H + Hkv:], q_gain=gains[0], k_gain=gains[1], eps=eps)
+    eps = float(np.float32(eps))
+    want, err = turned64(torch, x[:, :H], gains[0], eps, None, 0, 0, None, 1.0)
+    # a product below f32's normal range is off by up to 2^-126
+    assert bool(((q.double() - want).abs() <= err + U * want.abs() + 2.0 ** -126).all())
+    gk, _ = pool.values(slots)
+    check_rows(torch, pool, form, gk, *turned64(torch, x[:, H:H + Hkv], gains[1], eps, None, 0, 0, None, 1.0))

@@ -110,13 +110,28 @@ __device__ __forceinline__ void cache_store_rows(const CacheStoreArgs& a, int t0
     slot = next_slot;
     load(t0 + min(t + P, rows - 1), next, next_slot);
     if (gain) {
-      float ss = 0.f;
+      const auto mean = [&](float k2) {  // of the squares, and eps k2
+        float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < NU; i++)
+        for (int i = 0; i < NU; i++)
 #pragma unroll
-        for (int e = 0; e < V; e++) ss += x.A[i][e] * x.A[i][e] + x.B[i][e] * x.B[i][e];
-      ss = cache_over_lanes<LPH>(ss, [](float p, float q) { return p + q; });
-      const float sc = 1.f / sqrtf(ss * (1.f / D) + a.eps);
+          for (int e = 0; e < V; e++) ss += x.A[i][e] * x.A[i][e] + x.B[i][e] * x.B[i][e];
+        return cache_over_lanes<LPH>(ss, [](float p, float q) { return p + q; }) * (1.f / D) + k2;
+      };
+      float ms = mean(a.eps);
+      if (!(ms > 0x1p-84f && ms < 0x1p120f)) {
+        // squares that leave f32's range, or may: the row by a power of two, eps by its square
+        const float k = ms < 1.f ? 0x1p100f : 0x1p-64f;
+#pragma unroll
+        for (int i = 0; i < NU; i++)
+#pragma unroll
+          for (int e = 0; e < V; e++) {
+            x.A[i][e] *= k;
+            x.B[i][e] *= k;
+          }
+        ms = mean(a.eps * k * k);
+      }
+      const float sc = 1.f / sqrtf(ms);
 #pragma unroll
       for (int i = 0; i < NU; i++)
 #pragma unroll
