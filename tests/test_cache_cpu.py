@@ -170,3 +170,56 @@ def test_attention_refusals(change, word):
     assert tgo_amd.lib().tgohip_cache_attention(None, 1, ctypes.byref(c), a["layer"], SLOTS, 512, a["scale"], BASE + (10 << 20), 512,
                                                 a["dtype"]) == tgo_amd.EINVAL
     assert re.search(word, tgo_amd.last_error()), tgo_amd.last_error()
+
+
+def host_context():
+    """A context that never was, and a cache of tensors of the host: its calls end where the library asks for it."""
+    import torch
+    tgo_amd.lib()
+    c = object.__new__(tgo_amd.Context)
+    c.h, c.device, c._plans = None, -1, {}
+    codes = [torch.zeros(1, 8, 2, 16, 64, dtype=torch.int8) for _ in "kv"]
+    return c, tgo_amd.Cache(*codes, *(torch.zeros(1, 8, 2, 16) for _ in "kv"))
+
+
+@pytest.mark.parametrize("good", [[5], (5,), np.array([5]), np.array([5], np.int32), np.array([5], np.uint8), [np.int64(5)]])
+@pytest.mark.parametrize("bad", [np.array([2 ** 32 + 5]), [2 ** 32 + 5], [-2 ** 31 - 1], [2 ** 70], [1.7], np.array([5.0]), ["5"],
+                                 np.array([2 ** 31], np.uint32), (2 ** 40,)])
+def test_host_arrays_of_other_numbers_are_refused(good, bad):
+    """Slots, extents, lengths, pages and parents that are no whole numbers of 32 bits are not made into some."""
+    ctx, c = host_context()
+    table = [[0, 1, 2, 3]]
+    for src, dst in ((good, bad), (bad, good)):
+        with pytest.raises(tgo_amd.TgoError, match="slots are whole numbers of 32 bits"):
+            ctx.cache_move(c, src, dst)
+    with pytest.raises(tgo_amd.TgoError, match="context is missing"):
+        ctx.cache_move(c, good, [7])
+    with pytest.raises(tgo_amd.TgoError, match="extents are whole numbers"):
+        ctx.cache_plan(c, bad, good, table, 4)
+    with pytest.raises(tgo_amd.TgoError, match="lengths are whole numbers"):
+        ctx.cache_plan(c, good, bad, table, 4)
+    with pytest.raises(tgo_amd.TgoError, match="parents are whole numbers"):
+        ctx.cache_plan(c, [1], good, table, 4, parents=bad)
+    with pytest.raises(tgo_amd.TgoError, match="context is missing"):
+        ctx.cache_plan(c, good, [60], table, 4, parents=list(range(-1, 4)))
+
+
+@pytest.mark.parametrize("pages,word", [
+    ([[2 ** 32 + 1]], "pages are whole numbers"), (np.array([[2 ** 32 + 1]]), "pages are whole numbers"), ([[1.5]], "pages are whole numbers"),
+    ([[-1]], "page 0 is 4294967295 of a pool of 8"), (np.array([[-1]], np.int32), "page 0 is 4294967295 of a pool of 8"),
+    ([[3, -1]], "context is missing"), (np.array([[3, -1]]), "context is missing"), (np.array([[3]], np.uint32), "context is missing"),
+    ([3], "a page table of \\(1,\\)"),
+])
+def test_page_tables(pages, word):
+    ctx, c = host_context()
+    with pytest.raises(tgo_amd.TgoError, match=word):
+        ctx.cache_plan(c, [1], [9], pages, 4)
+
+
+def test_lists_of_other_shapes_are_refused():
+    ctx, c = host_context()
+    for extents, lengths in (([[1, 1]], [9]), ([1], [[9]]), ([1, 1], [9])):
+        with pytest.raises(tgo_amd.TgoError, match="cache_plan: extents of"):
+            ctx.cache_plan(c, extents, lengths, [[0]], 4)
+    with pytest.raises(tgo_amd.TgoError, match="slots are a list"):
+        ctx.cache_move(c, np.array([[1]]), [1])

@@ -271,6 +271,17 @@ def i32(a):
     return np.ascontiguousarray(np.asarray(a, dtype=np.int32))
 
 
+def _host_ints(a, what, dtype=np.int32):
+    """Whole numbers as a contiguous array of 32 bits; what does not fit is refused. In a page table's uint32
+    -1, say, is a page outside any pool."""
+    a = np.asarray(a)
+    if a.dtype != dtype and a.size:
+        top = 2 ** 31 if dtype is np.int32 else 2 ** 32
+        if a.dtype.kind not in "iub" or a.min() < -2 ** 31 or a.max() >= top:
+            raise TgoError(EINVAL, "%s are whole numbers of 32 bits" % what)
+    return np.ascontiguousarray(a.astype(dtype, copy=False))
+
+
 def _host_slots(a):
     """Slots as int32 on the host: what holds them, its address, their number. A list of ints goes through
     array, 18 ns each; through numpy 28."""
@@ -278,9 +289,9 @@ def _host_slots(a):
         try:
             a = array.array("i", a)
             return (a,) + a.buffer_info()
-        except TypeError:  # no ints
+        except (TypeError, OverflowError):  # no ints, or not of 32 bits
             pass
-    a = i32(a)
+    a = _host_ints(a, "slots")
     if a.ndim != 1:
         raise TgoError(EINVAL, "slots are a list, not of shape %s" % (a.shape,))
     return a, a.ctypes.data, a.size
@@ -1022,11 +1033,12 @@ class Context:
         """Decomposes a batch for cache_attention; returns the plan's handle. extents[b] new tokens end
         lengths[b] positions, pages [B, max_pages] their page table, parents (one per new token) their trees'.
         plan: a handle whose plan this one replaces."""
-        n, l, h = i32(extents), i32(lengths), ctypes.c_int(plan)
-        t = u32(pages)
-        if t.ndim != 2 or not len(n) == len(l) == len(t):
-            raise TgoError(EINVAL, "cache_plan: %d extents, %d lengths and a page table of %s" % (len(n), len(l), t.shape))
-        up = None if parents is None else i32(parents)
+        n, l, h = _host_ints(extents, "extents"), _host_ints(lengths, "lengths"), ctypes.c_int(plan)
+        t = _host_ints(pages, "pages", np.uint32)
+        if n.ndim != 1 or l.ndim != 1 or t.ndim != 2 or not len(n) == len(l) == len(t):
+            raise TgoError(EINVAL, "cache_plan: extents of %s, lengths of %s and a page table of %s" %
+                           (n.shape, l.shape, t.shape))
+        up = None if parents is None else _host_ints(parents, "parents")
         if up is not None and up.size != int(n.sum(dtype=np.int64)):
             raise TgoError(EINVAL, "cache_plan: %d parents for %d new tokens" % (up.size, int(n.sum(dtype=np.int64))))
         check(lib().tgohip_cache_plan(self.h, cache.at, len(n), ptr(n), ptr(l), ptr(t), t.shape[1], ptr(up), H, q_dtype,
