@@ -516,7 +516,8 @@ int tgohip_cache_store(tgohip_ctx* ctx, const tgohip_cache* cache, int layer, in
 /* Rows of slots (device int32 [T]) of a layer back as values: K's to k_out, V's to v_out
  * (either may be NULL), [T, kv_heads, head_dim] with the strides given, f32 (exact but for the
  * product's rounding) or f16 (rounded once more, past its range infinite). A slot outside the
- * pool reads as zeros. T kv_heads below 2^29. Can be captured. */
+ * pool reads as zeros. T kv_heads below 2^29, strides at most 2^36, T times a row's at most 2^60. Can be
+ * captured. */
 int tgohip_cache_read(tgohip_ctx* ctx, const tgohip_cache* cache, int layer, const int32_t* slots, int T,
                       void* k_out, int64_t k_row, int64_t k_head, void* v_out, int64_t v_row,
                       int64_t v_head, int out_dtype);

@@ -223,3 +223,19 @@ def test_lists_of_other_shapes_are_refused():
             ctx.cache_plan(c, extents, lengths, [[0]], 4)
     with pytest.raises(tgo_amd.TgoError, match="slots are a list"):
         ctx.cache_move(c, np.array([[1]]), [1])
+
+
+@pytest.mark.parametrize("T,row,word", [
+    (1 << 28, 1 << 36, "k_out's 268435456 rows are 68719476736 elements apart"), (1 << 28, (1 << 32) + 1, "at most 2\\^60"),
+    (1 << 28, 1 << 32, "context is missing"), ((1 << 29) - 1, 1 << 31, "context is missing"),
+    ((1 << 29) - 1, 1 << 34, "v_out's 536870911 rows"), (3, 1 << 36, "context is missing"),
+])
+def test_reads_of_rows_far_apart(T, row, word):
+    """What is computed of operands' places stays in 64 bits, whatever rows and strides are asked for."""
+    c = cache(kv_heads=1)
+    out = [BASE + (1 << 40), None]
+    if "v_out" in word:
+        out.reverse()
+    assert tgo_amd.lib().tgohip_cache_read(None, ctypes.byref(c), 0, SLOTS, T, out[0], row, 64, out[1], row, 64,
+                                           0) == tgo_amd.EINVAL
+    assert re.search(word, tgo_amd.last_error()), tgo_amd.last_error()

@@ -8,7 +8,9 @@
 
 namespace {
 
-constexpr int64_t kTopStride = (int64_t)1 << 36;  // beyond any tensor; products with it stay in 64 bits
+// Beyond any tensor. Bytes from an operand's first row to its last stay in 64 bits: a stride of at most
+// kTopStride elements times fewer than 2^24 rows, or rows times their stride at most kTopReach.
+constexpr int64_t kTopStride = (int64_t)1 << 36, kTopReach = (int64_t)1 << 60;
 
 std::string str(int64_t v) { return std::to_string(v); }
 
@@ -341,6 +343,9 @@ int tgohip_cache_read(tgohip_ctx* c, const tgohip_cache* cache, int layer, const
       if ((uintptr_t)out[i] % ob) return refuse(std::string("cache_read: ") + names[i] + " is not aligned to its type");
       if (bad_stride(row[i]) || bad_stride(head[i]))
         return refuse("cache_read: strides are not negative, and at most 2^36 elements");
+      if (row[i] > kTopReach / T)
+        return refuse(std::string("cache_read: ") + names[i] + "'s " + str(T) + " rows are " + str(row[i]) +
+                      " elements apart; rows times their stride is at most 2^60");
       if (overlap(T, row[i], Hkv, head[i], d))
         return refuse(std::string("cache_read: heads of ") + names[i] + " overlap (strides " + str(row[i]) + ", " +
                       str(head[i]) + ")");
