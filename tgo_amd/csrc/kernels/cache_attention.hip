@@ -94,36 +94,6 @@ __device__ __forceinline__ half2_t cache_rest2(float2_t p, half2_t h) {
   return __builtin_convertvector(r, half2_t);
 }
 
-template <bool QF16>
-__device__ __forceinline__ void cache_load_q(const void* q, int64_t off, half8_t& hi, half8_t& lo) {
-  if constexpr (QF16) {
-    hi = *(const half8_t*)((const half_t*)q + off);
-  } else {
-    const float4_t a = *(const float4_t*)((const float*)q + off), b = *(const float4_t*)((const float*)q + off + 4);
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const float f = j < 4 ? a[j & 3] : b[j & 3];
-      hi[j] = (half_t)f;
-      lo[j] = (half_t)(f - (float)hi[j]);
-    }
-  }
-}
-
-__device__ __forceinline__ void cache_out4(const CacheAttnArgs& a, int64_t off, float4_t v) {
-  if (a.out_form == OUT_F32) {
-    *(float4_t*)((float*)a.out + off) = v;
-    return;
-  }
-  half4_t hv, lv;
-#pragma unroll
-  for (int e = 0; e < 4; e++) {
-    hv[e] = (half_t)v[e];
-    lv[e] = (half_t)(v[e] - (float)hv[e]);
-  }
-  *(half4_t*)((half_t*)a.out + off) = hv;
-  if (a.out_form == OUT_X2) *(half4_t*)((half_t*)a.out + a.out_lo + off) = lv;
-}
-
 // Which of the 32 keys from position t0 on a token sees, as bits. mask: its tree's.
 // 64-bit shifts here go by amounts of the whole wave only: with a lane's amount in the last
 // register that the wave has allocated, v_lshlrev_b64 has shifted by the lane's v0 instead
@@ -224,7 +194,7 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, const Ca
     // 16-byte read of K serves two steps
 #pragma unroll
     for (int s = 0; s < NS; s++)
-      cache_load_q<QF16>(a.q, at + 64 * (s / 2) + 16 * g + 8 * (s % 2), qh[b][s], ql[b][QF16 ? 0 : s]);
+      pack_load_q<QF16>(a.q, at + 64 * (s / 2) + 16 * g + 8 * (s % 2), qh[b][s], ql[b][QF16 ? 0 : s]);
     m[b] = kCacheNoMax;
     l[b] = 0.f;
 #pragma unroll
@@ -392,7 +362,7 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, const Ca
       if (!live) continue;
       v *= mul;
       if (part) *(float4_t*)(a.part_o + ((int64_t)it.part + r) * D + 16 * d + 4 * g) = v;
-      else cache_out4(a, (int64_t)(it.q0 + t) * a.out_row + head * D + 16 * d + 4 * g, v);
+      else pack_store4(a, (int64_t)(it.q0 + t) * a.out_row + head * D + 16 * d + 4 * g, v);
     }
   };
   static_assert(RB <= 2, "a pair of buffers for each block");

@@ -69,8 +69,9 @@ __device__ __forceinline__ void pack_load_q(const void* q, int64_t off, half8_t&
   }
 }
 
-// Four neighbouring values of a result, `off` elements from its start.
-__device__ __forceinline__ void pack_store4(const PackedArgs& a, int64_t off, float4_t v) {
+// Four neighbouring values of a result, `off` elements from its start. A: PackedArgs, CacheAttnArgs.
+template <typename A>
+__device__ __forceinline__ void pack_store4(const A& a, int64_t off, float4_t v) {
   if (a.out_form == OUT_F32) {
     *(float4_t*)((float*)a.out + off) = v;
     return;
