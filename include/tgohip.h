@@ -551,8 +551,9 @@ int tgohip_cache_plan_free(tgohip_ctx* ctx, int handle);
  * elements apart (at most 2^30), heads dense, 16-byte aligned; scale is from 2^-64 to
  * 2^32. Both products take the codes as they are, scales are f32 in the softmax; f32 queries go
  * as f16 hi + lo pairs and so do their probabilities (|q| < 65504, carried to 2^-22 of
- * itself or 2^-25), f16 queries take f16 probabilities. Scores, sums and partial results are
- * f32. A row that sees a key or value standing for NaN is NaN; nothing that it does not see
+ * itself or 2^-25). f16 queries' probabilities are pairs too for a sequence with up to 64 rows a kv
+ * head (new tokens times H / kv_heads) and for the last up to 64 rows of others, f16 (2^-11 of each) for
+ * the rest. Scores, sums and partial results are f32. A row that sees a key or value standing for NaN is NaN; nothing that it does not see
  * reaches it. Memory behind the last row stays as it is; out meets neither q nor the cache. Can
  * be captured. */
 int tgohip_cache_attention(tgohip_ctx* ctx, int handle, const tgohip_cache* cache, int layer, const void* q,

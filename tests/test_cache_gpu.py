@@ -1183,3 +1183,17 @@ def test_norms_of_rows_of_every_size(ctx, torch_gpu, size, eps, form):
     assert bool(((q.double() - want).abs() <= err + U * want.abs() + 2.0 ** -126).all())
     gk, _ = pool.values(slots)
     check_rows(torch, pool, form, gk, *turned64(torch, x[:, H:H + Hkv], gains[1], eps, None, 0, 0, None, 1.0))
+
+
+@pytest.mark.parametrize("H,Hkv,d,form", [(8, 2, 128, "i8"), (32, 1, 64, "f8"), (16, 16, 128, "f8")])
+def test_f16_queries_of_few_rows_to_f32(ctx, torch_gpu, H, Hkv, d, form):
+    """Single tokens, small trees and chunks of f16 queries are as near as f32 ones that hold the same values: the
+    tolerance without an f16 term."""
+    r = np.random.default_rng(2)
+    most = 64 * Hkv // H
+    extents = [1, 1, most, min(most, 12), 1, 2]
+    lengths = [1, 9000, most + 300, 1500, 64, 700]
+    b = Batch(torch_gpu, extents, lengths, H, Hkv, d, form, True, trees=[None, None, None, random_tree(r, extents[3], 4), None, None])
+    got = b.run(ctx, out=torch_gpu.empty(b.q.shape, device="cuda"))
+    b.q = b.q.float()
+    b.check(got)

@@ -133,7 +133,8 @@ __device__ __forceinline__ int cache_v_swz(int r) {
 // LDS. S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16: lane (l16, g) holds row
 // l16 of each block of 16 rows, its scores at keys 16 kb + 4g + i, and of O^T dims
 // 16 db + 4g + i. A tile stays 8 bits in LDS and is converted by the wave that uses it, V by
-// the transposing read of bytes. Single tokens (4 rows of 16 used) by items of 16 / 32 rows, us: 128 of
+// the transposing read of bytes. Probabilities are pairs for f16 queries too: 128 tokens 62.7 us, with f16
+// ones 62.1 and 1.1e-4 from the definition beside the output's rounding. Single tokens (4 rows of 16 used) by items of 16 / 32 rows, us: 128 of
 // 16 to 8192 keys 65 / 81, one of 8192 11.6 / 13.3. The next tile's loads before the wait for this
 // one (twice the bytes in flight): no faster, 64.7 beside 64.0.
 template <int D, bool QF16, bool F8, int RB>
@@ -285,11 +286,9 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, const Ca
           const half2_t h = __builtin_convertvector(p, half2_t);
           ph[b][4 * kb + i] = h[0];
           ph[b][4 * kb + i + 1] = h[1];
-          if (!QF16) {
-            const half2_t r = cache_rest2(p, h);
-            pl[b][4 * kb + i] = r[0];
-            pl[b][4 * kb + i + 1] = r[1];
-          }
+          const half2_t r = cache_rest2(p, h);
+          pl[b][4 * kb + i] = r[0];
+          pl[b][4 * kb + i + 1] = r[1];
           l[b] = fmaf(p[0], inv[i], l[b]);
           l[b] = fmaf(p[1], inv[i + 1], l[b]);
         }
@@ -308,7 +307,7 @@ __device__ __forceinline__ void cache_rows_body(const CacheAttnArgs& a, const Ca
 #pragma unroll
       for (int b = 0; b < RB; b++) {
         o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, ph[b], o[b][d], 0, 0, 0);
-        if (!QF16) o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[b], o[b][d], 0, 0, 0);
+        o[b][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va, pl[b], o[b][d], 0, 0, 0);
       }
     }
   };
@@ -562,7 +561,10 @@ __device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const Ca
         // All terms by the reference as it is; only where one of a row's has passed f16's range (its
         // first tile, or a key far above the ones before), or its reference is far, is its largest looked
         // for. Each row by itself: no bit of it depends on the wave's others. Scores rounded in every
-        // tile, as f32 queries' are: 1210 us beside 1177 for 2048 tokens behind 30720 positions.
+        // tile, as f32 queries' are: 1210 us beside 1177 for 2048 tokens behind 30720 positions. f16
+        // probabilities are within 2^-11 each, 1e-4 of the result beside the 2.1e-4 that an f16 output is rounded by;
+        // as pairs (in f32 queries' order of steps) that call takes 1519 us beside 1165, a prompt of 2048 88 beside
+        // 76, 32 trees 82 beside 74.
         half8_t ph[4], none;
         float l[4] = {}, most = 0.f;
 #pragma unroll
