@@ -10,13 +10,15 @@
 // scales are, and the sum takes it out again. m moves along (online softmax), and only
 // when a probability would leave its range.
 //
-// What bounds it: few rows read the codes once, at HBM's rate; many are bound by the matrix
-// unit and the exponentials beside it. Measured (32 heads over 8 of 128 dims, us with the
-// merge): one f32 token over 8192 int8 keys 11.4 (two launches and chains of dependent loads);
-// 128 over 16 to 8192 keys 64, 5.9 TB/s in the kernel (a plain read here 6.6); 32 trees of
-// 17 to 60 tokens over 256 to 4096 keys 92; four f32 chunks of 187 to 405 over 2616 to 5417 e4m3
-// keys 135; 2048 f16 tokens, the last of 32768, 1112 to 1185 from card to card, 0.90 to 0.96 PFLOP/s (a large f16 matrix
-// product here 1.27).
+// What bounds it: few rows read the codes once, at HBM's rate; with many a wave's products and its
+// exponentials take turns, the matrix unit and the VALU each busy 41 to 52% of the time. Measured (32
+// heads over 8 of 128 dims, us a call among others, merges in it, from card to card): one f32 token over 8192 int8
+// keys 11.4 (two launches and chains of dependent loads; 1.2 more where 36 layers take turns and the
+// keys come from HBM); 128 over 16 to 8192 keys 64, the kernel 61, 5.7 TB/s (a plain read here 6.6); 32 trees
+// of 16 to 64 tokens over 285 to 4030 keys 92 to 95, of f16 queries 69 to 75; four f32 chunks of 187 to 405 over
+// 2616 to 5417 e4m3 keys 133 to 141, f16 111 to 115; 128 tokens over 256 to 4096 keys and two chunks of 512 in one call 154 to
+// 159, f16 129 to 133; 2048 f16 tokens, the last of 32768, 1126 to 1177, 0.91 to 0.95 PFLOP/s (a large f16
+// matrix product here 1.27).
 #include "pack_rows.h"
 
 #include <algorithm>
@@ -42,7 +44,7 @@ constexpr int kFewTile = 32;   // keys of a wave's tile
 constexpr int kFewWaves = 4;
 constexpr int kFewRows = 32;   // rows of an item
 // Up to so many rows at the end of a (sequence, head)'s go as such items. Up to 32 / 64 / 96 / 256,
-// us: 32 trees of 68 to 240 rows 97.6 / 94.4 / 95.0 / 100.8, four chunks of 748 to 1620
+// us: 32 trees of 64 to 256 rows 97.6 / 94.4 / 95.0 / 100.8, four chunks of 748 to 1620
 // 141.5 / 141.5 / 141.4 / 144.1.
 constexpr int kFewLast = 64;
 
@@ -69,8 +71,8 @@ __device__ __forceinline__ half8_t cache_half8(uint32_t a, uint32_t b) {
 }
 
 // What a key's scales are in the softmax: a_k, b_k / a_k and 1 / v_scale_k. The products
-// accumulate onto b_k / a_k, so that one multiply-add makes a term's exponent of them,
-// a_k (b_k / a_k + S_k) - m. A row that stands for NaN makes its key's start NaN, not a_k:
+// accumulate onto b_k / a_k, so that one product makes a score of them, or one multiply-add a
+// term's exponent, a_k (b_k / a_k + S_k) - m. A row that stands for NaN makes its key's start NaN, not a_k:
 // a masked score, -inf by then, stays so.
 struct KeyScales {
   float a, start, inv;
@@ -629,7 +631,8 @@ __device__ __forceinline__ void cache_tile_body(const CacheAttnArgs& a, const Ca
 }
 
 // Items of all kinds, two workgroups a CU: chunks, trees and single tokens of a batch run
-// beside each other.
+// beside each other. Registers end at 256 for that: with 128 dims the tile body spills 10 or 11 of them for
+// f16 queries (40 bytes a lane), none or 2 for f32.
 template <int D, bool QF16, bool F8>
 __global__ __launch_bounds__(256, 2) void cache_attention_kernel(CacheAttnArgs a) {
   // an array for each buffer: a read of one does not wait for the DMA into another
@@ -656,6 +659,8 @@ __global__ __launch_bounds__(512, 1) void cache_wide_kernel(CacheAttnArgs a) {
 // host
 // ---------------------------------------------------------------------------
 
+// Host time of a plan, its upload and the binding: 18 to 24 us for one sequence or a few, 76 for 128 single tokens,
+// 131 for 512, 78 for 32 trees; once for all layers of a step.
 void cache_build_plan(int B, const int32_t* extents, const int32_t* lengths, const uint8_t* tree, int H, int Hkv, int D,
                       bool q_f16, int ncu, CachePlan& plan) {
   plan = CachePlan();

@@ -6,9 +6,9 @@
 // c s. A row with a value that is not finite, or past 2^40, has the scale NaN and codes 0:
 // all of it stands for NaN, and no code is ever one.
 //
-// All three are bound by the rows' bytes. Measured (a large copy here 4.7 TB/s): store of
-// 16384 rows of 80 f16 heads of 128 dims, normed, half of each rotated, 639 MB, 137 us, 4.7 TB/s;
-// of 1152 rows of 48 f32 heads, 50 MB, 11.3; of one row 2.8, 7 with the call.
+// All three are bound by the rows' bytes. Measured (a large copy here 4.7 TB/s), us of the kernel: store
+// of 16384 rows of 80 f16 heads of 128 dims, normed, half of each rotated, 639 MB, 141, 4.5 TB/s;
+// of 1152 rows of 48 f32 heads, 50 MB, 12; of one row 3.3, 7 with the call.
 #include "heads.h"
 
 #include <algorithm>
@@ -265,10 +265,10 @@ void launch_cache_store(const CacheStoreArgs& args, int ncu, hipStream_t st) {
   CacheStoreArgs a = args;
   const int heads = a.H + 2 * a.c.Hkv, at_once = 256 / (a.c.d / 8);
   // Few rows: their heads spread over workgroups, down to one head for each group of lanes. Spread /
-  // all by one workgroup, us of 48 f32 heads: one row 2.8 / 4.3, 64 rows 3.4 / 4.8. Many: a
+  // all by one workgroup, us of 48 f32 heads in a graph: one row 3.1 / 4.7, 64 rows 3.6 / 5.2. Many: a
   // workgroup takes all heads of up to 16 rows, and their angles once. Up to 1 / 4 / 16 / 64
-  // rows, us with 17 and 3 of reading them back: 16384 of 80 f16 heads 169 / 160 / 154 / 154,
-  // 1152 of 48 f32 heads 14.6 each.
+  // rows, us with 17 and 4 of reading them back: 16384 of 80 f16 heads 169 / 161 / 157 / 157,
+  // 1152 of 48 f32 heads 14.8 each.
   a.slice = heads;
   while (a.slice > at_once && (int64_t)a.T * ((heads + a.slice - 1) / a.slice) < 2 * ncu)
     a.slice = std::max(at_once, (a.slice + 1) / 2);
@@ -279,7 +279,7 @@ void launch_cache_store(const CacheStoreArgs& args, int ncu, hipStream_t st) {
     return (uintptr_t)p % 16 == 0 && row % n == 0 && head % n == 0;
   };
   // Units of eight elements, where every head starts on 16 bytes, / of two, us with the same: 16384
-  // rows 154 / 212, 1152 14.6 / 17.8.
+  // rows 157 / 214, 1152 14.8 / 17.8.
   const bool wide = a.rd % 8 == 0 && fits(a.k, a.k_row, a.k_head, a.x_f16) && fits(a.v, a.v_row, a.v_head, a.x_f16) &&
                     (!a.H || (fits(a.q, a.q_row, a.q_head, a.x_f16) && fits(a.q_out, a.out_row, a.out_head, a.out_f16))) &&
                     (uintptr_t)a.q_gain % 16 == 0 && (uintptr_t)a.k_gain % 16 == 0;
