@@ -515,9 +515,9 @@ int tgohip_cache_store(tgohip_ctx* ctx, const tgohip_cache* cache, int layer, in
 
 /* Rows of slots (device int32 [T]) of a layer back as values: K's to k_out, V's to v_out
  * (either may be NULL), [T, kv_heads, head_dim] with the strides given, f32 (exact but for the
- * product's rounding) or f16 (rounded once more, past its range infinite). A slot outside the
- * pool reads as zeros. T kv_heads below 2^29, strides at most 2^36, T times a row's at most 2^60. Can be
- * captured. */
+ * product's rounding) or f16 (that rounded, or the product itself; past its range infinite). A slot
+ * outside the pool reads as zeros. T kv_heads below 2^29, strides at most 2^36 elements, T times a
+ * row's at most 2^60. Can be captured. */
 int tgohip_cache_read(tgohip_ctx* ctx, const tgohip_cache* cache, int layer, const int32_t* slots, int T,
                       void* k_out, int64_t k_row, int64_t k_head, void* v_out, int64_t v_row,
                       int64_t v_head, int out_dtype);
@@ -552,10 +552,11 @@ int tgohip_cache_plan_free(tgohip_ctx* ctx, int handle);
  * 2^32. Both products take the codes as they are, scales are f32 in the softmax; f32 queries go
  * as f16 hi + lo pairs and so do their probabilities (|q| < 65504, carried to 2^-22 of
  * itself or 2^-25). f16 queries' probabilities are pairs too for a sequence with up to 64 rows a kv
- * head (new tokens times H / kv_heads) and for the last up to 64 rows of others, f16 (2^-11 of each) for
- * the rest. Scores, sums and partial results are f32. A row that sees a key or value standing for NaN is NaN; nothing that it does not see
- * reaches it. Memory behind the last row stays as it is; out meets neither q nor the cache. Can
- * be captured. */
+ * head (new tokens times H / kv_heads), and may be for the last up to 64 of others; f16 (2^-11 of
+ * each) for the rest. Scores, sums and partial results are f32: keys whose scores differ by less than
+ * a step of f32 may weigh alike. A row that sees a key or value standing for NaN is NaN, and one whose
+ * scores are all infinite; nothing that it does not see reaches it. Memory behind the last row stays
+ * as it is; out meets neither q nor the cache. Can be captured. */
 int tgohip_cache_attention(tgohip_ctx* ctx, int handle, const tgohip_cache* cache, int layer, const void* q,
                            int64_t q_row, float scale, void* out, int64_t out_row, int out_dtype);
 
